@@ -35,6 +35,8 @@ EXPORTS = [
     "caifx_moe_dispatch_map_workspace_bytes", "caifx_moe_build_dispatch_map", "caifx_moe_dispatch",
     "caifx_moe_combine", "caifx_moe_combine_backward_grad_expert", "caifx_moe_combine_backward_grad_weights",
     "caifx_moe_dispatch_backward", "caifx_moe_dispatch_fresh", "caifx_moe_combine_backward_grad_expert_fresh",
+    "caifx_adapters_forward", "caifx_adapters_backward", "caifx_adapters_workspace_bytes",
+    "caifx_checkpoint_pack", "caifx_checkpoint_unpack", "caifx_silu_multiply_checkpoint", "caifx_swiglu_backward_checkpoint",
 ]
 
 
@@ -116,6 +118,15 @@ def lib():
         L.caifx_moe_combine_backward_grad_expert.argtypes = [_p, _p, _p, _p, _p, _p, _i64, _i64, _int, _int, _int, _p]
         L.caifx_moe_combine_backward_grad_weights.argtypes = [_p, _p, _p, _p, _p, _p, _i64, _i64, _int, _int, _int, _p]
         L.caifx_moe_dispatch_backward.argtypes = [_p, _p, _p, _p, _p, _i64, _i64, _int, _int, _int, _p]
+        shape = [_i64, _i64, _i64, _int, _int]
+        L.caifx_adapters_workspace_bytes.restype = _sz
+        L.caifx_adapters_workspace_bytes.argtypes = shape + [_int, _int]
+        L.caifx_adapters_forward.argtypes = shape + [_p] * 8 + [_int, _p, _sz, _p]
+        L.caifx_adapters_backward.argtypes = shape + [_p] * 12 + [_int, _p, _sz, _p]
+        L.caifx_checkpoint_pack.argtypes = [_p, _p, _p, _i64, _i64, _int, _p]
+        L.caifx_checkpoint_unpack.argtypes = [_p, _p, _p, _i64, _i64, _int, _p]
+        L.caifx_silu_multiply_checkpoint.argtypes = [_p] * 7 + [_i64, _i64, _int, _p]
+        L.caifx_swiglu_backward_checkpoint.argtypes = [_p] * 8 + [_i64, _i64, _int, _p]
         _lib = L
     return _lib
 

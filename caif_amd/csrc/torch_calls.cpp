@@ -10,11 +10,13 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
 #include <stdexcept>
+#include <vector>
 
 #include "caifx.h"
 
@@ -30,7 +32,9 @@ namespace {
   X(caifx_moe_build_dispatch_map) X(caifx_moe_dispatch) X(caifx_moe_combine) X(caifx_moe_combine_backward_grad_expert)   \
   X(caifx_moe_combine_backward_grad_weights) X(caifx_moe_dispatch_backward) X(caifx_moe_dispatch_fresh)                  \
   X(caifx_moe_combine_backward_grad_expert_fresh) X(caifx_quantize_int8_per_channel)           \
-  X(caifx_quantize_int8_per_tensor) X(caifx_quantize_to_int4)
+  X(caifx_quantize_int8_per_tensor) X(caifx_quantize_to_int4) X(caifx_adapters_forward) X(caifx_adapters_backward)         \
+  X(caifx_adapters_workspace_bytes) X(caifx_checkpoint_pack) X(caifx_checkpoint_unpack) X(caifx_silu_multiply_checkpoint)   \
+  X(caifx_swiglu_backward_checkpoint)
 
 struct Api {
 #define X(name) decltype(&::name) name = nullptr;
@@ -512,11 +516,220 @@ PyObject *moe_combine_backward_grad_weights(PyObject *, PyObject *const *a, Py_s
   });
 }
 
+// ------------------------------------------------------------------ low-rank adapters, activation checkpoints
+// These calls run on the device their first tensor lives on, whichever is current, and on that device's current stream.
+struct Device {
+  at::Device at;
+  c10::DeviceGuard guard;
+  explicit Device(const at::Tensor &t) : at(t.device()), guard(at) {}
+  void *stream() const { return static_cast<void *>(c10::hip::getCurrentHIPStream(at.index()).stream()); }
+  // device memory of this device, contiguous, of the type and number of elements that the call takes
+  const at::Tensor &operand(PyObject *o, at::ScalarType type, int64_t elements, const char *what) const
+  {
+    const at::Tensor &t = device_tensor(o);
+    if (t.device() != at) throw Error{PyExc_RuntimeError, "tensors must be on one device"};
+    if (t.scalar_type() != type || t.numel() != elements) throw Error{PyExc_ValueError, what};
+    return t;
+  }
+  const at::Tensor *optional(PyObject *o, at::ScalarType type, int64_t elements, const char *what) const
+  {
+    return o == Py_None ? nullptr : &operand(o, type, elements, what);
+  }
+};
+
+void *data(const at::Tensor *t) { return t ? t->data_ptr() : nullptr; }
+
+bool truth(PyObject *o)
+{
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Error{nullptr, nullptr};
+  return v != 0;
+}
+
+// the factors of the adapters: a [L, rank, K], b [L, N, rank]
+struct Factors {
+  int64_t L, rank, K, N;
+  Factors(const Device &d, const at::Tensor &a, const at::Tensor &b, at::ScalarType type)
+  {
+    if (a.dim() != 3 || b.dim() != 3 || a.size(0) != b.size(0) || a.size(1) != b.size(2))
+      throw Error{PyExc_ValueError, "the factors must be a [adapters, rank, K] and b [adapters, N, rank]"};
+    if (a.scalar_type() != type || b.scalar_type() != type) throw Error{PyExc_ValueError, "the factors must have the activations' dtype"};
+    if (a.device() != d.at || b.device() != d.at) throw Error{PyExc_RuntimeError, "tensors must be on one device"};
+    L = a.size(0), rank = a.size(1), K = a.size(2), N = b.size(1);
+    if (L > INT32_MAX || rank > INT32_MAX) throw Error{PyExc_OverflowError, "too many adapters"};
+    if (a.numel() == 0 || b.numel() == 0) throw Error{PyExc_ValueError, "the factors have no elements"};
+  }
+};
+
+int64_t rows_of(const at::Tensor &t, int64_t columns)
+{
+  if (t.dim() == 0 || t.size(t.dim() - 1) != columns) throw Error{PyExc_ValueError, "a row of activations must be as long as the factors' rows"};
+  return t.numel() / columns;
+}
+
+struct Scratch {
+  at::Tensor held;
+  size_t bytes;
+  Scratch(const at::Tensor &x, size_t n) : bytes(n)
+  {
+    if (n > 0) held = bytes_like(x, n);
+  }
+  void *p() const { return bytes ? held.data_ptr() : nullptr; }
+};
+
+// adapters_forward(x, ids, a, b, scaling, base, keep_hidden, out) -> y, (y, hidden) or status
+PyObject *adapters_forward(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  return guarded(n, 8, [&]() -> PyObject * {
+    const at::Tensor &x = device_tensor(v[0]), &a = device_tensor(v[2]), &b = device_tensor(v[3]);
+    const Device d(x);
+    const int dt = code_of(x.scalar_type());
+    const Factors f(d, a, b, x.scalar_type());
+    const int64_t M = rows_of(x, f.K);
+    const at::Tensor &ids = d.operand(v[1], at::kInt, M, "ids must be int32, one per row");
+    const at::Tensor &scaling = d.operand(v[4], at::kFloat, f.L, "scaling must be fp32, one per adapter");
+    const at::Tensor *base = d.optional(v[5], x.scalar_type(), M * f.N, "base must have the activations' dtype and rows x N elements");
+    const bool keep = truth(v[6]);
+    const at::Tensor *out = d.optional(v[7], x.scalar_type(), M * f.N, "out must have the activations' dtype and rows x N elements");
+    const at::Tensor y = out ? *out : at::empty({M, f.N}, x.options());
+    const at::Tensor hidden = keep ? at::empty({M, f.rank}, x.options().dtype(at::kFloat)) : at::Tensor();
+    const int L = static_cast<int>(f.L), r = static_cast<int>(f.rank);
+    const Scratch ws(x, api.caifx_adapters_workspace_bytes(M, f.N, f.K, r, L, dt, 0));
+    const int st = launch(api.caifx_adapters_forward, M, f.N, f.K, r, L, x.data_ptr(), static_cast<const int32_t *>(ids.data_ptr()), a.data_ptr(),
+                          b.data_ptr(), static_cast<const float *>(scaling.data_ptr()), data(base), y.data_ptr(),
+                          static_cast<float *>(keep ? hidden.data_ptr() : nullptr), dt, ws.p(), ws.bytes, d.stream());
+    return keep ? pair(st, y, hidden) : result(st, y);
+  });
+}
+
+// adapters_backward(dy, x or codes, scales or None, hidden, ids, a, b, scaling, base, need_dx) -> (dx or None, grad_a, grad_b) or status
+PyObject *adapters_backward(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  return guarded(n, 10, [&]() -> PyObject * {
+    const at::Tensor &dy = device_tensor(v[0]), &a = device_tensor(v[5]), &b = device_tensor(v[6]);
+    const Device d(dy);
+    const int dt = code_of(dy.scalar_type());
+    const Factors f(d, a, b, dy.scalar_type());
+    const int64_t M = rows_of(dy, f.N), groups = (f.K + CAIFX_CHECKPOINT_GROUP - 1) / CAIFX_CHECKPOINT_GROUP;
+    const bool packed = v[2] != Py_None;
+    const at::Tensor &x = d.operand(v[1], packed ? at::kChar : dy.scalar_type(), M * f.K, "x must have rows x K elements of the gradient's dtype, or be int8 codes with scales");
+    const at::Tensor *scales = d.optional(v[2], at::kFloat, M * groups, "the checkpoint's scales must be fp32, one per 128 values of a row");
+    const at::Tensor &hidden = d.operand(v[3], at::kFloat, M * f.rank, "hidden must be fp32 [rows, rank]");
+    const at::Tensor &ids = d.operand(v[4], at::kInt, M, "ids must be int32, one per row");
+    const at::Tensor &scaling = d.operand(v[7], at::kFloat, f.L, "scaling must be fp32, one per adapter");
+    const at::Tensor *base = d.optional(v[8], dy.scalar_type(), M * f.K, "base must have the gradient's dtype and rows x K elements");
+    const bool need = truth(v[9]);
+    const at::Tensor dx = need ? at::empty({M, f.K}, dy.options()) : at::Tensor();
+    const at::Tensor ga = at::empty_like(a), gb = at::empty_like(b);
+    const int L = static_cast<int>(f.L), r = static_cast<int>(f.rank);
+    const Scratch ws(dy, api.caifx_adapters_workspace_bytes(M, f.N, f.K, r, L, dt, 1));
+    const int st = launch(api.caifx_adapters_backward, M, f.N, f.K, r, L, dy.data_ptr(), x.data_ptr(), static_cast<const float *>(data(scales)),
+                          static_cast<const float *>(hidden.data_ptr()), static_cast<const int32_t *>(ids.data_ptr()), a.data_ptr(), b.data_ptr(),
+                          static_cast<const float *>(scaling.data_ptr()), data(base), need ? dx.data_ptr() : nullptr, ga.data_ptr(), gb.data_ptr(), dt,
+                          ws.p(), ws.bytes, d.stream());
+    if (st != CAIFX_OK) return PyLong_FromLong(st);
+    Owned p(need ? THPVariable_Wrap(dx) : Py_NewRef(Py_None)), q(THPVariable_Wrap(ga)), t(THPVariable_Wrap(gb));
+    return PyTuple_Pack(3, p.p, q.p, t.p);
+  });
+}
+
+// rows and columns of an activation, and its checkpoint's tensors
+struct Packed {
+  int64_t rows = 0, cols = 0, groups = 0;
+  explicit Packed(const at::Tensor &t)
+  {
+    if (t.dim() == 0) throw Error{PyExc_ValueError, "an activation has at least one dimension"};
+    cols = t.size(t.dim() - 1);
+    rows = cols > 0 ? t.numel() / cols : 0;
+    groups = (cols + CAIFX_CHECKPOINT_GROUP - 1) / CAIFX_CHECKPOINT_GROUP;
+  }
+  static at::Tensor codes(const at::Tensor &like) { return at::empty(like.sizes(), like.options().dtype(at::kChar)); }
+  at::Tensor scales(const at::Tensor &like) const
+  {
+    std::vector<int64_t> shape = like.sizes().vec();
+    shape.back() = groups;
+    return at::empty(shape, like.options().dtype(at::kFloat));
+  }
+};
+
+float *floats(const at::Tensor &t) { return static_cast<float *>(t.data_ptr()); }
+
+// checkpoint_pack(x) -> (codes, scales) or status
+PyObject *checkpoint_pack(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  return guarded(n, 1, [&]() -> PyObject * {
+    const at::Tensor &x = device_tensor(v[0]);
+    const Device d(x);
+    const int dt = code_of(x.scalar_type());
+    const Packed p(x);
+    const at::Tensor codes = Packed::codes(x), scales = p.scales(x);
+    return pair(launch(api.caifx_checkpoint_pack, x.data_ptr(), codes.data_ptr(), floats(scales), p.rows, p.cols, dt, d.stream()), codes, scales);
+  });
+}
+
+// checkpoint_unpack(codes, scales, dtype code) -> values or status
+PyObject *checkpoint_unpack(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  return guarded(n, 3, [&]() -> PyObject * {
+    const at::Tensor &codes = device_tensor(v[0]);
+    const Device d(codes);
+    if (codes.scalar_type() != at::kChar) throw Error{PyExc_ValueError, "a checkpoint's codes are int8"};
+    const Packed p(codes);
+    const at::Tensor &scales = d.operand(v[1], at::kFloat, p.rows * p.groups, "the checkpoint's scales must be fp32, one per 128 values of a row");
+    const int dt = static_cast<int>(integer(v[2]));
+    const at::Tensor y = at::empty(codes.sizes(), codes.options().dtype(type_of(dt)));
+    return result(launch(api.caifx_checkpoint_unpack, codes.data_ptr(), floats(scales), y.data_ptr(), p.rows, p.cols, dt, d.stream()), y);
+  });
+}
+
+// silu_multiply_checkpoint(gate, up) -> (hidden, gate codes, gate scales, up codes, up scales) or status
+PyObject *silu_multiply_checkpoint(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  return guarded(n, 2, [&]() -> PyObject * {
+    const at::Tensor &gate = device_tensor(v[0]);
+    const Device d(gate);
+    const int dt = code_of(gate.scalar_type());
+    const at::Tensor &up = d.operand(v[1], gate.scalar_type(), gate.numel(), "gate and up must have one shape and dtype");
+    if (up.sizes() != gate.sizes()) throw Error{PyExc_ValueError, "gate and up must have one shape and dtype"};
+    const Packed p(gate);
+    const at::Tensor hidden = at::empty_like(gate), gc = Packed::codes(gate), gs = p.scales(gate), uc = Packed::codes(gate), us = p.scales(gate);
+    const int st = launch(api.caifx_silu_multiply_checkpoint, gate.data_ptr(), up.data_ptr(), hidden.data_ptr(), gc.data_ptr(), floats(gs), uc.data_ptr(),
+                          floats(us), p.rows, p.cols, dt, d.stream());
+    if (st != CAIFX_OK) return PyLong_FromLong(st);
+    Owned o1(THPVariable_Wrap(hidden)), o2(THPVariable_Wrap(gc)), o3(THPVariable_Wrap(gs)), o4(THPVariable_Wrap(uc)), o5(THPVariable_Wrap(us));
+    return PyTuple_Pack(5, o1.p, o2.p, o3.p, o4.p, o5.p);
+  });
+}
+
+// swiglu_backward_checkpoint(gate codes, gate scales, up codes, up scales, grad_hidden, with_hidden) -> (grad_gate, grad_up[, hidden]) or status
+PyObject *swiglu_backward_checkpoint(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  return guarded(n, 6, [&]() -> PyObject * {
+    const at::Tensor &grad = device_tensor(v[4]);
+    const Device d(grad);
+    const int dt = code_of(grad.scalar_type());
+    const Packed p(grad);
+    const char *codes_are = "a checkpoint's codes are int8, of the gradient's shape", *scales_are = "the checkpoint's scales must be fp32, one per 128 values of a row";
+    const at::Tensor &gc = d.operand(v[0], at::kChar, grad.numel(), codes_are), &uc = d.operand(v[2], at::kChar, grad.numel(), codes_are);
+    const at::Tensor &gs = d.operand(v[1], at::kFloat, p.rows * p.groups, scales_are), &us = d.operand(v[3], at::kFloat, p.rows * p.groups, scales_are);
+    if (Packed(gc).cols != p.cols || Packed(uc).cols != p.cols) throw Error{PyExc_ValueError, codes_are};
+    const bool with = truth(v[5]);
+    const at::Tensor gg = at::empty_like(grad), gu = at::empty_like(grad), hidden = with ? at::empty_like(grad) : at::Tensor();
+    const int st = launch(api.caifx_swiglu_backward_checkpoint, gc.data_ptr(), floats(gs), uc.data_ptr(), floats(us), grad.data_ptr(), gg.data_ptr(),
+                          gu.data_ptr(), with ? hidden.data_ptr() : nullptr, p.rows, p.cols, dt, d.stream());
+    if (!with) return pair(st, gg, gu);
+    if (st != CAIFX_OK) return PyLong_FromLong(st);
+    Owned o1(THPVariable_Wrap(gg)), o2(THPVariable_Wrap(gu)), o3(THPVariable_Wrap(hidden));
+    return PyTuple_Pack(3, o1.p, o2.p, o3.p);
+  });
+}
+
 PyMethodDef methods[] = {
     {"bind", bind, METH_O, nullptr},
 #define M(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr},
     M(qlinear) M(grouped) M(quantize_int8) M(quantize_int4) M(elementwise) M(swiglu_backward) M(moe_build_dispatch_map) M(moe_dispatch) M(moe_combine)
     M(moe_combine_backward_grad_expert) M(moe_dispatch_backward) M(moe_combine_backward_grad_weights)
+    M(adapters_forward) M(adapters_backward) M(checkpoint_pack) M(checkpoint_unpack) M(silu_multiply_checkpoint) M(swiglu_backward_checkpoint)
 #undef M
     {nullptr, nullptr, 0, nullptr}};
 

@@ -273,3 +273,49 @@ def moe_combine_backward_grad_weights(grad_output, expert_buffer, expert_indices
     return _done((_native or _calls()).moe_combine_backward_grad_weights(
         grad_output, expert_buffer, expert_indices, dispatch_map, expert_offsets),
         "caifx_moe_combine_backward_grad_weights")
+
+
+# ------------------------------------------------------------------ low-rank adapters
+def adapters_forward(x, ids, a, b, scaling, base=None, keep_hidden=False, out=None):
+    """The low-rank branches of many requests beside the projection that they share (CAIF_DeviceLoRAAdapter's branch,
+    src/caif_device_lora_adapter.cpp:161-198, for rows of different adapters): with l = ids[m],
+    hidden[m] = x[m] a[l]^T and y[m] = T(base[m] + scaling[l] * hidden[m] b[l]^T).
+
+    x [..., K], ids int32 (one per row; outside [0, L): no adapter), a [L, rank, K], b [L, N, rank], scaling fp32 [L],
+    base [M, N] the projection's result (None: zero).  Returns y [M, N], with keep_hidden (y, hidden fp32 [M, rank]), which
+    adapters_backward takes.  `out` may be `base`.  Tensors are contiguous, on one device, and run on its current stream."""
+    return _done((_native or _calls()).adapters_forward(x, ids, a, b, scaling, base, keep_hidden, out), "caifx_adapters_forward")
+
+
+def adapters_backward(dy, x, hidden, ids, a, b, scaling, base=None, need_dx=True):
+    """(dx, grad_a, grad_b) of adapters_forward: dx [M, K] is `base` (the projection's own input gradient, None: zero) plus the
+    branch's, the factors' gradients have their shapes and type.  `x` is the forward's input or its checkpoint, the pair that
+    checkpoint_pack returned.  need_dx=False (a first layer): dx is None."""
+    codes, scales = x if isinstance(x, (tuple, list)) else (x, None)
+    return _done((_native or _calls()).adapters_backward(dy, codes, scales, hidden, ids, a, b, scaling, base, need_dx), "caifx_adapters_backward")
+
+
+# ------------------------------------------------------------------ activation checkpoints in 8 bits
+def checkpoint_pack(x):
+    """(codes int8 of x's shape, scales fp32 [..., ceil(columns / 128)]): an activation kept for the backward pass, one scale per
+    128 neighbouring values of a row."""
+    return _done((_native or _calls()).checkpoint_pack(x), "caifx_checkpoint_pack")
+
+
+def checkpoint_unpack(codes, scales, dtype):
+    """The values a checkpoint stands for, as a tensor of `dtype` (a torch type)."""
+    if dtype not in CODE_OF:
+        raise KeyError("checkpoint_unpack: dtype must be fp32, fp16 or bf16")
+    return _done((_native or _calls()).checkpoint_unpack(codes, scales, CODE_OF[dtype]), "caifx_checkpoint_unpack")
+
+
+def silu_multiply_checkpoint(gate, up):
+    """(hidden, gate's checkpoint, up's checkpoint): silu_multiply, bit for bit, and checkpoint_pack of both inputs in one pass."""
+    r = _done((_native or _calls()).silu_multiply_checkpoint(gate, up), "caifx_silu_multiply_checkpoint")
+    return r[0], (r[1], r[2]), (r[3], r[4])
+
+
+def swiglu_backward_checkpoint(gate, up, grad_hidden, with_hidden=False):
+    """(grad_gate, grad_up) of hidden = silu(gate) * up from the checkpoints of gate and up; with_hidden adds hidden itself, computed
+    from the checkpoints."""
+    return _done((_native or _calls()).swiglu_backward_checkpoint(*gate, *up, grad_hidden, with_hidden), "caifx_swiglu_backward_checkpoint")

@@ -464,6 +464,68 @@ CAIFX_API int caifx_moe_dispatch_backward(const void *grad_expert_buffer, const 
                                 int64_t num_tokens, int64_t dim, int top_k, int num_experts, int dtype,
                                 caifx_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside a frozen projection: the branch that CAIF_DeviceLoRAAdapter forms with
+ * MatMulTransposeB, Scale and Add (src/caif_device_lora_adapter.cpp:161-198) and its gradients (:234-276), for a batch
+ * whose rows belong to different adapters.
+ * Shapes: x [M,K], base and y [M,N], adapter factors a [num_adapters,rank,K] and b [num_adapters,N,rank], all of
+ * `dtype`; ids int32 [M], scaling fp32 [num_adapters] (alpha / rank), hidden fp32 [M,rank].  Rows may come in any order;
+ * neighbouring rows of one adapter share its factors' reads.  A row whose id is outside [0, num_adapters) has no
+ * adapter: its result is base (zero without one) bit for bit, its hidden row is zero, and it adds to no gradient.
+ * 1 <= rank <= CAIFX_ADAPTER_RANK_MAX; adapters of a smaller rank are padded with zeros.  Sums are fp32 in a fixed
+ * order.  Any alignment of the element type will do.
+ * ------------------------------------------------------------------------- */
+#define CAIFX_ADAPTER_RANK_MAX 128
+
+/* hidden[m,:] = x[m,:] a[l]^T,  y[m,:] = T(base[m,:] + scaling[l] * hidden[m,:] b[l]^T),  l = ids[m].
+ * hidden is kept in fp32 (the reference rounds it to the tensor type) and the sum is rounded once.  base may be NULL
+ * (zero) and may be y itself; hidden may be NULL.  workspace: caifx_adapters_workspace_bytes(..., backward = 0). */
+CAIFX_API int caifx_adapters_forward(int64_t M, int64_t N, int64_t K, int rank, int num_adapters, const void *x,
+                           const int32_t *ids, const void *a, const void *b, const float *scaling, const void *base,
+                           void *y, float *hidden, int dtype, void *workspace, size_t workspace_bytes,
+                           caifx_stream_t stream);
+
+/* With g[m,:] = scaling[l] * dy[m,:] b[l] (fp32):
+ *   dx[m,:]   = T(base[m,:] + g[m,:] a[l])                      base [M,K], NULL for zero, may be dx itself
+ *   grad_a[l] = T(sum over the rows m of l of g[m,:]^T x[m,:])           [num_adapters,rank,K]
+ *   grad_b[l] = T(sum over the rows m of l of scaling[l] * dy[m,:]^T hidden[m,:])   [num_adapters,N,rank]
+ * An adapter without rows gets zero gradients.  Any of dx, grad_a, grad_b may be NULL; what only they need (x, hidden, a) may then be
+ * NULL too.  x_scales != NULL: x holds the int8 codes of caifx_checkpoint_pack and x_scales their scales.
+ * workspace: caifx_adapters_workspace_bytes(..., backward = 1). */
+CAIFX_API int caifx_adapters_backward(int64_t M, int64_t N, int64_t K, int rank, int num_adapters, const void *dy,
+                            const void *x, const float *x_scales, const float *hidden, const int32_t *ids,
+                            const void *a, const void *b, const float *scaling, const void *base, void *dx,
+                            void *grad_a, void *grad_b, int dtype, void *workspace, size_t workspace_bytes,
+                            caifx_stream_t stream);
+CAIFX_API size_t caifx_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K, int rank, int num_adapters, int dtype,
+                                      int backward);
+
+/* ---------------------------------------------------------------------------
+ * Activation checkpoints in 8 bits: what a backward pass needs of the forward's activations, kept as one int8 code per
+ * value and one fp32 scale per CAIFX_CHECKPOINT_GROUP neighbouring values of a row (a row's last group may be shorter).
+ *   scale = fl32(max|x| / 127), 1 where that is zero, NaN where the group holds an infinity or a NaN (code 0 then, so
+ *   that the overflow shows in what is computed from the checkpoint);  code = clamp(rne(fl32(x / scale)), -127, 127)
+ * codes [rows,cols], scales [rows, ceil(cols / CAIFX_CHECKPOINT_GROUP)].
+ * ------------------------------------------------------------------------- */
+#define CAIFX_CHECKPOINT_GROUP 128
+
+CAIFX_API int caifx_checkpoint_pack(const void *input, void *codes, float *scales, int64_t rows, int64_t cols, int dtype,
+                          caifx_stream_t stream);
+/* output = T(code * scale) */
+CAIFX_API int caifx_checkpoint_unpack(const void *codes, const float *scales, void *output, int64_t rows, int64_t cols,
+                            int dtype, caifx_stream_t stream);
+/* caifx_silu_multiply (hidden has its bits) and the checkpoints of gate and up, in one pass over the two. */
+CAIFX_API int caifx_silu_multiply_checkpoint(const void *gate, const void *up, void *hidden, void *gate_codes,
+                                   float *gate_scales, void *up_codes, float *up_scales, int64_t rows, int64_t cols,
+                                   int dtype, caifx_stream_t stream);
+/* The gating's backward from checkpoints: with g, u = code * scale in fp32,
+ *   grad_up = T(grad_hidden * silu(g)),  grad_gate = T(grad_hidden * u * silu'(g)),
+ * each rounded once (caifx_swiglu_backward also rounds in between, as the reference's kernels do).  hidden != NULL also
+ * receives T(silu(g) * u): the input of the projection behind the gating, for the gradient of that projection's adapter. */
+CAIFX_API int caifx_swiglu_backward_checkpoint(const void *gate_codes, const float *gate_scales, const void *up_codes,
+                                     const float *up_scales, const void *grad_hidden, void *grad_gate, void *grad_up,
+                                     void *hidden, int64_t rows, int64_t cols, int dtype, caifx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
