@@ -1,7 +1,7 @@
 // Activation checkpoints in 8 bits: an activation of the forward pass kept as one int8 code per value and one fp32 scale per
 // 128 neighbouring values of a row, and the gating of a feed-forward block that writes and reads such checkpoints.
 //
-//   scale = fl32(max|x| / 127), 1 where that is zero, NaN where the group holds an infinity or a NaN
+//   scale = fl32(max|x| * fl32(1 / 127)), 1 where that is zero, NaN where the group holds an infinity or a NaN
 //   code  = clamp(rint(fl32(x / scale)), -127, 127)            value = code * scale
 //
 // Everything here is bound by memory.  Sixteen lanes take a group, eight values each, so that a lane's part is one 16-byte
@@ -86,7 +86,7 @@ template <typename T> __device__ __forceinline__ Eight<int8_t> quantise(const Ei
   }
   top = group_max(top);
   const bool finite = top < 0x7F800000u;
-  scale = finite ? __builtin_bit_cast(float, top) / 127.0f : __builtin_nanf("");
+  scale = finite ? __builtin_bit_cast(float, top) * (1.0f / 127.0f) : __builtin_nanf("");
   if (scale == 0.0f) scale = 1.0f;
   Eight<int8_t> q;
 #pragma unroll

@@ -503,8 +503,9 @@ CAIFX_API size_t caifx_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K,
 /* ---------------------------------------------------------------------------
  * Activation checkpoints in 8 bits: what a backward pass needs of the forward's activations, kept as one int8 code per
  * value and one fp32 scale per CAIFX_CHECKPOINT_GROUP neighbouring values of a row (a row's last group may be shorter).
- *   scale = fl32(max|x| / 127), 1 where that is zero, NaN where the group holds an infinity or a NaN (code 0 then, so
- *   that the overflow shows in what is computed from the checkpoint);  code = clamp(rne(fl32(x / scale)), -127, 127)
+ *   scale = fl32(max|x| * fl32(1 / 127)), 1 where that is zero, NaN where the group holds an infinity or a NaN (code 0
+ *   then, so that the overflow shows in what is computed from the checkpoint);
+ *   code = clamp(rne(fl32(x / scale)), -127, 127)
  * codes [rows,cols], scales [rows, ceil(cols / CAIFX_CHECKPOINT_GROUP)].
  * ------------------------------------------------------------------------- */
 #define CAIFX_CHECKPOINT_GROUP 128

@@ -24,7 +24,7 @@ def definition(x):
     wide[:, :cols] = v
     wide = wide.reshape(rows, groups, GROUP)
     with np.errstate(all="ignore"):
-        scale = (np.abs(wide).max(-1) / np.float32(127)).astype(np.float32)
+        scale = (np.abs(wide).max(-1) * (np.float32(1) / np.float32(127))).astype(np.float32)
         scale[scale == 0] = 1
         odd = ~np.isfinite(wide).all(-1)
         codes = np.clip(np.rint((wide / scale[..., None]).astype(np.float32)), -127, 127)
