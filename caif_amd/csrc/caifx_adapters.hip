@@ -124,9 +124,9 @@ __device__ __forceinline__ floatx4_t mma(const Pieces &u, const bf16x8_t &w, flo
 // transposing instruction: of the sixteen lanes of a q, lane t asks for four neighbouring values of row t / 4, columns
 // spread (t % 4) .. + 3, and receives column t of the four rows.
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4_t;
-template <typename T> __device__ __forceinline__ vec8<T> down(const T *m, int pitch, int spread, int lane)
+template <typename T> __device__ __forceinline__ vec8<T> down(const T *m, int pitch, int spread, int lane, int q)
 {
-  const int q = lane >> 4, t = lane & 15;
+  const int t = lane & 15;
   if constexpr (sizeof(T) == 2) {
     typedef __attribute__((address_space(3))) s16x4_t lds_t;
     const T *p = m + (8 * q + (t >> 2)) * pitch + spread * (t & 3);
@@ -166,33 +166,177 @@ struct TileIds {
   }
 };
 
+// ------------------------------------------------------------------ rows sorted by adapter
+// What the products over an adapter's rows are cut into: a slot is up to `chunk` of the rows of one adapter, as they stand in the list of
+// rows sorted by adapter.  An adapter with one slot (also one without rows) writes its gradient, the slots of the others go to
+// `part` and are added by join_kernel.
+struct Slot {
+  int32_t adapter, first, count, part;                // part -1: none
+};
+struct Multi {
+  int32_t adapter, part, parts, unused;
+};
+struct Cut {
+  int32_t *header;                                    // number of slots, number of entries in multi
+  Slot *slots;
+  Multi *multi;
+  int32_t chunk;
+};
+
+constexpr int kSortThreads = 512;
+
+struct Sort {
+  int32_t *rows;                                      // [M]
+  int32_t *spare;                                     // [adapters], where they do not fit LDS
+  Cut a, b;
+};
+
+// number of lanes with the same adapter, and of those below this lane; `bits` of an adapter's number are looked at
+__device__ __forceinline__ uint64_t same_lanes(int l, int bits)
+{
+  uint64_t same = __ballot(l >= 0);
+  for (int k = 0; k < bits; ++k) {
+    const bool one = l >= 0 && ((l >> k) & 1);
+    const uint64_t with = __ballot(one);
+    same &= one ? with : ~with;
+  }
+  return l >= 0 ? same : 0;
+}
+
+// One workgroup lists the rows of each adapter, in their order, and cuts the lists into slots.  The rows are shared among as many waves as
+// have room for a counter for each adapter; counters first, their running sums next, then every wave places its rows in order.
+__device__ __forceinline__ void sort_rows(const Problem &p, const Sort &o, int32_t *lds, int room)
+{
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const bool inside = p.L <= room;
+  int waves = inside ? room / p.L : 1;
+  if (waves > kSortThreads / 64) waves = kSortThreads / 64;
+  int32_t *counts = inside ? lds : o.spare;           // [waves][L]
+  for (int k = threadIdx.x; k < waves * p.L; k += kSortThreads) counts[k] = 0;
+  const int64_t share = ((p.M + waves - 1) / waves + 63) / 64 * 64, lo = wave * share, hi = lo + share < p.M ? lo + share : p.M;
+  int32_t *mine = counts + wave * p.L;
+  __syncthreads();
+  if (wave < waves) {
+    for (int64_t m = lo + lane; m < hi; m += 64) {
+      const int l = p.ids[m];
+      if (l >= 0 && l < p.L) atomicAdd(mine + l, 1);
+    }
+  }
+  __threadfence_block();
+  __syncthreads();
+  if (wave == 0) {
+    // running sums over the adapters: rows, slots and parts of either gradient, entries of the lists of those with several slots
+    int32_t row0 = 0, slot0[2] = {0, 0}, part0[2] = {0, 0}, multi0[2] = {0, 0};
+    for (int base = 0; base < p.L; base += 64) {
+      const int l = base + lane;
+      int n = 0;
+      if (l < p.L) {
+        for (int w = 0; w < waves; ++w) n += counts[w * p.L + l];
+      }
+      auto running = [&](int v, int32_t &carry) {     // the sum of the lanes before this one
+        int up = v;
+#pragma unroll
+        for (int k = 1; k < 64; k <<= 1) {
+          const int x = __shfl_up(up, k, 64);
+          if (lane >= k) up += x;
+        }
+        const int before = carry + up - v;
+        carry += __shfl(up, 63, 64);
+        return before;
+      };
+      const int row = running(n, row0);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const Cut &cut = g ? o.b : o.a;
+        const int slots = l >= p.L ? 0 : (n > cut.chunk ? (n + cut.chunk - 1) / cut.chunk : 1);
+        const int slot = running(slots, slot0[g]), part = running(slots > 1 ? slots : 0, part0[g]), multi = running(slots > 1 ? 1 : 0, multi0[g]);
+        for (int k = 0; k < slots; ++k) {
+          const int left = n - k * cut.chunk;
+          cut.slots[slot + k] = Slot{l, row + k * cut.chunk, left < cut.chunk ? left : cut.chunk, slots > 1 ? part + k : -1};
+        }
+        if (slots > 1) cut.multi[multi] = Multi{l, part, slots, 0};
+      }
+      if (l < p.L) {
+        int at = row;
+        for (int w = 0; w < waves; ++w) {
+          const int c = counts[w * p.L + l];
+          counts[w * p.L + l] = at;
+          at += c;
+        }
+      }
+    }
+    if (lane == 0) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const Cut &cut = g ? o.b : o.a;
+        cut.header[0] = slot0[g];
+        cut.header[1] = multi0[g];
+      }
+    }
+  }
+  __threadfence_block();
+  __syncthreads();
+  if (wave < waves) {
+    const int bits = 32 - __builtin_clz(static_cast<unsigned>(p.L > 1 ? p.L - 1 : 1));
+    for (int64_t base = lo; base < hi; base += 64) {
+      const int64_t m = base + lane;
+      int l = -1;
+      if (m < hi) {
+        const int id = p.ids[m];
+        if (id >= 0 && id < p.L) l = id;
+      }
+      const uint64_t same = same_lanes(l, bits);
+      const int below = __builtin_popcountll(same & ((uint64_t{1} << lane) - 1));
+      if (l >= 0) {
+        const int at = mine[l];
+        o.rows[at + below] = static_cast<int32_t>(m);
+        __builtin_amdgcn_wave_barrier();
+        if (below == 0) mine[l] = at + __builtin_popcountll(same);
+      }
+      __threadfence_block();
+    }
+  }
+}
+
 // ------------------------------------------------------------------ shrink
 constexpr int kShrinkWaves = 8;
-constexpr int kUnit = 64;                             // columns that a wave takes at a time: a line of a row in 16 bits
+
+// Columns that a wave asks for at a time: as much as its registers hold, so that a memory round trip is paid for few times.
+template <typename T, int JT, bool kDown> struct ShrinkUnit {
+  static constexpr int kBytes = JT * static_cast<int>(sizeof(T));       // 2 .. 32: registers of the factor grow with it
+  static constexpr int kSteps = kDown ? (kBytes >= 16 ? 1 : 2) : (kBytes >= 32 ? 1 : kBytes >= 8 ? 2 : 4);
+  static constexpr int kCols = 32 * kSteps;
+};
 
 // out[slice][m][j] = scale sum over the slice's columns c of z[m][c] f[l][j][c] (kDown: f[l][c][j]), rows without adapter zero.
 // The factor is the A operand (rows j), the rows are the B operand, so a lane's results belong to one row m = i.
 template <typename T, int JT, bool kDown>
 __global__ __launch_bounds__(64 * kShrinkWaves) void shrink_kernel(Problem p, const T *__restrict__ z, int64_t C, const T *__restrict__ f, int64_t per_slice,
-                                                                   bool scaled, float *__restrict__ out)
+                                                                   bool scaled, float *__restrict__ out, Sort sort)
 {
   constexpr int R = 16 * JT;
-  constexpr int kSteps = R * sizeof(T) >= (kDown ? 256 : 512) ? 1 : 2;       // of 32 columns, staged or loaded together
-  constexpr int kCols = 32 * kSteps;
+  constexpr int kSteps = ShrinkUnit<T, JT, kDown>::kSteps, kCols = 32 * kSteps;
   constexpr int kStage = kDown ? kCols * R * sizeof(T) : 0;             // bytes of a wave's staged factor
   constexpr int kSums = 16 * R * 4;
   __shared__ __align__(32) unsigned char lds[kShrinkWaves * (kStage > kSums ? kStage : kSums)];
+  if constexpr (kDown) {
+    static_assert(64 * kShrinkWaves == kSortThreads);
+    if (blockIdx.x == 0 && sort.rows != nullptr) {     // the gradients' list of rows, beside the others' work
+      if (blockIdx.y == 0) sort_rows(p, sort, reinterpret_cast<int32_t *>(lds), static_cast<int>(sizeof lds / 4));
+      return;
+    }
+  }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
-  const int64_t m = static_cast<int64_t>(blockIdx.x) * 16 + i;
+  const int64_t tile = static_cast<int64_t>(blockIdx.x) - (kDown && sort.rows != nullptr ? 1 : 0);
+  const int64_t m = tile * 16 + i;
   const int64_t lo = blockIdx.y * per_slice, hi = lo + per_slice < C ? lo + per_slice : C;
   TileIds ids(p, m);
   floatx4_t sum[JT];
 #pragma unroll
   for (int j = 0; j < JT; ++j) sum[j] = floatx4_t{0, 0, 0, 0};
-  const T *row = z + (m < p.M ? m : 0) * C;
+  const T *row = z + (m < p.M ? m : p.M - 1) * C;
   T *stage = reinterpret_cast<T *>(lds) + wave * (kStage / sizeof(T));
   for (int l = ids.next(); l >= 0; l = ids.next()) {
-    const bool mine = ids.mine == l;
     const T *factor = f + static_cast<int64_t>(l) * p.r * C;
     floatx4_t acc[JT];
 #pragma unroll
@@ -203,17 +347,17 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void shrink_kernel(Problem p, co
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         const int64_t c = c0 + 32 * s + 8 * q;
-        zv[s] = zero8<vec8<T>>();
-        if (mine) zv[s] = kFull ? load8<T>(row + c) : load8<T>(row + c, clamp8(hi - c));
-        if constexpr (!kDown) {
-#pragma unroll
-          for (int j = 0; j < JT; ++j) {
-            const int at = 16 * j + i < p.r ? 16 * j + i : p.r - 1;         // rows past the rank repeat the last; their sums are not kept
-            fv[s][j] = kFull ? load8<T>(factor + at * C + c) : load8<T>(factor + at * C + c, clamp8(hi - c));
-          }
-        }
+        zv[s] = kFull ? load8<T>(row + c) : load8<T>(row + c, clamp8(hi - c));
       }
-      if constexpr (kDown) {
+      if constexpr (!kDown) {
+#pragma unroll
+        for (int j = 0; j < JT; ++j) {
+          const int at = 16 * j + i < p.r ? 16 * j + i : p.r - 1;           // rows past the rank repeat the last; their sums are not kept
+          const T *from = factor + at * C + c0 + 8 * q;
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) fv[s][j] = kFull ? load8<T>(from + 32 * s) : load8<T>(from + 32 * s, clamp8(hi - c0 - 32 * s - 8 * q));
+        }
+      } else {
         // the factor's rows c0 .. + kCols, eight ranks at a time, zeros past the rank and past the last column
         constexpr int kOct = R / 8;
         vec8<T> st[kCols * kOct / 64];
@@ -228,7 +372,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void shrink_kernel(Problem p, co
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-          for (int j = 0; j < JT; ++j) fv[s][j] = down<T>(stage + 32 * s * R + 16 * j, R, 4, lane);
+          for (int j = 0; j < JT; ++j) fv[s][j] = down<T>(stage + 32 * s * R + 16 * j, R, 4, lane, q);
         __builtin_amdgcn_wave_barrier();
       }
 #pragma unroll
@@ -239,6 +383,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void shrink_kernel(Problem p, co
     int64_t c0 = lo + wave * kCols;
     for (; c0 + kCols <= hi; c0 += kShrinkWaves * kCols) unit(c0, std::true_type{});
     if (c0 < hi) unit(c0, std::false_type{});
+    const bool mine = ids.mine == l;
 #pragma unroll
     for (int j = 0; j < JT; ++j)
 #pragma unroll
@@ -251,7 +396,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void shrink_kernel(Problem p, co
   for (int j = 0; j < JT; ++j) *reinterpret_cast<floatx4_t *>(sums + (wave * 16 + i) * R + 16 * j + 4 * q) = sum[j];
   __syncthreads();
   for (int o = threadIdx.x; o < 16 * R; o += 64 * kShrinkWaves) {
-    const int64_t mm = static_cast<int64_t>(blockIdx.x) * 16 + o / R;
+    const int64_t mm = tile * 16 + o / R;
     const int j = o % R;
     if (mm >= p.M || j >= p.r) continue;
     float v = 0.0f;
@@ -286,109 +431,220 @@ __device__ __forceinline__ f32x8_t rank8(const Problem &p, const Rows &u, int64_
 }
 
 // ------------------------------------------------------------------ expand
-constexpr int kExpandWaves = 4;
-constexpr int kExpandCols = 64;                       // of a wave
+// The fp32 side of the expanding products.  16-bit tensors are multiplied by the row in two pieces of their own type, hi + lo: bf16 has
+// fp32's range, an fp16 row is first scaled by a power of two that brings its largest value to 2^14 (the pieces then add up to the value
+// but for 2^-22 of it, down to 2^-28 of the largest), and the results are scaled back.
+template <typename T> struct TwoPieces {
+  vec8<T> hi, lo;
+};
+template <typename T> __device__ __forceinline__ TwoPieces<T> two_pieces(const f32x8_t &v)
+{
+  TwoPieces<T> p;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    p.hi[e] = from_f32<T>(v[e]);
+    p.lo[e] = from_f32<T>(v[e] - to_f32<T>(p.hi[e]));
+  }
+  return p;
+}
+// A row's operand for one step.  kHalf: ranks up to 16, where the 32 elements of a step hold both pieces, hi in the lanes q = 0, 1 and lo in
+// q = 2, 3, each beside the same sixteen values of the factor.
+template <typename T, bool kHalf> struct RowOperand {
+  TwoPieces<T> u;
+  __device__ __forceinline__ void set(const f32x8_t &v, int) { u = two_pieces<T>(v); }
+  __device__ __forceinline__ floatx4_t with(const vec8<T> &f, floatx4_t acc) const { return mma(f, u.lo, mma(f, u.hi, acc)); }
+};
+template <typename T> struct RowOperand<T, true> {
+  vec8<T> u;
+  __device__ __forceinline__ void set(const f32x8_t &v, int q)
+  {
+    const TwoPieces<T> p = two_pieces<T>(v);
+    u = q < 2 ? p.hi : p.lo;
+  }
+  __device__ __forceinline__ floatx4_t with(const vec8<T> &f, floatx4_t acc) const { return mma(f, u, acc); }
+};
+struct RowOperandF32 {
+  f32x8_t u;
+  __device__ __forceinline__ void set(const f32x8_t &v, int) { u = v; }
+  __device__ __forceinline__ floatx4_t with(const f32x8_t &f, floatx4_t acc) const { return mma(f, u, acc); }
+};
+template <> struct RowOperand<float, true> : RowOperandF32 {};
+template <> struct RowOperand<float, false> : RowOperandF32 {};
+// the power of two that an fp16 row is multiplied by: its largest magnitude, a value of any lane i, q, comes to [2^14, 2^15); 1 for rows of
+// zeros, infinities, NaN, and for the other types
+template <typename T, int N> __device__ __forceinline__ float row_scale(const f32x8_t (&v)[N])
+{
+  if constexpr (dtype_code<T>::value != CAIFX_F16) return 1.0f;
+  uint32_t top = 0;
+#pragma unroll
+  for (int s = 0; s < N; ++s)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = v[s][e];
+      const uint32_t b = __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu;
+      top = top > b ? top : b;
+    }
+#pragma unroll
+  for (int o = 16; o < 64; o <<= 1) {
+    const uint32_t w = __shfl_xor(top, o, 64);
+    top = top > w ? top : w;
+  }
+  const int exponent = static_cast<int>(top >> 23);                     // biased; the scale's own exponent stays in the normal range
+  if (exponent == 0 || exponent == 255) return 1.0f;
+  const int e = 127 + 14 + 127 - exponent;
+  return __builtin_bit_cast(float, static_cast<uint32_t>(e > 253 ? 253 : (e < 1 ? 1 : e)) << 23);
+}
 
-// out[m][c] = T(base[m][c] + scale sum_j u[m][j] f[l][c][j])  (kDown: f[l][j][c]).  Of the 16 x 16 results of a product a lane holds
-// four neighbouring columns of one row; two products whose columns alternate by fours give it eight, one 16-byte access.
+constexpr int kExpandWaves = 4;                       // of 16 rows each
+constexpr int kExpandCols = 64;                       // of a wave at a time
+constexpr int kExpandGroups = 4;                      // of such columns
+
+// out[m][c] = T(base[m][c] + scale sum_j u[m][j] f[l][c][j])  (kDown: f[l][j][c]).  The factor's columns are the A operand, the rows the B
+// operand: of the 16 x 16 results of a product a lane holds four neighbouring columns of one row, and two products whose columns
+// alternate by fours give it eight, one 16-byte access.  A wave keeps its rows' operands for all its columns: what is not
+// a load, a store or a product costs as much as the memory otherwise (built for each 64 columns: 56 us for 4096 x 11008 in bf16).
 // hidden: the rows themselves, written by the first columns' waves.
 template <typename T, int RS, bool kDown>
 __global__ __launch_bounds__(64 * kExpandWaves) void expand_kernel(Problem p, Rows u, int64_t C, int64_t col_tiles, const T *__restrict__ f, bool scaled,
                                                                    const T *base, T *out, float *__restrict__ hidden)
 {
+  constexpr bool kHalf = RS == 0;
+  constexpr int S = RS == 0 ? 1 : RS;
+  constexpr bool kPieces = kHalf && sizeof(T) == 2;    // both pieces in one step
+  constexpr int kStageRows = kPieces ? 16 : 32;
   constexpr int kPitch = kExpandCols + 8;
-  __shared__ __align__(32) T lds[kDown ? kExpandWaves * 32 * kPitch : 1];
+  __shared__ __align__(32) T lds[kDown ? kExpandWaves * kStageRows * kPitch : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
   const int64_t tile = static_cast<int64_t>(blockIdx.x) / col_tiles;
-  const int64_t c0 = ((static_cast<int64_t>(blockIdx.x) - tile * col_tiles) * kExpandWaves + wave) * kExpandCols;
-  if (c0 >= C) return;
-  const int64_t m = tile * 16 + i;
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) - tile * col_tiles) * (kExpandCols * kExpandGroups);
+  const int64_t m = (tile * kExpandWaves + wave) * 16 + i;
+  if (m - i >= p.M) return;
   const bool in = m < p.M;
-  vec8<T> old[2];
-  int have[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int64_t c = c0 + 32 * h + 8 * q;
-    have[h] = in ? clamp8(C - c) : 0;
-    old[h] = zero8<vec8<T>>();
-    if (base) old[h] = load8<T>(base + m * C + c, have[h]);
-  }
   TileIds ids(p, m);
-  typename Fine<T>::type uv[RS];
-  const float scale = scaled && ids.mine >= 0 ? p.scaling[ids.mine] : 1.0f;
+  const int qj = kPieces ? q & 1 : q;                  // which eight ranks of a step
+  f32x8_t v[S];
 #pragma unroll
-  for (int s = 0; s < RS; ++s) {
-    f32x8_t v = zero8<f32x8_t>();
-    if (in) v = rank8(p, u, m, 32 * s + 8 * q);
-    if (hidden && c0 == 0 && in) {
+  for (int s = 0; s < S; ++s) v[s] = rank8(p, u, in ? m : p.M - 1, 32 * s + 8 * qj);
+  if (hidden && first == 0 && in && (!kPieces || q < 2)) {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
       for (int e = 0; e < 8; ++e)
-        if (32 * s + 8 * q + e < p.r) hidden[m * p.r + 32 * s + 8 * q + e] = v[e];
-    }
-    if (scaled) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= scale;
-    }
-    uv[s] = fine<T>(v);
+        if (32 * s + 8 * qj + e < p.r) hidden[m * p.r + 32 * s + 8 * qj + e] = v[s][e];
   }
-  floatx4_t sum[4];
+  if (scaled) {
+    const float scale = ids.mine >= 0 ? p.scaling[ids.mine] : 0.0f;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) sum[t] = floatx4_t{0, 0, 0, 0};
-  T *stage = lds + (kDown ? wave * 32 * kPitch : 0);
-  for (int l = ids.next(); l >= 0; l = ids.next()) {
-    const bool mine = ids.mine == l;
-    const T *factor = f + static_cast<int64_t>(l) * p.r * C;
-    floatx4_t acc[4];
+    for (int s = 0; s < S; ++s)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) acc[t] = floatx4_t{0, 0, 0, 0};
+      for (int e = 0; e < 8; ++e) v[s][e] *= scale;
+  }
+  const float up = row_scale<T>(v);                    // a power of two, and its inverse
+  const float back = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, up));
+  RowOperand<T, kHalf> row[S];
 #pragma unroll
-    for (int s = 0; s < RS; ++s) {
-      vec8<T> fv[4];
-      if constexpr (kDown) {
-        // ranks 32 s .. + 31 of the wave's columns, zeros past the rank and past the last column
-        vec8<T> st[4];
+  for (int s = 0; s < S; ++s) {
+    if constexpr (dtype_code<T>::value == CAIFX_F16) {
 #pragma unroll
-        for (int o = 0; o < 4; ++o) {
-          const int j = 32 * s + 8 * o + (lane >> 3);
-          const int64_t c = c0 + 8 * (lane & 7);
-          st[o] = load8<T>(factor + j * C + c, j < p.r ? clamp8(C - c) : 0);
+      for (int e = 0; e < 8; ++e) v[s][e] *= up;
+    }
+    row[s].set(v[s], q);
+  }
+  const uint64_t pending = ids.pending;
+  T *stage = lds + (kDown ? wave * kStageRows * kPitch : 0);
+
+  auto group = [&](int64_t c0, auto is_full) {
+    constexpr bool kFull = decltype(is_full)::value;    // all 16 rows, all 64 columns, ranks in whole octets
+    vec8<T> old[2];
+    int have[2];
+    T *to = out + m * C + c0 + 8 * q;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      have[h] = kFull ? 8 : (in ? clamp8(C - c0 - 32 * h - 8 * q) : 0);
+      if (base) old[h] = kFull ? load8<T>(base + m * C + c0 + 8 * q + 32 * h) : load8<T>(base + m * C + c0 + 8 * q + 32 * h, have[h]);
+      else old[h] = zero8<vec8<T>>();
+    }
+    floatx4_t sum[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum[k] = floatx4_t{0, 0, 0, 0};
+    ids.pending = pending;
+    bool again = false;
+    for (int l = ids.next(); l >= 0; l = ids.next()) {
+      const T *factor = f + static_cast<int64_t>(l) * p.r * C;
+      floatx4_t acc[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] = floatx4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        vec8<T> fv[4];
+        if constexpr (kDown) {
+          // a step's ranks of the 64 columns, zeros past the rank and past the last column
+          vec8<T> st[kStageRows / 8];
+#pragma unroll
+          for (int o = 0; o < kStageRows / 8; ++o) {
+            const int j = 32 * s + 8 * o + (lane >> 3);
+            const T *from = factor + j * C + c0 + 8 * (lane & 7);
+            if (kFull) st[o] = j < p.r ? load8<T>(from) : zero8<vec8<T>>();
+            else st[o] = load8<T>(from, j < p.r ? clamp8(C - c0 - 8 * (lane & 7)) : 0);
+          }
+#pragma unroll
+          for (int o = 0; o < kStageRows / 8; ++o) *reinterpret_cast<vec8<T> *>(stage + (8 * o + (lane >> 3)) * kPitch + 8 * (lane & 7)) = st[o];
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) fv[k] = down<T>(stage + 32 * (k >> 1) + 4 * (k & 1), kPitch, 8, lane, qj);
+          __builtin_amdgcn_wave_barrier();
+        } else {
+          const int j = 32 * s + 8 * qj;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int64_t c = c0 + 32 * (k >> 1) + 8 * (i >> 2) + 4 * (k & 1) + (i & 3);
+            // past the rank (where the row's operand is zero) the factor's last values again: they are there, and of the same adapter
+            if (kFull) fv[k] = load8<T>(factor + c * p.r + (j < p.r ? j : p.r - 8));
+            else fv[k] = load8<T>(factor + c * p.r + j, c < C ? clamp8(p.r - j) : 0);
+          }
         }
 #pragma unroll
-        for (int o = 0; o < 4; ++o) *reinterpret_cast<vec8<T> *>(stage + (8 * o + (lane >> 3)) * kPitch + 8 * (lane & 7)) = st[o];
-        __builtin_amdgcn_wave_barrier();
+        for (int k = 0; k < 4; ++k) acc[k] = row[s].with(fv[k], acc[k]);
+      }
+      // the tile's first adapter fills all rows, the others replace their own
+      if (!again) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) fv[t] = down<T>(stage + 32 * (t >> 1) + 4 * (t & 1), kPitch, 8, lane);
-        __builtin_amdgcn_wave_barrier();
+        for (int k = 0; k < 4; ++k) sum[k] = acc[k];
       } else {
-        const int j = 32 * s + 8 * q, hj = clamp8(p.r - j);
+        const bool mine = ids.mine == l;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int64_t c = c0 + 32 * (t >> 1) + 8 * (i >> 2) + 4 * (t & 1) + (i & 3);
-          fv[t] = load8<T>(factor + c * p.r + j, c < C ? hj : 0);
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[k][e] = mine ? acc[k][e] : sum[k][e];
+      }
+      again = true;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // a row without adapter keeps its base bit for bit, also a NaN's
+      if (ids.mine >= 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float add = sum[2 * h + (e >> 2)][e & 3];
+          if constexpr (dtype_code<T>::value == CAIFX_F16) add *= back;
+          old[h][e] = from_f32<T>(to_f32<T>(old[h][e]) + add);
         }
       }
+      if (kFull || have[h] == 8) {
+        __builtin_memcpy(to + 32 * h, &old[h], sizeof old[h]);
+      } else {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) acc[t] = mma(whole(fv[t]), uv[s], acc[t], 0);
+        for (int e = 0; e < 7; ++e)
+          if (e < have[h]) to[32 * h + e] = old[h][e];
+      }
     }
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum[t][e] = mine ? acc[t][e] : sum[t][e];
-  }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    // a row without adapter keeps its base bit for bit, also a NaN's
-    if (ids.mine >= 0) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) old[h][e] = from_f32<T>(to_f32<T>(old[h][e]) + sum[2 * h + (e >> 2)][e & 3]);
-    }
-    T *to = out + m * C + c0 + 32 * h + 8 * q;
-    if (have[h] == 8) {
-      __builtin_memcpy(to, &old[h], sizeof old[h]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 7; ++e)
-        if (e < have[h]) to[e] = old[h][e];
-    }
+  };
+  const bool whole_rows = m - i + 16 <= p.M && p.r % 8 == 0;
+#pragma unroll 1
+  for (int g = 0; g < kExpandGroups; ++g) {
+    const int64_t c0 = first + g * kExpandCols;
+    if (c0 >= C) break;
+    if (whole_rows && c0 + kExpandCols <= C) group(c0, std::true_type{});
+    else group(c0, std::false_type{});
   }
 }
 
@@ -475,26 +731,45 @@ __global__ __launch_bounds__(64 * kRowWaves) void row_kernel(Problem p, const T 
 // ------------------------------------------------------------------ outer
 constexpr int kOuterThreads = 256;
 constexpr int kOuterCols = 128;                       // of a workgroup, 32 of a wave; a checkpoint's group
-constexpr int kOuterRows = 32;                        // of a step
-constexpr int kOuterList = 1024;                      // rows looked through at a time
+constexpr int kOuterRows = 64;                        // of a step
 
 // what a tensor's values are in LDS: int8 codes are exact in bf16
 template <typename Z, typename T> struct Staged { typedef Z type; };
 template <typename T> struct Staged<int8_t, T> { typedef bf16_t type; };
 template <> struct Staged<int8_t, float> { typedef float type; };
-template <typename Z> __device__ __forceinline__ void load8_as(vec8<Z> &v, const Z *p, int have) { v = load8<Z>(p, have); }
-template <typename V> __device__ __forceinline__ void load8_as(V &v, const int8_t *p, int have)
+template <typename Z> struct Raw { typedef vec8<Z> type; };
+template <> struct Raw<int8_t> { typedef u32x2_t type; };
+template <typename S, typename Z> __device__ __forceinline__ vec8<S> staged(const typename Raw<Z>::type &v)
 {
-  int8_t c[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (have >= 8) {
-    __builtin_memcpy(c, p, 8);
+  if constexpr (sizeof(Z) > 1) {
+    return v;
   } else {
+    vec8<S> w;
+    float lo[4], hi[4];
+    int8x4_to_f32(v[0], lo);
+    int8x4_to_f32(v[1], hi);
 #pragma unroll
-    for (int e = 0; e < 7; ++e)
-      if (e < have) c[e] = p[e];
+    for (int e = 0; e < 4; ++e) {
+      w[e] = from_f32<S>(lo[e]);
+      w[4 + e] = from_f32<S>(hi[e]);
+    }
+    return w;
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(c[e]);
+}
+template <typename Z> __device__ __forceinline__ typename Raw<Z>::type load_raw(const Z *p, int have)
+{
+  if constexpr (sizeof(Z) > 1) {
+    return load8<Z>(p, have);
+  } else {
+    typename Raw<Z>::type v;
+    __builtin_memset(&v, 0, sizeof v);
+    if (have >= 8) {
+      __builtin_memcpy(&v, p, 8);
+    } else {
+      for (int e = 0; e < have; ++e) v[e >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(p[e])) << (8 * (e & 3));
+    }
+    return v;
+  }
 }
 
 struct Outer {
@@ -504,178 +779,192 @@ struct Outer {
   int64_t C;
   bool scaled;
   int64_t js, cs;                                     // of the result: [l][j * js + c * cs]
-  void *grad;                                         // T, or fp32 [splits] of it
-  int splits;
-  int64_t rows;                                       // of a split
+  void *grad;                                         // T
+  float *part;                                        // fp32, as many of an adapter's gradients as there are parts
+  const int32_t *rows;                                // sorted by adapter, in order for each
+  Cut cut;
 };
 
 // grad[l][c][j] = scale sum over the rows m of l of z[m][c] u[m][j]: both operands run down their rows, so both are staged in LDS as
-// they lie in memory and read with the transposing instruction.  The rows of the adapter are listed first (in order: results repeat),
-// so rows of other adapters cost nothing but their id.
-template <typename Z, typename T, int JT, bool kPartial>
+// they lie in memory and read with the transposing instruction.  The rows come from the sorted list: whatever their order in the batch,
+// they are read once.  The pitches leave the four rows of a transposing read in different banks.
+// kRanksDown: of a product's results a lane holds four ranks of one column (grad_a, whose columns are neighbours), else four columns of
+// one rank (grad_b, whose ranks are).
+template <typename Z, typename T, int JT, bool kRanksDown>
 __global__ __launch_bounds__(kOuterThreads) void outer_kernel(Problem p, Outer o)
 {
   typedef typename Staged<Z, T>::type S;
-  constexpr int R = 16 * JT;
-  constexpr int kZPitch = kOuterCols + 8, kUPitch = R + 8;
   constexpr bool k16 = sizeof(T) == 2;
   typedef typename std::conditional<k16, bf16_t, float>::type UT;
+  constexpr int R = 16 * JT, kOf = R / 4;              // values of u of a thread
+  constexpr int kZPitch = kOuterCols + 16, kUPitch = R + (R == 64 ? 8 : R == 128 ? 16 : 0);
   __shared__ __align__(32) S zs[kOuterRows * kZPitch];
-  __shared__ __align__(16) UT us[k16 ? 2 : 1][kOuterRows * kUPitch];
-  __shared__ int32_t list[kOuterList];
-  __shared__ int counts[kOuterThreads / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, q = lane >> 4;
+  __shared__ __align__(32) UT us[k16 ? 2 : 1][kOuterRows * kUPitch];
+  __shared__ int32_t list[1024];
   const int64_t tiles = (o.C + kOuterCols - 1) / kOuterCols;
-  int64_t at = blockIdx.x;
-  const int64_t c0 = at % tiles * kOuterCols;
-  at /= tiles;
-  const int l = static_cast<int>(at % p.L);
-  const int64_t split = at / p.L;
-  const int64_t lo = split * o.rows, hi = lo + o.rows < p.M ? lo + o.rows : p.M;
-  const Z *z = static_cast<const Z *>(o.z);
+  const int64_t at = blockIdx.x / tiles;
+  if (at >= o.cut.header[0]) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, q = lane >> 4;
+  const Slot slot = o.cut.slots[at];
+  const int64_t c0 = (blockIdx.x - at * tiles) * kOuterCols;
+  for (int k = tid; k < slot.count; k += kOuterThreads) list[k] = o.rows[slot.first + k];
   const int64_t groups = (o.C + CAIFX_CHECKPOINT_GROUP - 1) / CAIFX_CHECKPOINT_GROUP, group = c0 / CAIFX_CHECKPOINT_GROUP;
+  const float scale = o.scaled && slot.count > 0 ? p.scaling[slot.adapter] : 1.0f;
   floatx4_t acc[2][JT];
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int j = 0; j < JT; ++j) acc[t][j] = floatx4_t{0, 0, 0, 0};
+  __syncthreads();
 
-  bool any = false;
-  for (int64_t base = lo; base < hi; base += kOuterList) {
-    // rows base .. + 1023 of this adapter, in order: thread t looks at four neighbouring rows
-    int mine[4], n = 0;
+  // a step's values of a thread: four octets of z, a quarter of a row of u
+  typename Raw<Z>::type zv[4];
+  float uv[kOf];
+  const int zrow = tid >> 4, zcol = (tid & 15) * 8, urow = tid >> 2, ucol = (tid & 3) * kOf;
+  const Z *z = static_cast<const Z *>(o.z) + c0 + zcol;
+  const int zhave = clamp8(o.C - c0 - zcol), uhave = p.r - ucol;
+  auto fetch = [&](int s) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int64_t m = base + tid * 4 + k;
-      mine[k] = m < hi && p.ids[m] == l;
-      n += mine[k];
+      const int e = s * kOuterRows + zrow + 16 * k;
+      if (e < slot.count) zv[k] = load_raw<Z>(z + list[e] * o.C, zhave);
+      else __builtin_memset(&zv[k], 0, sizeof zv[k]);
     }
-    int before = n;
+    const int e = s * kOuterRows + urow;
 #pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const int up = __shfl_up(before, s, 64);
-      if (lane >= s) before += up;
-    }
-    __syncthreads();                                  // the last window's list has been read
-    if (lane == 63) counts[wave] = before;
-    __syncthreads();
-    int total = 0;
-    before -= n;
+    for (int k = 0; k < kOf; ++k) uv[k] = 0.0f;
+    if (e < slot.count) {
+      const int64_t m = list[e];
+      const float by = o.z_scales ? o.z_scales[m * groups + group] : 1.0f;
+      const float *from = o.u.at + m * p.r + ucol;
+      for (int w = 0; w < o.u.slices; ++w, from += p.M * p.r) {
+        if (uhave >= kOf) {
+          float add[kOf];
+          __builtin_memcpy(add, from, sizeof add);
 #pragma unroll
-    for (int w = 0; w < kOuterThreads / 64; ++w) {
-      if (w < wave) before += counts[w];
-      total += counts[w];
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (mine[k]) list[before++] = tid * 4 + k;
-    __syncthreads();
-
-    // a step's values of a thread: two octets of z, 2 JT values of u
-    vec8<S> zv[2];
-    float uv[2 * JT];
-    const int zrow = tid >> 4, zcol = (tid & 15) * 8, urow = tid >> 3, ucol = (tid & 7) * 2 * JT;
-    auto fetch = [&](int s) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int e = s * kOuterRows + zrow + 16 * k;
-        zv[k] = zero8<vec8<S>>();
-        if (e < total) load8_as(zv[k], z + (base + list[e]) * o.C + c0 + zcol, clamp8(o.C - c0 - zcol));
-      }
-      const int e = s * kOuterRows + urow;
-#pragma unroll
-      for (int k = 0; k < 2 * JT; ++k) uv[k] = 0.0f;
-      if (e < total) {
-        const int64_t m = base + list[e];
-        const float by = o.z_scales ? o.z_scales[m * groups + group] : 1.0f;
-#pragma unroll
-        for (int k = 0; k < 2 * JT; ++k) {
-          if (ucol + k < p.r) {
-            const float *from = o.u.at + m * p.r + ucol + k;
-            float v = *from;
-            for (int w = 1; w < o.u.slices; ++w) v += from[w * p.M * p.r];
-            uv[k] = v * by;
-          }
-        }
-      }
-    };
-    const int steps = (total + kOuterRows - 1) / kOuterRows;
-    any |= steps > 0;
-    if (steps > 0) fetch(0);
-    for (int s = 0; s < steps; ++s) {
-      if (s > 0) __syncthreads();                     // the step before has been read
-#pragma unroll
-      for (int k = 0; k < 2; ++k) *reinterpret_cast<vec8<S> *>(zs + (zrow + 16 * k) * kZPitch + zcol) = zv[k];
-#pragma unroll
-      for (int k = 0; k < 2 * JT; ++k) {
-        if constexpr (k16) {
-          const bf16_t top = from_f32<bf16_t>(uv[k]);
-          us[0][urow * kUPitch + ucol + k] = top;
-          us[1][urow * kUPitch + ucol + k] = from_f32<bf16_t>(uv[k] - to_f32<bf16_t>(top));
+          for (int k = 0; k < kOf; ++k) uv[k] += add[k];
         } else {
-          us[0][urow * kUPitch + ucol + k] = uv[k];
+#pragma unroll
+          for (int k = 0; k < kOf; ++k)
+            if (k < uhave) uv[k] += from[k];
         }
       }
-      __syncthreads();
-      if (s + 1 < steps) fetch(s + 1);
+      if (o.z_scales) {
+#pragma unroll
+        for (int k = 0; k < kOf; ++k) uv[k] *= by;
+      }
+    }
+  };
+  const int steps = (slot.count + kOuterRows - 1) / kOuterRows;
+  if (steps > 0) fetch(0);
+  for (int s = 0; s < steps; ++s) {
+    if (s > 0) __syncthreads();                       // the step before has been read
+#pragma unroll
+    for (int k = 0; k < 4; ++k) *reinterpret_cast<vec8<S> *>(zs + (zrow + 16 * k) * kZPitch + zcol) = staged<S, Z>(zv[k]);
+    if constexpr (k16) {
+      bf16_t hi[kOf], lo[kOf];
+#pragma unroll
+      for (int k = 0; k < kOf; ++k) {
+        hi[k] = from_f32<bf16_t>(uv[k]);
+        lo[k] = from_f32<bf16_t>(uv[k] - to_f32<bf16_t>(hi[k]));
+      }
+      __builtin_memcpy(__builtin_assume_aligned(us[0] + urow * kUPitch + ucol, 8), hi, sizeof hi);
+      __builtin_memcpy(__builtin_assume_aligned(us[1] + urow * kUPitch + ucol, 8), lo, sizeof lo);
+    } else {
+      __builtin_memcpy(__builtin_assume_aligned(us[0] + urow * kUPitch + ucol, 16), uv, sizeof uv);
+    }
+    __syncthreads();
+    if (s + 1 < steps) fetch(s + 1);
+#pragma unroll
+    for (int h = 0; h < kOuterRows / 32; ++h) {
       typename Fine<T>::type uf[JT];
 #pragma unroll
       for (int j = 0; j < JT; ++j) {
+        const UT *from = us[0] + 32 * h * kUPitch + 16 * j;
         if constexpr (k16) {
-          uf[j].hi = down<UT>(us[0] + 16 * j, kUPitch, 4, lane);
-          uf[j].lo = down<UT>(us[1] + 16 * j, kUPitch, 4, lane);
+          uf[j].hi = down<UT>(from, kUPitch, 4, lane, q);
+          uf[j].lo = down<UT>(from + kOuterRows * kUPitch, kUPitch, 4, lane, q);
         } else {
-          uf[j] = down<UT>(us[0] + 16 * j, kUPitch, 4, lane);
+          uf[j] = down<UT>(from, kUPitch, 4, lane, q);
         }
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const auto w = whole(down<S>(zs + 32 * wave + 16 * t, kZPitch, 4, lane));
+        const auto w = whole(down<S>(zs + 32 * h * kZPitch + 32 * wave + 16 * t, kZPitch, 4, lane, q));
 #pragma unroll
-        for (int j = 0; j < JT; ++j) acc[t][j] = mma(w, uf[j], acc[t][j], 0);
+        for (int j = 0; j < JT; ++j) acc[t][j] = kRanksDown ? mma(uf[j], w, acc[t][j], 0) : mma(w, uf[j], acc[t][j], 0);
       }
     }
   }
-  // an adapter without rows has zero gradients whatever its scaling
-  const float scale = o.scaled && any ? p.scaling[l] : 1.0f;
-  const int64_t first = static_cast<int64_t>(l) * p.r * o.C;
+  const int64_t size = p.r * o.C;
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int j = 0; j < JT; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int64_t c = c0 + 32 * wave + 16 * t + 4 * q + e;
-        const int jj = 16 * j + i;
+        const int64_t c = c0 + 32 * wave + 16 * t + (kRanksDown ? i : 4 * q + e);
+        const int jj = 16 * j + (kRanksDown ? 4 * q + e : i);
         if (c >= o.C || jj >= p.r) continue;
-        const int64_t to = first + jj * o.js + c * o.cs;
+        const int64_t to = jj * o.js + c * o.cs;
         const float v = acc[t][j][e] * scale;
-        if constexpr (kPartial) static_cast<float *>(o.grad)[split * p.L * p.r * o.C + to] = v;
-        else static_cast<T *>(o.grad)[to] = from_f32<T>(v);
+        if (slot.part >= 0) o.part[slot.part * size + to] = v;
+        else static_cast<T *>(o.grad)[slot.adapter * size + to] = from_f32<T>(v);
       }
 }
 
-// both gradients' splits added in order
+// the slots of an adapter that has several, added in order
 struct Join {
   const float *part;
   void *grad;
-  int64_t n;
-  int splits;
+  int64_t size;                                       // of an adapter's gradient
+  Cut cut;
 };
-template <typename T> __global__ __launch_bounds__(256) void join_kernel(Join a, Join b)
+constexpr int kJoinPer = 4;
+template <typename T> __device__ __forceinline__ void join(const Join &j, int64_t block, int which)
 {
-  int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const bool second = i >= a.n;
-  if (second) i -= a.n;
-  const Join &j = second ? b : a;
-  if (i >= j.n) return;
-  float v = j.part[i];
-  for (int s = 1; s < j.splits; ++s) v += j.part[s * j.n + i];
-  static_cast<T *>(j.grad)[i] = from_f32<T>(v);
+  if (which >= j.cut.header[1]) return;
+  const Multi m = j.cut.multi[which];
+  const int64_t i = (block * 256 + threadIdx.x) * kJoinPer;
+  if (i >= j.size) return;
+  const float *from = j.part + m.part * j.size + i;
+  T *to = static_cast<T *>(j.grad) + m.adapter * j.size + i;
+  if (i + kJoinPer <= j.size) {
+    float v[kJoinPer];
+    __builtin_memcpy(v, from, sizeof v);
+#pragma unroll 4
+    for (int s = 1; s < m.parts; ++s) {
+      float w[kJoinPer];
+      __builtin_memcpy(w, from + s * j.size, sizeof w);
+#pragma unroll
+      for (int k = 0; k < kJoinPer; ++k) v[k] += w[k];
+    }
+    T out[kJoinPer];
+#pragma unroll
+    for (int k = 0; k < kJoinPer; ++k) out[k] = from_f32<T>(v[k]);
+    __builtin_memcpy(to, out, sizeof out);
+  } else {
+    for (int64_t k = 0; i + k < j.size; ++k) {
+      float v = from[k];
+      for (int s = 1; s < m.parts; ++s) v += from[s * j.size + k];
+      to[k] = from_f32<T>(v);
+    }
+  }
+}
+template <typename T> __global__ __launch_bounds__(256) void join_kernel(Join a, Join b, unsigned blocks_a)
+{
+  if (blockIdx.x < blocks_a) join<T>(a, blockIdx.x, blockIdx.y);
+  else join<T>(b, blockIdx.x - blocks_a, blockIdx.y);
+}
+
+__global__ __launch_bounds__(256) void zero_kernel(unsigned char *at, int64_t bytes)
+{
+  zero_bytes(at, 0, bytes, static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, static_cast<int64_t>(gridDim.x) * 256);
 }
 
 // ------------------------------------------------------------------ host
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+size_t up16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
 
 // Workgroups of the shrinking product per 16 rows: enough that some 512 run, a slice no shorter than one unit for each wave.
 struct Slices {
@@ -684,6 +973,7 @@ struct Slices {
 };
 Slices plan_slices(int64_t M, int64_t C)
 {
+  constexpr int kUnit = 64;
   const int64_t tiles = ceil_div(M, 16), whole = ceil_div(C, kShrinkWaves * kUnit);
   int64_t n = 512 / (tiles > 0 ? tiles : 1);
   n = n < 1 ? 1 : (n > 16 ? 16 : n);
@@ -692,24 +982,38 @@ Slices plan_slices(int64_t M, int64_t C)
   return {static_cast<int>(ceil_div(C, columns)), columns};
 }
 
-// Shares of the rows for the gradients of the factors: enough that some 512 workgroups run, none shorter than 128 rows.
-int plan_splits(int64_t M, int64_t C, int L)
+// Rows of a slot of the gradients' products: so many that some 512 workgroups run, in whole steps.
+int32_t plan_chunk(int64_t M, int64_t C)
 {
-  const int64_t tiles = ceil_div(C, kOuterCols) * L;
-  int64_t n = ceil_div(512, tiles);
-  if (n > M / 128) n = M / 128;
-  return static_cast<int>(n < 1 ? 1 : (n > 16 ? 16 : n));
+  const int64_t rows = ceil_div(ceil_div(M * ceil_div(C, kOuterCols), 512), kOuterRows) * kOuterRows;
+  return static_cast<int32_t>(rows < 128 ? 128 : (rows > 1024 ? 1024 : rows));
 }
 
 // a decode step: the rows' factors are read from the caches for every part of the columns
 bool row_at_a_time(int64_t M) { return M <= 64; }
 
-size_t up16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
-
+struct Side {                                         // one gradient
+  int32_t chunk;
+  int64_t slots, parts, multi;                        // at most
+  size_t header, slot_bytes, multi_bytes, part_bytes;
+};
+Side plan_side(int64_t M, int64_t C, int rank, int L)
+{
+  Side w{};
+  w.chunk = plan_chunk(M, C);
+  w.slots = M / w.chunk + L;
+  w.parts = M > w.chunk ? 2 * (M / w.chunk) : 0;      // an adapter of n > chunk rows has ceil(n / chunk) <= 2 n / chunk
+  w.multi = M / (w.chunk + 1) < L ? M / (w.chunk + 1) : L;
+  w.header = 16;
+  w.slot_bytes = up16(w.slots * sizeof(Slot));
+  w.multi_bytes = up16(w.multi * sizeof(Multi));
+  w.part_bytes = up16(static_cast<size_t>(w.parts) * rank * C * 4);
+  return w;
+}
 struct Plan {
   Slices slices;
-  int splits_a, splits_b;
-  size_t rows, part_a, part_b, total;                 // bytes
+  Side a, b;
+  size_t rows, list, spare, total;                    // bytes
 };
 Plan plan(int64_t M, int64_t N, int64_t K, int rank, int L, bool backward)
 {
@@ -718,34 +1022,36 @@ Plan plan(int64_t M, int64_t N, int64_t K, int rank, int L, bool backward)
   w.rows = up16(static_cast<size_t>(w.slices.count) * M * rank * 4);
   if (!backward && row_at_a_time(M)) w.rows = 0;
   if (backward) {
-    w.splits_a = plan_splits(M, K, L);
-    w.splits_b = plan_splits(M, N, L);
-    w.part_a = w.splits_a > 1 ? up16(static_cast<size_t>(w.splits_a) * L * rank * K * 4) : 0;
-    w.part_b = w.splits_b > 1 ? up16(static_cast<size_t>(w.splits_b) * L * rank * N * 4) : 0;
+    w.a = plan_side(M, K, rank, L);
+    w.b = plan_side(M, N, rank, L);
+    w.list = up16(static_cast<size_t>(M) * 4);
+    w.spare = L > 2048 ? up16(static_cast<size_t>(L) * 4) : 0;      // the sorting workgroup has at least 8 KB of LDS
   }
-  w.total = w.rows + w.part_a + w.part_b;
+  w.total = w.rows + w.list + w.spare;
+  for (const Side *x : {&w.a, &w.b}) w.total += x->header + x->slot_bytes + x->multi_bytes + x->part_bytes;
   return w;
 }
 
 template <typename T, bool kDown>
-void shrink(const Problem &p, const Slices &sl, const void *z, int64_t C, const void *f, bool scaled, float *out, hipStream_t s)
+void shrink(const Problem &p, const Slices &sl, const void *z, int64_t C, const void *f, bool scaled, float *out, const Sort &sort, hipStream_t s)
 {
-  const dim3 grid(static_cast<unsigned>(ceil_div(p.M, 16)), sl.count), block(64 * kShrinkWaves);
+  const dim3 grid(static_cast<unsigned>(ceil_div(p.M, 16) + (sort.rows ? 1 : 0)), sl.count), block(64 * kShrinkWaves);
   const T *zz = static_cast<const T *>(z), *ff = static_cast<const T *>(f);
-  if (p.r <= 16) hipLaunchKernelGGL((shrink_kernel<T, 1, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out);
-  else if (p.r <= 32) hipLaunchKernelGGL((shrink_kernel<T, 2, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out);
-  else if (p.r <= 64) hipLaunchKernelGGL((shrink_kernel<T, 4, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out);
-  else hipLaunchKernelGGL((shrink_kernel<T, 8, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out);
+  if (p.r <= 16) hipLaunchKernelGGL((shrink_kernel<T, 1, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out, sort);
+  else if (p.r <= 32) hipLaunchKernelGGL((shrink_kernel<T, 2, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out, sort);
+  else if (p.r <= 64) hipLaunchKernelGGL((shrink_kernel<T, 4, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out, sort);
+  else hipLaunchKernelGGL((shrink_kernel<T, 8, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out, sort);
 }
 
 template <typename T, bool kDown>
 void expand(const Problem &p, const Rows &u, int64_t C, const void *f, bool scaled, const void *base, void *out, float *hidden, hipStream_t s)
 {
-  const int64_t tiles = ceil_div(C, kExpandWaves * kExpandCols);
-  const dim3 grid(static_cast<unsigned>(ceil_div(p.M, 16) * tiles)), block(64 * kExpandWaves);
+  const int64_t tiles = ceil_div(C, kExpandCols * kExpandGroups);
+  const dim3 grid(static_cast<unsigned>(ceil_div(p.M, 16 * kExpandWaves) * tiles)), block(64 * kExpandWaves);
   const T *ff = static_cast<const T *>(f), *bb = static_cast<const T *>(base);
   T *oo = static_cast<T *>(out);
-  if (p.r <= 32) hipLaunchKernelGGL((expand_kernel<T, 1, kDown>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
+  if (p.r <= 16) hipLaunchKernelGGL((expand_kernel<T, 0, kDown>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
+  else if (p.r <= 32) hipLaunchKernelGGL((expand_kernel<T, 1, kDown>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
   else if (p.r <= 64) hipLaunchKernelGGL((expand_kernel<T, 2, kDown>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
   else hipLaunchKernelGGL((expand_kernel<T, 4, kDown>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
 }
@@ -767,67 +1073,80 @@ template <typename T> int forward(const Problem &p, const void *x, const void *b
   const Plan w = plan(p.M, p.N, p.K, p.r, p.L, false);
   float *h = static_cast<float *>(workspace);
   if (hidden && w.slices.count == 1) h = hidden, hidden = nullptr;
-  shrink<T, false>(p, w.slices, x, p.K, p.a, false, h, s);
+  shrink<T, false>(p, w.slices, x, p.K, p.a, false, h, Sort{}, s);
   expand<T, false>(p, Rows{h, w.slices.count}, p.N, p.b, true, base, y, hidden, s);
   return launch_status();
 }
 
-template <typename Z, typename T> void outer(const Problem &p, const Outer &o, hipStream_t s)
+template <typename Z, typename T, bool kRanksDown> void outer(const Problem &p, const Outer &o, int64_t slots, hipStream_t s)
 {
-  const dim3 grid(static_cast<unsigned>(ceil_div(o.C, kOuterCols) * p.L * o.splits)), block(kOuterThreads);
-#define CAIFX_GO(JT)                                                                                   \
-  if (o.splits > 1) hipLaunchKernelGGL((outer_kernel<Z, T, JT, true>), grid, block, 0, s, p, o);       \
-  else hipLaunchKernelGGL((outer_kernel<Z, T, JT, false>), grid, block, 0, s, p, o)
-  if (p.r <= 16) {
-    CAIFX_GO(1);
-  } else if (p.r <= 32) {
-    CAIFX_GO(2);
-  } else if (p.r <= 64) {
-    CAIFX_GO(4);
-  } else {
-    CAIFX_GO(8);
-  }
-#undef CAIFX_GO
+  const dim3 grid(static_cast<unsigned>(ceil_div(o.C, kOuterCols) * slots)), block(kOuterThreads);
+  if (p.r <= 16) hipLaunchKernelGGL((outer_kernel<Z, T, 1, kRanksDown>), grid, block, 0, s, p, o);
+  else if (p.r <= 32) hipLaunchKernelGGL((outer_kernel<Z, T, 2, kRanksDown>), grid, block, 0, s, p, o);
+  else if (p.r <= 64) hipLaunchKernelGGL((outer_kernel<Z, T, 4, kRanksDown>), grid, block, 0, s, p, o);
+  else hipLaunchKernelGGL((outer_kernel<Z, T, 8, kRanksDown>), grid, block, 0, s, p, o);
 }
 
 template <typename T>
 int backward(const Problem &p, const void *dy, const void *x, const float *x_scales, const float *hidden, const void *base, void *dx, void *ga, void *gb,
              void *workspace, hipStream_t s)
 {
+  const int64_t size_a = static_cast<int64_t>(p.r) * p.K, size_b = static_cast<int64_t>(p.r) * p.N;
+  if (p.M == 0) {                                     // sums of nothing
+    if (ga) hipLaunchKernelGGL(zero_kernel, dim3(1024), dim3(256), 0, s, static_cast<unsigned char *>(ga), static_cast<int64_t>(sizeof(T)) * p.L * size_a);
+    if (gb) hipLaunchKernelGGL(zero_kernel, dim3(1024), dim3(256), 0, s, static_cast<unsigned char *>(gb), static_cast<int64_t>(sizeof(T)) * p.L * size_b);
+    return launch_status();
+  }
   const Plan w = plan(p.M, p.N, p.K, p.r, p.L, true);
   unsigned char *at = static_cast<unsigned char *>(workspace);
-  float *g = reinterpret_cast<float *>(at), *pa = reinterpret_cast<float *>(at + w.rows), *pb = reinterpret_cast<float *>(at + w.rows + w.part_a);
+  auto take = [&](size_t n) {
+    unsigned char *here = at;
+    at += n;
+    return here;
+  };
+  float *g = reinterpret_cast<float *>(take(w.rows));
+  Sort sort{};
+  sort.rows = reinterpret_cast<int32_t *>(take(w.list));
+  sort.spare = reinterpret_cast<int32_t *>(take(w.spare));
+  float *part[2];
+  for (int k = 0; k < 2; ++k) {
+    const Side &side = k ? w.b : w.a;
+    Cut &cut = k ? sort.b : sort.a;
+    cut.header = reinterpret_cast<int32_t *>(take(side.header));
+    cut.slots = reinterpret_cast<Slot *>(take(side.slot_bytes));
+    cut.multi = reinterpret_cast<Multi *>(take(side.multi_bytes));
+    cut.chunk = side.chunk;
+    part[k] = reinterpret_cast<float *>(take(side.part_bytes));
+  }
   const Rows rows{g, w.slices.count};
-  if (p.M > 0 && (dx || ga)) shrink<T, true>(p, w.slices, dy, p.N, p.b, true, g, s);
-  if (p.M > 0 && dx) expand<T, true>(p, rows, p.K, p.a, false, base, dx, nullptr, s);
-  Join ja{nullptr, nullptr, 0, 0}, jb = ja;
+  shrink<T, true>(p, w.slices, dy, p.N, p.b, true, g, ga || gb ? sort : Sort{}, s);
+  if (dx) expand<T, true>(p, rows, p.K, p.a, false, base, dx, nullptr, s);
+  if (gb) outer<T, T, false>(p, Outer{dy, nullptr, Rows{hidden, 1}, p.N, true, 1, p.r, gb, part[1], sort.rows, sort.b}, w.b.slots, s);
   if (ga) {
-    const bool many = w.splits_a > 1;
-    const Outer o{x, x_scales, rows, p.K, false, p.K, 1, many ? pa : ga, w.splits_a, ceil_div(p.M, w.splits_a)};
-    if (x_scales) outer<int8_t, T>(p, o, s);
-    else outer<T, T>(p, o, s);
-    if (many) ja = Join{pa, ga, static_cast<int64_t>(p.L) * p.r * p.K, w.splits_a};
+    const Outer o{x, x_scales, rows, p.K, false, p.K, 1, ga, part[0], sort.rows, sort.a};
+    if (x_scales) outer<int8_t, T, true>(p, o, w.a.slots, s);
+    else outer<T, T, true>(p, o, w.a.slots, s);
   }
-  if (gb) {
-    const bool many = w.splits_b > 1;
-    const Outer o{dy, nullptr, Rows{hidden, 1}, p.N, true, 1, p.r, many ? pb : gb, w.splits_b, ceil_div(p.M, w.splits_b)};
-    outer<T, T>(p, o, s);
-    if (many) jb = Join{pb, gb, static_cast<int64_t>(p.L) * p.r * p.N, w.splits_b};
+  const int64_t multi_a = ga ? w.a.multi : 0, multi_b = gb ? w.b.multi : 0, multi = multi_a > multi_b ? multi_a : multi_b;
+  if (multi > 0) {
+    const unsigned blocks_a = multi_a > 0 ? static_cast<unsigned>(ceil_div(size_a, 256 * kJoinPer)) : 0;
+    const unsigned blocks_b = multi_b > 0 ? static_cast<unsigned>(ceil_div(size_b, 256 * kJoinPer)) : 0;
+    hipLaunchKernelGGL(join_kernel<T>, dim3(blocks_a + blocks_b, static_cast<unsigned>(multi)), dim3(256), 0, s, Join{part[0], ga, size_a, sort.a},
+                       Join{part[1], gb, size_b, sort.b}, blocks_a);
   }
-  if (ja.n + jb.n > 0) hipLaunchKernelGGL(join_kernel<T>, dim3(static_cast<unsigned>(ceil_div(ja.n + jb.n, 256))), dim3(256), 0, s, ja, jb);
   return launch_status();
 }
 
 int check(int64_t M, int64_t N, int64_t K, int rank, int num_adapters, int dtype)
 {
   if (!valid_dtype(dtype) || M < 0 || N <= 0 || K <= 0 || rank <= 0 || num_adapters <= 0) return CAIFX_ERR_INVALID_ARGUMENT;
-  constexpr int64_t kMost = int64_t{1} << 30;
-  if (rank > CAIFX_ADAPTER_RANK_MAX || M > kMost || N > kMost || K > kMost) return CAIFX_ERR_UNSUPPORTED;
+  if (rank > CAIFX_ADAPTER_RANK_MAX || M > (int64_t{1} << 23) || N > (int64_t{1} << 26) || K > (int64_t{1} << 26)) return CAIFX_ERR_UNSUPPORTED;
   // a grid has fewer than 2^32 threads
-  const int64_t longest = N > K ? N : K, grid = (int64_t{1} << 24) - 1;
-  if (ceil_div(M, 16) > grid / ceil_div(longest, kExpandWaves * kExpandCols) || num_adapters > grid / 16 / ceil_div(longest, kOuterCols) ||
-      ceil_div(M, 16) > (int64_t{1} << 23) / 16)
-    return CAIFX_ERR_UNSUPPORTED;
+  constexpr int64_t kBlocks = (int64_t{1} << 24) - 1;
+  for (const int64_t C : {N, K}) {
+    if (ceil_div(M, 16 * kExpandWaves) > kBlocks / ceil_div(C, kExpandCols)) return CAIFX_ERR_UNSUPPORTED;
+    if (M / plan_chunk(M, C) + num_adapters > kBlocks / ceil_div(C, kOuterCols)) return CAIFX_ERR_UNSUPPORTED;
+  }
   return CAIFX_OK;
 }
 
