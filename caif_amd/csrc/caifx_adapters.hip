@@ -143,11 +143,14 @@ template <typename T> __device__ __forceinline__ vec8<T> down(const T *m, int pi
 }
 
 // ------------------------------------------------------------------ adapters of a tile of rows
-// Lane (i, q) holds row i's adapter, -1 for none.  next() goes through the adapters of the tile, each once.
+// Lane (i, q) holds row i's adapter, -1 for none.  next() goes through the adapters of the tile, each once.  Where few rows run, several
+// workgroups take a tile and share its adapters: `of` of them, this one the `turn`-th, in turn; a row belongs to its adapter's, a row
+// without adapter to the first.  (32 rows of 32 adapters of rank 64, 4096 to 14336, went from 54 to XX us by it.)
 struct TileIds {
   int mine;
   uint64_t pending;
-  __device__ TileIds(const Problem &p, int64_t m)
+  int turn, of;
+  __device__ TileIds(const Problem &p, int64_t m, int turn_ = 0, int of_ = 1) : turn(turn_), of(of_)
   {
     mine = -1;
     if (m < p.M) {
@@ -155,7 +158,19 @@ struct TileIds {
       if (l >= 0 && l < p.L) mine = l;
     }
     pending = __ballot(mine >= 0);
+    if (of > 1) {
+      uint64_t all = pending, kept = turn == 0 ? __ballot(mine < 0) : 0;
+      for (int k = 0; all != 0; ++k) {
+        const int l = __builtin_amdgcn_readlane(mine, __builtin_ctzll(all));
+        const uint64_t rows = __ballot(mine == l);
+        all &= ~rows;
+        if (k % of == turn) kept |= rows;
+      }
+      pending &= kept;
+      owned = (kept >> (threadIdx.x & 63)) & 1;
+    }
   }
+  bool owned = true;
   // the next adapter of the tile, the same for all lanes; -1 when there is none
   __device__ int next()
   {
@@ -322,7 +337,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void shrink_kernel(Problem p, co
   if constexpr (kDown) {
     static_assert(64 * kShrinkWaves == kSortThreads);
     if (blockIdx.x == 0 && sort.rows != nullptr) {     // the gradients' list of rows, beside the others' work
-      if (blockIdx.y == 0) sort_rows(p, sort, reinterpret_cast<int32_t *>(lds), static_cast<int>(sizeof lds / 4));
+      if (blockIdx.y == 0 && blockIdx.z == 0) sort_rows(p, sort, reinterpret_cast<int32_t *>(lds), static_cast<int>(sizeof lds / 4));
       return;
     }
   }
@@ -330,7 +345,10 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void shrink_kernel(Problem p, co
   const int64_t tile = static_cast<int64_t>(blockIdx.x) - (kDown && sort.rows != nullptr ? 1 : 0);
   const int64_t m = tile * 16 + i;
   const int64_t lo = blockIdx.y * per_slice, hi = lo + per_slice < C ? lo + per_slice : C;
-  TileIds ids(p, m);
+  TileIds ids(p, m, blockIdx.z, gridDim.z);
+  if (__ballot(ids.owned) == 0) return;               // the same for all waves
+  __shared__ bool owned[16];
+  if (threadIdx.x < 16) owned[threadIdx.x] = ids.owned;
   floatx4_t sum[JT];
 #pragma unroll
   for (int j = 0; j < JT; ++j) sum[j] = floatx4_t{0, 0, 0, 0};
@@ -347,7 +365,8 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void shrink_kernel(Problem p, co
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         const int64_t c = c0 + 32 * s + 8 * q;
-        zv[s] = kFull ? load8<T>(row + c) : load8<T>(row + c, clamp8(hi - c));
+        zv[s] = zero8<vec8<T>>();
+        if (ids.owned) zv[s] = kFull ? load8<T>(row + c) : load8<T>(row + c, clamp8(hi - c));
       }
       if constexpr (!kDown) {
 #pragma unroll
@@ -398,7 +417,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void shrink_kernel(Problem p, co
   for (int o = threadIdx.x; o < 16 * R; o += 64 * kShrinkWaves) {
     const int64_t mm = tile * 16 + o / R;
     const int j = o % R;
-    if (mm >= p.M || j >= p.r) continue;
+    if (mm >= p.M || j >= p.r || !owned[o / R]) continue;
     float v = 0.0f;
 #pragma unroll
     for (int w = 0; w < kShrinkWaves; ++w) v += sums[w * 16 * R + o];
@@ -422,8 +441,19 @@ __device__ __forceinline__ f32x8_t rank8(const Problem &p, const Rows &u, int64_
   const int have = clamp8(p.r - j);
   const float *at = u.at + m * p.r + j;
   f32x8_t v = load8<float>(at, have);
-  for (int s = 1; s < u.slices; ++s) {
-    const f32x8_t w = load8<float>(at + s * p.M * p.r, have);
+  const int64_t apart = p.M * p.r;
+  int s = 1;
+  for (; s + 4 <= u.slices; s += 4) {                 // four asked for at a time
+    f32x8_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = load8<float>(at + (s + k) * apart, have);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += w[k][e];
+  }
+  for (; s < u.slices; ++s) {
+    const f32x8_t w = load8<float>(at + s * apart, have);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += w[e];
   }
@@ -453,6 +483,7 @@ template <typename T, bool kHalf> struct RowOperand {
   TwoPieces<T> u;
   __device__ __forceinline__ void set(const f32x8_t &v, int) { u = two_pieces<T>(v); }
   __device__ __forceinline__ floatx4_t with(const vec8<T> &f, floatx4_t acc) const { return mma(f, u.lo, mma(f, u.hi, acc)); }
+  __device__ __forceinline__ floatx4_t as_rows(const vec8<T> &f, floatx4_t acc) const { return mma(u.lo, f, mma(u.hi, f, acc)); }
 };
 template <typename T> struct RowOperand<T, true> {
   vec8<T> u;
@@ -462,11 +493,13 @@ template <typename T> struct RowOperand<T, true> {
     u = q < 2 ? p.hi : p.lo;
   }
   __device__ __forceinline__ floatx4_t with(const vec8<T> &f, floatx4_t acc) const { return mma(f, u, acc); }
+  __device__ __forceinline__ floatx4_t as_rows(const vec8<T> &f, floatx4_t acc) const { return mma(u, f, acc); }
 };
 struct RowOperandF32 {
   f32x8_t u;
   __device__ __forceinline__ void set(const f32x8_t &v, int) { u = v; }
   __device__ __forceinline__ floatx4_t with(const f32x8_t &f, floatx4_t acc) const { return mma(f, u, acc); }
+  __device__ __forceinline__ floatx4_t as_rows(const f32x8_t &f, floatx4_t acc) const { return mma(u, f, acc); }
 };
 template <> struct RowOperand<float, true> : RowOperandF32 {};
 template <> struct RowOperand<float, false> : RowOperandF32 {};
@@ -497,14 +530,13 @@ template <typename T, int N> __device__ __forceinline__ float row_scale(const f3
 
 constexpr int kExpandWaves = 4;                       // of 16 rows each
 constexpr int kExpandCols = 64;                       // of a wave at a time
-constexpr int kExpandGroups = 4;                      // of such columns
 
 // out[m][c] = T(base[m][c] + scale sum_j u[m][j] f[l][c][j])  (kDown: f[l][j][c]).  The factor's columns are the A operand, the rows the B
 // operand: of the 16 x 16 results of a product a lane holds four neighbouring columns of one row, and two products whose columns
 // alternate by fours give it eight, one 16-byte access.  A wave keeps its rows' operands for all its columns: what is not
 // a load, a store or a product costs as much as the memory otherwise (built for each 64 columns: 56 us for 4096 x 11008 in bf16).
 // hidden: the rows themselves, written by the first columns' waves.
-template <typename T, int RS, bool kDown>
+template <typename T, int RS, bool kDown, int G>
 __global__ __launch_bounds__(64 * kExpandWaves) void expand_kernel(Problem p, Rows u, int64_t C, int64_t col_tiles, const T *__restrict__ f, bool scaled,
                                                                    const T *base, T *out, float *__restrict__ hidden)
 {
@@ -516,16 +548,30 @@ __global__ __launch_bounds__(64 * kExpandWaves) void expand_kernel(Problem p, Ro
   __shared__ __align__(32) T lds[kDown ? kExpandWaves * kStageRows * kPitch : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
   const int64_t tile = static_cast<int64_t>(blockIdx.x) / col_tiles;
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) - tile * col_tiles) * (kExpandCols * kExpandGroups);
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) - tile * col_tiles) * (kExpandCols * G);
   const int64_t m = (tile * kExpandWaves + wave) * 16 + i;
   if (m - i >= p.M) return;
   const bool in = m < p.M;
-  TileIds ids(p, m);
+  TileIds ids(p, m, blockIdx.y, gridDim.y);
+  if (__ballot(ids.owned) == 0) return;
+  // a tile that is whole in every direction asks for all of its base at once
+  const bool whole_tile = m - i + 16 <= p.M && p.r % 8 == 0 && first + G * kExpandCols <= C;
+  vec8<T> early[G][2];
+  if (whole_tile) {
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        early[g][h] = base && ids.owned ? load8<T>(base + m * C + first + kExpandCols * g + 32 * h + 8 * q) : zero8<vec8<T>>();
+  }
   const int qj = kPieces ? q & 1 : q;                  // which eight ranks of a step
   f32x8_t v[S];
 #pragma unroll
-  for (int s = 0; s < S; ++s) v[s] = rank8(p, u, in ? m : p.M - 1, 32 * s + 8 * qj);
-  if (hidden && first == 0 && in && (!kPieces || q < 2)) {
+  for (int s = 0; s < S; ++s) {
+    v[s] = zero8<f32x8_t>();
+    if (in && ids.owned) v[s] = rank8(p, u, m, 32 * s + 8 * qj);
+  }
+  if (hidden && first == 0 && in && ids.owned && (!kPieces || q < 2)) {
 #pragma unroll
     for (int s = 0; s < S; ++s)
       for (int e = 0; e < 8; ++e)
@@ -552,16 +598,16 @@ __global__ __launch_bounds__(64 * kExpandWaves) void expand_kernel(Problem p, Ro
   const uint64_t pending = ids.pending;
   T *stage = lds + (kDown ? wave * kStageRows * kPitch : 0);
 
-  auto group = [&](int64_t c0, auto is_full) {
+  auto group = [&](int64_t c0, const vec8<T> (&early)[2], auto is_full) {
     constexpr bool kFull = decltype(is_full)::value;    // all 16 rows, all 64 columns, ranks in whole octets
     vec8<T> old[2];
     int have[2];
     T *to = out + m * C + c0 + 8 * q;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      have[h] = kFull ? 8 : (in ? clamp8(C - c0 - 32 * h - 8 * q) : 0);
-      if (base) old[h] = kFull ? load8<T>(base + m * C + c0 + 8 * q + 32 * h) : load8<T>(base + m * C + c0 + 8 * q + 32 * h, have[h]);
-      else old[h] = zero8<vec8<T>>();
+      have[h] = kFull ? 8 : (in && ids.owned ? clamp8(C - c0 - 32 * h - 8 * q) : 0);
+      if (kFull) old[h] = early[h];
+      else old[h] = base ? load8<T>(base + m * C + c0 + 8 * q + 32 * h, have[h]) : zero8<vec8<T>>();
     }
     floatx4_t sum[4];
 #pragma unroll
@@ -629,6 +675,7 @@ __global__ __launch_bounds__(64 * kExpandWaves) void expand_kernel(Problem p, Ro
           old[h][e] = from_f32<T>(to_f32<T>(old[h][e]) + add);
         }
       }
+      if (!ids.owned) continue;
       if (kFull || have[h] == 8) {
         __builtin_memcpy(to + 32 * h, &old[h], sizeof old[h]);
       } else {
@@ -638,51 +685,88 @@ __global__ __launch_bounds__(64 * kExpandWaves) void expand_kernel(Problem p, Ro
       }
     }
   };
-  const bool whole_rows = m - i + 16 <= p.M && p.r % 8 == 0;
+  if (whole_tile) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) group(first + g * kExpandCols, early[g], std::true_type{});
+  } else {
 #pragma unroll 1
-  for (int g = 0; g < kExpandGroups; ++g) {
-    const int64_t c0 = first + g * kExpandCols;
-    if (c0 >= C) break;
-    if (whole_rows && c0 + kExpandCols <= C) group(c0, std::true_type{});
-    else group(c0, std::false_type{});
+    for (int g = 0; g < G; ++g)
+      if (first + g * kExpandCols < C) group(first + g * kExpandCols, early[g], std::false_type{});
   }
 }
 
 // ------------------------------------------------------------------ one row, both products
 constexpr int kRowWaves = 8;
+constexpr int kRowCols = 64 * kRowWaves;              // of a workgroup at a time
+#ifndef KA
+#define KA 16
+#endif
+constexpr int kRowRounds = 4;                         // of such columns, all asked for before the first product where registers allow
 
-// A workgroup takes one row and a part of the result's columns and forms the row's h itself: the other parts do the same from the
-// caches, which costs less than a second launch.  Both products use one row (column) of sixteen; the matrix cores are not what
-// bounds them.
-template <typename T, int JT>
-__global__ __launch_bounds__(64 * kRowWaves) void row_kernel(Problem p, const T *__restrict__ x, const T *__restrict__ a, const T *__restrict__ b,
+// A workgroup takes one row and up to 2048 columns of its result and forms the row's h itself: the row's other workgroups do the same from
+// the caches, which costs less than a second launch.  Both products use one row (column) of sixteen; the matrix cores are not what
+// bounds them, round trips to memory are: a wave asks for eight steps of the first product at a time, and for its part of the second
+// factor before the first product is done.
+template <typename T, int RS>
+__global__ __launch_bounds__(64 * kRowWaves) void row_kernel(Problem p, int rows_padded, const T *__restrict__ x, const T *__restrict__ a, const T *__restrict__ b,
                                                              int64_t per_block, const T *base, T *out, float *__restrict__ hidden)
 {
-  constexpr int R = 16 * JT, RS = (JT + 1) / 2;
-  __shared__ float shares[kRowWaves][R], total[RS * 32];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
-  const int64_t m = blockIdx.y;
-  const int64_t lo = blockIdx.x * per_block, hi = lo + per_block < p.N ? lo + per_block : p.N;
+  constexpr bool kHalf = RS == 0, kPieces = kHalf && sizeof(T) == 2;
+  constexpr int S = kHalf ? 1 : RS, JT = kHalf ? 1 : 2 * RS, R = 16 * JT;
+  constexpr int kAhead = JT * static_cast<int>(sizeof(T)) <= 2 ? KA : JT * static_cast<int>(sizeof(T)) <= 4 ? 8 : JT * static_cast<int>(sizeof(T)) <= 8 ? 4 : 2;      // steps of the first product
+  constexpr int kEarly = S * static_cast<int>(sizeof(T)) <= 2 ? kRowRounds : 1;                                          // rounds of the second
+  __shared__ float shares[kRowWaves][R];
+  __shared__ __align__(32) float total[S * 32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4, qj = kPieces ? q & 1 : q;
+  // neighbouring workgroups are of neighbouring rows: with a multiple of eight of them a row's workgroups share an L2
+  const int64_t part = blockIdx.x / rows_padded, m = blockIdx.x - part * rows_padded;
+  if (m >= p.M) return;
+  const int64_t lo = part * per_block, hi = lo + per_block < p.N ? lo + per_block : p.N;
   const int l = p.ids[m];
   if (l < 0 || l >= p.L) {
-    for (int64_t c = lo + threadIdx.x; c < hi; c += 64 * kRowWaves) out[m * p.N + c] = base ? base[m * p.N + c] : T(0.0f);
-    if (hidden && blockIdx.x == 0 && threadIdx.x < static_cast<unsigned>(p.r)) hidden[m * p.r + threadIdx.x] = 0.0f;
+    for (int64_t c = lo + threadIdx.x; c < hi; c += kRowCols) out[m * p.N + c] = base ? base[m * p.N + c] : T(0.0f);
+    if (hidden && part == 0 && threadIdx.x < static_cast<unsigned>(p.r)) hidden[m * p.r + threadIdx.x] = 0.0f;
     return;
   }
   const T *fa = a + static_cast<int64_t>(l) * p.r * p.K, *fb = b + static_cast<int64_t>(l) * p.N * p.r, *row = x + m * p.K;
   floatx4_t acc[JT];
 #pragma unroll
   for (int j = 0; j < JT; ++j) acc[j] = floatx4_t{0, 0, 0, 0};
-  for (int64_t c = wave * 32; c < p.K; c += 32 * kRowWaves) {
+  const T *fr[JT];
+#pragma unroll
+  for (int j = 0; j < JT; ++j) fr[j] = fa + (16 * j + i < p.r ? 16 * j + i : p.r - 1) * p.K;
+  vec8<T> fv[kEarly][S][4];
+  auto second = [&](int64_t c0, vec8<T> (&to)[S][4]) {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) to[s][t] = load8<T>(fb + (c0 + 16 * t + i) * p.r + 32 * s + 8 * qj, c0 + 16 * t + i < hi ? clamp8(p.r - 32 * s - 8 * qj) : 0);
+  };
+  int64_t c = wave * 32;
+  for (; c + (kAhead - 1) * 32 * kRowWaves + 32 <= p.K; c += kAhead * 32 * kRowWaves) {
+    vec8<T> xv[kAhead], av[kAhead][JT];
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      const int64_t at = c + s * 32 * kRowWaves + 8 * q;
+      xv[s] = load8<T>(row + at);
+#pragma unroll
+      for (int j = 0; j < JT; ++j) av[s][j] = load8<T>(fr[j] + at);
+    }
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s)
+#pragma unroll
+      for (int j = 0; j < JT; ++j) acc[j] = mma(av[s][j], xv[s], acc[j]);
+  }
+  for (; c < p.K; c += 32 * kRowWaves) {
     const int64_t at = c + 8 * q;
     const int have = clamp8(p.K - at);
     const vec8<T> xv = load8<T>(row + at, have);
 #pragma unroll
-    for (int j = 0; j < JT; ++j) {
-      const int64_t r = 16 * j + i < p.r ? 16 * j + i : p.r - 1;
-      acc[j] = mma(load8<T>(fa + r * p.K + at, have), xv, acc[j]);
-    }
+    for (int j = 0; j < JT; ++j) acc[j] = mma(load8<T>(fr[j] + at, have), xv, acc[j]);
   }
+#pragma unroll
+  for (int e = 0; e < kEarly; ++e)
+    if (lo + e * kRowCols + wave * 64 < hi) second(lo + e * kRowCols + wave * 64, fv[e]);
   if (i == 0) {
 #pragma unroll
     for (int j = 0; j < JT; ++j)
@@ -690,41 +774,48 @@ __global__ __launch_bounds__(64 * kRowWaves) void row_kernel(Problem p, const T 
       for (int e = 0; e < 4; ++e) shares[wave][16 * j + 4 * q + e] = acc[j][e];
   }
   __syncthreads();
-  if (threadIdx.x < RS * 32) {
+  if (threadIdx.x < S * 32) {
     float v = 0.0f;
     if (threadIdx.x < static_cast<unsigned>(p.r)) {
 #pragma unroll
       for (int w = 0; w < kRowWaves; ++w) v += shares[w][threadIdx.x];
-      if (hidden && blockIdx.x == 0) hidden[m * p.r + threadIdx.x] = v;
+      if (hidden && part == 0) hidden[m * p.r + threadIdx.x] = v;
+      v *= p.scaling[l];
     }
-    total[threadIdx.x] = v * p.scaling[l];
+    total[threadIdx.x] = v;
   }
   __syncthreads();
-  typename Fine<T>::type uv[RS];
+  f32x8_t v[S];
 #pragma unroll
-  for (int s = 0; s < RS; ++s) {
-    f32x8_t v;
+  for (int s = 0; s < S; ++s) v[s] = *reinterpret_cast<const f32x8_t *>(total + 32 * s + 8 * qj);
+  const float up = row_scale<T>(v);
+  const float back = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, up));
+  RowOperand<T, kHalf> u[S];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 32 * s + 8 * q + e < p.r ? total[32 * s + 8 * q + e] : 0.0f;
-    uv[s] = fine<T>(v);
+  for (int s = 0; s < S; ++s) {
+    if constexpr (dtype_code<T>::value == CAIFX_F16) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[s][e] *= up;
+    }
+    u[s].set(v[s], q);
   }
-  for (int64_t c0 = lo + wave * 64; c0 < hi; c0 += 64 * kRowWaves) {
+#pragma unroll
+  for (int e = 0; e < kRowRounds; ++e) {
+    const int64_t c0 = lo + e * kRowCols + wave * 64;
+    if (c0 >= hi) break;
+    if (e >= kEarly) second(c0, fv[0]);
     floatx4_t y[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) y[t] = floatx4_t{0, 0, 0, 0};
+    for (int t = 0; t < 4; ++t) {
+      y[t] = floatx4_t{0, 0, 0, 0};
 #pragma unroll
-    for (int s = 0; s < RS; ++s) {
-      const int j = 32 * s + 8 * q, hj = clamp8(p.r - j);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int64_t c = c0 + 16 * t + i;
-        y[t] = mma(uv[s], whole(load8<T>(fb + c * p.r + j, c < hi ? hj : 0)), y[t], 0);
-      }
+      for (int s = 0; s < S; ++s) y[t] = u[s].as_rows(fv[e < kEarly ? e : 0][s][t], y[t]);
     }
     // every row of a product is the same: the lanes of q keep column tile q
-    const float v = q == 0 ? y[0][0] : q == 1 ? y[1][0] : q == 2 ? y[2][0] : y[3][0];
-    const int64_t c = c0 + lane;
-    if (c < hi) out[m * p.N + c] = from_f32<T>((base ? to_f32<T>(base[m * p.N + c]) : 0.0f) + v);
+    float add = q == 0 ? y[0][0] : q == 1 ? y[1][0] : q == 2 ? y[2][0] : y[3][0];
+    if constexpr (dtype_code<T>::value == CAIFX_F16) add *= back;
+    const int64_t at = c0 + lane;
+    if (at < hi) out[m * p.N + at] = from_f32<T>((base ? to_f32<T>(base[m * p.N + at]) : 0.0f) + add);
   }
 }
 
@@ -989,8 +1080,23 @@ int32_t plan_chunk(int64_t M, int64_t C)
   return static_cast<int32_t>(rows < 128 ? 128 : (rows > 1024 ? 1024 : rows));
 }
 
-// a decode step: the rows' factors are read from the caches for every part of the columns
-bool row_at_a_time(int64_t M) { return M <= 64; }
+// Whether the forward takes its rows one by one: every workgroup reads its row's first factor again, so that factor must be short (256 KB
+// is four memory round trips of a workgroup's waves) and all reads together less than what the caches give in some ten us.  Measured, us,
+// row by row / in tiles, rows of one adapter each (neighbours of one adapter), K = 4096, bf16: rank 16, one row 7.4 / 10.1; 32 rows to
+// N = 14336 10.1 / 18.6 (8.9 / 10.1); 128 rows to 4096 10.2 / 22.5 (8.8 / 9.8), to 14336 (112 MB) 27.6 / 35.6 (23.9 / 11.8); rank 64
+// (512 KB), one row 18.5 / 14.2, 32 rows to 4096 19.9 / 17.3 (19.0 / 13.8).
+bool row_at_a_time(int64_t M, int64_t N, int64_t K, int rank, size_t es)
+{
+  const int64_t factor = static_cast<int64_t>(rank) * K * static_cast<int64_t>(es);
+  return factor <= 256 << 10 && M * ceil_div(N, kRowCols * kRowRounds) <= (int64_t{64} << 20) / factor;
+}
+
+// Workgroups that share the adapters of a tile of 16 rows, `waves` waves working on it otherwise: as many as leave some 16384 in all.
+unsigned turns(const Problem &p, int64_t waves)
+{
+  const int64_t most = p.L < 16 ? p.L : 16, n = 16384 / (ceil_div(p.M, 16) * waves);
+  return static_cast<unsigned>(n < 1 ? 1 : (n > most ? most : n));
+}
 
 struct Side {                                         // one gradient
   int32_t chunk;
@@ -1015,12 +1121,12 @@ struct Plan {
   Side a, b;
   size_t rows, list, spare, total;                    // bytes
 };
-Plan plan(int64_t M, int64_t N, int64_t K, int rank, int L, bool backward)
+Plan plan(int64_t M, int64_t N, int64_t K, int rank, int L, size_t es, bool backward)
 {
   Plan w{};
   w.slices = plan_slices(M, backward ? N : K);
   w.rows = up16(static_cast<size_t>(w.slices.count) * M * rank * 4);
-  if (!backward && row_at_a_time(M)) w.rows = 0;
+  if (!backward && row_at_a_time(M, N, K, rank, es)) w.rows = 0;
   if (backward) {
     w.a = plan_side(M, K, rank, L);
     w.b = plan_side(M, N, rank, L);
@@ -1035,7 +1141,7 @@ Plan plan(int64_t M, int64_t N, int64_t K, int rank, int L, bool backward)
 template <typename T, bool kDown>
 void shrink(const Problem &p, const Slices &sl, const void *z, int64_t C, const void *f, bool scaled, float *out, const Sort &sort, hipStream_t s)
 {
-  const dim3 grid(static_cast<unsigned>(ceil_div(p.M, 16) + (sort.rows ? 1 : 0)), sl.count), block(64 * kShrinkWaves);
+  const dim3 grid(static_cast<unsigned>(ceil_div(p.M, 16) + (sort.rows ? 1 : 0)), sl.count, turns(p, sl.count * kShrinkWaves)), block(64 * kShrinkWaves);
   const T *zz = static_cast<const T *>(z), *ff = static_cast<const T *>(f);
   if (p.r <= 16) hipLaunchKernelGGL((shrink_kernel<T, 1, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out, sort);
   else if (p.r <= 32) hipLaunchKernelGGL((shrink_kernel<T, 2, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out, sort);
@@ -1043,34 +1149,47 @@ void shrink(const Problem &p, const Slices &sl, const void *z, int64_t C, const 
   else hipLaunchKernelGGL((shrink_kernel<T, 8, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out, sort);
 }
 
+template <typename T, bool kDown, int G>
+void expand(const Problem &p, const Rows &u, int64_t C, const void *f, bool scaled, const void *base, void *out, float *hidden, hipStream_t s)
+{
+  const int64_t tiles = ceil_div(C, kExpandCols * G);
+  const dim3 grid(static_cast<unsigned>(ceil_div(p.M, 16 * kExpandWaves) * tiles), turns(p, tiles)), block(64 * kExpandWaves);
+  const T *ff = static_cast<const T *>(f), *bb = static_cast<const T *>(base);
+  T *oo = static_cast<T *>(out);
+  if (p.r <= 16) hipLaunchKernelGGL((expand_kernel<T, 0, kDown, G>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
+  else if (p.r <= 32) hipLaunchKernelGGL((expand_kernel<T, 1, kDown, G>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
+  else if (p.r <= 64) hipLaunchKernelGGL((expand_kernel<T, 2, kDown, G>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
+  else hipLaunchKernelGGL((expand_kernel<T, 4, kDown, G>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
+}
+
+// columns of a wave: 64 while there are few waves
 template <typename T, bool kDown>
 void expand(const Problem &p, const Rows &u, int64_t C, const void *f, bool scaled, const void *base, void *out, float *hidden, hipStream_t s)
 {
-  const int64_t tiles = ceil_div(C, kExpandCols * kExpandGroups);
-  const dim3 grid(static_cast<unsigned>(ceil_div(p.M, 16 * kExpandWaves) * tiles)), block(64 * kExpandWaves);
-  const T *ff = static_cast<const T *>(f), *bb = static_cast<const T *>(base);
-  T *oo = static_cast<T *>(out);
-  if (p.r <= 16) hipLaunchKernelGGL((expand_kernel<T, 0, kDown>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
-  else if (p.r <= 32) hipLaunchKernelGGL((expand_kernel<T, 1, kDown>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
-  else if (p.r <= 64) hipLaunchKernelGGL((expand_kernel<T, 2, kDown>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
-  else hipLaunchKernelGGL((expand_kernel<T, 4, kDown>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
+#ifndef EG
+#define EG 4
+#endif
+  if (ceil_div(p.M, 16) * ceil_div(C, kExpandCols) < 16384) expand<T, kDown, 1>(p, u, C, f, scaled, base, out, hidden, s);
+  else expand<T, kDown, EG>(p, u, C, f, scaled, base, out, hidden, s);
 }
 
 template <typename T> int forward(const Problem &p, const void *x, const void *base, void *y, float *hidden, void *workspace, hipStream_t s)
 {
-  if (row_at_a_time(p.M)) {
-    const int64_t units = ceil_div(p.N, 64 * kRowWaves), parts = 256 / p.M < units ? 256 / p.M : units;
-    const int64_t per = ceil_div(units, parts) * 64 * kRowWaves;
-    const dim3 grid(static_cast<unsigned>(ceil_div(p.N, per)), static_cast<unsigned>(p.M)), block(64 * kRowWaves);
+  if (row_at_a_time(p.M, p.N, p.K, p.r, sizeof(T))) {
+    // as many parts of the columns as make some 256 workgroups, or as many as are needed
+    const int64_t units = ceil_div(p.N, kRowCols), least = ceil_div(units, kRowRounds), most = 256 / p.M < units ? 256 / p.M : units;
+    const int64_t per = ceil_div(units, most > least ? most : least) * kRowCols;
+    const int padded = static_cast<int>(p.M < 8 ? p.M : ceil_div(p.M, 8) * 8);
+    const dim3 grid(static_cast<unsigned>(ceil_div(p.N, per) * padded)), block(64 * kRowWaves);
     const T *xx = static_cast<const T *>(x), *a = static_cast<const T *>(p.a), *b = static_cast<const T *>(p.b), *bb = static_cast<const T *>(base);
     T *yy = static_cast<T *>(y);
-    if (p.r <= 16) hipLaunchKernelGGL((row_kernel<T, 1>), grid, block, 0, s, p, xx, a, b, per, bb, yy, hidden);
-    else if (p.r <= 32) hipLaunchKernelGGL((row_kernel<T, 2>), grid, block, 0, s, p, xx, a, b, per, bb, yy, hidden);
-    else if (p.r <= 64) hipLaunchKernelGGL((row_kernel<T, 4>), grid, block, 0, s, p, xx, a, b, per, bb, yy, hidden);
-    else hipLaunchKernelGGL((row_kernel<T, 8>), grid, block, 0, s, p, xx, a, b, per, bb, yy, hidden);
+    if (p.r <= 16) hipLaunchKernelGGL((row_kernel<T, 0>), grid, block, 0, s, p, padded, xx, a, b, per, bb, yy, hidden);
+    else if (p.r <= 32) hipLaunchKernelGGL((row_kernel<T, 1>), grid, block, 0, s, p, padded, xx, a, b, per, bb, yy, hidden);
+    else if (p.r <= 64) hipLaunchKernelGGL((row_kernel<T, 2>), grid, block, 0, s, p, padded, xx, a, b, per, bb, yy, hidden);
+    else hipLaunchKernelGGL((row_kernel<T, 4>), grid, block, 0, s, p, padded, xx, a, b, per, bb, yy, hidden);
     return launch_status();
   }
-  const Plan w = plan(p.M, p.N, p.K, p.r, p.L, false);
+  const Plan w = plan(p.M, p.N, p.K, p.r, p.L, sizeof(T), false);
   float *h = static_cast<float *>(workspace);
   if (hidden && w.slices.count == 1) h = hidden, hidden = nullptr;
   shrink<T, false>(p, w.slices, x, p.K, p.a, false, h, Sort{}, s);
@@ -1097,7 +1216,7 @@ int backward(const Problem &p, const void *dy, const void *x, const float *x_sca
     if (gb) hipLaunchKernelGGL(zero_kernel, dim3(1024), dim3(256), 0, s, static_cast<unsigned char *>(gb), static_cast<int64_t>(sizeof(T)) * p.L * size_b);
     return launch_status();
   }
-  const Plan w = plan(p.M, p.N, p.K, p.r, p.L, true);
+  const Plan w = plan(p.M, p.N, p.K, p.r, p.L, sizeof(T), true);
   unsigned char *at = static_cast<unsigned char *>(workspace);
   auto take = [&](size_t n) {
     unsigned char *here = at;
@@ -1160,7 +1279,7 @@ extern "C" {
 size_t caifx_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K, int rank, int num_adapters, int dtype, int backward)
 {
   if (check(M, N, K, rank, num_adapters, dtype) != CAIFX_OK || M == 0) return 0;
-  return plan(M, N, K, rank, num_adapters, backward != 0).total;
+  return plan(M, N, K, rank, num_adapters, dtype_size(dtype), backward != 0).total;
 }
 
 int caifx_adapters_forward(int64_t M, int64_t N, int64_t K, int rank, int num_adapters, const void *x, const int32_t *ids, const void *a, const void *b,
@@ -1170,7 +1289,7 @@ int caifx_adapters_forward(int64_t M, int64_t N, int64_t K, int rank, int num_ad
   const int st = check(M, N, K, rank, num_adapters, dtype);
   if (st != CAIFX_OK || M == 0) return st;
   if (!x || !ids || !a || !b || !scaling || !y) return CAIFX_ERR_INVALID_ARGUMENT;
-  const size_t es = dtype_size(dtype), need = plan(M, N, K, rank, num_adapters, false).total;
+  const size_t es = dtype_size(dtype), need = plan(M, N, K, rank, num_adapters, es, false).total;
   if (!aligned_to(x, es) || !aligned_to(a, es) || !aligned_to(b, es) || !aligned_to(base, es) || !aligned_to(y, es) || !aligned_to(ids, 4) ||
       !aligned_to(scaling, 4) || !aligned_to(hidden, 4) || !aligned_to(workspace, 4))
     return CAIFX_ERR_MISALIGNED;
@@ -1191,7 +1310,7 @@ int caifx_adapters_backward(int64_t M, int64_t N, int64_t K, int rank, int num_a
   const int st = check(M, N, K, rank, num_adapters, dtype);
   if (st != CAIFX_OK || ((M == 0 || !dx) && !grad_a && !grad_b)) return st;
   if (M > 0 && (!dy || !ids || !scaling || (dx && !a) || ((dx || grad_a) && !b) || (grad_a && !x) || (grad_b && !hidden))) return CAIFX_ERR_INVALID_ARGUMENT;
-  const size_t es = dtype_size(dtype), need = plan(M, N, K, rank, num_adapters, true).total;
+  const size_t es = dtype_size(dtype), need = plan(M, N, K, rank, num_adapters, es, true).total;
   if (!aligned_to(dy, es) || (!x_scales && !aligned_to(x, es)) || !aligned_to(x_scales, 4) || !aligned_to(hidden, 4) || !aligned_to(ids, 4) ||
       !aligned_to(a, es) || !aligned_to(b, es) || !aligned_to(scaling, 4) || !aligned_to(base, es) || !aligned_to(dx, es) || !aligned_to(grad_a, es) ||
       !aligned_to(grad_b, es) || !aligned_to(workspace, 4))
