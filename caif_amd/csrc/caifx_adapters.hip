@@ -143,23 +143,27 @@ template <typename T> __device__ __forceinline__ vec8<T> down(const T *m, int pi
 }
 
 // ------------------------------------------------------------------ adapters of a tile of rows
-// Lane (i, q) holds row i's adapter, -1 for none.  next() goes through the adapters of the tile, each once.  Where few rows run, several
-// workgroups take a tile and share its adapters: `of` of them, this one the `turn`-th, in turn; a row belongs to its adapter's, a row
-// without adapter to the first.  (32 rows of 32 adapters of rank 64, 4096 to 14336, went from 54 to XX us by it.)
-struct TileIds {
+// The adapters of ROWS rows from m0 on: lane l holds that of row l % ROWS, -1 for none.  next() goes through the adapters, each once.
+// Where few rows run, several workgroups take a tile and share its adapters: `of` of them, this one the `turn`-th, in turn; a row belongs to
+// its adapter's, a row without adapter to the first.  (32 rows of 32 adapters of rank 64 from 4096 to 14336 took 54 us with one workgroup
+// for each tile, 29 with sixteen.)
+template <int ROWS> struct TileIds {
   int mine;
-  uint64_t pending;
-  int turn, of;
-  __device__ TileIds(const Problem &p, int64_t m, int turn_ = 0, int of_ = 1) : turn(turn_), of(of_)
+  uint64_t pending, kept;
+  bool owned;
+  __device__ __forceinline__ TileIds(const Problem &p, int64_t m0, int turn, int of)
   {
+    const int64_t m = m0 + (threadIdx.x & (ROWS - 1));
     mine = -1;
     if (m < p.M) {
       const int l = p.ids[m];
       if (l >= 0 && l < p.L) mine = l;
     }
     pending = __ballot(mine >= 0);
+    kept = ~uint64_t{0};
     if (of > 1) {
-      uint64_t all = pending, kept = turn == 0 ? __ballot(mine < 0) : 0;
+      uint64_t all = pending;
+      kept = turn == 0 ? __ballot(mine < 0) : 0;
       for (int k = 0; all != 0; ++k) {
         const int l = __builtin_amdgcn_readlane(mine, __builtin_ctzll(all));
         const uint64_t rows = __ballot(mine == l);
@@ -167,12 +171,13 @@ struct TileIds {
         if (k % of == turn) kept |= rows;
       }
       pending &= kept;
-      owned = (kept >> (threadIdx.x & 63)) & 1;
     }
+    owned = owned_row(threadIdx.x & (ROWS - 1));
   }
-  bool owned = true;
+  __device__ __forceinline__ int of_row(int row) const { return __shfl(mine, row, 64); }
+  __device__ __forceinline__ bool owned_row(int row) const { return (kept >> row) & 1; }
   // the next adapter of the tile, the same for all lanes; -1 when there is none
-  __device__ int next()
+  __device__ __forceinline__ int next()
   {
     if (pending == 0) return -1;
     const int l = __builtin_amdgcn_readlane(mine, __builtin_ctzll(pending));
@@ -316,11 +321,17 @@ __device__ __forceinline__ void sort_rows(const Problem &p, const Sort &o, int32
 // ------------------------------------------------------------------ shrink
 constexpr int kShrinkWaves = 8;
 
-// Columns that a wave asks for at a time: as much as its registers hold, so that a memory round trip is paid for few times.
+#ifndef TT1
+#define TT1 2
+#endif
+// Columns that a wave asks for at a time (as much as its registers hold, so that a memory round trip is paid for few times), and tiles of
+// 16 rows of a workgroup.
 template <typename T, int JT, bool kDown> struct ShrinkUnit {
   static constexpr int kBytes = JT * static_cast<int>(sizeof(T));       // 2 .. 32: registers of the factor grow with it
   static constexpr int kSteps = kDown ? (kBytes >= 16 ? 1 : 2) : (kBytes >= 32 ? 1 : kBytes >= 8 ? 2 : 4);
   static constexpr int kCols = 32 * kSteps;
+  // kDown stages the factor once for all rows of a workgroup
+  static constexpr int kTiles = !kDown || kBytes >= 32 ? 1 : kBytes == 2 ? TT1 : 2;
 };
 
 // out[slice][m][j] = scale sum over the slice's columns c of z[m][c] f[l][j][c] (kDown: f[l][c][j]), rows without adapter zero.
@@ -330,10 +341,11 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void shrink_kernel(Problem p, co
                                                                    bool scaled, float *__restrict__ out, Sort sort)
 {
   constexpr int R = 16 * JT;
-  constexpr int kSteps = ShrinkUnit<T, JT, kDown>::kSteps, kCols = 32 * kSteps;
+  constexpr int kSteps = ShrinkUnit<T, JT, kDown>::kSteps, kCols = 32 * kSteps, MT = ShrinkUnit<T, JT, kDown>::kTiles;
   constexpr int kStage = kDown ? kCols * R * sizeof(T) : 0;             // bytes of a wave's staged factor
-  constexpr int kSums = 16 * R * 4;
+  constexpr int kSums = 16 * MT * R * 4;
   __shared__ __align__(32) unsigned char lds[kShrinkWaves * (kStage > kSums ? kStage : kSums)];
+  __shared__ bool owned[16 * MT];
   if constexpr (kDown) {
     static_assert(64 * kShrinkWaves == kSortThreads);
     if (blockIdx.x == 0 && sort.rows != nullptr) {     // the gradients' list of rows, beside the others' work
@@ -342,85 +354,126 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void shrink_kernel(Problem p, co
     }
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
-  const int64_t tile = static_cast<int64_t>(blockIdx.x) - (kDown && sort.rows != nullptr ? 1 : 0);
-  const int64_t m = tile * 16 + i;
+  const int64_t m0 = (static_cast<int64_t>(blockIdx.x) - (kDown && sort.rows != nullptr ? 1 : 0)) * (16 * MT);
   const int64_t lo = blockIdx.y * per_slice, hi = lo + per_slice < C ? lo + per_slice : C;
-  TileIds ids(p, m, blockIdx.z, gridDim.z);
+  // lanes hold the rows m0 + lane for the list of adapters, and m0 + 16 t + i for the products
+  TileIds<16 * MT> ids(p, m0, blockIdx.z, gridDim.z);
   if (__ballot(ids.owned) == 0) return;               // the same for all waves
-  __shared__ bool owned[16];
-  if (threadIdx.x < 16) owned[threadIdx.x] = ids.owned;
-  floatx4_t sum[JT];
+  if (threadIdx.x < 16 * MT) owned[threadIdx.x] = ids.owned;
+  int mine[MT];
+  bool have_row[MT];
+  const T *row[MT];
 #pragma unroll
-  for (int j = 0; j < JT; ++j) sum[j] = floatx4_t{0, 0, 0, 0};
-  const T *row = z + (m < p.M ? m : p.M - 1) * C;
+  for (int t = 0; t < MT; ++t) {
+    mine[t] = ids.of_row(16 * t + i);
+    have_row[t] = ids.owned_row(16 * t + i);
+    const int64_t m = m0 + 16 * t + i;
+    row[t] = z + (m < p.M ? m : p.M - 1) * C;
+  }
+  floatx4_t sum[MT][JT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int j = 0; j < JT; ++j) sum[t][j] = floatx4_t{0, 0, 0, 0};
   T *stage = reinterpret_cast<T *>(lds) + wave * (kStage / sizeof(T));
   for (int l = ids.next(); l >= 0; l = ids.next()) {
     const T *factor = f + static_cast<int64_t>(l) * p.r * C;
-    floatx4_t acc[JT];
+    floatx4_t acc[MT][JT];
 #pragma unroll
-    for (int j = 0; j < JT; ++j) acc[j] = floatx4_t{0, 0, 0, 0};
-    auto unit = [&](int64_t c0, auto is_full) {
-      constexpr bool kFull = decltype(is_full)::value;
-      vec8<T> zv[kSteps], fv[kSteps][JT];
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int64_t c = c0 + 32 * s + 8 * q;
-        zv[s] = zero8<vec8<T>>();
-        if (ids.owned) zv[s] = kFull ? load8<T>(row + c) : load8<T>(row + c, clamp8(hi - c));
-      }
-      if constexpr (!kDown) {
+      for (int j = 0; j < JT; ++j) acc[t][j] = floatx4_t{0, 0, 0, 0};
+    vec8<T> zv[MT][kSteps];
+    auto fetch_rows = [&](int64_t c0, bool full) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          const int64_t c = c0 + 32 * s + 8 * q;
+          zv[t][s] = zero8<vec8<T>>();
+          if (have_row[t]) zv[t][s] = full ? load8<T>(row[t] + c) : load8<T>(row[t] + c, clamp8(hi - c));
+        }
+    };
+    int64_t c0 = lo + wave * kCols;
+    if constexpr (!kDown) {
+      auto unit = [&](bool full) {
+        vec8<T> fv[kSteps][JT];
+        fetch_rows(c0, full);
 #pragma unroll
         for (int j = 0; j < JT; ++j) {
           const int at = 16 * j + i < p.r ? 16 * j + i : p.r - 1;           // rows past the rank repeat the last; their sums are not kept
           const T *from = factor + at * C + c0 + 8 * q;
 #pragma unroll
-          for (int s = 0; s < kSteps; ++s) fv[s][j] = kFull ? load8<T>(from + 32 * s) : load8<T>(from + 32 * s, clamp8(hi - c0 - 32 * s - 8 * q));
+          for (int s = 0; s < kSteps; ++s) fv[s][j] = full ? load8<T>(from + 32 * s) : load8<T>(from + 32 * s, clamp8(hi - c0 - 32 * s - 8 * q));
         }
-      } else {
-        // the factor's rows c0 .. + kCols, eight ranks at a time, zeros past the rank and past the last column
-        constexpr int kOct = R / 8;
-        vec8<T> st[kCols * kOct / 64];
-#pragma unroll
-        for (int o = 0; o < kCols * kOct / 64; ++o) {
-          const int at = o * 64 + lane, c = at / kOct, j = at % kOct * 8;
-          st[o] = load8<T>(factor + (c0 + c) * p.r + j, kFull || c0 + c < hi ? clamp8(p.r - j) : 0);
-        }
-#pragma unroll
-        for (int o = 0; o < kCols * kOct / 64; ++o) *reinterpret_cast<vec8<T> *>(stage + (o * 64 + lane) * 8) = st[o];
-        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-          for (int j = 0; j < JT; ++j) fv[s][j] = down<T>(stage + 32 * s * R + 16 * j, R, 4, lane, q);
+          for (int j = 0; j < JT; ++j)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t][j] = mma(fv[s][j], zv[t][s], acc[t][j]);
+      };
+      for (; c0 + kCols <= hi; c0 += kShrinkWaves * kCols) unit(true);
+      if (c0 < hi) unit(false);
+    } else {
+      // the factor's rows c0 .. + kCols, eight ranks at a time, zeros past the rank and past the last column; a unit's values are asked for
+      // before the products of the unit in front
+      constexpr int kOct = R / 8, kEach = kCols * kOct / 64;
+      vec8<T> st[kEach];
+      auto fetch = [&]() {
+        const bool full = c0 + kCols <= hi;
+        fetch_rows(c0, full);
+#pragma unroll
+        for (int o = 0; o < kEach; ++o) {
+          const int at = o * 64 + lane, c = at / kOct, j = at % kOct * 8;
+          st[o] = load8<T>(factor + (c0 + c) * p.r + j, full || c0 + c < hi ? clamp8(p.r - j) : 0);
+        }
+      };
+      if (c0 < hi) fetch();
+      while (c0 < hi) {
+#pragma unroll
+        for (int o = 0; o < kEach; ++o) *reinterpret_cast<vec8<T> *>(stage + (o * 64 + lane) * 8) = st[o];
+        vec8<T> now[MT][kSteps];
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) now[t][s] = zv[t][s];
+        __builtin_amdgcn_wave_barrier();
+        c0 += kShrinkWaves * kCols;
+        if (c0 < hi) fetch();
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int j = 0; j < JT; ++j) {
+            const vec8<T> fv = down<T>(stage + 32 * s * R + 16 * j, R, 4, lane, q);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t][j] = mma(fv, now[t][s], acc[t][j]);
+          }
         __builtin_amdgcn_wave_barrier();
       }
+    }
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s)
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int j = 0; j < JT; ++j) acc[j] = mma(fv[s][j], zv[s], acc[j]);
-    };
-    int64_t c0 = lo + wave * kCols;
-    for (; c0 + kCols <= hi; c0 += kShrinkWaves * kCols) unit(c0, std::true_type{});
-    if (c0 < hi) unit(c0, std::false_type{});
-    const bool mine = ids.mine == l;
+      for (int j = 0; j < JT; ++j)
 #pragma unroll
-    for (int j = 0; j < JT; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum[j][e] = mine ? acc[j][e] : sum[j][e];
+        for (int e = 0; e < 4; ++e) sum[t][j][e] = mine[t] == l ? acc[t][j][e] : sum[t][j][e];
   }
   // the waves' shares, [wave][m][j], added in the waves' order
   __syncthreads();
   float *sums = reinterpret_cast<float *>(lds);
 #pragma unroll
-  for (int j = 0; j < JT; ++j) *reinterpret_cast<floatx4_t *>(sums + (wave * 16 + i) * R + 16 * j + 4 * q) = sum[j];
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int j = 0; j < JT; ++j) *reinterpret_cast<floatx4_t *>(sums + ((wave * MT + t) * 16 + i) * R + 16 * j + 4 * q) = sum[t][j];
   __syncthreads();
-  for (int o = threadIdx.x; o < 16 * R; o += 64 * kShrinkWaves) {
-    const int64_t mm = tile * 16 + o / R;
+  for (int o = threadIdx.x; o < 16 * MT * R; o += 64 * kShrinkWaves) {
+    const int64_t mm = m0 + o / R;
     const int j = o % R;
     if (mm >= p.M || j >= p.r || !owned[o / R]) continue;
     float v = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kShrinkWaves; ++w) v += sums[w * 16 * R + o];
+    for (int w = 0; w < kShrinkWaves; ++w) v += sums[w * 16 * MT * R + o];
     if (scaled) {
       const int l = p.ids[mm];
       v = l >= 0 && l < p.L ? v * p.scaling[l] : 0.0f;
@@ -435,15 +488,15 @@ struct Rows {
   const float *at;
   int slices;
 };
-// values j .. j + 7 of row m, zeros past the rank
-__device__ __forceinline__ f32x8_t rank8(const Problem &p, const Rows &u, int64_t m, int j)
+// values j .. j + 7 of row m, zeros past the rank; kMany: more than a few slices, asked for four at a time
+template <bool kMany> __device__ __forceinline__ f32x8_t rank8(const Problem &p, const Rows &u, int64_t m, int j)
 {
   const int have = clamp8(p.r - j);
   const float *at = u.at + m * p.r + j;
   f32x8_t v = load8<float>(at, have);
   const int64_t apart = p.M * p.r;
   int s = 1;
-  for (; s + 4 <= u.slices; s += 4) {                 // four asked for at a time
+  for (; kMany && s + 4 <= u.slices; s += 4) {
     f32x8_t w[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) w[k] = load8<float>(at + (s + k) * apart, have);
@@ -552,24 +605,30 @@ __global__ __launch_bounds__(64 * kExpandWaves) void expand_kernel(Problem p, Ro
   const int64_t m = (tile * kExpandWaves + wave) * 16 + i;
   if (m - i >= p.M) return;
   const bool in = m < p.M;
-  TileIds ids(p, m, blockIdx.y, gridDim.y);
-  if (__ballot(ids.owned) == 0) return;
   // a tile that is whole in every direction asks for all of its base at once
   const bool whole_tile = m - i + 16 <= p.M && p.r % 8 == 0 && first + G * kExpandCols <= C;
   vec8<T> early[G][2];
-  if (whole_tile) {
+  auto ask = [&]() {
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        early[g][h] = base && ids.owned ? load8<T>(base + m * C + first + kExpandCols * g + 32 * h + 8 * q) : zero8<vec8<T>>();
-  }
+      for (int h = 0; h < 2; ++h) early[g][h] = base ? load8<T>(base + m * C + first + kExpandCols * g + 32 * h + 8 * q) : zero8<vec8<T>>();
+  };
+  constexpr bool kTurns = G == 1;                      // of the tiles' adapters, where few waves run
+  if (whole_tile && !kTurns) ask();
+  TileIds<16> ids(p, m - i, kTurns ? blockIdx.y : 0, kTurns ? gridDim.y : 1);
+  if (__ballot(ids.owned) == 0) return;
+  if (whole_tile && kTurns && ids.owned) ask();
   const int qj = kPieces ? q & 1 : q;                  // which eight ranks of a step
   f32x8_t v[S];
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    v[s] = zero8<f32x8_t>();
-    if (in && ids.owned) v[s] = rank8(p, u, m, 32 * s + 8 * qj);
+    if constexpr (kTurns) {
+      v[s] = zero8<f32x8_t>();
+      if (in && ids.owned) v[s] = rank8<true>(p, u, m, 32 * s + 8 * qj);
+    } else {
+      v[s] = rank8<false>(p, u, in ? m : p.M - 1, 32 * s + 8 * qj);
+    }
   }
   if (hidden && first == 0 && in && ids.owned && (!kPieces || q < 2)) {
 #pragma unroll
@@ -698,9 +757,6 @@ __global__ __launch_bounds__(64 * kExpandWaves) void expand_kernel(Problem p, Ro
 // ------------------------------------------------------------------ one row, both products
 constexpr int kRowWaves = 8;
 constexpr int kRowCols = 64 * kRowWaves;              // of a workgroup at a time
-#ifndef KA
-#define KA 16
-#endif
 constexpr int kRowRounds = 4;                         // of such columns, all asked for before the first product where registers allow
 
 // A workgroup takes one row and up to 2048 columns of its result and forms the row's h itself: the row's other workgroups do the same from
@@ -713,7 +769,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void row_kernel(Problem p, int rows
 {
   constexpr bool kHalf = RS == 0, kPieces = kHalf && sizeof(T) == 2;
   constexpr int S = kHalf ? 1 : RS, JT = kHalf ? 1 : 2 * RS, R = 16 * JT;
-  constexpr int kAhead = JT * static_cast<int>(sizeof(T)) <= 2 ? KA : JT * static_cast<int>(sizeof(T)) <= 4 ? 8 : JT * static_cast<int>(sizeof(T)) <= 8 ? 4 : 2;      // steps of the first product
+  constexpr int kAhead = JT * static_cast<int>(sizeof(T)) <= 4 ? 8 : JT * static_cast<int>(sizeof(T)) <= 8 ? 4 : 2;      // steps of the first product
   constexpr int kEarly = S * static_cast<int>(sizeof(T)) <= 2 ? kRowRounds : 1;                                          // rounds of the second
   __shared__ float shares[kRowWaves][R];
   __shared__ __align__(32) float total[S * 32];
@@ -1055,17 +1111,24 @@ __global__ __launch_bounds__(256) void zero_kernel(unsigned char *at, int64_t by
 
 // ------------------------------------------------------------------ host
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int up_to(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }      // the ranks that a kernel computes
 size_t up16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
 
-// Workgroups of the shrinking product per 16 rows: enough that some 512 run, a slice no shorter than one unit for each wave.
+// Workgroups of the shrinking product per `rows` rows: enough that some 512 run, a slice no shorter than one unit for each wave.
+int shrink_rows(int rank, size_t es)
+{
+  const int bytes = up_to(rank) / 16 * static_cast<int>(es);
+  return bytes >= 32 ? 16 : bytes == 2 ? 16 * TT1 : 32;
+}
+
 struct Slices {
   int count;
   int64_t columns;
 };
-Slices plan_slices(int64_t M, int64_t C)
+Slices plan_slices(int64_t M, int64_t C, int rows)
 {
   constexpr int kUnit = 64;
-  const int64_t tiles = ceil_div(M, 16), whole = ceil_div(C, kShrinkWaves * kUnit);
+  const int64_t tiles = ceil_div(M, rows), whole = ceil_div(C, kShrinkWaves * kUnit);
   int64_t n = 512 / (tiles > 0 ? tiles : 1);
   n = n < 1 ? 1 : (n > 16 ? 16 : n);
   if (n > whole) n = whole;
@@ -1091,10 +1154,11 @@ bool row_at_a_time(int64_t M, int64_t N, int64_t K, int rank, size_t es)
   return factor <= 256 << 10 && M * ceil_div(N, kRowCols * kRowRounds) <= (int64_t{64} << 20) / factor;
 }
 
-// Workgroups that share the adapters of a tile of 16 rows, `waves` waves working on it otherwise: as many as leave some 16384 in all.
+// Workgroups that share the adapters of a tile of 16 rows, `waves` waves working on it otherwise: as many as leave some 4096 in
+// all (999 rows in runs, 4096 to 4096, turns of four: 23.5 us, without turns XX).
 unsigned turns(const Problem &p, int64_t waves)
 {
-  const int64_t most = p.L < 16 ? p.L : 16, n = 16384 / (ceil_div(p.M, 16) * waves);
+  const int64_t most = p.L < 16 ? p.L : 16, n = 4096 / (ceil_div(p.M, 16) * waves);
   return static_cast<unsigned>(n < 1 ? 1 : (n > most ? most : n));
 }
 
@@ -1124,7 +1188,7 @@ struct Plan {
 Plan plan(int64_t M, int64_t N, int64_t K, int rank, int L, size_t es, bool backward)
 {
   Plan w{};
-  w.slices = plan_slices(M, backward ? N : K);
+  w.slices = plan_slices(M, backward ? N : K, backward ? shrink_rows(rank, es) : 16);
   w.rows = up16(static_cast<size_t>(w.slices.count) * M * rank * 4);
   if (!backward && row_at_a_time(M, N, K, rank, es)) w.rows = 0;
   if (backward) {
@@ -1141,7 +1205,8 @@ Plan plan(int64_t M, int64_t N, int64_t K, int rank, int L, size_t es, bool back
 template <typename T, bool kDown>
 void shrink(const Problem &p, const Slices &sl, const void *z, int64_t C, const void *f, bool scaled, float *out, const Sort &sort, hipStream_t s)
 {
-  const dim3 grid(static_cast<unsigned>(ceil_div(p.M, 16) + (sort.rows ? 1 : 0)), sl.count, turns(p, sl.count * kShrinkWaves)), block(64 * kShrinkWaves);
+  const int rows = kDown ? shrink_rows(p.r, sizeof(T)) : 16;
+  const dim3 grid(static_cast<unsigned>(ceil_div(p.M, rows) + (sort.rows ? 1 : 0)), sl.count, turns(p, sl.count * kShrinkWaves)), block(64 * kShrinkWaves);
   const T *zz = static_cast<const T *>(z), *ff = static_cast<const T *>(f);
   if (p.r <= 16) hipLaunchKernelGGL((shrink_kernel<T, 1, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out, sort);
   else if (p.r <= 32) hipLaunchKernelGGL((shrink_kernel<T, 2, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out, sort);
@@ -1153,7 +1218,7 @@ template <typename T, bool kDown, int G>
 void expand(const Problem &p, const Rows &u, int64_t C, const void *f, bool scaled, const void *base, void *out, float *hidden, hipStream_t s)
 {
   const int64_t tiles = ceil_div(C, kExpandCols * G);
-  const dim3 grid(static_cast<unsigned>(ceil_div(p.M, 16 * kExpandWaves) * tiles), turns(p, tiles)), block(64 * kExpandWaves);
+  const dim3 grid(static_cast<unsigned>(ceil_div(p.M, 16 * kExpandWaves) * tiles), G == 1 ? turns(p, tiles) : 1), block(64 * kExpandWaves);
   const T *ff = static_cast<const T *>(f), *bb = static_cast<const T *>(base);
   T *oo = static_cast<T *>(out);
   if (p.r <= 16) hipLaunchKernelGGL((expand_kernel<T, 0, kDown, G>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
