@@ -1144,14 +1144,16 @@ int32_t plan_chunk(int64_t M, int64_t C)
 }
 
 // Whether the forward takes its rows one by one: every workgroup reads its row's first factor again, so that factor must be short (256 KB
-// is four memory round trips of a workgroup's waves) and all reads together less than what the caches give in some ten us.  Measured, us,
+// is four memory round trips of a workgroup's waves), the workgroups few enough to run at once, and all reads together less than what the
+// caches give in some ten us.  Measured, us,
 // row by row / in tiles, rows of one adapter each (neighbours of one adapter), K = 4096, bf16: rank 16, one row 7.4 / 10.1; 32 rows to
 // N = 14336 10.1 / 18.6 (8.9 / 10.1); 128 rows to 4096 10.2 / 22.5 (8.8 / 9.8), to 14336 (112 MB) 27.6 / 35.6 (23.9 / 11.8); rank 64
 // (512 KB), one row 18.5 / 14.2, 32 rows to 4096 19.9 / 17.3 (19.0 / 13.8).
 bool row_at_a_time(int64_t M, int64_t N, int64_t K, int rank, size_t es)
 {
   const int64_t factor = static_cast<int64_t>(rank) * K * static_cast<int64_t>(es);
-  return factor <= 256 << 10 && M * ceil_div(N, kRowCols * kRowRounds) <= (int64_t{64} << 20) / factor;
+  const int64_t workgroups = M * ceil_div(N, kRowCols * kRowRounds);
+  return factor <= 256 << 10 && workgroups <= 512 && workgroups <= (int64_t{64} << 20) / factor;
 }
 
 // Workgroups that share the adapters of a tile of 16 rows, `waves` waves working on it otherwise: as many as leave some 4096 in

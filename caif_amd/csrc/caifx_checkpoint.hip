@@ -4,8 +4,9 @@
 //   scale = fl32(max|x| * fl32(1 / 127)), 1 where that is zero, NaN where the group holds an infinity or a NaN
 //   code  = clamp(rint(fl32(x / scale)), -127, 127)            value = code * scale
 //
-// Everything here is bound by memory.  Sixteen lanes take a group, eight values each, so that a lane's part is one 16-byte
-// access of a 16-bit type; rows of any length and alignment take the same path (the hardware splits an access that straddles
+// Everything here is bound by memory, if the arithmetic is kept short: 45 M values through silu and two divisions each are as long a way
+// for the vector units as their 360 MB for the memory.  Sixteen lanes take a group, eight values each, so that a lane's part is one
+// 16-byte access of a 16-bit type; rows of any length and alignment take the same path (the hardware splits an access that straddles
 // a line), only a row's last values are moved one by one.
 #include "caifx_common.hpp"
 
@@ -18,7 +19,8 @@ constexpr int kGroup = CAIFX_CHECKPOINT_GROUP;
 constexpr int kPer = 8;                               // values of a lane
 constexpr int kLanes = kGroup / kPer;                 // lanes of a group
 constexpr int kThreads = 256;
-constexpr int kUnits = kThreads / kLanes;             // groups of a workgroup
+constexpr int kTurns = 2;                             // groups of a lane, both asked for before the first is used
+constexpr int kUnits = kTurns * kThreads / kLanes;    // groups of a workgroup
 
 template <typename T> struct Eight { T v[kPer]; };
 
@@ -45,149 +47,231 @@ template <typename T> __device__ __forceinline__ void store8(T *p, const Eight<T
   }
 }
 
-// The place of a lane: its group (row, column of the group) and its eight values in it.
-struct Place {
-  int64_t at;                                         // flat index of the lane's first value
-  int64_t scale_at;                                   // flat index of the group's scale
-  int have;                                           // values of the lane inside the row, 0 past the last group
+// rows x cols in groups of a row.  Rows of whole groups need no row: their groups stand in one line.
+struct Shape {
+  uint32_t units, groups, magic;                      // groups in all, of a row, floor(2^32 / groups) or 2^32 - 1
+  int64_t cols;
 };
-__device__ __forceinline__ Place place(int64_t rows, int64_t cols, int64_t groups)
+// The place of a lane: its eight values in a group.
+struct Place {
+  int64_t at;                                         // flat index of the first
+  uint32_t unit;                                      // flat index of the group
+  int have;                                           // values inside the row, 0 past the last group
+};
+template <bool kWhole> __device__ __forceinline__ Place place(const Shape &s, int turn)
 {
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kUnits;             // the workgroup's first group, the same for all lanes
-  const int64_t row0 = first / groups;
-  const uint32_t in_row = static_cast<uint32_t>(first - row0 * groups) + threadIdx.x / kLanes;
-  const uint32_t down = in_row / static_cast<uint32_t>(groups);
-  const int64_t row = row0 + down;
-  const int64_t col = static_cast<int64_t>(in_row - down * static_cast<uint32_t>(groups)) * kGroup + (threadIdx.x % kLanes) * kPer;
-  const int64_t left = row < rows ? cols - col : 0;
-  return {row * cols + col, first + threadIdx.x / kLanes, left >= kPer ? kPer : (left > 0 ? static_cast<int>(left) : 0)};
+  const uint32_t unit = (blockIdx.x * kTurns + turn) * (kThreads / kLanes) + threadIdx.x / kLanes, in = (threadIdx.x % kLanes) * kPer;
+  if constexpr (kWhole) {
+    return {static_cast<int64_t>(unit) * kGroup + in, unit, unit < s.units ? kPer : 0};
+  } else {
+    uint32_t row = __umulhi(unit, s.magic);           // the quotient or one less
+    if (unit - row * s.groups >= s.groups) ++row;
+    const int64_t col = static_cast<int64_t>(unit - row * s.groups) * kGroup + in, left = unit < s.units ? s.cols - col : 0;
+    return {row * s.cols + col, unit, left >= kPer ? kPer : (left > 0 ? static_cast<int>(left) : 0)};
+  }
 }
 
-// maximum over the sixteen lanes of a group
+// Maximum over the sixteen lanes of a group, which are a row of the wave's data-parallel moves: neighbours, pairs, mirrored halves.
 __device__ __forceinline__ uint32_t group_max(uint32_t v)
 {
-#pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) {
-    const uint32_t w = __shfl_xor(v, o, kLanes);
-    v = v > w ? v : w;
-  }
+  auto with = [&](uint32_t w) { v = v > w ? v : w; };
+  with(__builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true));              // lanes 1 0 3 2
+  with(__builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true));              // lanes 2 3 0 1
+  with(__builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, true));             // eight lanes backwards
+  with(__builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, true));             // sixteen lanes backwards
   return v;
 }
 
-// Codes of a lane's eight values, and the group's scale.  The magnitudes are compared as bit patterns: an infinity is larger
-// than any number and a NaN larger than that, so one comparison at the end tells whether the group holds either.
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+
+// The largest magnitude of a group, as the bits of an fp32 number.  Magnitudes are compared as bit patterns: an infinity is larger than
+// any number and a NaN larger than that, so one comparison tells whether the group holds either.
+template <typename T> __device__ __forceinline__ uint32_t group_top(const Eight<T> &x)
+{
+  if constexpr (sizeof(T) == 4) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t b = __builtin_bit_cast(uint32_t, x.v[i]) & 0x7FFFFFFFu;
+      top = top > b ? top : b;
+    }
+    return group_max(top);
+  } else {
+    struct Words { uint32_t w[kPer / 2]; };
+    const Words words = __builtin_bit_cast(Words, x);
+    u16x2_t top = __builtin_bit_cast(u16x2_t, words.w[0] & 0x7FFF7FFFu);
+#pragma unroll
+    for (int i = 1; i < kPer / 2; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, words.w[i] & 0x7FFF7FFFu));
+    const uint32_t most = group_max(top[0] > top[1] ? top[0] : top[1]);
+    const float value = to_f32<T>(__builtin_bit_cast(T, static_cast<uint16_t>(most)));
+    return __builtin_bit_cast(uint32_t, value);
+  }
+}
+
+// Codes of a lane's eight values, and the group's scale.  The quotient is rounded as a division rounds it without being one: with the
+// rounded inverse y of the scale, q = x y is at most 1.5 steps off, q + (x - q s) y within a step, and the same once more is the rounded
+// quotient (Markstein: a quotient within a step, corrected by its exact remainder times the rounded inverse).  Adding 1.5 2^23 rounds it to
+// an integer, ties to even, and leaves the integer in the low byte.  Scales below 2^-100, where the remainders would underflow, divide.
 template <typename T> __device__ __forceinline__ Eight<int8_t> quantise(const Eight<T> &x, float &scale)
 {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, to_f32<T>(x.v[i])) & 0x7FFFFFFFu;
-    top = top > b ? top : b;
-  }
-  top = group_max(top);
+  const uint32_t top = group_top(x);
   const bool finite = top < 0x7F800000u;
   scale = finite ? __builtin_bit_cast(float, top) * (1.0f / 127.0f) : __builtin_nanf("");
   if (scale == 0.0f) scale = 1.0f;
-  Eight<int8_t> q;
+  uint32_t bits[kPer];
+  if (scale < 0x1p-100f) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const float n = fminf(fmaxf(rintf(to_f32<T>(x.v[i]) / scale), -127.0f), 127.0f);
-    q.v[i] = static_cast<int8_t>(finite ? static_cast<int>(n) : 0);
+    for (int i = 0; i < kPer; ++i) {
+      const float n = fminf(fmaxf(rintf(to_f32<T>(x.v[i]) / scale), -127.0f), 127.0f);
+      bits[i] = static_cast<uint32_t>(static_cast<int>(n));
+    }
+  } else {
+    const float y = 1.0f / scale;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const float v = to_f32<T>(x.v[i]);
+      float q = v * y;
+      q = __builtin_fmaf(__builtin_fmaf(-q, scale, v), y, q);
+      q = __builtin_fmaf(__builtin_fmaf(-q, scale, v), y, q);
+      bits[i] = __builtin_bit_cast(uint32_t, q + 12582912.0f);
+    }
   }
-  return q;
+  struct Words { uint32_t w[2]; } words;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t lo = __builtin_amdgcn_perm(bits[4 * h + 1], bits[4 * h], 0x0C0C0400u), hi = __builtin_amdgcn_perm(bits[4 * h + 3], bits[4 * h + 2], 0x04000C0Cu);
+    words.w[h] = finite ? lo | hi : 0u;
+  }
+  return __builtin_bit_cast(Eight<int8_t>, words);
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void pack_kernel(const T *__restrict__ x, int8_t *__restrict__ codes, float *__restrict__ scales, int64_t rows,
-                                                        int64_t cols, int64_t groups)
+template <typename T, bool kWhole>
+__global__ __launch_bounds__(kThreads) void pack_kernel(const T *__restrict__ x, int8_t *__restrict__ codes, float *__restrict__ scales, Shape s)
 {
-  const Place p = place(rows, cols, groups);
-  const Eight<T> v = load8(x + p.at, p.have);
-  float scale;
-  const Eight<int8_t> q = quantise(v, scale);
-  store8(codes + p.at, q, p.have);
-  if (threadIdx.x % kLanes == 0 && p.have > 0) scales[p.scale_at] = scale;
+  Place p[kTurns];
+  Eight<T> v[kTurns];
+#pragma unroll
+  for (int k = 0; k < kTurns; ++k) {
+    p[k] = place<kWhole>(s, k);
+    v[k] = load8(x + p[k].at, p[k].have);
+  }
+#pragma unroll
+  for (int k = 0; k < kTurns; ++k) {
+    float scale;
+    const Eight<int8_t> q = quantise(v[k], scale);
+    store8(codes + p[k].at, q, p[k].have);
+    if (threadIdx.x % kLanes == 0 && p[k].have > 0) scales[p[k].unit] = scale;
+  }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void unpack_kernel(const int8_t *__restrict__ codes, const float *__restrict__ scales, T *__restrict__ out,
-                                                          int64_t rows, int64_t cols, int64_t groups)
+template <typename T, bool kWhole>
+__global__ __launch_bounds__(kThreads) void unpack_kernel(const int8_t *__restrict__ codes, const float *__restrict__ scales, T *__restrict__ out, Shape s)
 {
-  const Place p = place(rows, cols, groups);
-  if (p.have == 0) return;
-  const Eight<int8_t> q = load8(codes + p.at, p.have);
-  const float scale = scales[p.scale_at];
-  Eight<T> v;
+  Place p[kTurns];
+  Eight<int8_t> q[kTurns];
+  float scale[kTurns];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    float value = static_cast<float>(q.v[i]) * scale;
-    // the product is an fp32 number first: fused with the conversion to fp16 it would be rounded once, to another value in places
-    asm("" : "+v"(value));
-    v.v[i] = from_f32<T>(value);
+  for (int k = 0; k < kTurns; ++k) {
+    p[k] = place<kWhole>(s, k);
+    q[k] = load8(codes + p[k].at, p[k].have);
+    scale[k] = p[k].have > 0 ? scales[p[k].unit] : 0.0f;
   }
-  store8(out + p.at, v, p.have);
+#pragma unroll
+  for (int k = 0; k < kTurns; ++k) {
+    Eight<T> v;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      float value = static_cast<float>(q[k].v[i]) * scale[k];
+      // the product is an fp32 number first: fused with the conversion to fp16 it would be rounded once, to another value in places
+      asm("" : "+v"(value));
+      v.v[i] = from_f32<T>(value);
+    }
+    store8(out + p[k].at, v, p[k].have);
+  }
 }
 
 // hidden = silu_multiply(gate, up), bit for bit (silu(gate) is rounded to T first), and both inputs' checkpoints
-template <typename T>
+template <typename T, bool kWhole>
 __global__ __launch_bounds__(kThreads) void gate_kernel(const T *__restrict__ gate, const T *__restrict__ up, T *__restrict__ hidden,
                                                         int8_t *__restrict__ gate_codes, float *__restrict__ gate_scales, int8_t *__restrict__ up_codes,
-                                                        float *__restrict__ up_scales, int64_t rows, int64_t cols, int64_t groups)
+                                                        float *__restrict__ up_scales, Shape s)
 {
-  const Place p = place(rows, cols, groups);
-  const Eight<T> g = load8(gate + p.at, p.have), u = load8(up + p.at, p.have);
-  Eight<T> h;
+  Place p[kTurns];
+  Eight<T> g[kTurns], u[kTurns];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) h.v[i] = swiglu_fwd_one<T>(g.v[i], u.v[i]);
-  store8(hidden + p.at, h, p.have);
-  float gs, us;
-  const Eight<int8_t> gq = quantise(g, gs), uq = quantise(u, us);
-  store8(gate_codes + p.at, gq, p.have);
-  store8(up_codes + p.at, uq, p.have);
-  if (threadIdx.x % kLanes == 0 && p.have > 0) {
-    gate_scales[p.scale_at] = gs;
-    up_scales[p.scale_at] = us;
+  for (int k = 0; k < kTurns; ++k) {
+    p[k] = place<kWhole>(s, k);
+    g[k] = load8(gate + p[k].at, p[k].have);
+    u[k] = load8(up + p[k].at, p[k].have);
+  }
+#pragma unroll
+  for (int k = 0; k < kTurns; ++k) {
+    Eight<T> h;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) h.v[i] = swiglu_fwd_one<T>(g[k].v[i], u[k].v[i]);
+    store8(hidden + p[k].at, h, p[k].have);
+    float gs, us;
+    const Eight<int8_t> gq = quantise(g[k], gs), uq = quantise(u[k], us);
+    store8(gate_codes + p[k].at, gq, p[k].have);
+    store8(up_codes + p[k].at, uq, p[k].have);
+    if (threadIdx.x % kLanes == 0 && p[k].have > 0) {
+      gate_scales[p[k].unit] = gs;
+      up_scales[p[k].unit] = us;
+    }
   }
 }
 
 // g, u = the checkpoints' values in fp32; grad_up = T(d silu(g)), grad_gate = T(d u silu'(g)) and, where it is asked for,
-// hidden = T(silu(g) u): each result is rounded once.
-template <typename T, bool kHidden>
+// hidden = T(silu(g) u): each result is rounded once.  The logistic function's inverse is the instruction's, within a step.
+template <typename T, bool kHidden, bool kWhole>
 __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(const int8_t *__restrict__ gate_codes, const float *__restrict__ gate_scales,
                                                             const int8_t *__restrict__ up_codes, const float *__restrict__ up_scales,
                                                             const T *__restrict__ grad, T *__restrict__ grad_gate, T *__restrict__ grad_up,
-                                                            T *__restrict__ hidden, int64_t rows, int64_t cols, int64_t groups)
+                                                            T *__restrict__ hidden, Shape s)
 {
-  const Place p = place(rows, cols, groups);
-  if (p.have == 0) return;
-  const Eight<int8_t> gq = load8(gate_codes + p.at, p.have), uq = load8(up_codes + p.at, p.have);
-  const Eight<T> d = load8(grad + p.at, p.have);
-  const float gs = gate_scales[p.scale_at], us = up_scales[p.scale_at];
-  Eight<T> og, ou, oh;
+  Place p[kTurns];
+  Eight<int8_t> gq[kTurns], uq[kTurns];
+  Eight<T> d[kTurns];
+  float gs[kTurns], us[kTurns];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const float g = static_cast<float>(gq.v[i]) * gs, u = static_cast<float>(uq.v[i]) * us, grad_h = to_f32<T>(d.v[i]);
-    const float s = 1.0f / (1.0f + expf(-g)), act = g * s;
-    ou.v[i] = from_f32<T>(grad_h * act);
-    og.v[i] = from_f32<T>(grad_h * u * (s * __builtin_fmaf(g, 1.0f - s, 1.0f)));
-    if constexpr (kHidden) oh.v[i] = from_f32<T>(act * u);
+  for (int k = 0; k < kTurns; ++k) {
+    p[k] = place<kWhole>(s, k);
+    gq[k] = load8(gate_codes + p[k].at, p[k].have);
+    uq[k] = load8(up_codes + p[k].at, p[k].have);
+    d[k] = load8(grad + p[k].at, p[k].have);
+    gs[k] = p[k].have > 0 ? gate_scales[p[k].unit] : 0.0f;
+    us[k] = p[k].have > 0 ? up_scales[p[k].unit] : 0.0f;
   }
-  store8(grad_gate + p.at, og, p.have);
-  store8(grad_up + p.at, ou, p.have);
-  if constexpr (kHidden) store8(hidden + p.at, oh, p.have);
+#pragma unroll
+  for (int k = 0; k < kTurns; ++k) {
+    Eight<T> og, ou, oh;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const float g = static_cast<float>(gq[k].v[i]) * gs[k], u = static_cast<float>(uq[k].v[i]) * us[k], grad_h = to_f32<T>(d[k].v[i]);
+      const float sg = __builtin_amdgcn_rcpf(1.0f + expf(-g)), act = g * sg;
+      ou.v[i] = from_f32<T>(grad_h * act);
+      og.v[i] = from_f32<T>(grad_h * u * (sg * __builtin_fmaf(g, 1.0f - sg, 1.0f)));
+      if constexpr (kHidden) oh.v[i] = from_f32<T>(act * u);
+    }
+    store8(grad_gate + p[k].at, og, p[k].have);
+    store8(grad_up + p[k].at, ou, p[k].have);
+    if constexpr (kHidden) store8(hidden + p[k].at, oh, p[k].have);
+  }
 }
 
-// CAIFX_OK and `go` for a launch that has work; blocks of the launch
-int check(int64_t rows, int64_t cols, int dtype, bool missing, bool misaligned, bool &go, dim3 &grid, int64_t &groups)
+// CAIFX_OK and `go` for a launch that has work, its shape and workgroups
+int check(int64_t rows, int64_t cols, int dtype, bool missing, bool misaligned, bool &go, dim3 &grid, Shape &shape)
 {
   go = false;
   if (!valid_dtype(dtype) || rows < 0 || cols < 0) return CAIFX_ERR_INVALID_ARGUMENT;
   if (rows == 0 || cols == 0) return CAIFX_OK;
   if (missing) return CAIFX_ERR_INVALID_ARGUMENT;
   if (misaligned) return CAIFX_ERR_MISALIGNED;
-  groups = (cols + kGroup - 1) / kGroup;
-  // a grid has fewer than 2^32 threads, and a row's groups fit 31 bits
-  if (groups > INT32_MAX / 2 || rows > (int64_t{1} << 30) || groups > ((int64_t{1} << 24) - 1) * kUnits / rows) return CAIFX_ERR_UNSUPPORTED;
+  const int64_t groups = (cols + kGroup - 1) / kGroup;
+  // a grid has fewer than 2^32 threads
+  if (rows > INT32_MAX || groups > INT32_MAX || groups > ((int64_t{1} << 24) - 1) * kUnits / rows) return CAIFX_ERR_UNSUPPORTED;
+  const uint32_t g = static_cast<uint32_t>(groups);
+  shape = Shape{static_cast<uint32_t>(rows * groups), g, g == 1 ? UINT32_MAX : static_cast<uint32_t>((uint64_t{1} << 32) / g), cols};
   grid = dim3(static_cast<unsigned>((rows * groups + kUnits - 1) / kUnits));
   go = true;
   return CAIFX_OK;
@@ -198,12 +282,15 @@ int check(int64_t rows, int64_t cols, int dtype, bool missing, bool misaligned, 
 
 using namespace caifx;
 
-// one launch for the element type of `dtype`
-#define CAIFX_BY_TYPE(go)                       \
-  switch (dtype) {                              \
-    case CAIFX_F32: { typedef float T; go; break; }   \
-    case CAIFX_F16: { typedef f16_t T; go; break; }   \
-    default: { typedef bf16_t T; go; break; }         \
+// one launch for the element type of `dtype`, and for rows of whole groups or others
+#define CAIFX_BY_WIDTH(...)                                                 \
+  if (cols % kGroup == 0) { constexpr bool kWhole = true; __VA_ARGS__; }            \
+  else { constexpr bool kWhole = false; __VA_ARGS__; }
+#define CAIFX_BY_TYPE(...)                                                  \
+  switch (dtype) {                                                         \
+    case CAIFX_F32: { typedef float T; CAIFX_BY_WIDTH(__VA_ARGS__) break; }         \
+    case CAIFX_F16: { typedef f16_t T; CAIFX_BY_WIDTH(__VA_ARGS__) break; }         \
+    default: { typedef bf16_t T; CAIFX_BY_WIDTH(__VA_ARGS__) break; }               \
   }
 
 extern "C" {
@@ -212,11 +299,11 @@ int caifx_checkpoint_pack(const void *input, void *codes, float *scales, int64_t
 {
   bool go;
   dim3 grid;
-  int64_t groups;
-  const int st = check(rows, cols, dtype, !input || !codes || !scales, !aligned_to(input, dtype_size(dtype)) || !aligned_to(scales, 4), go, grid, groups);
+  Shape shape;
+  const int st = check(rows, cols, dtype, !input || !codes || !scales, !aligned_to(input, dtype_size(dtype)) || !aligned_to(scales, 4), go, grid, shape);
   if (!go) return st;
-  CAIFX_BY_TYPE(hipLaunchKernelGGL(pack_kernel<T>, grid, dim3(kThreads), 0, as_stream(stream), static_cast<const T *>(input),
-                                   static_cast<int8_t *>(codes), scales, rows, cols, groups));
+  CAIFX_BY_TYPE(hipLaunchKernelGGL((pack_kernel<T, kWhole>), grid, dim3(kThreads), 0, as_stream(stream), static_cast<const T *>(input),
+                                   static_cast<int8_t *>(codes), scales, shape));
   return launch_status();
 }
 
@@ -224,11 +311,11 @@ int caifx_checkpoint_unpack(const void *codes, const float *scales, void *output
 {
   bool go;
   dim3 grid;
-  int64_t groups;
-  const int st = check(rows, cols, dtype, !output || !codes || !scales, !aligned_to(output, dtype_size(dtype)) || !aligned_to(scales, 4), go, grid, groups);
+  Shape shape;
+  const int st = check(rows, cols, dtype, !output || !codes || !scales, !aligned_to(output, dtype_size(dtype)) || !aligned_to(scales, 4), go, grid, shape);
   if (!go) return st;
-  CAIFX_BY_TYPE(hipLaunchKernelGGL(unpack_kernel<T>, grid, dim3(kThreads), 0, as_stream(stream), static_cast<const int8_t *>(codes), scales,
-                                   static_cast<T *>(output), rows, cols, groups));
+  CAIFX_BY_TYPE(hipLaunchKernelGGL((unpack_kernel<T, kWhole>), grid, dim3(kThreads), 0, as_stream(stream), static_cast<const int8_t *>(codes), scales,
+                                   static_cast<T *>(output), shape));
   return launch_status();
 }
 
@@ -237,15 +324,15 @@ int caifx_silu_multiply_checkpoint(const void *gate, const void *up, void *hidde
 {
   bool go;
   dim3 grid;
-  int64_t groups;
+  Shape shape;
   const size_t es = dtype_size(dtype);
   const int st = check(rows, cols, dtype, !gate || !up || !hidden || !gate_codes || !gate_scales || !up_codes || !up_scales,
                        !aligned_to(gate, es) || !aligned_to(up, es) || !aligned_to(hidden, es) || !aligned_to(gate_scales, 4) || !aligned_to(up_scales, 4),
-                       go, grid, groups);
+                       go, grid, shape);
   if (!go) return st;
-  CAIFX_BY_TYPE(hipLaunchKernelGGL(gate_kernel<T>, grid, dim3(kThreads), 0, as_stream(stream), static_cast<const T *>(gate), static_cast<const T *>(up),
+  CAIFX_BY_TYPE(hipLaunchKernelGGL((gate_kernel<T, kWhole>), grid, dim3(kThreads), 0, as_stream(stream), static_cast<const T *>(gate), static_cast<const T *>(up),
                                    static_cast<T *>(hidden), static_cast<int8_t *>(gate_codes), gate_scales, static_cast<int8_t *>(up_codes), up_scales,
-                                   rows, cols, groups));
+                                   shape));
   return launch_status();
 }
 
@@ -255,17 +342,17 @@ int caifx_swiglu_backward_checkpoint(const void *gate_codes, const float *gate_s
 {
   bool go;
   dim3 grid;
-  int64_t groups;
+  Shape shape;
   const size_t es = dtype_size(dtype);
   const int st = check(rows, cols, dtype, !gate_codes || !gate_scales || !up_codes || !up_scales || !grad_hidden || !grad_gate || !grad_up,
                        !aligned_to(gate_scales, 4) || !aligned_to(up_scales, 4) || !aligned_to(grad_hidden, es) || !aligned_to(grad_gate, es) ||
-                           !aligned_to(grad_up, es) || !aligned_to(hidden, es), go, grid, groups);
+                           !aligned_to(grad_up, es) || !aligned_to(hidden, es), go, grid, shape);
   if (!go) return st;
   hipStream_t s = as_stream(stream);
 #define CAIFX_GO(kHidden)                                                                                                                          \
-  hipLaunchKernelGGL((gate_bwd_kernel<T, kHidden>), grid, dim3(kThreads), 0, s, static_cast<const int8_t *>(gate_codes), gate_scales,              \
+  hipLaunchKernelGGL((gate_bwd_kernel<T, kHidden, kWhole>), grid, dim3(kThreads), 0, s, static_cast<const int8_t *>(gate_codes), gate_scales,              \
                      static_cast<const int8_t *>(up_codes), up_scales, static_cast<const T *>(grad_hidden), static_cast<T *>(grad_gate),           \
-                     static_cast<T *>(grad_up), static_cast<T *>(hidden), rows, cols, groups)
+                     static_cast<T *>(grad_up), static_cast<T *>(hidden), shape)
   if (hidden) {
     CAIFX_BY_TYPE(CAIFX_GO(true));
   } else {

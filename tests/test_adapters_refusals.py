@@ -30,8 +30,8 @@ def backward(**over):
     (dict(N=2 ** 40), UNSUPPORTED), (dict(K=2 ** 31), UNSUPPORTED), (dict(x=None), INVALID), (dict(ids=None), INVALID), (dict(a=None), INVALID),
     (dict(b=None), INVALID), (dict(scaling=None), INVALID), (dict(x=AT + 1), MISALIGNED), (dict(ids=AT + 2), MISALIGNED), (dict(a=AT + 1), MISALIGNED),
     (dict(b=AT + 1), MISALIGNED), (dict(base=AT + 1), MISALIGNED), (dict(scaling=AT + 2), MISALIGNED), (dict(hidden=AT + 2), MISALIGNED),
-    (dict(x=AT + 2, dtype=T.F32), MISALIGNED), (dict(ws=AT + 1), MISALIGNED), (dict(M=200, ws=None), SMALL),
-    (dict(M=200, bytes=15), SMALL)])
+    (dict(x=AT + 2, dtype=T.F32), MISALIGNED), (dict(ws=AT + 1), MISALIGNED), (dict(M=5000, ws=None), SMALL),
+    (dict(M=5000, bytes=15), SMALL)])
 def test_adapter_calls(call, over, status):
     assert call(**over) == status
 
