@@ -589,20 +589,38 @@ constexpr int kExpandCols = 64;                       // of a wave at a time
 // alternate by fours give it eight, one 16-byte access.  A wave keeps its rows' operands for all its columns: what is not
 // a load, a store or a product costs as much as the memory otherwise (built for each 64 columns: 56 us for 4096 x 11008 in bf16).
 // hidden: the rows themselves, written by the first columns' waves.
+struct Expand {
+  Rows u;
+  int64_t C, col_tiles;
+  const void *f;                                      // the factor, T
+  bool scaled;
+  const void *base;                                   // T, null for zero
+  void *out;                                          // T, may be base
+  float *hidden;                                      // null: not wanted
+  unsigned turns;                                     // workgroups of a tile
+};
+template <typename T, int RS> constexpr int expand_lds() { return kExpandWaves * (RS == 0 && sizeof(T) == 2 ? 16 : 32) * (kExpandCols + 8) * static_cast<int>(sizeof(T)); }
 template <typename T, int RS, bool kDown, int G>
-__global__ __launch_bounds__(64 * kExpandWaves) void expand_kernel(Problem p, Rows u, int64_t C, int64_t col_tiles, const T *__restrict__ f, bool scaled,
-                                                                   const T *base, T *out, float *__restrict__ hidden)
+__device__ __forceinline__ void expand_block(const Problem &p, const Expand &o, unsigned block, T *lds)
 {
+  const Rows &u = o.u;
+  const int64_t C = o.C;
+  const T *__restrict__ f = static_cast<const T *>(o.f);
+  const bool scaled = o.scaled;
+  const T *base = static_cast<const T *>(o.base);
+  T *out = static_cast<T *>(o.out);
+  float *__restrict__ hidden = o.hidden;
   constexpr bool kHalf = RS == 0;
   constexpr int S = RS == 0 ? 1 : RS;
   constexpr bool kPieces = kHalf && sizeof(T) == 2;    // both pieces in one step
   constexpr int kStageRows = kPieces ? 16 : 32;
   constexpr int kPitch = kExpandCols + 8;
-  __shared__ __align__(32) T lds[kDown ? kExpandWaves * kStageRows * kPitch : 1];
+  constexpr bool kTurns = G == 1;                      // of the tiles' adapters, where few waves run
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
-  const int64_t tile = static_cast<int64_t>(blockIdx.x) / col_tiles;
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) - tile * col_tiles) * (kExpandCols * G);
-  const int64_t m = (tile * kExpandWaves + wave) * 16 + i;
+  const unsigned turn = kTurns ? block % o.turns : 0, place = kTurns ? block / o.turns : block;
+  const unsigned tile = place / static_cast<unsigned>(o.col_tiles);
+  const int64_t first = static_cast<int64_t>(place - tile * static_cast<unsigned>(o.col_tiles)) * (kExpandCols * G);
+  const int64_t m = (static_cast<int64_t>(tile) * kExpandWaves + wave) * 16 + i;
   if (m - i >= p.M) return;
   const bool in = m < p.M;
   // a tile that is whole in every direction asks for all of its base at once
@@ -614,9 +632,8 @@ __global__ __launch_bounds__(64 * kExpandWaves) void expand_kernel(Problem p, Ro
 #pragma unroll
       for (int h = 0; h < 2; ++h) early[g][h] = base ? load8<T>(base + m * C + first + kExpandCols * g + 32 * h + 8 * q) : zero8<vec8<T>>();
   };
-  constexpr bool kTurns = G == 1;                      // of the tiles' adapters, where few waves run
   if (whole_tile && !kTurns) ask();
-  TileIds<16> ids(p, m - i, kTurns ? blockIdx.y : 0, kTurns ? gridDim.y : 1);
+  TileIds<16> ids(p, m - i, turn, kTurns ? o.turns : 1);
   if (__ballot(ids.owned) == 0) return;
   if (whole_tile && kTurns && ids.owned) ask();
   const int qj = kPieces ? q & 1 : q;                  // which eight ranks of a step
@@ -752,6 +769,11 @@ __global__ __launch_bounds__(64 * kExpandWaves) void expand_kernel(Problem p, Ro
     for (int g = 0; g < G; ++g)
       if (first + g * kExpandCols < C) group(first + g * kExpandCols, early[g], std::false_type{});
   }
+}
+
+template <typename T, int RS, int G> __global__ __launch_bounds__(64 * kExpandWaves) void expand_kernel(Problem p, Expand o)
+{
+  expand_block<T, RS, false, G>(p, o, blockIdx.x, nullptr);
 }
 
 // ------------------------------------------------------------------ one row, both products
@@ -937,23 +959,31 @@ struct Outer {
 // they are read once.  The pitches leave the four rows of a transposing read in different banks.
 // kRanksDown: of a product's results a lane holds four ranks of one column (grad_a, whose columns are neighbours), else four columns of
 // one rank (grad_b, whose ranks are).
+constexpr int kOuterList = 1024;                      // rows of a slot at most
+constexpr int kZPitch = kOuterCols + 16;
+constexpr int u_pitch(int R) { return R + (R == 64 ? 8 : R == 128 ? 16 : 0); }
+template <typename T, int JT> constexpr int outer_lds()
+{
+  return kOuterRows * kZPitch * static_cast<int>(sizeof(T)) + 4 * kOuterRows * u_pitch(16 * JT) + 4 * kOuterList;
+}
 template <typename Z, typename T, int JT, bool kRanksDown>
-__global__ __launch_bounds__(kOuterThreads) void outer_kernel(Problem p, Outer o)
+__device__ __forceinline__ void outer_block(const Problem &p, const Outer &o, unsigned block, unsigned char *lds)
 {
   typedef typename Staged<Z, T>::type S;
   constexpr bool k16 = sizeof(T) == 2;
   typedef typename std::conditional<k16, bf16_t, float>::type UT;
   constexpr int R = 16 * JT, kOf = R / 4;              // values of u of a thread
-  constexpr int kZPitch = kOuterCols + 16, kUPitch = R + (R == 64 ? 8 : R == 128 ? 16 : 0);
-  __shared__ __align__(32) S zs[kOuterRows * kZPitch];
-  __shared__ __align__(32) UT us[k16 ? 2 : 1][kOuterRows * kUPitch];
-  __shared__ int32_t list[1024];
+  constexpr int kUPitch = u_pitch(R);
+  static_assert(sizeof(S) == sizeof(T));
+  S *zs = reinterpret_cast<S *>(lds);
+  UT *us = reinterpret_cast<UT *>(lds + kOuterRows * kZPitch * sizeof(S));             // two of them in 16 bits, one behind the other
+  int32_t *list = reinterpret_cast<int32_t *>(lds + kOuterRows * kZPitch * sizeof(S) + 4 * kOuterRows * kUPitch);
   const int64_t tiles = (o.C + kOuterCols - 1) / kOuterCols;
-  const int64_t at = blockIdx.x / tiles;
+  const int64_t at = block / static_cast<unsigned>(tiles);
   if (at >= o.cut.header[0]) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, q = lane >> 4;
   const Slot slot = o.cut.slots[at];
-  const int64_t c0 = (blockIdx.x - at * tiles) * kOuterCols;
+  const int64_t c0 = (block - at * tiles) * kOuterCols;
   for (int k = tid; k < slot.count; k += kOuterThreads) list[k] = o.rows[slot.first + k];
   const int64_t groups = (o.C + CAIFX_CHECKPOINT_GROUP - 1) / CAIFX_CHECKPOINT_GROUP, group = c0 / CAIFX_CHECKPOINT_GROUP;
   const float scale = o.scaled && slot.count > 0 ? p.scaling[slot.adapter] : 1.0f;
@@ -1015,10 +1045,10 @@ __global__ __launch_bounds__(kOuterThreads) void outer_kernel(Problem p, Outer o
         hi[k] = from_f32<bf16_t>(uv[k]);
         lo[k] = from_f32<bf16_t>(uv[k] - to_f32<bf16_t>(hi[k]));
       }
-      __builtin_memcpy(__builtin_assume_aligned(us[0] + urow * kUPitch + ucol, 8), hi, sizeof hi);
-      __builtin_memcpy(__builtin_assume_aligned(us[1] + urow * kUPitch + ucol, 8), lo, sizeof lo);
+      __builtin_memcpy(__builtin_assume_aligned(us + urow * kUPitch + ucol, 8), hi, sizeof hi);
+      __builtin_memcpy(__builtin_assume_aligned(us + (kOuterRows + urow) * kUPitch + ucol, 8), lo, sizeof lo);
     } else {
-      __builtin_memcpy(__builtin_assume_aligned(us[0] + urow * kUPitch + ucol, 16), uv, sizeof uv);
+      __builtin_memcpy(__builtin_assume_aligned(us + urow * kUPitch + ucol, 16), uv, sizeof uv);
     }
     __syncthreads();
     if (s + 1 < steps) fetch(s + 1);
@@ -1027,7 +1057,7 @@ __global__ __launch_bounds__(kOuterThreads) void outer_kernel(Problem p, Outer o
       typename Fine<T>::type uf[JT];
 #pragma unroll
       for (int j = 0; j < JT; ++j) {
-        const UT *from = us[0] + 32 * h * kUPitch + 16 * j;
+        const UT *from = us + 32 * h * kUPitch + 16 * j;
         if constexpr (k16) {
           uf[j].hi = down<UT>(from, kUPitch, 4, lane, q);
           uf[j].lo = down<UT>(from + kOuterRows * kUPitch, kUPitch, 4, lane, q);
@@ -1058,6 +1088,20 @@ __global__ __launch_bounds__(kOuterThreads) void outer_kernel(Problem p, Outer o
         if (slot.part >= 0) o.part[slot.part * size + to] = v;
         else static_cast<T *>(o.grad)[slot.adapter * size + to] = from_f32<T>(v);
       }
+}
+
+// What of the backward needs g or the sorted rows, in one launch: blocks of grad_b, of grad_a, of dx.  Each of the three alone leaves the
+// chip half empty at its beginning and its end, and a launch of its own costs the small calls 3 us.
+template <typename T, typename Z, int JT, int G>
+__global__ __launch_bounds__(kOuterThreads) void gradients_kernel(Problem p, Outer b, unsigned blocks_b, Outer a, unsigned blocks_a, Expand dx)
+{
+  static_assert(kOuterThreads == 64 * kExpandWaves);
+  constexpr int RS = JT / 2;
+  constexpr int kLds = outer_lds<T, JT>() > expand_lds<T, RS>() ? outer_lds<T, JT>() : expand_lds<T, RS>();
+  __shared__ __align__(32) unsigned char lds[kLds];
+  if (blockIdx.x < blocks_b) outer_block<T, T, JT, false>(p, b, blockIdx.x, lds);
+  else if (blockIdx.x < blocks_b + blocks_a) outer_block<Z, T, JT, true>(p, a, blockIdx.x - blocks_b, lds);
+  else expand_block<T, RS, true, G>(p, dx, blockIdx.x - blocks_b - blocks_a, reinterpret_cast<T *>(lds));
 }
 
 // the slots of an adapter that has several, added in order
@@ -1216,28 +1260,15 @@ void shrink(const Problem &p, const Slices &sl, const void *z, int64_t C, const 
   else hipLaunchKernelGGL((shrink_kernel<T, 8, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out, sort);
 }
 
-template <typename T, bool kDown, int G>
-void expand(const Problem &p, const Rows &u, int64_t C, const void *f, bool scaled, const void *base, void *out, float *hidden, hipStream_t s)
+// columns of a wave of the expanding product: 64 while there are few waves, else 256
+bool few_waves(int64_t M, int64_t C) { return ceil_div(M, 16) * ceil_div(C, kExpandCols) < 16384; }
+Expand plan_expand(const Problem &p, const Rows &u, int64_t C, const void *f, bool scaled, const void *base, void *out, float *hidden, unsigned &blocks)
 {
-  const int64_t tiles = ceil_div(C, kExpandCols * G);
-  const dim3 grid(static_cast<unsigned>(ceil_div(p.M, 16 * kExpandWaves) * tiles), G == 1 ? turns(p, tiles) : 1), block(64 * kExpandWaves);
-  const T *ff = static_cast<const T *>(f), *bb = static_cast<const T *>(base);
-  T *oo = static_cast<T *>(out);
-  if (p.r <= 16) hipLaunchKernelGGL((expand_kernel<T, 0, kDown, G>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
-  else if (p.r <= 32) hipLaunchKernelGGL((expand_kernel<T, 1, kDown, G>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
-  else if (p.r <= 64) hipLaunchKernelGGL((expand_kernel<T, 2, kDown, G>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
-  else hipLaunchKernelGGL((expand_kernel<T, 4, kDown, G>), grid, block, 0, s, p, u, C, tiles, ff, scaled, bb, oo, hidden);
-}
-
-// columns of a wave: 64 while there are few waves
-template <typename T, bool kDown>
-void expand(const Problem &p, const Rows &u, int64_t C, const void *f, bool scaled, const void *base, void *out, float *hidden, hipStream_t s)
-{
-#ifndef EG
-#define EG 4
-#endif
-  if (ceil_div(p.M, 16) * ceil_div(C, kExpandCols) < 16384) expand<T, kDown, 1>(p, u, C, f, scaled, base, out, hidden, s);
-  else expand<T, kDown, EG>(p, u, C, f, scaled, base, out, hidden, s);
+  const bool few = few_waves(p.M, C);
+  const int64_t tiles = ceil_div(C, kExpandCols * (few ? 1 : 4));
+  const Expand o{u, C, tiles, f, scaled, base, out, hidden, few ? turns(p, tiles) : 1};
+  blocks = static_cast<unsigned>(ceil_div(p.M, 16 * kExpandWaves) * tiles * o.turns);
+  return o;
 }
 
 template <typename T> int forward(const Problem &p, const void *x, const void *base, void *y, float *hidden, void *workspace, hipStream_t s)
@@ -1260,17 +1291,43 @@ template <typename T> int forward(const Problem &p, const void *x, const void *b
   float *h = static_cast<float *>(workspace);
   if (hidden && w.slices.count == 1) h = hidden, hidden = nullptr;
   shrink<T, false>(p, w.slices, x, p.K, p.a, false, h, Sort{}, s);
-  expand<T, false>(p, Rows{h, w.slices.count}, p.N, p.b, true, base, y, hidden, s);
+  unsigned blocks;
+  const Expand o = plan_expand(p, Rows{h, w.slices.count}, p.N, p.b, true, base, y, hidden, blocks);
+  const dim3 grid(blocks), block(64 * kExpandWaves);
+#define CAIFX_GO(RS)                                                                                           \
+  if (few_waves(p.M, p.N)) hipLaunchKernelGGL((expand_kernel<T, RS, 1>), grid, block, 0, s, p, o);             \
+  else hipLaunchKernelGGL((expand_kernel<T, RS, 4>), grid, block, 0, s, p, o)
+  if (p.r <= 16) {
+    CAIFX_GO(0);
+  } else if (p.r <= 32) {
+    CAIFX_GO(1);
+  } else if (p.r <= 64) {
+    CAIFX_GO(2);
+  } else {
+    CAIFX_GO(4);
+  }
+#undef CAIFX_GO
   return launch_status();
 }
 
-template <typename Z, typename T, bool kRanksDown> void outer(const Problem &p, const Outer &o, int64_t slots, hipStream_t s)
+template <typename T, typename Z>
+void gradients(const Problem &p, const Outer &b, unsigned blocks_b, const Outer &a, unsigned blocks_a, const Expand &dx, unsigned blocks_x, hipStream_t s)
 {
-  const dim3 grid(static_cast<unsigned>(ceil_div(o.C, kOuterCols) * slots)), block(kOuterThreads);
-  if (p.r <= 16) hipLaunchKernelGGL((outer_kernel<Z, T, 1, kRanksDown>), grid, block, 0, s, p, o);
-  else if (p.r <= 32) hipLaunchKernelGGL((outer_kernel<Z, T, 2, kRanksDown>), grid, block, 0, s, p, o);
-  else if (p.r <= 64) hipLaunchKernelGGL((outer_kernel<Z, T, 4, kRanksDown>), grid, block, 0, s, p, o);
-  else hipLaunchKernelGGL((outer_kernel<Z, T, 8, kRanksDown>), grid, block, 0, s, p, o);
+  const dim3 grid(blocks_b + blocks_a + blocks_x), block(kOuterThreads);
+  if (grid.x == 0) return;
+#define CAIFX_GO(JT)                                                                                                                             \
+  if (few_waves(p.M, p.K)) hipLaunchKernelGGL((gradients_kernel<T, Z, JT, 1>), grid, block, 0, s, p, b, blocks_b, a, blocks_a, dx);              \
+  else hipLaunchKernelGGL((gradients_kernel<T, Z, JT, 4>), grid, block, 0, s, p, b, blocks_b, a, blocks_a, dx)
+  if (p.r <= 16) {
+    CAIFX_GO(1);
+  } else if (p.r <= 32) {
+    CAIFX_GO(2);
+  } else if (p.r <= 64) {
+    CAIFX_GO(4);
+  } else {
+    CAIFX_GO(8);
+  }
+#undef CAIFX_GO
 }
 
 template <typename T>
@@ -1306,13 +1363,15 @@ int backward(const Problem &p, const void *dy, const void *x, const float *x_sca
   }
   const Rows rows{g, w.slices.count};
   shrink<T, true>(p, w.slices, dy, p.N, p.b, true, g, ga || gb ? sort : Sort{}, s);
-  if (dx) expand<T, true>(p, rows, p.K, p.a, false, base, dx, nullptr, s);
-  if (gb) outer<T, T, false>(p, Outer{dy, nullptr, Rows{hidden, 1}, p.N, true, 1, p.r, gb, part[1], sort.rows, sort.b}, w.b.slots, s);
-  if (ga) {
-    const Outer o{x, x_scales, rows, p.K, false, p.K, 1, ga, part[0], sort.rows, sort.a};
-    if (x_scales) outer<int8_t, T, true>(p, o, w.a.slots, s);
-    else outer<T, T, true>(p, o, w.a.slots, s);
-  }
+  unsigned blocks_b = 0, blocks_a = 0, blocks_x = 0;
+  const Outer ob{dy, nullptr, Rows{hidden, 1}, p.N, true, 1, p.r, gb, part[1], sort.rows, sort.b};
+  const Outer oa{x, x_scales, rows, p.K, false, p.K, 1, ga, part[0], sort.rows, sort.a};
+  if (gb) blocks_b = static_cast<unsigned>(ceil_div(p.N, kOuterCols) * w.b.slots);
+  if (ga) blocks_a = static_cast<unsigned>(ceil_div(p.K, kOuterCols) * w.a.slots);
+  Expand ox{};
+  if (dx) ox = plan_expand(p, rows, p.K, p.a, false, base, dx, nullptr, blocks_x);
+  if (x_scales) gradients<T, int8_t>(p, ob, blocks_b, oa, blocks_a, ox, blocks_x, s);
+  else gradients<T, T>(p, ob, blocks_b, oa, blocks_a, ox, blocks_x, s);
   const int64_t multi_a = ga ? w.a.multi : 0, multi_b = gb ? w.b.multi : 0, multi = multi_a > multi_b ? multi_a : multi_b;
   if (multi > 0) {
     const unsigned blocks_a = multi_a > 0 ? static_cast<unsigned>(ceil_div(size_a, 256 * kJoinPer)) : 0;
@@ -1327,8 +1386,8 @@ int check(int64_t M, int64_t N, int64_t K, int rank, int num_adapters, int dtype
 {
   if (!valid_dtype(dtype) || M < 0 || N <= 0 || K <= 0 || rank <= 0 || num_adapters <= 0) return CAIFX_ERR_INVALID_ARGUMENT;
   if (rank > CAIFX_ADAPTER_RANK_MAX || M > (int64_t{1} << 23) || N > (int64_t{1} << 26) || K > (int64_t{1} << 26)) return CAIFX_ERR_UNSUPPORTED;
-  // a grid has fewer than 2^32 threads
-  constexpr int64_t kBlocks = (int64_t{1} << 24) - 1;
+  // a grid has fewer than 2^32 threads; a launch holds three kinds of blocks
+  constexpr int64_t kBlocks = int64_t{1} << 22;
   for (const int64_t C : {N, K}) {
     if (ceil_div(M, 16 * kExpandWaves) > kBlocks / ceil_div(C, kExpandCols)) return CAIFX_ERR_UNSUPPORTED;
     if (M / plan_chunk(M, C) + num_adapters > kBlocks / ceil_div(C, kOuterCols)) return CAIFX_ERR_UNSUPPORTED;
