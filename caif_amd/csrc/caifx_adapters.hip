@@ -6,17 +6,22 @@
 //              dA[l] = T(sum over m of l of g[m]^T x[m])      dB[l] = T(sum over m of l of scaling[l] dy[m]^T h[m])
 //
 // with x [M,K], A [L,r,K], B [L,N,r], h and g [M,r] in fp32.  A rank of 16 leaves 16 multiply-adds for a value read or written,
-// so all of it is bound by memory: x, dy, base and the result pass once, the factors come from the caches, and the matrix cores
+// so all of it is bound by memory: x, dy (twice), base and the results pass, the factors come from the caches, and the matrix cores
 // keep the arithmetic out of the way.  Four kinds of product:
 //
-//   shrink   rows x factor over the long axis (h, g): a workgroup takes 16 rows, its waves share the axis
-//   expand   rank -> long axis (y, dx): a wave takes 16 rows x 64 columns, adds base and rounds once
-//   outer    sums over the rows of an adapter (dA, dB): a workgroup takes 128 columns of one adapter and lists its rows first
+//   shrink   rows x factor over the long axis (h, g): a workgroup takes 16 or 32 rows, its waves share the axis
+//   expand   rank -> long axis (y, dx): a wave takes 16 rows x 256 columns (64 in small calls), adds base and rounds once
+//   outer    sums over the rows of an adapter (dA, dB): a workgroup takes 128 columns and a run of the adapter's rows
 //   row      shrink and expand of one row in one launch, for decode steps
 //
+// The forward is row, or shrink and expand; the backward is shrink (with a workgroup that sorts the rows by adapter beside it), outer and
+// expand in one launch, and the sum of an adapter's runs where it has several.  Measured on one MI355X against the copy of as many bytes (in
+// three buffers in turn, 5.0 TB/s): y of 4096 x 11008 in bf16 45 us of 35, h of 4096 x 4096 12 of 8, g of 4096 x 11008 25 of 18 (rank 64:
+// 51, where the factor's reads count), both gradients and dx of the two together 47 of 42.
+//
 // Precision: products of two 16-bit values are exact in fp32 and summed in fp32.  h and g stay fp32; on the 16-bit matrix cores they
-// are two bf16 pieces that add up to them but for 2^-17 (and an fp16 partner two bf16 pieces that add up to it exactly, so no value
-// leaves the range of a piece), which is far below the one rounding of the result.  fp32 tensors use the fp32 instruction.
+// are two pieces that add up to them but for 2^-17 or less, which is far below the one rounding of the result.  fp32 tensors use the
+// fp32 instruction.
 //
 // Rows of different adapters never meet in a product: a tile with several adapters is multiplied by each of them and every row
 // keeps the result of its own, so that an infinity in one adapter's factors stays out of the other rows.
@@ -321,9 +326,6 @@ __device__ __forceinline__ void sort_rows(const Problem &p, const Sort &o, int32
 // ------------------------------------------------------------------ shrink
 constexpr int kShrinkWaves = 8;
 
-#ifndef TT1
-#define TT1 2
-#endif
 // Columns that a wave asks for at a time (as much as its registers hold, so that a memory round trip is paid for few times), and tiles of
 // 16 rows of a workgroup.
 template <typename T, int JT, bool kDown> struct ShrinkUnit {
@@ -331,7 +333,7 @@ template <typename T, int JT, bool kDown> struct ShrinkUnit {
   static constexpr int kSteps = kDown ? (kBytes >= 16 ? 1 : 2) : (kBytes >= 32 ? 1 : kBytes >= 8 ? 2 : 4);
   static constexpr int kCols = 32 * kSteps;
   // kDown stages the factor once for all rows of a workgroup
-  static constexpr int kTiles = !kDown || kBytes >= 32 ? 1 : kBytes == 2 ? TT1 : 2;
+  static constexpr int kTiles = !kDown || kBytes >= 32 ? 1 : 2;
 };
 
 // out[slice][m][j] = scale sum over the slice's columns c of z[m][c] f[l][j][c] (kDown: f[l][c][j]), rows without adapter zero.
@@ -1162,7 +1164,7 @@ size_t up16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
 int shrink_rows(int rank, size_t es)
 {
   const int bytes = up_to(rank) / 16 * static_cast<int>(es);
-  return bytes >= 32 ? 16 : bytes == 2 ? 16 * TT1 : 32;
+  return bytes >= 32 ? 16 : 32;
 }
 
 struct Slices {
@@ -1201,7 +1203,7 @@ bool row_at_a_time(int64_t M, int64_t N, int64_t K, int rank, size_t es)
 }
 
 // Workgroups that share the adapters of a tile of 16 rows, `waves` waves working on it otherwise: as many as leave some 4096 in
-// all (999 rows in runs, 4096 to 4096, turns of four: 23.5 us, without turns XX).
+// all (999 rows in runs, 4096 to 4096, turns of four: 23.5 us, without turns 18.8).
 unsigned turns(const Problem &p, int64_t waves)
 {
   const int64_t most = p.L < 16 ? p.L : 16, n = 4096 / (ceil_div(p.M, 16) * waves);

@@ -319,3 +319,57 @@ def test_a_block_with_adapters_and_checkpoints(orc, tokens):
         R.check(g, *want[name], BF16, R.sums(dim, max(tokens, r)) + R.pieces(BF16), name)
     want, mag = R.forward(hidden, ids, *fac[2], scaling, T.qlinear_forward(hidden, base[2], T.BF16, T.BF16))[:2]
     R.check(y, want, mag, BF16, R.sums(wide, r) + R.pieces(BF16), "y")
+
+
+def call_backward(p, more, adapters, dx, ga, gb, base):
+    """caifx_adapters_backward with any of its results, null for None."""
+    at = lambda t: None if t is None else t.data_ptr()                                                    # noqa: E731
+    (m, k), n, r = p["x"].shape, p["b"].shape[1], p["a"].shape[1]
+    code = T.CODE_OF[p["x"].dtype]
+    need = capi.lib().caifx_adapters_workspace_bytes(m, n, k, r, adapters, code, 1)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    capi.call("caifx_adapters_backward", m, n, k, r, adapters, at(more["dy"]), at(p["x"]) if ga is not None else None, None,
+              at(more["hidden"]) if gb is not None else None, at(p["ids"]), at(p["a"]) if dx is not None else None, at(p["b"]), at(p["scaling"]),
+              at(base), at(dx), at(ga), at(gb), code, at(ws), need, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("m", [30, 700])
+def test_each_result_alone_and_dx_into_its_base(m):
+    p, more = problem(m, 264, 392, 16, 3, BF16, "runs")
+    want = T.adapters_backward(more["dy"], p["x"], more["hidden"], **{key: p[key] for key in ("ids", "a", "b", "scaling")}, base=more["dbase"])
+    for i in range(3):
+        out = [None, None, None]
+        out[i] = torch.full_like(want[i], float("nan"))
+        call_backward(p, more, 3, *out, more["dbase"])
+        assert torch.equal(out[i], want[i])
+    into = more["dbase"].clone()
+    call_backward(p, more, 3, into, None, None, into)
+    assert torch.equal(into, want[0])
+
+
+@pytest.mark.parametrize("adapters", [700, 5000])
+def test_more_adapters_than_rows(adapters):
+    """Counters of the sorting workgroup for fewer waves than it has, and beyond its local memory."""
+    p, more = problem(300, 72, 40, 8, adapters, BF16, "mixed")
+    y, hidden = T.adapters_forward(**p, base=more["base"], keep_hidden=True)
+    want, mag = R.forward(**p, base=more["base"])[:2]
+    R.check(y, want, mag, BF16, R.sums(72, 8) + R.pieces(BF16), "y")
+    x = p.pop("x")
+    got = T.adapters_backward(more["dy"], x, more["hidden"], **p, base=more["dbase"])
+    want = R.backward(more["dy"], x, more["hidden"], **p, base=more["dbase"])
+    for name, g in zip(("dx", "grad_a", "grad_b"), got):
+        R.check(g, *want[name], BF16, R.sums(40, 300) + R.pieces(BF16), name)
+
+
+def test_one_adapter_of_many_rows_in_any_order():
+    """Several runs of one adapter's rows, the rows of the others between them, through every kernel of the large calls."""
+    p, more = problem(4500, 520, 4100, 16, 2, BF16, "mixed")
+    y = T.adapters_forward(**p, base=more["base"])
+    want, mag = R.forward(**p, base=more["base"])[:2]
+    R.check(y, want, mag, BF16, R.sums(520, 16) + R.pieces(BF16), "y")
+    x = p.pop("x")
+    got = T.adapters_backward(more["dy"], x, more["hidden"], **p, base=more["dbase"])
+    want = R.backward(more["dy"], x, more["hidden"], **p, base=more["dbase"])
+    for name, g in zip(("dx", "grad_a", "grad_b"), got):
+        R.check(g, *want[name], BF16, R.sums(4100, 4500) + R.pieces(BF16), name)
