@@ -110,7 +110,8 @@ template <typename T> __device__ __forceinline__ uint32_t group_top(const Eight<
 
 // Codes of a lane's eight values, and the group's scale.  The quotient is rounded as a division rounds it without being one: with the
 // rounded inverse y of the scale, q = x y is at most 1.5 steps off, q + (x - q s) y within a step, and the same once more is the rounded
-// quotient (Markstein: a quotient within a step, corrected by its exact remainder times the rounded inverse).  Adding 1.5 2^23 rounds it to
+// quotient (Markstein: a quotient within a step, corrected by its exact remainder times the rounded inverse).  For 16-bit values one
+// correction gives the same codes: all pairs of a maximum's and a value's 11 bits were compared.  Adding 1.5 2^23 rounds the quotient to
 // an integer, ties to even, and leaves the integer in the low byte.  Scales below 2^-100, where the remainders would underflow, divide.
 template <typename T> __device__ __forceinline__ Eight<int8_t> quantise(const Eight<T> &x, float &scale)
 {
@@ -132,7 +133,7 @@ template <typename T> __device__ __forceinline__ Eight<int8_t> quantise(const Ei
       const float v = to_f32<T>(x.v[i]);
       float q = v * y;
       q = __builtin_fmaf(__builtin_fmaf(-q, scale, v), y, q);
-      q = __builtin_fmaf(__builtin_fmaf(-q, scale, v), y, q);
+      if constexpr (sizeof(T) == 4) q = __builtin_fmaf(__builtin_fmaf(-q, scale, v), y, q);
       bits[i] = __builtin_bit_cast(uint32_t, q + 12582912.0f);
     }
   }

@@ -85,6 +85,23 @@ def test_every_quotient_near_a_tie():
     assert np.array_equal(scales.cpu().numpy(), want_scales) and np.array_equal(codes.cpu().numpy(), want)
 
 
+def test_every_pair_of_a_maximum_and_a_value_in_16_bits():
+    """The quotient of two numbers of 11 bits, scaled by powers of two: all of them, the value up to 2^9 times smaller than the maximum
+    (below that its code is zero)."""
+    top = torch.arange(1024, 2048, device="cuda")
+    value = torch.arange(1024, 2048, device="cuda")
+    for shift in range(10):
+        v = (value.float() * 2.0 ** -shift).expand(1024, -1)
+        keep = torch.where(v <= top[:, None].float(), v, torch.zeros((), device="cuda"))
+        x = torch.cat([top.float()[:, None].expand(-1, 8).reshape(1024, 8, 1), keep.reshape(1024, 8, 128)[:, :, :127]], 2).reshape(8192, 128)
+        last = torch.cat([top.float()[:, None], keep.reshape(1024, 8, 128)[:, :, 127], torch.zeros(1024, 119, device="cuda")], 1)
+        x = torch.cat([x, last]).to(F16)
+        assert torch.equal(x.float().amax(1)[:8192:8], top.float())
+        codes, scales = T.checkpoint_pack(x)
+        want, want_scales = definition(x)
+        assert np.array_equal(scales.cpu().numpy(), want_scales) and np.array_equal(codes.cpu().numpy(), want)
+
+
 def test_more_dimensions_and_no_elements():
     x = torch.randn(3, 5, 200, device="cuda")
     codes, scales = T.checkpoint_pack(x)
