@@ -326,11 +326,12 @@ __device__ __forceinline__ void sort_rows(const Problem &p, const Sort &o, int32
 // ------------------------------------------------------------------ shrink
 constexpr int kShrinkWaves = 8;
 
+constexpr int shrink_steps(int bytes, bool down) { return down ? (bytes >= 16 ? 1 : 2) : (bytes >= 32 ? 1 : bytes >= 8 ? 2 : 4); }
 // Columns that a wave asks for at a time (as much as its registers hold, so that a memory round trip is paid for few times), and tiles of
 // 16 rows of a workgroup.
 template <typename T, int JT, bool kDown> struct ShrinkUnit {
   static constexpr int kBytes = JT * static_cast<int>(sizeof(T));       // 2 .. 32: registers of the factor grow with it
-  static constexpr int kSteps = kDown ? (kBytes >= 16 ? 1 : 2) : (kBytes >= 32 ? 1 : kBytes >= 8 ? 2 : 4);
+  static constexpr int kSteps = shrink_steps(kBytes, kDown);
   static constexpr int kCols = 32 * kSteps;
   // kDown stages the factor once for all rows of a workgroup
   static constexpr int kTiles = !kDown || kBytes >= 32 ? 1 : 2;
@@ -599,7 +600,8 @@ struct Expand {
   const void *base;                                   // T, null for zero
   void *out;                                          // T, may be base
   float *hidden;                                      // null: not wanted
-  unsigned turns;                                     // workgroups of a tile
+  unsigned turns, places;                             // workgroups of a tile, tiles: all tiles' first workgroups come first, so
+                                                      // that those with work (often the first alone) spread over the XCDs
 };
 template <typename T, int RS> constexpr int expand_lds() { return kExpandWaves * (RS == 0 && sizeof(T) == 2 ? 16 : 32) * (kExpandCols + 8) * static_cast<int>(sizeof(T)); }
 template <typename T, int RS, bool kDown, int G>
@@ -619,7 +621,7 @@ __device__ __forceinline__ void expand_block(const Problem &p, const Expand &o, 
   constexpr int kPitch = kExpandCols + 8;
   constexpr bool kTurns = G == 1;                      // of the tiles' adapters, where few waves run
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
-  const unsigned turn = kTurns ? block % o.turns : 0, place = kTurns ? block / o.turns : block;
+  const unsigned turn = kTurns ? block / o.places : 0, place = kTurns ? block - turn * o.places : block;
   const unsigned tile = place / static_cast<unsigned>(o.col_tiles);
   const int64_t first = static_cast<int64_t>(place - tile * static_cast<unsigned>(o.col_tiles)) * (kExpandCols * G);
   const int64_t m = (static_cast<int64_t>(tile) * kExpandWaves + wave) * 16 + i;
@@ -1167,18 +1169,24 @@ int shrink_rows(int rank, size_t es)
   return bytes >= 32 ? 16 : 32;
 }
 
+// columns of a unit
+int shrink_unit(int rank, size_t es, bool down)
+{
+  const int bytes = up_to(rank) / 16 * static_cast<int>(es);
+  return 32 * shrink_steps(bytes, down);
+}
+
 struct Slices {
   int count;
   int64_t columns;
 };
-Slices plan_slices(int64_t M, int64_t C, int rows)
+Slices plan_slices(int64_t M, int64_t C, int rows, int unit)
 {
-  constexpr int kUnit = 64;
-  const int64_t tiles = ceil_div(M, rows), whole = ceil_div(C, kShrinkWaves * kUnit);
+  const int64_t tiles = ceil_div(M, rows), whole = ceil_div(C, kShrinkWaves * unit);
   int64_t n = 512 / (tiles > 0 ? tiles : 1);
   n = n < 1 ? 1 : (n > 16 ? 16 : n);
   if (n > whole) n = whole;
-  const int64_t columns = ceil_div(whole, n) * kShrinkWaves * kUnit;
+  const int64_t columns = ceil_div(whole, n) * kShrinkWaves * unit;
   return {static_cast<int>(ceil_div(C, columns)), columns};
 }
 
@@ -1236,7 +1244,7 @@ struct Plan {
 Plan plan(int64_t M, int64_t N, int64_t K, int rank, int L, size_t es, bool backward)
 {
   Plan w{};
-  w.slices = plan_slices(M, backward ? N : K, backward ? shrink_rows(rank, es) : 16);
+  w.slices = plan_slices(M, backward ? N : K, backward ? shrink_rows(rank, es) : 16, shrink_unit(rank, es, backward));
   w.rows = up16(static_cast<size_t>(w.slices.count) * M * rank * 4);
   if (!backward && row_at_a_time(M, N, K, rank, es)) w.rows = 0;
   if (backward) {
@@ -1268,8 +1276,8 @@ Expand plan_expand(const Problem &p, const Rows &u, int64_t C, const void *f, bo
 {
   const bool few = few_waves(p.M, C);
   const int64_t tiles = ceil_div(C, kExpandCols * (few ? 1 : 4));
-  const Expand o{u, C, tiles, f, scaled, base, out, hidden, few ? turns(p, tiles) : 1};
-  blocks = static_cast<unsigned>(ceil_div(p.M, 16 * kExpandWaves) * tiles * o.turns);
+  const Expand o{u, C, tiles, f, scaled, base, out, hidden, few ? turns(p, tiles) : 1, static_cast<unsigned>(ceil_div(p.M, 16 * kExpandWaves) * tiles)};
+  blocks = o.places * o.turns;
   return o;
 }
 
