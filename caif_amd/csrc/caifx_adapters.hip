@@ -1162,7 +1162,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int up_to(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }      // the ranks that a kernel computes
 size_t up16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
 
-// Workgroups of the shrinking product per `rows` rows: enough that some 512 run, a slice no shorter than one unit for each wave.
+// rows of a workgroup of the backward's shrinking product
 int shrink_rows(int rank, size_t es)
 {
   const int bytes = up_to(rank) / 16 * static_cast<int>(es);
@@ -1176,14 +1176,17 @@ int shrink_unit(int rank, size_t es, bool down)
   return 32 * shrink_steps(bytes, down);
 }
 
+// Workgroups of the shrinking product per `rows` rows: enough that some 512 run, a slice no shorter than one unit for each wave.  Above rank 32
+// some 256: every slice is read again by all consumers of the rows (four adapters of rank 64, 4096 rows: 62 + 50 us for the consumers and
+// the product, 71 + 51 with twice as many slices; forward of 999 rows to 4096 29.5 and 36.0).
 struct Slices {
   int count;
   int64_t columns;
 };
-Slices plan_slices(int64_t M, int64_t C, int rows, int unit)
+Slices plan_slices(int64_t M, int64_t C, int rank, int rows, int unit)
 {
   const int64_t tiles = ceil_div(M, rows), whole = ceil_div(C, kShrinkWaves * unit);
-  int64_t n = 512 / (tiles > 0 ? tiles : 1);
+  int64_t n = (rank > 32 ? 256 : 512) / (tiles > 0 ? tiles : 1);
   n = n < 1 ? 1 : (n > 16 ? 16 : n);
   if (n > whole) n = whole;
   const int64_t columns = ceil_div(whole, n) * kShrinkWaves * unit;
@@ -1244,7 +1247,7 @@ struct Plan {
 Plan plan(int64_t M, int64_t N, int64_t K, int rank, int L, size_t es, bool backward)
 {
   Plan w{};
-  w.slices = plan_slices(M, backward ? N : K, backward ? shrink_rows(rank, es) : 16, shrink_unit(rank, es, backward));
+  w.slices = plan_slices(M, backward ? N : K, rank, backward ? shrink_rows(rank, es) : 16, shrink_unit(rank, es, backward));
   w.rows = up16(static_cast<size_t>(w.slices.count) * M * rank * 4);
   if (!backward && row_at_a_time(M, N, K, rank, es)) w.rows = 0;
   if (backward) {
@@ -1270,8 +1273,9 @@ void shrink(const Problem &p, const Slices &sl, const void *z, int64_t C, const 
   else hipLaunchKernelGGL((shrink_kernel<T, 8, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out, sort);
 }
 
-// columns of a wave of the expanding product: 64 while there are few waves, else 256
-bool few_waves(int64_t M, int64_t C) { return ceil_div(M, 16) * ceil_div(C, kExpandCols) < 16384; }
+// Columns of a wave of the expanding product: 64 while there are few waves, else 256.  (In runs of 100 rows, to 14336, 64 / 256 columns: 300
+// rows, 4256 waves of 64, rank 16 15.6 / 17.7 us, rank 64 35.0 / 29.4; 600 rows 21.1 / 20.7 and 57.5 / 38.4; 999 rows 28.6 / 25.5 and 84.8 / 56.9.)
+bool few_waves(int64_t M, int64_t C) { return ceil_div(M, 16) * ceil_div(C, kExpandCols) < 8192; }
 Expand plan_expand(const Problem &p, const Rows &u, int64_t C, const void *f, bool scaled, const void *base, void *out, float *hidden, unsigned &blocks)
 {
   const bool few = few_waves(p.M, C);
