@@ -1261,11 +1261,14 @@ Plan plan(int64_t M, int64_t N, int64_t K, int rank, int L, size_t es, bool back
   return w;
 }
 
+// `product` false: the sorting workgroup alone, which reads neither z nor f
 template <typename T, bool kDown>
-void shrink(const Problem &p, const Slices &sl, const void *z, int64_t C, const void *f, bool scaled, float *out, const Sort &sort, hipStream_t s)
+void shrink(const Problem &p, const Slices &sl, const void *z, int64_t C, const void *f, bool scaled, float *out, const Sort &sort, hipStream_t s,
+            bool product = true)
 {
   const int rows = kDown ? shrink_rows(p.r, sizeof(T)) : 16;
-  const dim3 grid(static_cast<unsigned>(ceil_div(p.M, rows) + (sort.rows ? 1 : 0)), sl.count, turns(p, sl.count * kShrinkWaves)), block(64 * kShrinkWaves);
+  const dim3 block(64 * kShrinkWaves),
+      grid = product ? dim3(static_cast<unsigned>(ceil_div(p.M, rows) + (sort.rows ? 1 : 0)), sl.count, turns(p, sl.count * kShrinkWaves)) : dim3(1);
   const T *zz = static_cast<const T *>(z), *ff = static_cast<const T *>(f);
   if (p.r <= 16) hipLaunchKernelGGL((shrink_kernel<T, 1, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out, sort);
   else if (p.r <= 32) hipLaunchKernelGGL((shrink_kernel<T, 2, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out, sort);
@@ -1376,7 +1379,7 @@ int backward(const Problem &p, const void *dy, const void *x, const float *x_sca
     part[k] = reinterpret_cast<float *>(take(side.part_bytes));
   }
   const Rows rows{g, w.slices.count};
-  shrink<T, true>(p, w.slices, dy, p.N, p.b, true, g, ga || gb ? sort : Sort{}, s);
+  shrink<T, true>(p, w.slices, dy, p.N, p.b, true, g, ga || gb ? sort : Sort{}, s, dx || ga);      // b may be null for grad_b alone, which needs no g
   unsigned blocks_b = 0, blocks_a = 0, blocks_x = 0;
   const Outer ob{dy, nullptr, Rows{hidden, 1}, p.N, true, 1, p.r, gb, part[1], sort.rows, sort.b};
   const Outer oa{x, x_scales, rows, p.K, false, p.K, 1, ga, part[0], sort.rows, sort.a};

@@ -490,8 +490,8 @@ CAIFX_API int caifx_adapters_forward(int64_t M, int64_t N, int64_t K, int rank, 
  *   dx[m,:]   = T(base[m,:] + g[m,:] a[l])                      base [M,K], NULL for zero, may be dx itself
  *   grad_a[l] = T(sum over the rows m of l of g[m,:]^T x[m,:])           [num_adapters,rank,K]
  *   grad_b[l] = T(sum over the rows m of l of scaling[l] * dy[m,:]^T hidden[m,:])   [num_adapters,N,rank]
- * An adapter without rows gets zero gradients.  Any of dx, grad_a, grad_b may be NULL; what only they need (x, hidden, a) may then be
- * NULL too.  x_scales != NULL: x holds the int8 codes of caifx_checkpoint_pack and x_scales their scales.
+ * An adapter without rows gets zero gradients.  Any of dx, grad_a, grad_b may be NULL, and so may what only they need: x without
+ * grad_a, hidden without grad_b, a without dx, b where grad_b alone is wanted.  x_scales != NULL: x holds the int8 codes of caifx_checkpoint_pack and x_scales their scales.
  * workspace: caifx_adapters_workspace_bytes(..., backward = 1). */
 CAIFX_API int caifx_adapters_backward(int64_t M, int64_t N, int64_t K, int rank, int num_adapters, const void *dy,
                             const void *x, const float *x_scales, const float *hidden, const int32_t *ids,
