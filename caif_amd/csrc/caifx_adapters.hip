@@ -24,7 +24,8 @@
 // fp32 instruction.
 //
 // Rows of different adapters never meet in a product: a tile with several adapters is multiplied by each of them and every row
-// keeps the result of its own, so that an infinity in one adapter's factors stays out of the other rows.
+// keeps the result of its own, so that an infinity in one adapter's factors stays out of the other rows.  Within a row infinities give what the
+// formulas give.
 #include "caifx_common.hpp"
 
 #include <type_traits>
@@ -516,6 +517,23 @@ template <bool kMany> __device__ __forceinline__ f32x8_t rank8(const Problem &p,
   return v;
 }
 
+// value j of row m, its slices added in rank8's order
+__device__ __forceinline__ float rank1(const Problem &p, const Rows &u, int64_t m, int j)
+{
+  const float *at = u.at + m * p.r + j;
+  const int64_t apart = p.M * p.r;
+  float v = at[0];
+  for (int s = 1; s < u.slices; ++s) v += at[s * apart];
+  return v;
+}
+
+// ------------------------------------------------------------------ infinities
+// The matrix cores' sum is a NaN in places where the definition's is not: the pieces of an infinity, and of a number beyond the 16-bit type's
+// range, are an infinity and a NaN or an infinity of the other sign; a zero piece or a spare rank's zero meets an infinite factor.  It is never a
+// number where the definition's is not.  So every result that comes out as a NaN is formed again in fp32, value by value.  The test for it is within
+// 1.5 % of a pass in every case (the largest: fp32 gradients, 2048 x 4096 x 4096 of rank 64, 104.6 -> 106.2 us).
+__device__ __forceinline__ bool any_nan(const floatx4_t &v) { return __builtin_isunordered(v[0], v[1]) | __builtin_isunordered(v[2], v[3]); }
+
 // ------------------------------------------------------------------ expand
 // The fp32 side of the expanding products.  16-bit tensors are multiplied by the row in two pieces of their own type, hi + lo: bf16 has
 // fp32's range, an fp16 row is first scaled by a power of two that brings its largest value to 2^14 (the pieces then add up to the value
@@ -677,6 +695,7 @@ __device__ __forceinline__ void expand_block(const Problem &p, const Expand &o, 
   }
   const uint64_t pending = ids.pending;
   T *stage = lds + (kDown ? wave * kStageRows * kPitch : 0);
+  unsigned odd = 0;                                    // half groups where this lane's results have a NaN, the last in bit 0: not stored yet
 
   auto group = [&](int64_t c0, const vec8<T> (&early)[2], auto is_full) {
     constexpr bool kFull = decltype(is_full)::value;    // all 16 rows, all 64 columns, ranks in whole octets
@@ -747,7 +766,9 @@ __device__ __forceinline__ void expand_block(const Problem &p, const Expand &o, 
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       // a row without adapter keeps its base bit for bit, also a NaN's
+      bool nan = false;
       if (ids.mine >= 0) {
+        nan = any_nan(sum[2 * h]) | any_nan(sum[2 * h + 1]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           float add = sum[2 * h + (e >> 2)][e & 3];
@@ -755,7 +776,8 @@ __device__ __forceinline__ void expand_block(const Problem &p, const Expand &o, 
           old[h][e] = from_f32<T>(to_f32<T>(old[h][e]) + add);
         }
       }
-      if (!ids.owned) continue;
+      odd = 2 * odd + nan;
+      if (!ids.owned || nan) continue;
       if (kFull || have[h] == 8) {
         __builtin_memcpy(to + 32 * h, &old[h], sizeof old[h]);
       } else {
@@ -772,6 +794,19 @@ __device__ __forceinline__ void expand_block(const Problem &p, const Expand &o, 
 #pragma unroll 1
     for (int g = 0; g < G; ++g)
       if (first + g * kExpandCols < C) group(first + g * kExpandCols, early[g], std::false_type{});
+      else odd *= 4;
+  }
+  if (__builtin_expect(odd == 0 || !ids.owned, 1)) return;
+  const float scale = scaled ? p.scaling[ids.mine] : 1.0f;
+  const T *factor = f + static_cast<int64_t>(ids.mine) * p.r * C;
+#pragma unroll 1
+  for (int n = 0; n < 16 * G; ++n) {
+    const int64_t c = first + 8 * q + 32 * (n >> 3) + (n & 7);
+    if (!(odd >> (2 * G - 1 - (n >> 3)) & 1) || c >= C) continue;
+    float add = 0.0f;
+#pragma unroll 1
+    for (int j = 0; j < p.r; ++j) add = __builtin_fmaf(rank1(p, u, m, j) * scale, to_f32<T>(factor[kDown ? j * C + c : c * p.r + j]), add);
+    out[m * C + c] = from_f32<T>((base ? to_f32<T>(base[m * C + c]) : 0.0f) + add);
   }
 }
 
@@ -897,6 +932,11 @@ __global__ __launch_bounds__(64 * kRowWaves) void row_kernel(Problem p, int rows
     float add = q == 0 ? y[0][0] : q == 1 ? y[1][0] : q == 2 ? y[2][0] : y[3][0];
     if constexpr (dtype_code<T>::value == CAIFX_F16) add *= back;
     const int64_t at = c0 + lane;
+    if (__builtin_expect(__builtin_isunordered(add, add) && at < hi, 0)) {
+      add = 0.0f;
+#pragma unroll 1
+      for (int j = 0; j < p.r; ++j) add = __builtin_fmaf(total[j], to_f32<T>(fb[at * p.r + j]), add);
+    }
     if (at < hi) out[m * p.N + at] = from_f32<T>((base ? to_f32<T>(base[m * p.N + at]) : 0.0f) + add);
   }
 }
@@ -1078,26 +1118,51 @@ __device__ __forceinline__ void outer_block(const Problem &p, const Outer &o, un
     }
   }
   const int64_t size = p.r * o.C;
+  auto put = [&](int t, int j, int e, auto value) {
+    const int64_t c = c0 + 32 * wave + 16 * t + (kRanksDown ? i : 4 * q + e);
+    const int jj = 16 * j + (kRanksDown ? 4 * q + e : i);
+    if (c >= o.C || jj >= p.r) return;
+    const int64_t to = jj * o.js + c * o.cs;
+    const float v = value(c, jj) * scale;
+    if (slot.part >= 0) o.part[slot.part * size + to] = v;
+    else static_cast<T *>(o.grad)[slot.adapter * size + to] = from_f32<T>(v);
+  };
+  bool odd = false;
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int t = 0; t < 2; ++t) {
 #pragma unroll
-    for (int j = 0; j < JT; ++j)
+    for (int j = 0; j < JT; ++j) {
+      odd |= any_nan(acc[t][j]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t c = c0 + 32 * wave + 16 * t + (kRanksDown ? i : 4 * q + e);
-        const int jj = 16 * j + (kRanksDown ? 4 * q + e : i);
-        if (c >= o.C || jj >= p.r) continue;
-        const int64_t to = jj * o.js + c * o.cs;
-        const float v = acc[t][j][e] * scale;
-        if (slot.part >= 0) o.part[slot.part * size + to] = v;
-        else static_cast<T *>(o.grad)[slot.adapter * size + to] = from_f32<T>(v);
-      }
+      for (int e = 0; e < 4; ++e) put(t, j, e, [&](int64_t, int) { return acc[t][j][e]; });
+    }
+  }
+  if (__builtin_expect(odd, 0)) {
+    // a lane with a NaN forms all of its values again
+#pragma unroll 1
+    for (int k = 0; k < 8 * JT; ++k)
+      put(k / (4 * JT), k / 4 % JT, k % 4, [&](int64_t c, int jj) {
+        float v = 0.0f;
+#pragma unroll 1
+        for (int n = 0; n < slot.count; ++n) {
+          const int64_t m = list[n];
+          float x;
+          if constexpr (sizeof(Z) > 1) x = to_f32<Z>(static_cast<const Z *>(o.z)[m * o.C + c]);
+          else x = static_cast<float>(static_cast<const Z *>(o.z)[m * o.C + c]) * o.z_scales[m * groups + group];
+          v = __builtin_fmaf(rank1(p, o.u, m, jj), x, v);
+        }
+        return v;
+      });
+  }
 }
 
 // What of the backward needs g or the sorted rows, in one launch: blocks of grad_b, of grad_a, of dx.  Each of the three alone leaves the
 // chip half empty at its beginning and its end, and a launch of its own costs the small calls 3 us.
+// gradients_waves: waves of a SIMD that registers have to allow.  fp32 up to rank 32: as many as local memory holds, three (4096 x 11008, rank 16, with
+// two 151 us the pass, with three 138).
+template <typename T, int JT> constexpr int gradients_waves() { return sizeof(T) == 4 && JT <= 2 ? 3 : 1; }
 template <typename T, typename Z, int JT, int G>
-__global__ __launch_bounds__(kOuterThreads) void gradients_kernel(Problem p, Outer b, unsigned blocks_b, Outer a, unsigned blocks_a, Expand dx)
+__global__ __launch_bounds__(kOuterThreads, (gradients_waves<T, JT>())) void gradients_kernel(Problem p, Outer b, unsigned blocks_b, Outer a, unsigned blocks_a, Expand dx)
 {
   static_assert(kOuterThreads == 64 * kExpandWaves);
   constexpr int RS = JT / 2;
