@@ -252,9 +252,11 @@ __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(const int8_t *__rest
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const float g = static_cast<float>(gq[k].v[i]) * gs[k], u = static_cast<float>(uq[k].v[i]) * us[k], grad_h = to_f32<T>(d[k].v[i]);
-      const float sg = __builtin_amdgcn_rcpf(1.0f + expf(-g)), act = g * sg;
+      // e / (1 + e) and 1 / (1 + e) with e = exp(-|g|): the inverse stays in (0.5, 1], where exp(-g) would take it below the normal numbers
+      const float e = expf(-fabsf(g)), high = __builtin_amdgcn_rcpf(1.0f + e), low = e * high;
+      const float sg = g < 0.0f ? low : high, rest = g < 0.0f ? high : low, act = g * sg;
       ou.v[i] = from_f32<T>(grad_h * act);
-      og.v[i] = from_f32<T>(grad_h * u * (sg * __builtin_fmaf(g, 1.0f - sg, 1.0f)));
+      og.v[i] = from_f32<T>(grad_h * u * (sg * __builtin_fmaf(g, rest, 1.0f)));
       if constexpr (kHidden) oh.v[i] = from_f32<T>(act * u);
     }
     store8(grad_gate + p[k].at, og, p[k].have);
