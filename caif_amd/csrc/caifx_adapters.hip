@@ -1464,15 +1464,15 @@ int backward(const Problem &p, const void *dy, const void *x, const float *x_sca
   return launch_status();
 }
 
-int check(int64_t M, int64_t N, int64_t K, int rank, int num_adapters, int dtype)
+int check(int64_t M, int64_t N, int64_t K, int rank, int num_adapters, int dtype, bool backward)
 {
   if (!valid_dtype(dtype) || M < 0 || N <= 0 || K <= 0 || rank <= 0 || num_adapters <= 0) return CAIFX_ERR_INVALID_ARGUMENT;
   if (rank > CAIFX_ADAPTER_RANK_MAX || M > (int64_t{1} << 23) || N > (int64_t{1} << 26) || K > (int64_t{1} << 26)) return CAIFX_ERR_UNSUPPORTED;
-  // a grid has fewer than 2^32 threads; a launch holds three kinds of blocks
+  // a grid has fewer than 2^32 threads; the backward's launch holds three kinds of blocks, two of them slots of rows
   constexpr int64_t kBlocks = int64_t{1} << 22;
   for (const int64_t C : {N, K}) {
     if (ceil_div(M, 16 * kExpandWaves) > kBlocks / ceil_div(C, kExpandCols)) return CAIFX_ERR_UNSUPPORTED;
-    if (M / plan_chunk(M, C) + num_adapters > kBlocks / ceil_div(C, kOuterCols)) return CAIFX_ERR_UNSUPPORTED;
+    if (backward && M / plan_chunk(M, C) + num_adapters > kBlocks / ceil_div(C, kOuterCols)) return CAIFX_ERR_UNSUPPORTED;
   }
   return CAIFX_OK;
 }
@@ -1486,7 +1486,7 @@ extern "C" {
 
 size_t caifx_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K, int rank, int num_adapters, int dtype, int backward)
 {
-  if (check(M, N, K, rank, num_adapters, dtype) != CAIFX_OK || M == 0) return 0;
+  if (check(M, N, K, rank, num_adapters, dtype, backward != 0) != CAIFX_OK || M == 0) return 0;
   return plan(M, N, K, rank, num_adapters, dtype_size(dtype), backward != 0).total;
 }
 
@@ -1494,7 +1494,7 @@ int caifx_adapters_forward(int64_t M, int64_t N, int64_t K, int rank, int num_ad
                            const float *scaling, const void *base, void *y, float *hidden, int dtype, void *workspace, size_t workspace_bytes,
                            caifx_stream_t stream)
 {
-  const int st = check(M, N, K, rank, num_adapters, dtype);
+  const int st = check(M, N, K, rank, num_adapters, dtype, false);
   if (st != CAIFX_OK || M == 0) return st;
   if (!x || !ids || !a || !b || !scaling || !y) return CAIFX_ERR_INVALID_ARGUMENT;
   const size_t es = dtype_size(dtype), need = plan(M, N, K, rank, num_adapters, es, false).total;
@@ -1515,7 +1515,7 @@ int caifx_adapters_backward(int64_t M, int64_t N, int64_t K, int rank, int num_a
                             const float *hidden, const int32_t *ids, const void *a, const void *b, const float *scaling, const void *base, void *dx,
                             void *grad_a, void *grad_b, int dtype, void *workspace, size_t workspace_bytes, caifx_stream_t stream)
 {
-  const int st = check(M, N, K, rank, num_adapters, dtype);
+  const int st = check(M, N, K, rank, num_adapters, dtype, true);
   if (st != CAIFX_OK || ((M == 0 || !dx) && !grad_a && !grad_b)) return st;
   if (M > 0 && (!dy || !ids || !scaling || (dx && !a) || ((dx || grad_a) && !b) || (grad_a && !x) || (grad_b && !hidden))) return CAIFX_ERR_INVALID_ARGUMENT;
   const size_t es = dtype_size(dtype), need = plan(M, N, K, rank, num_adapters, es, true).total;

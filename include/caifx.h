@@ -473,8 +473,10 @@ CAIFX_API int caifx_moe_dispatch_backward(const void *grad_expert_buffer, const 
  * neighbouring rows of one adapter share its factors' reads.  A row whose id is outside [0, num_adapters) has no
  * adapter: its result is base (zero without one) bit for bit, its hidden row is zero, and it adds to no gradient.
  * 1 <= rank <= CAIFX_ADAPTER_RANK_MAX; adapters of a smaller rank are padded with zeros.  Sums are fp32 in a fixed
- * order; infinities and NaN give what the formulas give.  Any alignment of the element type will do.  Results alias no input but base.  CAIFX_ERR_UNSUPPORTED beyond
- * 2^23 rows, N or K of 2^26, and where M * N, M * K (2^34) or num_adapters * N / 128 (2^22) is more than one grid holds.
+ * order; infinities and NaN give what the formulas give.  Any alignment of the element type will do.  Results alias no
+ * input but base.  CAIFX_ERR_UNSUPPORTED beyond 2^23 rows, beyond an N or K of 2^26, and where a grid is too small: M * N
+ * or M * K beyond 2^34 (rounded up to multiples of 64 each); for the backward also num_adapters * ceil(N / 128) or
+ * num_adapters * ceil(K / 128) beyond some 2^22 (2^22 - 2^18 is always taken).
  * ------------------------------------------------------------------------- */
 #define CAIFX_ADAPTER_RANK_MAX 128
 
