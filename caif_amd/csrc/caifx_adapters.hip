@@ -10,7 +10,7 @@
 // keep the arithmetic out of the way.  Four kinds of product:
 //
 //   shrink   rows x factor over the long axis (h, g): a workgroup takes 16 or 32 rows, its waves share the axis
-//   expand   rank -> long axis (y, dx): a wave takes 16 rows x 256 columns (64 in small calls), adds base and rounds once
+//   expand   rank -> long axis (y, dx): a wave takes 16 rows x 256 columns (64 in small calls and in fp32 above rank 64), adds base and rounds once
 //   outer    sums over the rows of an adapter (dA, dB): a workgroup takes 128 columns and a run of the adapter's rows
 //   row      shrink and expand of one row in one launch, for decode steps
 //
@@ -810,7 +810,9 @@ __device__ __forceinline__ void expand_block(const Problem &p, const Expand &o, 
   }
 }
 
-template <typename T, int RS, int G> __global__ __launch_bounds__(64 * kExpandWaves) void expand_kernel(Problem p, Expand o)
+// as for the gradients: three waves of a SIMD for fp32 above rank 64 (300 rows, 1024 to 14336, rank 128: with two 60.6 us the pass, with three 57.0)
+template <typename T, int RS> constexpr int expand_waves() { return sizeof(T) == 4 && RS == 4 ? 3 : 1; }
+template <typename T, int RS, int G> __global__ __launch_bounds__(64 * kExpandWaves, (expand_waves<T, RS>())) void expand_kernel(Problem p, Expand o)
 {
   expand_block<T, RS, false, G>(p, o, blockIdx.x, nullptr);
 }
@@ -1341,14 +1343,25 @@ void shrink(const Problem &p, const Slices &sl, const void *z, int64_t C, const 
   else hipLaunchKernelGGL((shrink_kernel<T, 8, kDown>), grid, block, 0, s, p, zz, C, ff, sl.columns, scaled, out, sort);
 }
 
-// Columns of a wave of the expanding product: 64 while there are few waves, else 256.  (In runs of 100 rows, to 14336, 64 / 256 columns: 300
-// rows, 4256 waves of 64, rank 16 15.6 / 17.7 us, rank 64 35.0 / 29.4; 600 rows 21.1 / 20.7 and 57.5 / 38.4; 999 rows 28.6 / 25.5 and 84.8 / 56.9.)
-bool few_waves(int64_t M, int64_t C) { return ceil_div(M, 16) * ceil_div(C, kExpandCols) < 8192; }
-Expand plan_expand(const Problem &p, const Rows &u, int64_t C, const void *f, bool scaled, const void *base, void *out, float *hidden, unsigned &blocks)
+// Whether a wave of the expanding product takes 64 columns, or 256 (in calls of `es` bytes a value).  64 while there are few waves and the rows that
+// they read again for each 64 columns (all slices, fp32) are few bytes; fp32 above rank 64 always, where 256 leave registers for one wave of a SIMD.
+// Measured, us with 64 / 256 columns, K -> N, runs of 100 rows, bf16 where nothing else is said: rank 16, 1024 -> 14336, 300 rows (4256 waves) 13.6 / 17.2,
+// 999 (14112) 22.9 / 23.3; 4096 -> 11008, 600 rows (6536) 19.3 / 20.3, 999 (10836) 25.8 / 24.3.  Rank 64, 1024 -> 14336, 300 rows (33 MB read again)
+// 22.3 / 24.3; 4096 -> 14336, 300 rows (133 MB) 36.4 / 30.4; 4096 -> 11008, 999 rows 52.9 / 40.5; its backward to 11008, 600 rows (204 MB) 63.7 / 54.6.
+// fp32, rank 64, 4096 -> 11008, 600 rows (102 MB) 54.5 / 57.9, its backward to 11008 (204 MB) 100.7 / 90.7; rank 128, 4096 rows 4096 -> 11008 516 / 530,
+// backward 11008 -> 4096 548 / 689.
+bool narrow_waves(const Problem &p, const Rows &u, int64_t C, size_t es)
 {
-  const bool few = few_waves(p.M, C);
-  const int64_t tiles = ceil_div(C, kExpandCols * (few ? 1 : 4));
-  const Expand o{u, C, tiles, f, scaled, base, out, hidden, few ? turns(p, tiles) : 1, static_cast<unsigned>(ceil_div(p.M, 16 * kExpandWaves) * tiles)};
+  if (es == 4 && p.r > 64) return true;
+  const int64_t waves = ceil_div(p.M, 16) * ceil_div(C, kExpandCols), again = waves * u.slices * 16 * 4 * p.r;
+  return waves < 8192 && again < (int64_t{es == 4 ? 120 : 72} << 20);
+}
+template <typename T, int RS> constexpr bool kWideWaves = sizeof(T) == 2 || RS <= 2;      // whether a call may take the wide ones
+Expand plan_expand(const Problem &p, const Rows &u, int64_t C, const void *f, bool scaled, const void *base, void *out, float *hidden, bool narrow,
+                   unsigned &blocks)
+{
+  const int64_t tiles = ceil_div(C, kExpandCols * (narrow ? 1 : 4));
+  const Expand o{u, C, tiles, f, scaled, base, out, hidden, narrow ? turns(p, tiles) : 1, static_cast<unsigned>(ceil_div(p.M, 16 * kExpandWaves) * tiles)};
   blocks = o.places * o.turns;
   return o;
 }
@@ -1374,11 +1387,13 @@ template <typename T> int forward(const Problem &p, const void *x, const void *b
   if (hidden && w.slices.count == 1) h = hidden, hidden = nullptr;
   shrink<T, false>(p, w.slices, x, p.K, p.a, false, h, Sort{}, s);
   unsigned blocks;
-  const Expand o = plan_expand(p, Rows{h, w.slices.count}, p.N, p.b, true, base, y, hidden, blocks);
+  const Rows rows{h, w.slices.count};
+  const bool narrow = narrow_waves(p, rows, p.N, sizeof(T));
+  const Expand o = plan_expand(p, rows, p.N, p.b, true, base, y, hidden, narrow, blocks);
   const dim3 grid(blocks), block(64 * kExpandWaves);
 #define CAIFX_GO(RS)                                                                                           \
-  if (few_waves(p.M, p.N)) hipLaunchKernelGGL((expand_kernel<T, RS, 1>), grid, block, 0, s, p, o);             \
-  else hipLaunchKernelGGL((expand_kernel<T, RS, 4>), grid, block, 0, s, p, o)
+  if (narrow) hipLaunchKernelGGL((expand_kernel<T, RS, 1>), grid, block, 0, s, p, o);                          \
+  else if constexpr (kWideWaves<T, RS>) hipLaunchKernelGGL((expand_kernel<T, RS, 4>), grid, block, 0, s, p, o)
   if (p.r <= 16) {
     CAIFX_GO(0);
   } else if (p.r <= 32) {
@@ -1393,13 +1408,15 @@ template <typename T> int forward(const Problem &p, const void *x, const void *b
 }
 
 template <typename T, typename Z>
-void gradients(const Problem &p, const Outer &b, unsigned blocks_b, const Outer &a, unsigned blocks_a, const Expand &dx, unsigned blocks_x, hipStream_t s)
+void gradients(const Problem &p, const Outer &b, unsigned blocks_b, const Outer &a, unsigned blocks_a, const Expand &dx, unsigned blocks_x, bool narrow,
+               hipStream_t s)
 {
   const dim3 grid(blocks_b + blocks_a + blocks_x), block(kOuterThreads);
   if (grid.x == 0) return;
 #define CAIFX_GO(JT)                                                                                                                             \
-  if (few_waves(p.M, p.K)) hipLaunchKernelGGL((gradients_kernel<T, Z, JT, 1>), grid, block, 0, s, p, b, blocks_b, a, blocks_a, dx);              \
-  else hipLaunchKernelGGL((gradients_kernel<T, Z, JT, 4>), grid, block, 0, s, p, b, blocks_b, a, blocks_a, dx)
+  if (narrow) hipLaunchKernelGGL((gradients_kernel<T, Z, JT, 1>), grid, block, 0, s, p, b, blocks_b, a, blocks_a, dx);                           \
+  else if constexpr (kWideWaves<T, JT / 2>)                                                                                                      \
+    hipLaunchKernelGGL((gradients_kernel<T, Z, JT, 4>), grid, block, 0, s, p, b, blocks_b, a, blocks_a, dx)
   if (p.r <= 16) {
     CAIFX_GO(1);
   } else if (p.r <= 32) {
@@ -1451,9 +1468,10 @@ int backward(const Problem &p, const void *dy, const void *x, const float *x_sca
   if (gb) blocks_b = static_cast<unsigned>(ceil_div(p.N, kOuterCols) * w.b.slots);
   if (ga) blocks_a = static_cast<unsigned>(ceil_div(p.K, kOuterCols) * w.a.slots);
   Expand ox{};
-  if (dx) ox = plan_expand(p, rows, p.K, p.a, false, base, dx, nullptr, blocks_x);
-  if (x_scales) gradients<T, int8_t>(p, ob, blocks_b, oa, blocks_a, ox, blocks_x, s);
-  else gradients<T, T>(p, ob, blocks_b, oa, blocks_a, ox, blocks_x, s);
+  const bool narrow = !dx || narrow_waves(p, rows, p.K, sizeof(T));
+  if (dx) ox = plan_expand(p, rows, p.K, p.a, false, base, dx, nullptr, narrow, blocks_x);
+  if (x_scales) gradients<T, int8_t>(p, ob, blocks_b, oa, blocks_a, ox, blocks_x, narrow, s);
+  else gradients<T, T>(p, ob, blocks_b, oa, blocks_a, ox, blocks_x, narrow, s);
   const int64_t multi_a = ga ? w.a.multi : 0, multi_b = gb ? w.b.multi : 0, multi = multi_a > multi_b ? multi_a : multi_b;
   if (multi > 0) {
     const unsigned blocks_a = multi_a > 0 ? static_cast<unsigned>(ceil_div(size_a, 256 * kJoinPer)) : 0;

@@ -1,5 +1,5 @@
-"""Adapters' calls large enough for the waves of 256 columns (8192 waves of 64 or more along either axis): rows and columns that end inside a tile, the
-last tile whole and not, every rank's kernel, every type."""
+"""Adapters' calls large enough for the waves of 256 columns (8192 waves of 64 or more along either axis; fp32 above rank 64 stays with 64): rows and
+columns that end inside a tile, the last tile whole and not, every rank's kernel, every type."""
 import pytest
 import torch
 
@@ -44,3 +44,21 @@ def test_backward(m, k, n, r, adapters, order, packed, dtype):
     R.check(dx, *want["dx"], dtype, R.sums(n, r) + R.pieces(dtype), "dx")
     R.check(ga, *want["grad_a"], dtype, R.sums(n, m) + R.pieces(dtype), "grad_a")
     R.check(gb, *want["grad_b"], dtype, R.sums(m) + R.pieces(dtype), "grad_b")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("r", [64, 128])
+@pytest.mark.parametrize("m,order", [(300, "mixed"), (607, "runs")])
+def test_few_rows_in_many_slices(m, order, r, dtype):
+    """Fewer waves than that, whose rows would be read in eight slices for every 64 columns."""
+    p, more = problem(m, 4100, 9000, r, 3, dtype, order)
+    y, hidden = T.adapters_forward(**p, base=more["base"], keep_hidden=True)
+    want, mag, h, hmag = R.forward(**p, base=more["base"])
+    R.check(hidden, h, hmag, F32, R.sums(4100), "hidden")
+    R.check(y, want, mag, dtype, R.sums(4100, r) + R.pieces(dtype), "y")
+    p, more = problem(m, 9000, 4100, r, 3, dtype, order)
+    x = p.pop("x")
+    got = T.adapters_backward(more["dy"], x, more["hidden"], **p, base=more["dbase"])
+    want = R.backward(more["dy"], x, more["hidden"], **p, base=more["dbase"])
+    for name, g, slack in zip(("dx", "grad_a", "grad_b"), got, (R.sums(4100, r), R.sums(4100, m), R.sums(m))):
+        R.check(g, *want[name], dtype, slack + R.pieces(dtype), name)
