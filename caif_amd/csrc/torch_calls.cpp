@@ -15,6 +15,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
+#include <initializer_list>
 #include <stdexcept>
 #include <vector>
 
@@ -567,6 +568,16 @@ int64_t rows_of(const at::Tensor &t, int64_t columns)
   return t.numel() / columns;
 }
 
+// a result that the caller gives may be the base, place for place, and shares no memory with what else is read while it is written
+void apart(const at::Tensor &out, const at::Tensor *base, std::initializer_list<const at::Tensor *> inputs)
+{
+  const auto from = [](const at::Tensor &t) { return reinterpret_cast<uintptr_t>(t.data_ptr()); };
+  const auto meet = [&](const at::Tensor &t) { return from(out) < from(t) + t.nbytes() && from(t) < from(out) + out.nbytes(); };
+  bool wrong = base && from(*base) != from(out) && meet(*base);
+  for (const at::Tensor *t : inputs) wrong = wrong || (t && meet(*t));
+  if (wrong) throw Error{PyExc_ValueError, "out must be base itself or share no memory with the inputs"};
+}
+
 struct Scratch {
   at::Tensor held;
   size_t bytes;
@@ -591,6 +602,7 @@ PyObject *adapters_forward(PyObject *, PyObject *const *v, Py_ssize_t n)
     const at::Tensor *base = d.optional(v[5], x.scalar_type(), M * f.N, "base must have the activations' dtype and rows x N elements");
     const bool keep = truth(v[6]);
     const at::Tensor *out = d.optional(v[7], x.scalar_type(), M * f.N, "out must have the activations' dtype and rows x N elements");
+    if (out) apart(*out, base, {&x, &ids, &a, &b, &scaling});
     const at::Tensor y = out ? *out : at::empty({M, f.N}, x.options());
     const at::Tensor hidden = keep ? at::empty({M, f.rank}, x.options().dtype(at::kFloat)) : at::Tensor();
     const int L = static_cast<int>(f.L), r = static_cast<int>(f.rank);
@@ -602,33 +614,41 @@ PyObject *adapters_forward(PyObject *, PyObject *const *v, Py_ssize_t n)
   });
 }
 
-// adapters_backward(dy, x or codes, scales or None, hidden, ids, a, b, scaling, base, need_dx) -> (dx or None, grad_a, grad_b) or status
+// adapters_backward(dy, x or codes, scales or None, hidden, ids, a, b, scaling, base, need_dx, need_a, need_b, out) -> (dx, grad_a, grad_b), None for
+// what is not needed, or status
 PyObject *adapters_backward(PyObject *, PyObject *const *v, Py_ssize_t n)
 {
-  return guarded(n, 10, [&]() -> PyObject * {
+  return guarded(n, 13, [&]() -> PyObject * {
     const at::Tensor &dy = device_tensor(v[0]), &a = device_tensor(v[5]), &b = device_tensor(v[6]);
     const Device d(dy);
     const int dt = code_of(dy.scalar_type());
     const Factors f(d, a, b, dy.scalar_type());
     const int64_t M = rows_of(dy, f.N), groups = (f.K + CAIFX_CHECKPOINT_GROUP - 1) / CAIFX_CHECKPOINT_GROUP;
-    const bool packed = v[2] != Py_None;
-    const at::Tensor &x = d.operand(v[1], packed ? at::kChar : dy.scalar_type(), M * f.K, "x must have rows x K elements of the gradient's dtype, or be int8 codes with scales");
+    const bool packed = v[2] != Py_None, need_x = truth(v[9]), need_a = truth(v[10]), need_b = truth(v[11]);
+    // what no wanted result reads may be left out
+    const at::Tensor *x = need_a || v[1] != Py_None
+                              ? &d.operand(v[1], packed ? at::kChar : dy.scalar_type(), M * f.K,
+                                           "x must have rows x K elements of the gradient's dtype, or be int8 codes with scales")
+                              : nullptr;
     const at::Tensor *scales = d.optional(v[2], at::kFloat, M * groups, "the checkpoint's scales must be fp32, one per 128 values of a row");
-    const at::Tensor &hidden = d.operand(v[3], at::kFloat, M * f.rank, "hidden must be fp32 [rows, rank]");
+    const at::Tensor *hidden = need_b || v[3] != Py_None ? &d.operand(v[3], at::kFloat, M * f.rank, "hidden must be fp32 [rows, rank]") : nullptr;
     const at::Tensor &ids = d.operand(v[4], at::kInt, M, "ids must be int32, one per row");
     const at::Tensor &scaling = d.operand(v[7], at::kFloat, f.L, "scaling must be fp32, one per adapter");
     const at::Tensor *base = d.optional(v[8], dy.scalar_type(), M * f.K, "base must have the gradient's dtype and rows x K elements");
-    const bool need = truth(v[9]);
-    const at::Tensor dx = need ? at::empty({M, f.K}, dy.options()) : at::Tensor();
-    const at::Tensor ga = at::empty_like(a), gb = at::empty_like(b);
+    const at::Tensor *out = d.optional(v[12], dy.scalar_type(), M * f.K, "out must have the gradient's dtype and rows x K elements");
+    if (out && !need_x) throw Error{PyExc_ValueError, "out is for dx, which is not needed"};
+    if (out) apart(*out, base, {&dy, need_a ? x : nullptr, need_a ? scales : nullptr, need_b ? hidden : nullptr, &ids, &a, &b, &scaling});
+    const at::Tensor dx = out ? *out : need_x ? at::empty({M, f.K}, dy.options()) : at::Tensor();
+    const at::Tensor ga = need_a ? at::empty_like(a) : at::Tensor(), gb = need_b ? at::empty_like(b) : at::Tensor();
     const int L = static_cast<int>(f.L), r = static_cast<int>(f.rank);
     const Scratch ws(dy, api.caifx_adapters_workspace_bytes(M, f.N, f.K, r, L, dt, 1));
-    const int st = launch(api.caifx_adapters_backward, M, f.N, f.K, r, L, dy.data_ptr(), x.data_ptr(), static_cast<const float *>(data(scales)),
-                          static_cast<const float *>(hidden.data_ptr()), static_cast<const int32_t *>(ids.data_ptr()), a.data_ptr(), b.data_ptr(),
-                          static_cast<const float *>(scaling.data_ptr()), data(base), need ? dx.data_ptr() : nullptr, ga.data_ptr(), gb.data_ptr(), dt,
-                          ws.p(), ws.bytes, d.stream());
+    const auto at = [](const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
+    const int st = launch(api.caifx_adapters_backward, M, f.N, f.K, r, L, dy.data_ptr(), data(x), static_cast<const float *>(data(scales)),
+                          static_cast<const float *>(data(hidden)), static_cast<const int32_t *>(ids.data_ptr()), a.data_ptr(), b.data_ptr(),
+                          static_cast<const float *>(scaling.data_ptr()), data(base), at(dx), at(ga), at(gb), dt, ws.p(), ws.bytes, d.stream());
     if (st != CAIFX_OK) return PyLong_FromLong(st);
-    Owned p(need ? THPVariable_Wrap(dx) : Py_NewRef(Py_None)), q(THPVariable_Wrap(ga)), t(THPVariable_Wrap(gb));
+    const auto wrap = [](const at::Tensor &t) { return t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None); };
+    Owned p(wrap(dx)), q(wrap(ga)), t(wrap(gb));
     return PyTuple_Pack(3, p.p, q.p, t.p);
   });
 }

@@ -283,16 +283,18 @@ def adapters_forward(x, ids, a, b, scaling, base=None, keep_hidden=False, out=No
 
     x [..., K], ids int32 (one per row; outside [0, L): no adapter), a [L, rank, K], b [L, N, rank], scaling fp32 [L],
     base [M, N] the projection's result (None: zero).  Returns y [M, N], with keep_hidden (y, hidden fp32 [M, rank]), which
-    adapters_backward takes.  `out` may be `base`.  Tensors are contiguous, on one device, and run on its current stream."""
+    adapters_backward takes.  `out` may be `base`, and shares no memory with the other inputs.  Tensors are contiguous, on one device, and run on its current stream."""
     return _done((_native or _calls()).adapters_forward(x, ids, a, b, scaling, base, keep_hidden, out), "caifx_adapters_forward")
 
 
-def adapters_backward(dy, x, hidden, ids, a, b, scaling, base=None, need_dx=True):
+def adapters_backward(dy, x, hidden, ids, a, b, scaling, base=None, need_dx=True, need_a=True, need_b=True, out=None):
     """(dx, grad_a, grad_b) of adapters_forward: dx [M, K] is `base` (the projection's own input gradient, None: zero) plus the
     branch's, the factors' gradients have their shapes and type.  `x` is the forward's input or its checkpoint, the pair that
-    checkpoint_pack returned.  need_dx=False (a first layer): dx is None."""
+    checkpoint_pack returned.  A result that is not needed (dx of a first layer, the gradient of a frozen factor) is None and costs
+    nothing; x may then be None without grad_a, hidden without grad_b.  dx goes into `out`, which may be `base`."""
     codes, scales = x if isinstance(x, (tuple, list)) else (x, None)
-    return _done((_native or _calls()).adapters_backward(dy, codes, scales, hidden, ids, a, b, scaling, base, need_dx), "caifx_adapters_backward")
+    return _done((_native or _calls()).adapters_backward(dy, codes, scales, hidden, ids, a, b, scaling, base, need_dx, need_a, need_b, out),
+                 "caifx_adapters_backward")
 
 
 # ------------------------------------------------------------------ activation checkpoints in 8 bits

@@ -46,3 +46,40 @@ def test_no_rows_need_no_operands():
     p, more = problem(0, 24, 40, 8, 3, BF16, "one")
     got = backward(p, more, 3, p["x"], ("gb",), dict.fromkeys(("x", "hidden", "a", "b", "base"), True))
     assert not got["gb"].any()
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("m", [30, 700])
+def test_the_torch_call_leaves_out_what_is_not_needed(m, packed):
+    p, more = problem(m, 264, 392, 16, 3, BF16, "runs")
+    x = T.checkpoint_pack(p["x"]) if packed else p["x"]
+    rest = {key: p[key] for key in ("ids", "a", "b", "scaling")}
+    every = T.adapters_backward(more["dy"], x, more["hidden"], **rest, base=more["dbase"])
+    for need in range(8):
+        dx, a, b = (bool(need >> k & 1) for k in range(3))
+        got = T.adapters_backward(more["dy"], x if a else None, more["hidden"] if b else None, **rest, base=more["dbase"], need_dx=dx, need_a=a, need_b=b)
+        for wanted, g, e in zip((dx, a, b), got, every):
+            assert torch.equal(g, e) if wanted else g is None
+    into = more["dbase"].clone()
+    got = T.adapters_backward(more["dy"], x, more["hidden"], **rest, base=into, out=into)
+    assert got[0].data_ptr() == into.data_ptr() and all(torch.equal(g, e) for g, e in zip(got, every))
+    fresh = torch.empty_like(into)
+    assert torch.equal(T.adapters_backward(more["dy"], x, more["hidden"], **rest, base=more["dbase"], out=fresh)[0], every[0])
+
+
+def test_results_that_share_memory_with_inputs_are_refused():
+    p, more = problem(20, 64, 64, 8, 2, BF16, "mixed")
+    x = p["x"]
+    rest = {key: p[key] for key in ("ids", "a", "b", "scaling")}
+    room = torch.zeros(21, 64, dtype=BF16, device="cuda")
+    for bad in (dict(out=x), dict(base=room[:20], out=room[1:])):
+        with pytest.raises(ValueError):
+            T.adapters_forward(x, **rest, **bad)
+    for bad in (dict(out=more["dy"]), dict(out=x), dict(base=room[1:], out=room[:20]), dict(out=more["dbase"], need_dx=False)):
+        with pytest.raises(ValueError):
+            T.adapters_backward(more["dy"], x, more["hidden"], **rest, **bad)
+    with pytest.raises(TypeError):
+        T.adapters_backward(more["dy"], None, more["hidden"], **rest)
+    with pytest.raises(TypeError):
+        T.adapters_backward(more["dy"], x, None, **rest)
+    assert T.adapters_backward(more["dy"], x, more["hidden"], **rest, out=x, need_a=False)[0].data_ptr() == x.data_ptr()
