@@ -1161,7 +1161,7 @@ __device__ __forceinline__ void outer_block(const Problem &p, const Outer &o, un
 // What of the backward needs g or the sorted rows, in one launch: blocks of grad_b, of grad_a, of dx.  Each of the three alone leaves the
 // chip half empty at its beginning and its end, and a launch of its own costs the small calls 3 us.
 // gradients_waves: waves of a SIMD that registers have to allow.  fp32 up to rank 32: as many as local memory holds, three (4096 x 11008, rank 16, with
-// two 151 us the pass, with three 138).
+// two 151 us the pass, with three 141).
 template <typename T, int JT> constexpr int gradients_waves() { return sizeof(T) == 4 && JT <= 2 ? 3 : 1; }
 template <typename T, typename Z, int JT, int G>
 __global__ __launch_bounds__(kOuterThreads, (gradients_waves<T, JT>())) void gradients_kernel(Problem p, Outer b, unsigned blocks_b, Outer a, unsigned blocks_a, Expand dx)

@@ -7,10 +7,10 @@
 // Everything here is bound by memory, if the arithmetic is kept short: 45 M values through silu and two divisions each are as long a way
 // for the vector units as their 360 MB for the memory.  Sixteen lanes take a group, eight values each, so that a lane's part is one
 // 16-byte access of a 16-bit type; rows of any length and alignment take the same path (the hardware splits an access that straddles
-// a line), only a row's last values are moved one by one.  Measured in bf16: 16384 x 4096 packed in 39 us and unpacked in 30 (5.2 and 6.8
-// TB/s, in part from the memory-side cache; with divisions and shuffles 64 and 42), 4096 x 11008 gated in 84 us, three
-// quarters of it vector instructions (silu's exponential and division are a third of the 54 for a pair of values), its backward in 66
-// (5.5 TB/s).
+// a line), only a row's last values are moved one by one.  Measured in bf16, three sets of tensors in turn: 16384 x 4096 packed in 34 us and unpacked in
+// 32 (6.0 and 6.4 TB/s, in part from the memory-side cache; with divisions and shuffles 64 and 42), 4096 x 11008 gated in 88 us, three
+// quarters of it vector instructions (silu's exponential and division are a third of the 54 for a pair of values), its backward in 71
+// (5.1 TB/s).
 #include "caifx_common.hpp"
 
 #pragma clang fp contract(off)
