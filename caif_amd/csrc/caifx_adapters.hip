@@ -530,7 +530,8 @@ __device__ __forceinline__ float rank1(const Problem &p, const Rows &u, int64_t 
 // ------------------------------------------------------------------ infinities
 // The matrix cores' sum is a NaN in places where the definition's is not: the pieces of an infinity, and of a number beyond the 16-bit type's
 // range, are an infinity and a NaN or an infinity of the other sign; a zero piece or a spare rank's zero meets an infinite factor.  It is never a
-// number where the definition's is not.  So every result that comes out as a NaN is formed again in fp32, value by value.  The test for it is within
+// number where the definition's is not.  So every result that comes out as a NaN is formed again in fp32, value by value, up to
+// the first NaN of the definition's own.  The test for it is within
 // 1.5 % of a pass in every case (the largest: fp32 gradients, 2048 x 4096 x 4096 of rank 64, 104.6 -> 106.2 us).
 __device__ __forceinline__ bool any_nan(const floatx4_t &v) { return __builtin_isunordered(v[0], v[1]) | __builtin_isunordered(v[2], v[3]); }
 
@@ -805,7 +806,7 @@ __device__ __forceinline__ void expand_block(const Problem &p, const Expand &o, 
     if (!(odd >> (2 * G - 1 - (n >> 3)) & 1) || c >= C) continue;
     float add = 0.0f;
 #pragma unroll 1
-    for (int j = 0; j < p.r; ++j) add = __builtin_fmaf(rank1(p, u, m, j) * scale, to_f32<T>(factor[kDown ? j * C + c : c * p.r + j]), add);
+    for (int j = 0; j < p.r && add == add; ++j) add = __builtin_fmaf(rank1(p, u, m, j) * scale, to_f32<T>(factor[kDown ? j * C + c : c * p.r + j]), add);
     out[m * C + c] = from_f32<T>((base ? to_f32<T>(base[m * C + c]) : 0.0f) + add);
   }
 }
@@ -937,7 +938,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void row_kernel(Problem p, int rows
     if (__builtin_expect(__builtin_isunordered(add, add) && at < hi, 0)) {
       add = 0.0f;
 #pragma unroll 1
-      for (int j = 0; j < p.r; ++j) add = __builtin_fmaf(total[j], to_f32<T>(fb[at * p.r + j]), add);
+      for (int j = 0; j < p.r && add == add; ++j) add = __builtin_fmaf(total[j], to_f32<T>(fb[at * p.r + j]), add);
     }
     if (at < hi) out[m * p.N + at] = from_f32<T>((base ? to_f32<T>(base[m * p.N + at]) : 0.0f) + add);
   }
@@ -1120,51 +1121,54 @@ __device__ __forceinline__ void outer_block(const Problem &p, const Outer &o, un
     }
   }
   const int64_t size = p.r * o.C;
-  auto put = [&](int t, int j, int e, auto value) {
-    const int64_t c = c0 + 32 * wave + 16 * t + (kRanksDown ? i : 4 * q + e);
-    const int jj = 16 * j + (kRanksDown ? 4 * q + e : i);
-    if (c >= o.C || jj >= p.r) return;
-    const int64_t to = jj * o.js + c * o.cs;
-    const float v = value(c, jj) * scale;
+  // a lane's columns and ranks
+  const auto column = [&](int t, int e) { return c0 + 32 * wave + 16 * t + (kRanksDown ? i : 4 * q + e); };
+  const auto rank = [&](int j, int e) { return 16 * j + (kRanksDown ? 4 * q + e : i); };
+  const auto put = [&](int64_t to, float v) {
     if (slot.part >= 0) o.part[slot.part * size + to] = v;
     else static_cast<T *>(o.grad)[slot.adapter * size + to] = from_f32<T>(v);
   };
   bool odd = false;
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int j = 0; j < JT; ++j) {
       odd |= any_nan(acc[t][j]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) put(t, j, e, [&](int64_t, int) { return acc[t][j][e]; });
+      for (int e = 0; e < 4; ++e)
+        if (column(t, e) < o.C && rank(j, e) < p.r) put(rank(j, e) * o.js + column(t, e) * o.cs, acc[t][j][e] * scale);
     }
-  }
-  if (__builtin_expect(odd, 0)) {
-    // a lane with a NaN forms all of its values again
+  if (__builtin_expect(odd && scale == scale, 0)) {
 #pragma unroll 1
-    for (int k = 0; k < 8 * JT; ++k)
-      put(k / (4 * JT), k / 4 % JT, k % 4, [&](int64_t c, int jj) {
-        float v = 0.0f;
+    for (int k = 0; k < 8 * JT; ++k) {
+      const int64_t c = column(k / (4 * JT), k % 4);
+      const int jj = rank(k / 4 % JT, k % 4);
+      if (c >= o.C || jj >= p.r) continue;
+      const int64_t to = jj * o.js + c * o.cs;
+      const float was = slot.part >= 0 ? o.part[slot.part * size + to] : to_f32<T>(static_cast<const T *>(o.grad)[slot.adapter * size + to]);
+      if (was == was) continue;
+      float v = 0.0f;
 #pragma unroll 1
-        for (int n = 0; n < slot.count; ++n) {
-          const int64_t m = list[n];
-          float x;
-          if constexpr (sizeof(Z) > 1) x = to_f32<Z>(static_cast<const Z *>(o.z)[m * o.C + c]);
-          else x = static_cast<float>(static_cast<const Z *>(o.z)[m * o.C + c]) * o.z_scales[m * groups + group];
-          v = __builtin_fmaf(rank1(p, o.u, m, jj), x, v);
-        }
-        return v;
-      });
+      for (int n = 0; n < slot.count && v == v; ++n) {
+        const int64_t m = list[n];
+        float x;
+        if constexpr (sizeof(Z) > 1) x = to_f32<Z>(static_cast<const Z *>(o.z)[m * o.C + c]);
+        else x = static_cast<float>(static_cast<const Z *>(o.z)[m * o.C + c]) * o.z_scales[m * groups + group];
+        v = __builtin_fmaf(rank1(p, o.u, m, jj), x, v);
+      }
+      put(to, v * scale);
+    }
   }
 }
 
 // What of the backward needs g or the sorted rows, in one launch: blocks of grad_b, of grad_a, of dx.  Each of the three alone leaves the
 // chip half empty at its beginning and its end, and a launch of its own costs the small calls 3 us.
-// gradients_waves: waves of a SIMD that registers have to allow.  fp32 up to rank 32: as many as local memory holds, three (4096 x 11008, rank 16, with
-// two 151 us the pass, with three 141).
-template <typename T, int JT> constexpr int gradients_waves() { return sizeof(T) == 4 && JT <= 2 ? 3 : 1; }
+// gradients_waves: waves of a SIMD that registers have to allow, as many as local memory holds where that is a matter of a few registers: three in fp32 up
+// to rank 32 (4096 x 11008, rank 16, with two 151 us the pass, with three 141), four with 64 columns in 16 bits
+// between ranks 33 and 64 (1200 rows, 1024 to 4096, rank 64: with three 34.0, with four 33.1).
+template <typename T, int JT, int G> constexpr int gradients_waves() { return sizeof(T) == 4 && JT <= 2 ? 3 : sizeof(T) == 2 && JT == 4 && G == 1 ? 4 : 1; }
 template <typename T, typename Z, int JT, int G>
-__global__ __launch_bounds__(kOuterThreads, (gradients_waves<T, JT>())) void gradients_kernel(Problem p, Outer b, unsigned blocks_b, Outer a, unsigned blocks_a, Expand dx)
+__global__ __launch_bounds__(kOuterThreads, (gradients_waves<T, JT, G>())) void gradients_kernel(Problem p, Outer b, unsigned blocks_b, Outer a, unsigned blocks_a, Expand dx)
 {
   static_assert(kOuterThreads == 64 * kExpandWaves);
   constexpr int RS = JT / 2;
