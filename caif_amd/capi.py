@@ -10,7 +10,7 @@ import os
 import subprocess
 
 F32, F16, BF16 = 0, 1, 2
-W_INT8, W_INT4_GROUP, W_F32, W_F16, W_BF16 = 0, 1, 2, 3, 4
+W_INT8, W_INT4_GROUP, W_F32, W_F16, W_BF16, W_MXFP4 = 0, 1, 2, 3, 4, 5
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libcaifx.so")
@@ -37,6 +37,8 @@ EXPORTS = [
     "caifx_moe_dispatch_backward", "caifx_moe_dispatch_fresh", "caifx_moe_combine_backward_grad_expert_fresh",
     "caifx_adapters_forward", "caifx_adapters_backward", "caifx_adapters_workspace_bytes",
     "caifx_checkpoint_pack", "caifx_checkpoint_unpack", "caifx_silu_multiply_checkpoint", "caifx_swiglu_backward_checkpoint",
+    "caifx_mxfp4_quantize", "caifx_mxfp4_dequantize", "caifx_mxfp4_matmul", "caifx_mxfp4_matmul_workspace_bytes",
+    "caifx_gated_forward", "caifx_gated_backward", "caifx_gated_workspace_bytes",
 ]
 
 
@@ -127,6 +129,15 @@ def lib():
         L.caifx_checkpoint_unpack.argtypes = [_p, _p, _p, _i64, _i64, _int, _p]
         L.caifx_silu_multiply_checkpoint.argtypes = [_p] * 7 + [_i64, _i64, _int, _p]
         L.caifx_swiglu_backward_checkpoint.argtypes = [_p] * 8 + [_i64, _i64, _int, _p]
+        L.caifx_mxfp4_quantize.argtypes = [_p, _p, _p, _i64, _i64, _int, _p]
+        L.caifx_mxfp4_dequantize.argtypes = [_p, _p, _p, _i64, _i64, _int, _p]
+        L.caifx_mxfp4_matmul.argtypes = [_i64] * 3 + [_p] * 5 + [_int, _p, _sz, _p]
+        L.caifx_mxfp4_matmul_workspace_bytes.restype = _sz
+        L.caifx_mxfp4_matmul_workspace_bytes.argtypes = [_i64] * 3
+        L.caifx_gated_forward.argtypes = [_i64] * 3 + [_p] * 5 + [_int] + [_p] * 3 + [_int, _p, _sz, _p]
+        L.caifx_gated_backward.argtypes = [_i64] * 3 + [_p] * 7 + [_int] + [_p] * 3 + [_int, _p, _sz, _p]
+        L.caifx_gated_workspace_bytes.restype = _sz
+        L.caifx_gated_workspace_bytes.argtypes = [_i64] * 3 + [_int] * 3
         _lib = L
     return _lib
 

@@ -48,7 +48,9 @@ int validate_weight(int64_t N, int64_t K, int w_kind, const void *scales, int64_
       if (scale_period <= 0) return CAIFX_ERR_INVALID_ARGUMENT;
       if (!aligned_to(scales, 4)) return CAIFX_ERR_MISALIGNED;
     }
-  } else if (!float_kind(w_kind)) {
+  } else if (w_kind != CAIFX_W_MXFP4 && !float_kind(w_kind)) {
+    return CAIFX_ERR_INVALID_ARGUMENT;
+  } else if (w_kind == CAIFX_W_MXFP4 && !scales) {
     return CAIFX_ERR_INVALID_ARGUMENT;
   }
   return CAIFX_OK;
@@ -119,6 +121,7 @@ static size_t workspace_bytes(int64_t M, int64_t N, int64_t K, int x_dtype, int 
   a.x_dtype = x_dtype;
   a.compute_dtype = compute_dtype;
   a.w.kind = w_kind;
+  if (w_kind == CAIFX_W_MXFP4) return mxfp4_workspace_bytes(a, backward);
   const size_t f32_bytes = mfma_f32_workspace_bytes(a, backward);
   // float storage runs on the fp32 matrix-core instruction unless it is stored in the 16-bit compute type itself
   if (float_kind(w_kind) && !same_16bit(w_kind, compute_dtype)) return f32_bytes;
@@ -150,6 +153,18 @@ static int finish_add(int st, const void *addend, void *y, int y_dtype, int64_t 
   return caifx_add(y, addend, y, n, y_dtype, stream);
 }
 
+// A weight in microscaled 4 bits: products over operands laid out in the workspace, without that room the shape-agnostic kernels
+static int mxfp4_or_generic(GemmArgs &a, bool backward, const void *addend, caifx_stream_t stream)
+{
+  if (!aligned_to(a.w.q, 16)) return CAIFX_ERR_MISALIGNED;
+  hipStream_t s = as_stream(stream);
+  a.addend = addend;
+  const int st = mxfp4_linear(a, backward, s);
+  if (st != CAIFX_ERR_UNSUPPORTED) return st;
+  a.addend = nullptr;
+  return finish_add(backward ? generic_backward(a, s) : generic_forward(a, s), addend, a.y, a.y_dtype, a.M * (backward ? a.K : a.N), stream);
+}
+
 static int forward_impl(int64_t M, int64_t N, int64_t K, const void *x, int x_dtype, int compute_dtype,
                         const void *wq, int w_kind, const void *scales, int64_t scale_period, int group_size,
                         void *y, int y_dtype, const void *addend, void *workspace, size_t workspace_bytes,
@@ -164,6 +179,7 @@ static int forward_impl(int64_t M, int64_t N, int64_t K, const void *x, int x_dt
   if (M == 0) return CAIFX_OK;
   GemmArgs a = make_args(M, N, K, x, x_dtype, compute_dtype, wq, w_kind, scales, scale_period, group_size, y,
                          y_dtype, workspace, workspace_bytes);
+  if (w_kind == CAIFX_W_MXFP4) return mxfp4_or_generic(a, false, addend, stream);
   hipStream_t s = as_stream(stream);
   if (float_kind(w_kind)) {
     // float storage: stored in the 16-bit compute type -> the tiled kernel on the 16-bit matrix cores; every other
@@ -288,6 +304,7 @@ static int backward_impl(int64_t M, int64_t N, int64_t K, const void *dy, int dy
   if (M == 0) return CAIFX_OK;
   GemmArgs a = make_args(M, N, K, dy, dy_dtype, compute_dtype, wq, w_kind, scales, scale_period, group_size,
                          dx, dx_dtype, workspace, workspace_bytes);
+  if (w_kind == CAIFX_W_MXFP4) return mxfp4_or_generic(a, true, addend, stream);
   hipStream_t s = as_stream(stream);
   // up to 16 rows of int8 codes (scale vectors through residue classes of the rows, one scale, none) or of int4
   // codes in groups of 128 or more: one pass over the weight, whatever the compute type (16-bit compute types on
@@ -368,6 +385,8 @@ static int grouped(bool backward, int num_experts, const int32_t *offsets, int64
     if (scales_ptrs && scale_period <= 0) return CAIFX_ERR_INVALID_ARGUMENT;
   } else if (float_kind(w_kind)) {
     scales_ptrs = nullptr;
+  } else if (w_kind == CAIFX_W_MXFP4) {
+    return CAIFX_ERR_UNSUPPORTED;
   } else {
     return CAIFX_ERR_INVALID_ARGUMENT;
   }
@@ -478,8 +497,8 @@ static int swiglu_grouped(bool backward, int num_experts, const int32_t *offsets
     if (group_size <= 0 || !scales_ptrs) return CAIFX_ERR_INVALID_ARGUMENT;
   } else if (w_kind == CAIFX_W_INT8) {
     if (scales_ptrs && scale_period <= 0) return CAIFX_ERR_INVALID_ARGUMENT;
-  } else if (float_kind(w_kind)) {
-    return CAIFX_ERR_UNSUPPORTED;        // the gated stores exist in the quantised kernels only
+  } else if (float_kind(w_kind) || w_kind == CAIFX_W_MXFP4) {
+    return CAIFX_ERR_UNSUPPORTED;        // the gated stores exist in the int8 and int4 kernels only
   } else {
     return CAIFX_ERR_INVALID_ARGUMENT;
   }

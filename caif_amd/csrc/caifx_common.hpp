@@ -336,6 +336,28 @@ template <typename CT> __device__ __forceinline__ uint32_t pack2(float lo, float
   return __builtin_bit_cast(uint32_t, p);
 }
 
+// Microscaled 4-bit values.  The conversions of gfx950 take the power of two as an fp32 whose exponent field is the scale's byte:
+// 0 stands for 2^-127 and 255 gives a NaN, as the format has it; results below the smallest normal number are kept.
+__device__ __forceinline__ float mxfp4_scale(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
+// the value of the low four bits of `code`
+__device__ __forceinline__ float mxfp4_value(uint32_t code, uint32_t byte)
+{
+  typedef float pair_t __attribute__((ext_vector_type(2)));
+  const pair_t p = __builtin_bit_cast(pair_t, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code & 15u, mxfp4_scale(byte), 0));
+  return p[0];
+}
+// the two values of byte kByte of `codes` in CT, the first in the low half
+template <typename CT, int kByte> __device__ __forceinline__ uint32_t mxfp4_pair(uint32_t codes, float scale)
+{
+  if constexpr (dtype_code<CT>::value == CAIFX_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, kByte));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, kByte));
+}
+// the eight values of a dword in CT
+template <typename CT> __device__ __forceinline__ u32x4_t mxfp4_eight(uint32_t codes, float scale)
+{
+  return u32x4_t{mxfp4_pair<CT, 0>(codes, scale), mxfp4_pair<CT, 1>(codes, scale), mxfp4_pair<CT, 2>(codes, scale), mxfp4_pair<CT, 3>(codes, scale)};
+}
+
 __device__ __forceinline__ float wave_max(float v)
 {
 #pragma unroll

@@ -28,12 +28,17 @@ __device__ __forceinline__ void store_rt(void *p, int dt, int64_t i, float v)
   else static_cast<float *>(p)[i] = v;
 }
 
-// W[flat] in the compute dtype, widened to fp32
-__device__ __forceinline__ float weight_rt(const QWeight &w, const void *wq, const void *scales, int64_t f,
+// W[n, k] in the compute dtype, widened to fp32
+__device__ __forceinline__ float weight_rt(const QWeight &w, const void *wq, const void *scales, int64_t n, int64_t k, int64_t K,
                                            int compute_dtype)
 {
+  const int64_t f = n * K + k;
   float v;
-  if (w.kind == CAIFX_W_F32) {
+  if (w.kind == CAIFX_W_MXFP4) {
+    const int64_t at = n * ((K + CAIFX_MXFP4_BLOCK - 1) / CAIFX_MXFP4_BLOCK) + k / CAIFX_MXFP4_BLOCK;
+    const int in = static_cast<int>(k % CAIFX_MXFP4_BLOCK);
+    v = mxfp4_value(static_cast<const uint8_t *>(wq)[16 * at + in / 2] >> (4 * (in & 1)), static_cast<const uint8_t *>(scales)[at]);
+  } else if (w.kind == CAIFX_W_F32) {
     v = static_cast<const float *>(wq)[f];
   } else if (w.kind == CAIFX_W_F16) {
     v = to_f32(static_cast<const f16_t *>(wq)[f]);
@@ -79,7 +84,7 @@ __global__ void generic_forward_kernel(GemmArgs a)
 #pragma unroll
     for (int i = 0; i < kMB; ++i) acc[i] = 0.0f;
     for (int64_t k = lane; k < a.K; k += 64) {
-      const float wv = weight_rt(a.w, wq, scales, n * a.K + k, a.compute_dtype);
+      const float wv = weight_rt(a.w, wq, scales, n, k, a.K, a.compute_dtype);
 #pragma unroll
       for (int i = 0; i < kMB; ++i)
         if (i < mcnt) acc[i] = __builtin_fmaf(round_rt(load_rt(a.x, a.x_dtype, (m0 + i) * a.K + k), a.compute_dtype), wv, acc[i]);
@@ -118,7 +123,7 @@ __global__ void generic_backward_kernel(GemmArgs a)
 #pragma unroll
     for (int i = 0; i < kMB; ++i) acc[i] = 0.0f;
     for (int64_t n = 0; n < a.N; ++n) {
-      const float wv = weight_rt(a.w, wq, scales, n * a.K + k, a.compute_dtype);
+      const float wv = weight_rt(a.w, wq, scales, n, k, a.K, a.compute_dtype);
 #pragma unroll
       for (int i = 0; i < kMB; ++i)
         if (i < mcnt) acc[i] = __builtin_fmaf(round_rt(load_rt(a.x, a.x_dtype, (m0 + i) * a.N + n), a.compute_dtype), wv, acc[i]);

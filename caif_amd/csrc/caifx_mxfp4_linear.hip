@@ -1,0 +1,377 @@
+// Products over frozen weights in microscaled 4 bits (forward, input gradient, both operands in 4 bits), and the gated feed-forward block
+// over two such weights or two stored in the 16-bit type: which kernels run on what, and the operands that they need in the workspace.
+#include "caifx_mxfp4.hpp"
+
+namespace caifx {
+namespace {
+
+int64_t up_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+int64_t chunks_of(int64_t reduction) { return (reduction + kRowsChunk - 1) / kRowsChunk; }
+
+// A workspace handed out in pieces of whole 256 bytes; without memory only the sizes are added up.
+struct Room {
+  char *p = nullptr;
+  size_t used = 0;
+  void *take(size_t bytes)
+  {
+    void *at = p ? p + used : nullptr;
+    used += (bytes + 255) / 256 * 256;
+    return at;
+  }
+};
+
+int pieces_of(int compute_dtype) { return compute_dtype == CAIFX_F32 ? 3 : 1; }
+size_t packed_bytes(int64_t rows, int64_t chunks, int compute_dtype)
+{
+  return static_cast<size_t>((rows + 15) / 16) * static_cast<size_t>(chunks) * static_cast<size_t>(pieces_of(compute_dtype)) * 8192;
+}
+// fp32 products of bf16 activations: every factor is a bf16 number as it is
+int computed_in(const GemmArgs &a) { return a.compute_dtype == CAIFX_F32 && a.x_dtype == CAIFX_BF16 ? CAIFX_BF16 : a.compute_dtype; }
+int stored_as(int compute_dtype) { return compute_dtype == CAIFX_F16 ? CAIFX_F16 : CAIFX_BF16; }
+
+// One weight of a product, in either form
+struct Weight {
+  const void *p;
+  const void *scales;      // MX only
+  bool mx;
+};
+
+// One or two products x w^T.  x [M, R] of x_dtype; w [N, R].
+struct Product {
+  int64_t M, N, R;
+  const void *x;
+  int x_dtype, compute_dtype;
+  int weights;
+  Weight w[2];
+  void *y, *gate, *up;
+  int y_dtype;
+  const void *addend;
+};
+
+RowsArgs rows_args(const Product &p)
+{
+  RowsArgs g{};
+  const int64_t blocks = (p.R + CAIFX_MXFP4_BLOCK - 1) / CAIFX_MXFP4_BLOCK;
+  for (int i = 0; i < p.weights; ++i) {
+    g.w[i] = p.w[i].p;
+    g.s[i] = static_cast<const uint8_t *>(p.w[i].scales);
+  }
+  g.M = p.M;
+  g.N = p.N;
+  g.R = p.R;
+  g.blocks = blocks;
+  g.w_pitch = p.w[0].mx ? 16 * blocks : 2 * p.R;
+  g.x_pitch = p.R;
+  g.chunks = static_cast<int>(chunks_of(p.R));
+  g.tiles = static_cast<int>((p.M + 15) / 16);
+  g.y = p.y;
+  g.gate = p.gate;
+  g.up = p.up;
+  g.addend = p.addend;
+  g.y_dtype = p.y_dtype;
+  return g;
+}
+
+int rows_run(const RowsArgs &g, bool mx, int weights, int compute_dtype, bool direct, hipStream_t s)
+{
+  const int kind = mx ? ROWS_MX : ROWS_DENSE;
+  return compute_dtype == CAIFX_F16 ? rows_f16(g, kind, weights, direct, s) : rows_bf16(g, kind, weights, pieces_of(compute_dtype), direct, s);
+}
+
+// whether the row kernels can read the activations where they are
+bool direct_type(const Product &p) { return p.compute_dtype != CAIFX_F32 && p.x_dtype == p.compute_dtype && p.R % 8 == 0; }
+
+// Runs the product, or with room.p == nullptr adds up what it needs of the workspace.
+int product(const Product &p, Room &room, bool only_size, hipStream_t s)
+{
+  Product d = p;
+  // rows of a stored weight start at any multiple of two bytes where R is odd: the row kernels take them from a copy
+  if (!p.w[0].mx && p.R % 8 != 0) {
+    const int64_t pitch = up_to(p.R, 8);
+    for (int i = 0; i < p.weights; ++i) {
+      void *copy = room.take(static_cast<size_t>(p.N) * static_cast<size_t>(pitch) * 2);
+      if (!only_size) {
+        const int st = operand_dense(p.w[i].p, nullptr, stored_as(p.compute_dtype), p.N, p.R, stored_as(p.compute_dtype), copy, pitch, pitch, 0, s);
+        if (st != CAIFX_OK) return st;
+      }
+      d.w[i].p = copy;
+    }
+  }
+  RowsArgs g = rows_args(d);
+  if (!p.w[0].mx && p.R % 8 != 0) {
+    g.R = up_to(p.R, 8);
+    g.w_pitch = 2 * g.R;
+  }
+  const bool direct = p.M <= 32 && direct_type(p) && (only_size || aligned_to(p.x, 16));
+  if (!direct) {
+    void *packed = room.take(packed_bytes(p.M, g.chunks, p.compute_dtype));
+    if (!only_size) {
+      const int st = operand_rows(p.x, p.x_dtype, p.M, p.R, p.compute_dtype, p.w[0].mx ? ROWS_MX : ROWS_DENSE, packed, 0, g.chunks, s);
+      if (st != CAIFX_OK) return st;
+    }
+    g.x = packed;
+  } else {
+    g.x = p.x;
+  }
+  return only_size ? CAIFX_OK : rows_run(g, p.w[0].mx, p.weights, p.compute_dtype, direct, s);
+}
+
+// y[M,K] = sum over the weights of x[i][M,N] w[i][N,K], as one reduction over their rows
+struct Gradient {
+  int64_t M, N, K;
+  const void *x[2];
+  int x_dtype, compute_dtype;
+  int weights;
+  Weight w[2];
+  void *y;
+  int y_dtype;
+  const void *addend;
+};
+
+int gradient(const Gradient &p, Room &room, bool only_size, hipStream_t s)
+{
+  const int to = stored_as(p.compute_dtype);
+  const int64_t pitch = up_to(p.N, kRowsChunk), stride = pitch * p.weights;       // whole chunks of each weight's rows
+  const int per = static_cast<int>(pitch / kRowsChunk), chunks = per * p.weights;
+  void *copy = room.take(static_cast<size_t>(p.K) * static_cast<size_t>(stride) * 2);
+  void *packed = room.take(packed_bytes(p.M, chunks, p.compute_dtype));
+  if (only_size) return CAIFX_OK;
+  for (int i = 0; i < p.weights; ++i) {
+    int st = operand_transposed(p.w[i].p, p.w[i].scales, p.w[i].mx ? OPERAND_MX : to, p.N, p.K, to, copy, pitch, stride, i * pitch, s);
+    if (st == CAIFX_OK) st = operand_rows(p.x[i], p.x_dtype, p.M, p.N, p.compute_dtype, ROWS_DENSE, packed, i * per, chunks, s);
+    if (st != CAIFX_OK) return st;
+  }
+  RowsArgs g{};
+  g.w[0] = copy;
+  g.M = p.M;
+  g.N = p.K;
+  g.R = stride;
+  g.w_pitch = 2 * stride;
+  g.chunks = chunks;
+  g.tiles = static_cast<int>((p.M + 15) / 16);
+  g.x = packed;
+  g.y = p.y;
+  g.addend = p.addend;
+  g.y_dtype = p.y_dtype;
+  return rows_run(g, false, 1, p.compute_dtype, false, s);
+}
+
+Product product_of(const GemmArgs &a)
+{
+  Product p{};
+  p.M = a.M;
+  p.N = a.N;
+  p.R = a.K;
+  p.x = a.x;
+  p.x_dtype = a.x_dtype;
+  p.compute_dtype = computed_in(a);
+  p.weights = 1;
+  p.w[0] = Weight{a.w.q, a.w.scales, true};
+  p.y = a.y;
+  p.y_dtype = a.y_dtype;
+  p.addend = a.addend;
+  return p;
+}
+Gradient gradient_of(const GemmArgs &a)
+{
+  Gradient p{};
+  p.M = a.M;
+  p.N = a.N;
+  p.K = a.K;
+  p.x[0] = a.x;
+  p.x_dtype = a.x_dtype;
+  p.compute_dtype = computed_in(a);
+  p.weights = 1;
+  p.w[0] = Weight{a.w.q, a.w.scales, true};
+  p.y = a.y;
+  p.y_dtype = a.y_dtype;
+  p.addend = a.addend;
+  return p;
+}
+
+// sizes that every launch here has a grid for
+bool fits(int64_t M, int64_t N, int64_t K) { return M <= (1 << 30) && N < (1 << 22) && K < (1 << 22); }
+
+}  // namespace
+
+size_t mxfp4_workspace_bytes(const GemmArgs &a, bool backward)
+{
+  if (a.M <= 0 || a.N <= 0 || a.K <= 0 || !fits(a.M, a.N, a.K)) return 0;
+  Room room;
+  if (backward) gradient(gradient_of(a), room, true, nullptr);
+  else product(product_of(a), room, true, nullptr);
+  return room.used;
+}
+
+int mxfp4_linear(const GemmArgs &a, bool backward, hipStream_t s)
+{
+  if (!fits(a.M, a.N, a.K)) return CAIFX_ERR_UNSUPPORTED;
+  const size_t need = mxfp4_workspace_bytes(a, backward);
+  const bool misaligned = !backward && need == 0 && !aligned_to(a.x, 16);      // (packed then, into room that the query did not count)
+  if (misaligned || (need > 0 && (!a.workspace || a.workspace_bytes < need || !aligned_to(a.workspace, 16)))) return CAIFX_ERR_UNSUPPORTED;
+  Room room{static_cast<char *>(a.workspace), 0};
+  return backward ? gradient(gradient_of(a), room, false, s) : product(product_of(a), room, false, s);
+}
+
+}  // namespace caifx
+
+using namespace caifx;
+
+namespace {
+
+// what both gated calls check; `go`: there is work
+int gated_check(int64_t M, int64_t N, int64_t K, int w_kind, int dtype, bool &go)
+{
+  go = false;
+  if (M < 0 || N <= 0 || K <= 0 || !valid_dtype(dtype)) return CAIFX_ERR_INVALID_ARGUMENT;
+  if (w_kind < CAIFX_W_INT8 || w_kind > CAIFX_W_MXFP4) return CAIFX_ERR_INVALID_ARGUMENT;
+  const bool stored = (w_kind == CAIFX_W_F16 && dtype == CAIFX_F16) || (w_kind == CAIFX_W_BF16 && dtype == CAIFX_BF16);
+  if ((w_kind != CAIFX_W_MXFP4 && !stored) || !fits(M, N, K)) return CAIFX_ERR_UNSUPPORTED;
+  go = M > 0;
+  return CAIFX_OK;
+}
+Product gated_product(int64_t M, int64_t N, int64_t K, int w_kind, int dtype)
+{
+  Product p{};
+  p.M = M;
+  p.N = N;
+  p.R = K;
+  p.x_dtype = p.compute_dtype = p.y_dtype = dtype;
+  p.weights = 2;
+  p.w[0].mx = p.w[1].mx = w_kind == CAIFX_W_MXFP4;
+  return p;
+}
+Gradient gated_gradient(int64_t M, int64_t N, int64_t K, int w_kind, int dtype)
+{
+  Gradient p{};
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.x_dtype = p.compute_dtype = p.y_dtype = dtype;
+  p.weights = 2;
+  p.w[0].mx = p.w[1].mx = w_kind == CAIFX_W_MXFP4;
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t caifx_mxfp4_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K)
+{
+  if (M <= 0 || N <= 0 || K <= 0 || !fits(M, N, K)) return 0;
+  Room room;
+  room.take(static_cast<size_t>(M) * static_cast<size_t>(up_to(K, CAIFX_MXFP4_BLOCK)) * 2);
+  GemmArgs a{};
+  a.M = M;
+  a.N = N;
+  a.K = up_to(K, CAIFX_MXFP4_BLOCK);
+  a.x_dtype = a.compute_dtype = CAIFX_BF16;
+  return room.used + mxfp4_workspace_bytes(a, false);
+}
+
+int caifx_mxfp4_matmul(int64_t M, int64_t N, int64_t K, const void *a_codes, const void *a_scales, const void *b_codes, const void *b_scales, void *y,
+                       int y_dtype, void *workspace, size_t workspace_bytes, caifx_stream_t stream)
+{
+  if (M < 0 || N < 0 || K <= 0 || !valid_dtype(y_dtype)) return CAIFX_ERR_INVALID_ARGUMENT;
+  if (M == 0 || N == 0) return CAIFX_OK;
+  if (!a_codes || !a_scales || !b_codes || !b_scales || !y) return CAIFX_ERR_INVALID_ARGUMENT;
+  if (!fits(M, N, K)) return CAIFX_ERR_UNSUPPORTED;
+  if (!aligned_to(a_codes, 16) || !aligned_to(b_codes, 16) || !aligned_to(y, dtype_size(y_dtype)) || !aligned_to(workspace, 16)) return CAIFX_ERR_MISALIGNED;
+  const size_t need = caifx_mxfp4_matmul_workspace_bytes(M, N, K);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return CAIFX_ERR_WORKSPACE_TOO_SMALL;
+  const int64_t R = up_to(K, CAIFX_MXFP4_BLOCK);
+  Room room{static_cast<char *>(workspace), 0};
+  void *x = room.take(static_cast<size_t>(M) * static_cast<size_t>(R) * 2);
+  const int st = operand_dense(a_codes, a_scales, OPERAND_MX, M, R, CAIFX_BF16, x, R, R, 0, as_stream(stream));
+  if (st != CAIFX_OK) return st;
+  Product p{};
+  p.M = M;
+  p.N = N;
+  p.R = R;
+  p.x = x;
+  p.x_dtype = p.compute_dtype = CAIFX_BF16;
+  p.weights = 1;
+  p.w[0] = Weight{b_codes, b_scales, true};
+  p.y = y;
+  p.y_dtype = y_dtype;
+  return product(p, room, false, as_stream(stream));
+}
+
+size_t caifx_gated_workspace_bytes(int64_t M, int64_t N, int64_t K, int w_kind, int dtype, int backward)
+{
+  bool go;
+  if (gated_check(M, N, K, w_kind, dtype, go) != CAIFX_OK || !go) return 0;
+  Room room;
+  if (backward) gradient(gated_gradient(M, N, K, w_kind, dtype), room, true, nullptr);
+  else product(gated_product(M, N, K, w_kind, dtype), room, true, nullptr);
+  // (activations at an address that no 16-byte access takes are packed; few rows are all the query leaves out otherwise)
+  if (!backward && room.used == 0) room.take(packed_bytes(M, chunks_of(K), dtype));
+  return room.used;
+}
+
+int caifx_gated_forward(int64_t M, int64_t N, int64_t K, const void *x, const void *w_gate, const void *scales_gate, const void *w_up,
+                        const void *scales_up, int w_kind, void *hidden, void *gate, void *up, int dtype, void *workspace, size_t workspace_bytes,
+                        caifx_stream_t stream)
+{
+  bool go;
+  const int st = gated_check(M, N, K, w_kind, dtype, go);
+  if (!go) return st;
+  const bool mx = w_kind == CAIFX_W_MXFP4;
+  if (!x || !w_gate || !w_up || !hidden || (mx && (!scales_gate || !scales_up)) || (gate == nullptr) != (up == nullptr)) return CAIFX_ERR_INVALID_ARGUMENT;
+  if (x == hidden || x == gate || x == up || hidden == gate || hidden == up || (gate && gate == up)) return CAIFX_ERR_INVALID_ARGUMENT;
+  const size_t es = dtype_size(dtype);
+  if (!aligned_to(x, es) || !aligned_to(hidden, es) || !aligned_to(gate, es) || !aligned_to(up, es) || !aligned_to(w_gate, 16) || !aligned_to(w_up, 16) ||
+      !aligned_to(workspace, 16))
+    return CAIFX_ERR_MISALIGNED;
+  const size_t need = caifx_gated_workspace_bytes(M, N, K, w_kind, dtype, 0);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return CAIFX_ERR_WORKSPACE_TOO_SMALL;
+  Product p = gated_product(M, N, K, w_kind, dtype);
+  p.x = x;
+  p.w[0].p = w_gate;
+  p.w[0].scales = scales_gate;
+  p.w[1].p = w_up;
+  p.w[1].scales = scales_up;
+  p.y = hidden;
+  p.gate = gate;
+  p.up = up;
+  Room room{static_cast<char *>(workspace), 0};
+  return product(p, room, false, as_stream(stream));
+}
+
+int caifx_gated_backward(int64_t M, int64_t N, int64_t K, const void *grad_hidden, const void *gate, const void *up, const void *w_gate,
+                         const void *scales_gate, const void *w_up, const void *scales_up, int w_kind, void *grad_gate, void *grad_up, void *dx, int dtype,
+                         void *workspace, size_t workspace_bytes, caifx_stream_t stream)
+{
+  bool go;
+  int st = gated_check(M, N, K, w_kind, dtype, go);
+  if (!go) return st;
+  const bool mx = w_kind == CAIFX_W_MXFP4;
+  if (!grad_hidden || !gate || !up || !grad_gate || !grad_up || (dx && (!w_gate || !w_up || (mx && (!scales_gate || !scales_up)))))
+    return CAIFX_ERR_INVALID_ARGUMENT;
+  const void *in[3] = {grad_hidden, gate, up};
+  for (const void *i : in)
+    if (i == grad_gate || i == grad_up || i == dx) return CAIFX_ERR_INVALID_ARGUMENT;
+  if (grad_gate == grad_up || grad_gate == dx || grad_up == dx) return CAIFX_ERR_INVALID_ARGUMENT;
+  const size_t es = dtype_size(dtype);
+  if (!aligned_to(grad_hidden, es) || !aligned_to(gate, es) || !aligned_to(up, es) || !aligned_to(grad_gate, es) || !aligned_to(grad_up, es) ||
+      !aligned_to(dx, es) || !aligned_to(w_gate, 16) || !aligned_to(w_up, 16) || !aligned_to(workspace, 16))
+    return CAIFX_ERR_MISALIGNED;
+  const size_t need = dx ? caifx_gated_workspace_bytes(M, N, K, w_kind, dtype, 1) : 0;
+  if (need > 0 && (!workspace || workspace_bytes < need)) return CAIFX_ERR_WORKSPACE_TOO_SMALL;
+  hipStream_t s = as_stream(stream);
+  st = gating_backward(grad_hidden, gate, up, grad_gate, grad_up, M * N, dtype, s);
+  if (st != CAIFX_OK || !dx) return st;
+  Gradient p = gated_gradient(M, N, K, w_kind, dtype);
+  p.x[0] = grad_gate;
+  p.x[1] = grad_up;
+  p.w[0].p = w_gate;
+  p.w[0].scales = scales_gate;
+  p.w[1].p = w_up;
+  p.w[1].scales = scales_up;
+  p.y = dx;
+  Room room{static_cast<char *>(workspace), 0};
+  return gradient(p, room, false, s);
+}
+
+}  // extern "C"

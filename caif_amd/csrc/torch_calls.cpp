@@ -35,7 +35,8 @@ namespace {
   X(caifx_moe_combine_backward_grad_expert_fresh) X(caifx_quantize_int8_per_channel)           \
   X(caifx_quantize_int8_per_tensor) X(caifx_quantize_to_int4) X(caifx_adapters_forward) X(caifx_adapters_backward)         \
   X(caifx_adapters_workspace_bytes) X(caifx_checkpoint_pack) X(caifx_checkpoint_unpack) X(caifx_silu_multiply_checkpoint)   \
-  X(caifx_swiglu_backward_checkpoint)
+  X(caifx_swiglu_backward_checkpoint) X(caifx_mxfp4_quantize) X(caifx_mxfp4_dequantize) X(caifx_mxfp4_matmul)               \
+  X(caifx_mxfp4_matmul_workspace_bytes) X(caifx_gated_forward) X(caifx_gated_backward) X(caifx_gated_workspace_bytes)
 
 struct Api {
 #define X(name) decltype(&::name) name = nullptr;
@@ -230,6 +231,17 @@ template <typename F> PyObject *guarded(Py_ssize_t have, Py_ssize_t want, F f)
   }
 }
 
+// the codes and scales of a weight in microscaled 4 bits, [N, K]: the kernels take both sizes from N and K
+void check_mxfp4(PyObject *w, int64_t N, int64_t K, const at::Tensor &x)
+{
+  const int64_t blocks = (K + CAIFX_MXFP4_BLOCK - 1) / CAIFX_MXFP4_BLOCK;
+  Owned codes(PyObject_GetAttr(w, attrs().wq.name)), scales(PyObject_GetAttr(w, attrs().scales.name));
+  const at::Tensor &c = device_tensor(codes.p), &s = device_tensor(scales.p);
+  if (c.scalar_type() != at::kByte || s.scalar_type() != at::kByte || c.numel() != N * 16 * blocks || s.numel() != N * blocks)
+    throw Error{PyExc_ValueError, "a W_MXFP4 weight's codes are uint8 [N, 16 * ceil(K / 32)], its scales uint8 [N, ceil(K / 32)]"};
+  if (c.device() != x.device() || s.device() != x.device()) throw Error{PyExc_RuntimeError, "tensors must be on one device"};
+}
+
 // ------------------------------------------------------------------ frozen linear
 // qlinear(backward, x, weight, compute_dtype, out_dtype, out, workspace, addend) -> result or status
 PyObject *qlinear(PyObject *, PyObject *const *a, Py_ssize_t n)
@@ -248,6 +260,15 @@ PyObject *qlinear(PyObject *, PyObject *const *a, Py_ssize_t n)
     const int kind = static_cast<int>(int_attr(w, at_.kind));
     const int64_t period = int_attr(w, at_.period);
     const int group = static_cast<int>(int_attr(w, at_.group));
+    c10::OptionalDeviceGuard guard;
+    if (kind == CAIFX_W_MXFP4) {
+      check_mxfp4(w, N, K, x);
+      if (x.numel() != M * in) throw Error{PyExc_ValueError, "the input's size is not a multiple of the reduction length"};
+      for (const int i : {5, 7})
+        if (a[i] != Py_None && (device_tensor(a[i]).numel() != M * out_dim || tensor(a[i]).scalar_type() != type_of(od) || tensor(a[i]).device() != x.device()))
+          throw Error{PyExc_ValueError, "the result and the addend must have the result's dtype and rows x columns elements, on the input's device"};
+      guard.reset_device(x.device());
+    }
     const void *wq = ptr_attr(w, at_.wq), *scales = ptr_attr(w, at_.scales);
     const at::Tensor y = a[5] != Py_None ? tensor(a[5]) : at::empty({M, out_dim}, x.options().dtype(type_of(od)));
     const Workspace ws(a[6], x, [&] { return api.caifx_qlinear_workspace_bytes(M, N, K, xd, compute, kind, backward ? 1 : 0); });
@@ -744,12 +765,159 @@ PyObject *swiglu_backward_checkpoint(PyObject *, PyObject *const *v, Py_ssize_t 
   });
 }
 
+// ------------------------------------------------------------------ microscaled 4-bit floating point, gated feed-forward block
+// the last extent of a tensor of at least one dimension
+int64_t last(const at::Tensor &t)
+{
+  if (t.dim() == 0) throw Error{PyExc_ValueError, "expected a tensor of at least one dimension"};
+  return t.size(t.dim() - 1);
+}
+
+// codes and scales of rows of values; the scales decide the number of blocks
+struct Micro {
+  const at::Tensor &codes, &scales;
+  int64_t rows, blocks;
+  Micro(const Device &d, PyObject *c, PyObject *s) : codes(device_tensor(c)), scales(device_tensor(s))
+  {
+    if (codes.device() != d.at || scales.device() != d.at) throw Error{PyExc_RuntimeError, "tensors must be on one device"};
+    if (codes.scalar_type() != at::kByte || scales.scalar_type() != at::kByte) throw Error{PyExc_ValueError, "codes and scales are uint8"};
+    blocks = last(scales);
+    if (codes.dim() != scales.dim() || last(codes) != 16 * blocks || codes.numel() != 16 * scales.numel())
+      throw Error{PyExc_ValueError, "codes must have 16 bytes for every scale"};
+    rows = blocks > 0 ? scales.numel() / blocks : 0;
+  }
+};
+
+// mxfp4_quantize(x) -> (codes, scales) or status
+PyObject *mxfp4_quantize(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  return guarded(n, 1, [&]() -> PyObject * {
+    const at::Tensor &x = device_tensor(v[0]);
+    const Device d(x);
+    const int dt = code_of(x.scalar_type());
+    const int64_t cols = last(x), rows = cols > 0 ? x.numel() / cols : 0, blocks = (cols + CAIFX_MXFP4_BLOCK - 1) / CAIFX_MXFP4_BLOCK;
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = 16 * blocks;
+    const at::Tensor codes = at::empty(shape, x.options().dtype(at::kByte));
+    shape.back() = blocks;
+    const at::Tensor scales = at::empty(shape, x.options().dtype(at::kByte));
+    return pair(launch(api.caifx_mxfp4_quantize, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, cols, dt, d.stream()), codes, scales);
+  });
+}
+
+// mxfp4_dequantize(codes, scales, columns, dtype code) -> values or status
+PyObject *mxfp4_dequantize(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  return guarded(n, 4, [&]() -> PyObject * {
+    const Device d(device_tensor(v[0]));
+    const Micro m(d, v[0], v[1]);
+    const int64_t cols = integer(v[2]);
+    if (cols < 0 || (cols + CAIFX_MXFP4_BLOCK - 1) / CAIFX_MXFP4_BLOCK != m.blocks) throw Error{PyExc_ValueError, "columns do not fill the blocks there are"};
+    const int dt = static_cast<int>(integer(v[3]));
+    std::vector<int64_t> shape = m.scales.sizes().vec();
+    shape.back() = cols;
+    const at::Tensor y = at::empty(shape, m.codes.options().dtype(type_of(dt)));
+    return result(launch(api.caifx_mxfp4_dequantize, m.codes.data_ptr(), m.scales.data_ptr(), y.data_ptr(), m.rows, cols, dt, d.stream()), y);
+  });
+}
+
+// mxfp4_matmul(a codes, a scales, b codes, b scales, result's dtype code, out) -> y or status
+PyObject *mxfp4_matmul(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  return guarded(n, 6, [&]() -> PyObject * {
+    const Device d(device_tensor(v[0]));
+    const Micro a(d, v[0], v[1]), b(d, v[2], v[3]);
+    if (a.blocks != b.blocks) throw Error{PyExc_ValueError, "both operands must have rows of one length"};
+    const int dt = static_cast<int>(integer(v[4]));
+    const at::Tensor *out = d.optional(v[5], type_of(dt), a.rows * b.rows, "out must have the result's dtype and M x N elements");
+    if (out) apart(*out, nullptr, {&a.codes, &a.scales, &b.codes, &b.scales});
+    const at::Tensor y = out ? *out : at::empty({a.rows, b.rows}, a.codes.options().dtype(type_of(dt)));
+    const int64_t K = CAIFX_MXFP4_BLOCK * a.blocks;
+    const Scratch ws(a.codes, api.caifx_mxfp4_matmul_workspace_bytes(a.rows, b.rows, K));
+    return result(launch(api.caifx_mxfp4_matmul, a.rows, b.rows, K, a.codes.data_ptr(), a.scales.data_ptr(), b.codes.data_ptr(), b.scales.data_ptr(),
+                         y.data_ptr(), dt, ws.p(), ws.bytes, d.stream()), y);
+  });
+}
+
+// the two weights of a gated block
+struct Gated {
+  int64_t N, K;
+  int kind;
+  const void *gate, *gate_scales, *up, *up_scales;
+  Gated(const Device &d, const at::Tensor &x, PyObject *g, PyObject *u)
+  {
+    const WeightAttrs &w = attrs();
+    N = int_attr(g, w.n), K = int_attr(g, w.k), kind = static_cast<int>(int_attr(g, w.kind));
+    if (N <= 0 || K <= 0) throw Error{PyExc_ValueError, "the weight has no elements"};
+    if (int_attr(u, w.n) != N || int_attr(u, w.k) != K || int_attr(u, w.kind) != kind) throw Error{PyExc_ValueError, "both weights must have one shape and kind"};
+    for (PyObject *o : {g, u}) {
+      if (kind == CAIFX_W_MXFP4) {
+        check_mxfp4(o, N, K, x);
+      } else if (kind == CAIFX_W_F16 || kind == CAIFX_W_BF16) {
+        const Owned t(PyObject_GetAttr(o, w.wq.name));
+        d.operand(t.p, kind == CAIFX_W_F16 ? at::kHalf : at::kBFloat16, N * K, "a stored weight has N x K elements of its kind's type");
+      }
+    }
+    gate = ptr_attr(g, w.wq), up = ptr_attr(u, w.wq);
+    gate_scales = kind == CAIFX_W_MXFP4 ? ptr_attr(g, w.scales) : nullptr;
+    up_scales = kind == CAIFX_W_MXFP4 ? ptr_attr(u, w.scales) : nullptr;
+  }
+};
+
+// gated_forward(x, gate weight, up weight, keep) -> hidden, (hidden, gate, up) or status
+PyObject *gated_forward(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  return guarded(n, 4, [&]() -> PyObject * {
+    const at::Tensor &x = device_tensor(v[0]);
+    const Device d(x);
+    const int dt = code_of(x.scalar_type());
+    const Gated w(d, x, v[1], v[2]);
+    if (last(x) != w.K) throw Error{PyExc_ValueError, "a row of activations must be as long as the weights' rows"};
+    const int64_t M = x.numel() / w.K;
+    const bool keep = truth(v[3]);
+    const at::Tensor hidden = at::empty({M, w.N}, x.options());
+    const at::Tensor gate = keep ? at::empty_like(hidden) : at::Tensor(), up = keep ? at::empty_like(hidden) : at::Tensor();
+    const Scratch ws(x, api.caifx_gated_workspace_bytes(M, w.N, w.K, w.kind, dt, 0));
+    const int st = launch(api.caifx_gated_forward, M, w.N, w.K, x.data_ptr(), w.gate, w.gate_scales, w.up, w.up_scales, w.kind, hidden.data_ptr(),
+                          keep ? gate.data_ptr() : nullptr, keep ? up.data_ptr() : nullptr, dt, ws.p(), ws.bytes, d.stream());
+    if (!keep) return result(st, hidden);
+    if (st != CAIFX_OK) return PyLong_FromLong(st);
+    Owned o1(THPVariable_Wrap(hidden)), o2(THPVariable_Wrap(gate)), o3(THPVariable_Wrap(up));
+    return PyTuple_Pack(3, o1.p, o2.p, o3.p);
+  });
+}
+
+// gated_backward(grad_hidden, gate, up, gate weight, up weight, need_dx) -> (dx or None, grad_gate, grad_up) or status
+PyObject *gated_backward(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  return guarded(n, 6, [&]() -> PyObject * {
+    const at::Tensor &grad = device_tensor(v[0]);
+    const Device d(grad);
+    const int dt = code_of(grad.scalar_type());
+    const Gated w(d, grad, v[3], v[4]);
+    if (last(grad) != w.N) throw Error{PyExc_ValueError, "a row of gradients must have a value for each of the weights' rows"};
+    const int64_t M = grad.numel() / w.N;
+    const char *same = "gate and up must have the gradient's dtype and number of elements";
+    const at::Tensor &gate = d.operand(v[1], grad.scalar_type(), grad.numel(), same), &up = d.operand(v[2], grad.scalar_type(), grad.numel(), same);
+    const bool need = truth(v[5]);
+    const at::Tensor gg = at::empty({M, w.N}, grad.options()), gu = at::empty({M, w.N}, grad.options());
+    const at::Tensor dx = need ? at::empty({M, w.K}, grad.options()) : at::Tensor();
+    const Scratch ws(grad, need ? api.caifx_gated_workspace_bytes(M, w.N, w.K, w.kind, dt, 1) : 0);
+    const int st = launch(api.caifx_gated_backward, M, w.N, w.K, grad.data_ptr(), gate.data_ptr(), up.data_ptr(), w.gate, w.gate_scales, w.up, w.up_scales,
+                          w.kind, gg.data_ptr(), gu.data_ptr(), need ? dx.data_ptr() : nullptr, dt, ws.p(), ws.bytes, d.stream());
+    if (st != CAIFX_OK) return PyLong_FromLong(st);
+    Owned o1(need ? THPVariable_Wrap(dx) : Py_NewRef(Py_None)), o2(THPVariable_Wrap(gg)), o3(THPVariable_Wrap(gu));
+    return PyTuple_Pack(3, o1.p, o2.p, o3.p);
+  });
+}
+
 PyMethodDef methods[] = {
     {"bind", bind, METH_O, nullptr},
 #define M(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr},
     M(qlinear) M(grouped) M(quantize_int8) M(quantize_int4) M(elementwise) M(swiglu_backward) M(moe_build_dispatch_map) M(moe_dispatch) M(moe_combine)
     M(moe_combine_backward_grad_expert) M(moe_dispatch_backward) M(moe_combine_backward_grad_weights)
     M(adapters_forward) M(adapters_backward) M(checkpoint_pack) M(checkpoint_unpack) M(silu_multiply_checkpoint) M(swiglu_backward_checkpoint)
+    M(mxfp4_quantize) M(mxfp4_dequantize) M(mxfp4_matmul) M(gated_forward) M(gated_backward)
 #undef M
     {nullptr, nullptr, 0, nullptr}};
 

@@ -9,7 +9,7 @@ ctypes.  Function names follow the reference's CAIF_Ops entry points
 import torch
 
 from . import capi
-from .capi import F32, F16, BF16, W_INT8, W_INT4_GROUP, W_F32, W_F16, W_BF16
+from .capi import F32, F16, BF16, W_INT8, W_INT4_GROUP, W_F32, W_F16, W_BF16, W_MXFP4
 
 TORCH_DTYPE = {F32: torch.float32, F16: torch.float16, BF16: torch.bfloat16}
 CODE_OF = {v: k for k, v in TORCH_DTYPE.items()}
@@ -111,7 +111,8 @@ def convert(x, dtype):
 
 # ------------------------------------------------------------------ frozen linear
 class FrozenWeight:
-    """Device storage of one CAIF_DeviceFrozenLinear: codes, scales and the scale scheme."""
+    """Device storage of one CAIF_DeviceFrozenLinear: codes, scales and the scale scheme.  W_MXFP4: what mxfp4_quantize returns of the
+    weight [N, K] (scale_period and group_size have no meaning there)."""
 
     def __init__(self, wq, w_kind, scales, N, K, scale_period=1, group_size=128):
         self.wq, self.w_kind, self.scales = wq, w_kind, scales
@@ -321,3 +322,39 @@ def swiglu_backward_checkpoint(gate, up, grad_hidden, with_hidden=False):
     """(grad_gate, grad_up) of hidden = silu(gate) * up from the checkpoints of gate and up; with_hidden adds hidden itself, computed
     from the checkpoints."""
     return _done((_native or _calls()).swiglu_backward_checkpoint(*gate, *up, grad_hidden, with_hidden), "caifx_swiglu_backward_checkpoint")
+
+
+# ------------------------------------------------------------------ microscaled 4-bit floating point
+def mxfp4_quantize(x):
+    """(codes uint8 [..., 16 * blocks], scales uint8 [..., blocks]) of x [..., K], blocks = ceil(K / 32): codes of 4 bits (0, 1/2, 1, 3/2,
+    2, 3, 4, 6 with a sign; two a byte, the even column in the low nibble), and byte b for the power of two 2^(b - 127) of each 32
+    neighbouring values of a row.  A block that holds an infinity or a NaN is NaN as a whole (b = 255)."""
+    return _done((_native or _calls()).mxfp4_quantize(x), "caifx_mxfp4_quantize")
+
+
+def mxfp4_dequantize(codes, scales, columns, dtype):
+    """The values [..., columns] that codes and scales stand for, as a tensor of `dtype` (a torch type)."""
+    if dtype not in CODE_OF:
+        raise KeyError("mxfp4_dequantize: dtype must be fp32, fp16 or bf16")
+    return _done((_native or _calls()).mxfp4_dequantize(codes, scales, columns, CODE_OF[dtype]), "caifx_mxfp4_dequantize")
+
+
+def mxfp4_matmul(a_codes, a_scales, b_codes, b_scales, y_dtype=F32, out=None):
+    """y [M, N] = A B^T of two tensors that mxfp4_quantize returned, A [..., K] and B [N, K], on the 4-bit matrix cores.  The codes that
+    fill up a row's last block take part in the sums (mxfp4_quantize leaves zeros there)."""
+    return _done((_native or _calls()).mxfp4_matmul(a_codes, a_scales, b_codes, b_scales, y_dtype, out), "caifx_mxfp4_matmul")
+
+
+# ------------------------------------------------------------------ gated feed-forward block
+def gated_forward(x, gate_weight, up_weight, keep=False):
+    """hidden [M, N] = silu(x W_gate^T) * (x W_up^T) of x [..., K] and two frozen weights, in x's type: what the expert's forward
+    (src/caif_device_moe_frozen_expert.cpp:119-153) chains up to the down projection, in one product.  The weights are W_MXFP4, or stored
+    in x's 16-bit type.  With keep: (hidden, gate, up), the projections that gated_backward takes.  Tensors are contiguous, on one device,
+    and run on its current stream."""
+    return _done((_native or _calls()).gated_forward(x, gate_weight, up_weight, keep), "caifx_gated_forward")
+
+
+def gated_backward(grad_hidden, gate, up, gate_weight, up_weight, need_dx=True):
+    """(dx, grad_gate, grad_up) of gated_forward, dx = grad_gate W_gate + grad_up W_up [M, K].  Without need_dx, dx is None and costs
+    nothing."""
+    return _done((_native or _calls()).gated_backward(grad_hidden, gate, up, gate_weight, up_weight, need_dx), "caifx_gated_backward")

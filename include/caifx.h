@@ -69,8 +69,11 @@ enum caifx_dtype { CAIFX_F32 = 0, CAIFX_F16 = 1, CAIFX_BF16 = 2 };
  *                      src/caif_device_frozen_linear.cpp:301-318 uses the buffer as it is when storage and
  *                      compute types agree, otherwise Weight().To(target)); scales, scale_period and group_size
  *                      are ignored.  These cells run on the fp32 matrix-core kernel (operands rounded to a
- *                      16-bit compute type first, fp32 products and sums), not on the fast paths of the quantised kinds. */
-enum caifx_weight_kind { CAIFX_W_INT8 = 0, CAIFX_W_INT4_GROUP = 1, CAIFX_W_F32 = 2, CAIFX_W_F16 = 3, CAIFX_W_BF16 = 4 };
+ *                      16-bit compute type first, fp32 products and sums), not on the fast paths of the quantised kinds.
+ *  CAIFX_W_MXFP4:      microscaled 4-bit floating point, codes and scales as caifx_mxfp4_quantize lays them out for N rows of K
+ *                      columns (codes aligned to 16 bytes; scale_period and group_size are ignored).  Taken by the plain calls,
+ *                      with an addend too; the grouped ones return CAIFX_ERR_UNSUPPORTED. */
+enum caifx_weight_kind { CAIFX_W_INT8 = 0, CAIFX_W_INT4_GROUP = 1, CAIFX_W_F32 = 2, CAIFX_W_F16 = 3, CAIFX_W_BF16 = 4, CAIFX_W_MXFP4 = 5 };
 
 CAIFX_API const char *caifx_status_string(int status);
 /* ABI version of this header: major*1000 + minor. */
@@ -530,6 +533,58 @@ CAIFX_API int caifx_silu_multiply_checkpoint(const void *gate, const void *up, v
 CAIFX_API int caifx_swiglu_backward_checkpoint(const void *gate_codes, const float *gate_scales, const void *up_codes,
                                      const float *up_scales, const void *grad_hidden, void *grad_gate, void *grad_up,
                                      void *hidden, int64_t rows, int64_t cols, int dtype, caifx_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Microscaled 4-bit floating point: codes of one sign, two exponent and one mantissa bit (0, 1/2, 1, 3/2, 2, 3, 4, 6 and their
+ * negatives) and one power of two per CAIFX_MXFP4_BLOCK neighbouring values of a row; no counterpart in the reference, whose
+ * 4-bit storage is CAIFX_W_INT4_GROUP.  A row is cut into ceil(cols / 32) blocks, the last one filled up with zeros:
+ *   codes  uint8 [rows, 16 * blocks], two codes per byte, the even column in the low nibble (bit 3 of a code is its sign);
+ *   scales uint8 [rows, blocks], byte b standing for 2^(b - 127), 255 for a NaN.
+ * Quantising: b = clamp(floor(log2 max|x|) - 2, -127, 127) + 127 (0 for a block of zeros), code = the nearest value to
+ * x 2^(127 - b), ties to the even mantissa, 6 for everything beyond 5.  A block that holds an infinity or a NaN gets byte 255 and
+ * codes of zero: all its values are NaN.  Results alias no input.  CAIFX_ERR_UNSUPPORTED beyond 2^29 blocks.
+ * ------------------------------------------------------------------------- */
+#define CAIFX_MXFP4_BLOCK 32
+
+/* input [rows, cols] of dtype, any alignment of its type; codes aligned to 16 bytes. */
+CAIFX_API int caifx_mxfp4_quantize(const void *input, void *codes, void *scales, int64_t rows, int64_t cols, int dtype,
+                         caifx_stream_t stream);
+/* output [rows, cols] = T(code * 2^(b - 127)) */
+CAIFX_API int caifx_mxfp4_dequantize(const void *codes, const void *scales, void *output, int64_t rows, int64_t cols, int dtype,
+                           caifx_stream_t stream);
+/* y[M,N] = A B^T with both operands in that form, A of M rows and B of N rows of K columns; products and sums are fp32, one rounding
+ * to y_dtype.  The codes that fill up a row's last block take part in the sums: they have to be zeros, as caifx_mxfp4_quantize leaves
+ * them.  Both codes aligned to 16 bytes.  workspace: caifx_mxfp4_matmul_workspace_bytes (may be 0, CAIFX_ERR_WORKSPACE_TOO_SMALL for
+ * less).  CAIFX_ERR_UNSUPPORTED beyond 2^30 rows of either and beyond K = 2^30. */
+CAIFX_API int caifx_mxfp4_matmul(int64_t M, int64_t N, int64_t K, const void *a_codes, const void *a_scales, const void *b_codes,
+                       const void *b_scales, void *y, int y_dtype, void *workspace, size_t workspace_bytes,
+                       caifx_stream_t stream);
+CAIFX_API size_t caifx_mxfp4_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
+
+/* ---------------------------------------------------------------------------
+ * Gated feed-forward block over two frozen weights [N,K] of one kind, gate and up: what CAIF_DeviceMoEFrozenExpert::ForwardImpl
+ * chains up to its down projection (src/caif_device_moe_frozen_expert.cpp:119-153), both projections and the gating in one product,
+ * and the backward pass of that part (:266-316).
+ * w_kind: CAIFX_W_MXFP4, or CAIFX_W_F16 / CAIFX_W_BF16 with dtype the same type (scales NULL then); CAIFX_ERR_UNSUPPORTED for other
+ * kinds.  All activations and results are of `dtype`, contiguous, any alignment of it; weights are aligned to 16 bytes.  Results alias
+ * no input and no other result.  fp32 uses three bf16 pieces of each activation, which add up to it.  CAIFX_ERR_UNSUPPORTED beyond
+ * 2^30 rows and an N or K of 2^26.  workspace: caifx_gated_workspace_bytes, CAIFX_ERR_WORKSPACE_TOO_SMALL for less.
+ * ------------------------------------------------------------------------- */
+
+/* With g = x w_gate^T and u = x w_up^T in fp32: hidden[M,N] = T(silu(g) * u), gate = T(g), up = T(u).  gate and up are what the
+ * backward needs; both or neither may be NULL.  hidden is rounded once (the reference's chain rounds the projections and silu too). */
+CAIFX_API int caifx_gated_forward(int64_t M, int64_t N, int64_t K, const void *x, const void *w_gate, const void *scales_gate,
+                        const void *w_up, const void *scales_up, int w_kind, void *hidden, void *gate, void *up, int dtype,
+                        void *workspace, size_t workspace_bytes, caifx_stream_t stream);
+/* With g, u = gate, up and s = 1 / (1 + exp(-g)):
+ *   grad_up = T(grad_hidden * g s),  grad_gate = T(grad_hidden * u * s (1 + g (1 - s))),
+ *   dx[M,K] = T(grad_gate w_gate + grad_up w_up), one sum of 2 N products.
+ * dx may be NULL (a first layer): then only the gating's gradients are formed, and the weights and scales may be NULL too. */
+CAIFX_API int caifx_gated_backward(int64_t M, int64_t N, int64_t K, const void *grad_hidden, const void *gate, const void *up,
+                         const void *w_gate, const void *scales_gate, const void *w_up, const void *scales_up, int w_kind,
+                         void *grad_gate, void *grad_up, void *dx, int dtype, void *workspace, size_t workspace_bytes,
+                         caifx_stream_t stream);
+CAIFX_API size_t caifx_gated_workspace_bytes(int64_t M, int64_t N, int64_t K, int w_kind, int dtype, int backward);
 
 #ifdef __cplusplus
 }
