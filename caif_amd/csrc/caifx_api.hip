@@ -121,7 +121,7 @@ static size_t workspace_bytes(int64_t M, int64_t N, int64_t K, int x_dtype, int 
   a.x_dtype = x_dtype;
   a.compute_dtype = compute_dtype;
   a.w.kind = w_kind;
-  if (w_kind == CAIFX_W_MXFP4) return mxfp4_workspace_bytes(a, backward);
+  if (w_kind == CAIFX_W_MXFP4) return mxfp4_workspace_bytes(a, backward, dense_copy);
   const size_t f32_bytes = mfma_f32_workspace_bytes(a, backward);
   // float storage runs on the fp32 matrix-core instruction unless it is stored in the 16-bit compute type itself
   if (float_kind(w_kind) && !same_16bit(w_kind, compute_dtype)) return f32_bytes;

@@ -16,6 +16,7 @@
 // Against the kernels that dequantise inside the product (forward 361 us, input gradient 390 us at M = 4096, N = 11008,
 // K = 4096, int4, bf16) the two launches take 293 and 251 us in the same run.
 #include "caifx_gemm_regw.hpp"
+#include "caifx_wide.hpp"
 
 #include <atomic>
 #include <type_traits>
@@ -40,6 +41,9 @@ struct WideArgs {
   bool zero_rest;
   unsigned long long *stamps;      // measurement only, see mfma_grouped_tile_stamps
   long long stamps_capacity;
+  // the forms over a pair of weights (WIDE_GATED, WIDE_CHAIN)
+  const void *a2, *b2;
+  void *gate, *up;
 };
 
 // A result tile has 64 WI rows and 64 WJ columns.  Wave (wm, wn) owns rows h 32 WI + wm 16 WI + [0, 16 WI) and columns
@@ -51,11 +55,16 @@ struct WideArgs {
 // unit for 256 x 256) are on their way at any time, and every request has one and a half steps to arrive.  Requests
 // complete in issue order, so the wait for the half tile that is read next is an exact count (a wave issues WI + WJ
 // per half).
-template <typename CT, int WI, int WJ, bool kGrouped>
+// WIDE_GATED: half g of the columns belongs to the g-th weight, the same BN / 2 columns of each, so that a wave's accumulators of the two
+// halves hold gate and up of the same values and the gating happens where they are.  WIDE_CHAIN: the steps run through the first pair
+// of operands and then through the second.
+template <typename CT, int WI, int WJ, bool kGrouped, int kForm = WIDE_PLAIN>
 __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(WideArgs g)
 {
   typedef typename Mfma32<CT>::vec_t vec_t;
+  constexpr bool kGated = kForm == WIDE_GATED, kChain = kForm == WIDE_CHAIN;
   constexpr int BM = 64 * WI, BN = 64 * WJ;
+  constexpr int BC = kGated ? BN / 2 : BN;      // columns of the result
   constexpr int kASlot = BM / 2 * 128, kBSlot = BN / 2 * 128;      // LDS bytes of half an operand tile
   constexpr int kBBase = 4 * kASlot;
   constexpr int kBand = kBandRows / BM;
@@ -69,7 +78,7 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(Wi
 
   // XCD x (workgroup id mod 8, each with its own L2) walks the x-th contiguous eighth of a list that runs through bands
   // of 1024 rows column by column: the 256 x 256 tiles it works on at a time share 4 row and 8 column panels
-  const int64_t col_tiles = (g.C + BN - 1) / BN, row_tiles = (g.M + BM - 1) / BM;
+  const int64_t col_tiles = (g.C + BC - 1) / BC, row_tiles = (g.M + BM - 1) / BM;
   int64_t row0, col0, row_end = g.M;
   uint64_t b_ptr = reinterpret_cast<uint64_t>(g.b);
   int64_t stamp_pos = -1;
@@ -99,7 +108,7 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(Wi
     const int64_t within = pos - band * kBand * col_tiles;
     const int64_t left = row_tiles - band * kBand;
     const int64_t band_rows = left < kBand ? left : kBand;
-    col0 = (within / band_rows) * BN;
+    col0 = (within / band_rows) * BC;
     row0 = (band * kBand + within % band_rows) * BM;
   }
 
@@ -120,20 +129,30 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(Wi
 #pragma unroll
     for (int i = 0; i < WJ; ++i) {
       const int lrow = 8 * (wave + 4 * i) + (lane >> 3);
-      int64_t c = col0 + h * (BN / 2) + lrow;
+      int64_t c = col0 + (kGated ? 0 : h * (BN / 2)) + lrow;
       if (c >= g.C) c = g.C - 1;
       b_voff[h][i] = static_cast<uint32_t>((c - col0) * g.R * 2 + (((lane & 7) ^ ((lrow ^ (lrow >> 3)) & 7)) << 4));
     }
   }
   const uint64_t a_base = uniform64(reinterpret_cast<uint64_t>(g.a) + static_cast<uint64_t>(row0 * g.R * 2));
   const uint64_t b_base = uniform64(b_ptr + static_cast<uint64_t>(col0 * g.R * 2));
-  const int steps = static_cast<int>(g.R / kBK);
+  const uint64_t b2_base = kForm != WIDE_PLAIN ? uniform64(reinterpret_cast<uint64_t>(g.b2) + static_cast<uint64_t>(col0 * g.R * 2)) : 0;
+  const uint64_t a2_base = kChain ? uniform64(reinterpret_cast<uint64_t>(g.a2) + static_cast<uint64_t>(row0 * g.R * 2)) : 0;
+  const int part = static_cast<int>(g.R / kBK);
+  const int steps = kChain ? 2 * part : part;
   const int last = steps - 1;
   auto request = [&](int s, int h, int slot, int x) __attribute__((always_inline)) {
     const uint32_t k0 = static_cast<uint32_t>(s < last ? s : last) * 128;          // past the end: the last step again
     const bool is_a = x < WI;
     const int i = is_a ? x : x - WI;
-    const uint64_t src = (is_a ? a_base : b_base) + k0;
+    uint64_t src;
+    if constexpr (kChain) {
+      // (the second pair begins `part` steps into the sum)
+      const bool second = s >= part;
+      src = (second ? (is_a ? a2_base : b2_base) - static_cast<uint64_t>(part) * 128 : (is_a ? a_base : b_base)) + k0;
+    } else {
+      src = (is_a ? a_base : kGated && h == 1 ? b2_base : b_base) + k0;
+    }
     const uint32_t dst = lds0 + (is_a ? slot * kASlot : kBBase + slot * kBSlot) + (wave + 4 * i) * 1024;
     const uint32_t voff = is_a ? a_voff[h][is_a ? i : 0] : b_voff[h][is_a ? 0 : i];
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(voff), "s"(src) : "memory");
@@ -306,6 +325,48 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(Wi
       }
     }
   };
+  // gated: the result and, where they are kept, the two projections, one after the other through LDS
+  auto store_gated = [&](auto what_) __attribute__((always_inline)) {
+    constexpr int what = decltype(what_)::value;         // 0 hidden, 1 gate, 2 up
+    constexpr int kPitch = BC * sizeof(CT) + 32;
+    constexpr int kLanesPerRow = BC / 8;
+    constexpr int kRowsPerInstr = 64 / kLanesPerRow;
+    constexpr int kInstr = BM / (4 * kRowsPerInstr);
+    CT *dp = static_cast<CT *>(what == 0 ? g.d : what == 1 ? g.gate : g.up);
+    const int chunk = lane % kLanesPerRow;
+    const int64_t gcol = col0 + chunk * 8;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < WI; ++i)
+#pragma unroll
+        for (int c = 0; c < WJ; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int lrow = h * (BM / 2) + wm * 16 * WI + i * 16 + 4 * kq + r;
+            const float a = acc[h][0][i][c][r], u = acc[h][1][i][c][r];
+            *reinterpret_cast<CT *>(smem + lrow * kPitch + (wn * 16 * WJ + c * 16 + r16) * sizeof(CT)) =
+                from_f32<CT>(what == 0 ? gate_act(a) * u : what == 1 ? a : u);
+          }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < kInstr; ++b) {
+      const int lrow = (b * 4 + wave) * kRowsPerInstr + lane / kLanesPerRow;
+      const int64_t grow = row0 + lrow;
+      const u32x4_t v = *reinterpret_cast<const u32x4_t *>(smem + lrow * kPitch + chunk * 16);
+      if (grow < row_end && gcol < g.C) *reinterpret_cast<u32x4_t *>(dp + grow * g.C + gcol) = v;
+    }
+  };
+  if constexpr (kGated) {
+    store_gated(std::integral_constant<int, 0>{});
+    if (g.gate) {
+      __syncthreads();
+      store_gated(std::integral_constant<int, 1>{});
+      __syncthreads();
+      store_gated(std::integral_constant<int, 2>{});
+    }
+    return;
+  }
   auto store_as = [&](auto type_) __attribute__((always_inline)) {
     if (g.addend) store(type_, std::true_type{});
     else store(type_, std::false_type{});
@@ -462,14 +523,14 @@ int launch_dense(const DenseArgs &g, int kind, bool transposed, int experts, hip
   return launch_status();
 }
 
-template <typename CT, int WI, int WJ, bool kGrouped>
+template <typename CT, int WI, int WJ, bool kGrouped, int kForm = WIDE_PLAIN>
 int launch_wide(const WideArgs &g, hipStream_t s)
 {
-  constexpr int BM = 64 * WI, BN = 64 * WJ;
+  constexpr int BM = 64 * WI, BN = 64 * WJ, BC = kForm == WIDE_GATED ? BN / 2 : BN;
   constexpr int kRing = (BM + BN) * 256, kStore16 = BM * (BN * 2 + 32), kStore32 = BM / 2 * (BN * 4 + 32);
   constexpr int kStore = kStore16 > kStore32 ? kStore16 : kStore32;
   constexpr int kLds = kRing > kStore ? kRing : kStore;
-  auto kern = wide_gemm_kernel<CT, WI, WJ, kGrouped>;
+  auto kern = wide_gemm_kernel<CT, WI, WJ, kGrouped, kForm>;
   static std::atomic<bool> raised{false};
   if (!raised.load(std::memory_order_relaxed)) {
     // the attribute is per kernel and sticky; two threads racing here both set it, which is harmless
@@ -478,7 +539,7 @@ int launch_wide(const WideArgs &g, hipStream_t s)
     raised.store(true, std::memory_order_relaxed);
   }
   // grouped: segment lengths live on the device; an upper bound, every expert can add one partial tile
-  const int64_t tiles = ((g.M + BM - 1) / BM + (kGrouped ? g.num_experts : 0)) * ((g.C + BN - 1) / BN);
+  const int64_t tiles = ((g.M + BM - 1) / BM + (kGrouped ? g.num_experts : 0)) * ((g.C + BC - 1) / BC);
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((tiles + 7) / 8 * 8)), dim3(256), kLds, s, g);
   return launch_status();
 }
@@ -577,13 +638,14 @@ double regw_us(const GemmArgs &a)
   return 4.0 * static_cast<double>((tiles + 255) / 256) + steps * rounds_cost(tiles, 256, 0.90, 0.55, 0.0014);
 }
 
-template <typename CT, bool kGrouped>
+template <typename CT, bool kGrouped, int kForm = WIDE_PLAIN>
 int pick_wide(const WideArgs &g, hipStream_t s)
 {
-  switch (best_tile(g.M, g.C, g.num_experts)) {
-    case TILE_256: return launch_wide<CT, 4, 4, kGrouped>(g, s);
-    case TILE_128x256: return launch_wide<CT, 2, 4, kGrouped>(g, s);
-    default: return launch_wide<CT, 2, 2, kGrouped>(g, s);
+  // (gated: as many tiles as a plain product with both weights' columns has)
+  switch (best_tile(g.M, kForm == WIDE_GATED ? 2 * g.C : g.C, g.num_experts)) {
+    case TILE_256: return launch_wide<CT, 4, 4, kGrouped, kForm>(g, s);
+    case TILE_128x256: return launch_wide<CT, 2, 4, kGrouped, kForm>(g, s);
+    default: return launch_wide<CT, 2, 2, kGrouped, kForm>(g, s);
   }
 }
 template <typename CT>
@@ -723,6 +785,37 @@ int mfma_wide(const GemmArgs &a, bool backward, hipStream_t s)
   if (st != CAIFX_OK) return st;
   g.b = a.workspace;
   return product();
+}
+
+bool wide_takes(int64_t M, int64_t C, int64_t R)
+{
+  // (row offsets inside a tile have 32 bits)
+  return M > 0 && M <= (int64_t{1} << 30) && C > 0 && C % 8 == 0 && R % kBK == 0 && R >= 2 * kBK && R < (int64_t{1} << 22) &&
+         ((M + 127) / 128) * ((C + 63) / 64) <= (int64_t{1} << 30);
+}
+
+int wide_product(const WideProduct &p, hipStream_t s)
+{
+  WideArgs g{};
+  g.a = p.a[0];
+  g.a2 = p.a[1];
+  g.b = p.b[0];
+  g.b2 = p.b[1];
+  g.d = p.d;
+  g.gate = p.gate;
+  g.up = p.up;
+  g.addend = p.addend;
+  g.M = p.M;
+  g.C = p.C;
+  g.R = p.R;
+  g.d_dtype = p.d_dtype;
+  const auto go = [&](auto type_) {
+    typedef decltype(type_) CT;
+    if (p.form == WIDE_GATED) return pick_wide<CT, false, WIDE_GATED>(g, s);
+    if (p.form == WIDE_CHAIN) return pick_wide<CT, false, WIDE_CHAIN>(g, s);
+    return pick_wide<CT, false>(g, s);
+  };
+  return p.compute_dtype == CAIFX_BF16 ? go(bf16_t{}) : go(f16_t{});
 }
 
 }  // namespace caifx

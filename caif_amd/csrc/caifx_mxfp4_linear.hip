@@ -81,8 +81,54 @@ int rows_run(const RowsArgs &g, bool mx, int weights, int compute_dtype, bool di
 // whether the row kernels can read the activations where they are
 bool direct_type(const Product &p) { return p.compute_dtype != CAIFX_F32 && p.x_dtype == p.compute_dtype && p.R % 8 == 0; }
 
-// Runs the product, or with room.p == nullptr adds up what it needs of the workspace.
-int product(const Product &p, Room &room, bool only_size, hipStream_t s)
+bool aligned16(const void *a, const void *b = nullptr, const void *c = nullptr, const void *d = nullptr)
+{
+  return aligned_to(a, 16) && aligned_to(b, 16) && aligned_to(c, 16) && aligned_to(d, 16);
+}
+
+// Whether a product with this many rows runs on dense operands (caifx_gemm_wide.hip) instead of the row kernels.
+bool wide_product_pays(const Product &p)
+{
+  if (p.compute_dtype == CAIFX_F32 || !wide_takes(p.M, p.N, up_to(p.R, 64)) || p.N * up_to(p.R, 64) >= (int64_t{1} << 32)) return false;
+  return p.M > (p.w[0].mx ? 256 : 64);
+}
+
+// The product on dense operands: the weights dequantised into the workspace, activations of another type or length copied.
+int product_wide(const Product &p, Room &room, bool only_size, hipStream_t s)
+{
+  const int64_t R = up_to(p.R, 64);
+  const int to = p.compute_dtype;
+  WideProduct d{};
+  d.form = p.weights == 2 ? WIDE_GATED : WIDE_PLAIN;
+  for (int i = 0; i < p.weights; ++i) {
+    d.b[i] = p.w[i].p;
+    if (!p.w[i].mx && R == p.R) continue;
+    void *copy = room.take(static_cast<size_t>(p.N) * static_cast<size_t>(R) * 2);
+    d.b[i] = copy;
+    const int st = only_size ? CAIFX_OK : operand_dense(p.w[i].p, p.w[i].scales, p.w[i].mx ? OPERAND_MX : to, p.N, p.R, to, copy, R, R, 0, s);
+    if (st != CAIFX_OK) return st;
+  }
+  d.a[0] = p.x;
+  if (p.x_dtype != to || R != p.R || (!only_size && !aligned_to(p.x, 16))) {
+    void *copy = room.take(static_cast<size_t>(p.M) * static_cast<size_t>(R) * 2);
+    d.a[0] = copy;
+    const int st = only_size ? CAIFX_OK : operand_dense(p.x, nullptr, p.x_dtype, p.M, p.R, to, copy, R, R, 0, s);
+    if (st != CAIFX_OK) return st;
+  }
+  d.d = p.y;
+  d.gate = p.gate;
+  d.up = p.up;
+  d.addend = p.addend;
+  d.M = p.M;
+  d.C = p.N;
+  d.R = R;
+  d.compute_dtype = to;
+  d.d_dtype = p.y_dtype;
+  return only_size ? CAIFX_OK : wide_product(d, s);
+}
+
+// The product on the row kernels, any sizes and types.
+int product_rows(const Product &p, Room &room, bool only_size, hipStream_t s)
 {
   Product d = p;
   // rows of a stored weight start at any multiple of two bytes where R is odd: the row kernels take them from a copy
@@ -116,6 +162,23 @@ int product(const Product &p, Room &room, bool only_size, hipStream_t s)
   return only_size ? CAIFX_OK : rows_run(g, p.w[0].mx, p.weights, p.compute_dtype, direct, s);
 }
 
+// What either way can need.  Results or activations at addresses that the dense product does not take run on the row kernels.
+size_t product_bytes(const Product &p, bool dense_copy = true)
+{
+  Room rows, wide;
+  product_rows(p, rows, true, nullptr);
+  if (!dense_copy || !wide_product_pays(p)) return rows.used;
+  product_wide(p, wide, true, nullptr);
+  return rows.used > wide.used ? rows.used : wide.used;
+}
+int product(const Product &p, void *workspace, size_t bytes, hipStream_t s)
+{
+  Room room{static_cast<char *>(workspace), 0};
+  // (activations at an odd address would need a copy that the query did not count: the row kernels' order has room)
+  if (wide_product_pays(p) && bytes >= product_bytes(p) && aligned16(p.x, p.y, p.addend) && aligned16(p.gate, p.up)) return product_wide(p, room, false, s);
+  return product_rows(p, room, false, s);
+}
+
 // y[M,K] = sum over the weights of x[i][M,N] w[i][N,K], as one reduction over their rows
 struct Gradient {
   int64_t M, N, K;
@@ -128,7 +191,41 @@ struct Gradient {
   const void *addend;
 };
 
-int gradient(const Gradient &p, Room &room, bool only_size, hipStream_t s)
+// Whether a gradient runs on the dense product behind the transposed copies.
+bool wide_gradient_pays(const Gradient &p)
+{
+  return p.compute_dtype != CAIFX_F32 && p.M > 64 && wide_takes(p.M, p.K, up_to(p.N, 64));
+}
+
+int gradient_wide(const Gradient &p, Room &room, bool only_size, hipStream_t s)
+{
+  const int to = p.compute_dtype;
+  const int64_t R = up_to(p.N, 64);
+  WideProduct d{};
+  d.form = p.weights == 2 ? WIDE_CHAIN : WIDE_PLAIN;
+  for (int i = 0; i < p.weights; ++i) {
+    void *copy = room.take(static_cast<size_t>(p.K) * static_cast<size_t>(R) * 2);
+    d.b[i] = copy;
+    int st = only_size ? CAIFX_OK : operand_transposed(p.w[i].p, p.w[i].scales, p.w[i].mx ? OPERAND_MX : to, p.N, p.K, to, copy, R, R, 0, s);
+    if (st != CAIFX_OK) return st;
+    d.a[i] = p.x[i];
+    if (p.x_dtype == to && R == p.N) continue;
+    void *x = room.take(static_cast<size_t>(p.M) * static_cast<size_t>(R) * 2);
+    d.a[i] = x;
+    st = only_size ? CAIFX_OK : operand_dense(p.x[i], nullptr, p.x_dtype, p.M, p.N, to, x, R, R, 0, s);
+    if (st != CAIFX_OK) return st;
+  }
+  d.d = p.y;
+  d.addend = p.addend;
+  d.M = p.M;
+  d.C = p.K;
+  d.R = R;
+  d.compute_dtype = to;
+  d.d_dtype = p.y_dtype;
+  return only_size ? CAIFX_OK : wide_product(d, s);
+}
+
+int gradient_rows(const Gradient &p, Room &room, bool only_size, hipStream_t s)
 {
   const int to = stored_as(p.compute_dtype);
   const int64_t pitch = up_to(p.N, kRowsChunk), stride = pitch * p.weights;       // whole chunks of each weight's rows
@@ -154,6 +251,21 @@ int gradient(const Gradient &p, Room &room, bool only_size, hipStream_t s)
   g.addend = p.addend;
   g.y_dtype = p.y_dtype;
   return rows_run(g, false, 1, p.compute_dtype, false, s);
+}
+
+size_t gradient_bytes(const Gradient &p)
+{
+  Room rows, wide;
+  gradient_rows(p, rows, true, nullptr);
+  if (!wide_gradient_pays(p)) return rows.used;
+  gradient_wide(p, wide, true, nullptr);
+  return rows.used > wide.used ? rows.used : wide.used;
+}
+int gradient(const Gradient &p, void *workspace, hipStream_t s)
+{
+  Room room{static_cast<char *>(workspace), 0};
+  if (wide_gradient_pays(p) && aligned16(p.x[0], p.x[1], p.y, p.addend)) return gradient_wide(p, room, false, s);
+  return gradient_rows(p, room, false, s);
 }
 
 Product product_of(const GemmArgs &a)
@@ -194,23 +306,21 @@ bool fits(int64_t M, int64_t N, int64_t K) { return M <= (1 << 30) && N < (1 << 
 
 }  // namespace
 
-size_t mxfp4_workspace_bytes(const GemmArgs &a, bool backward)
+size_t mxfp4_workspace_bytes(const GemmArgs &a, bool backward, bool dense_copy)
 {
   if (a.M <= 0 || a.N <= 0 || a.K <= 0 || !fits(a.M, a.N, a.K)) return 0;
-  Room room;
-  if (backward) gradient(gradient_of(a), room, true, nullptr);
-  else product(product_of(a), room, true, nullptr);
-  return room.used;
+  if (backward) return dense_copy ? gradient_bytes(gradient_of(a)) : 0;
+  return product_bytes(product_of(a), dense_copy);
 }
 
 int mxfp4_linear(const GemmArgs &a, bool backward, hipStream_t s)
 {
   if (!fits(a.M, a.N, a.K)) return CAIFX_ERR_UNSUPPORTED;
-  const size_t need = mxfp4_workspace_bytes(a, backward);
+  const size_t need = mxfp4_workspace_bytes(a, backward, backward);
   const bool misaligned = !backward && need == 0 && !aligned_to(a.x, 16);      // (packed then, into room that the query did not count)
   if (misaligned || (need > 0 && (!a.workspace || a.workspace_bytes < need || !aligned_to(a.workspace, 16)))) return CAIFX_ERR_UNSUPPORTED;
-  Room room{static_cast<char *>(a.workspace), 0};
-  return backward ? gradient(gradient_of(a), room, false, s) : product(product_of(a), room, false, s);
+  if (backward) return gradient(gradient_of(a), a.workspace, s);
+  return product(product_of(a), a.workspace, a.workspace && aligned_to(a.workspace, 16) ? a.workspace_bytes : 0, s);
 }
 
 }  // namespace caifx
@@ -218,6 +328,10 @@ int mxfp4_linear(const GemmArgs &a, bool backward, hipStream_t s)
 using namespace caifx;
 
 namespace {
+
+int64_t blocks_of(int64_t columns) { return (columns + CAIFX_MXFP4_BLOCK - 1) / CAIFX_MXFP4_BLOCK; }
+// whether a product of two operands in 4 bits runs in tiles rather than on the row kernels
+bool tiles_pay(int64_t M, int64_t N, int64_t blocks) { return M > 64 && mx_gemm_takes(M, N, blocks); }
 
 // what both gated calls check; `go`: there is work
 int gated_check(int64_t M, int64_t N, int64_t K, int w_kind, int dtype, bool &go)
@@ -260,14 +374,8 @@ extern "C" {
 size_t caifx_mxfp4_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K)
 {
   if (M <= 0 || N <= 0 || K <= 0 || !fits(M, N, K)) return 0;
-  Room room;
-  room.take(static_cast<size_t>(M) * static_cast<size_t>(up_to(K, CAIFX_MXFP4_BLOCK)) * 2);
-  GemmArgs a{};
-  a.M = M;
-  a.N = N;
-  a.K = up_to(K, CAIFX_MXFP4_BLOCK);
-  a.x_dtype = a.compute_dtype = CAIFX_BF16;
-  return room.used + mxfp4_workspace_bytes(a, false);
+  const int64_t blocks = blocks_of(K);
+  return tiles_pay(M, N, blocks) ? mx_gemm_workspace_bytes(M, N, blocks) : 0;
 }
 
 int caifx_mxfp4_matmul(int64_t M, int64_t N, int64_t K, const void *a_codes, const void *a_scales, const void *b_codes, const void *b_scales, void *y,
@@ -280,34 +388,34 @@ int caifx_mxfp4_matmul(int64_t M, int64_t N, int64_t K, const void *a_codes, con
   if (!aligned_to(a_codes, 16) || !aligned_to(b_codes, 16) || !aligned_to(y, dtype_size(y_dtype)) || !aligned_to(workspace, 16)) return CAIFX_ERR_MISALIGNED;
   const size_t need = caifx_mxfp4_matmul_workspace_bytes(M, N, K);
   if (need > 0 && (!workspace || workspace_bytes < need)) return CAIFX_ERR_WORKSPACE_TOO_SMALL;
-  const int64_t R = up_to(K, CAIFX_MXFP4_BLOCK);
-  Room room{static_cast<char *>(workspace), 0};
-  void *x = room.take(static_cast<size_t>(M) * static_cast<size_t>(R) * 2);
-  const int st = operand_dense(a_codes, a_scales, OPERAND_MX, M, R, CAIFX_BF16, x, R, R, 0, as_stream(stream));
-  if (st != CAIFX_OK) return st;
-  Product p{};
-  p.M = M;
-  p.N = N;
-  p.R = R;
-  p.x = x;
-  p.x_dtype = p.compute_dtype = CAIFX_BF16;
-  p.weights = 1;
-  p.w[0] = Weight{b_codes, b_scales, true};
-  p.y = y;
-  p.y_dtype = y_dtype;
-  return product(p, room, false, as_stream(stream));
+  const int64_t blocks = blocks_of(K);
+  // (scales at an odd address would need a copy that the query did not count)
+  if (tiles_pay(M, N, blocks) && (need > 0 || (aligned_to(a_scales, 16) && aligned_to(b_scales, 16))))
+    return mx_gemm(M, N, blocks, a_codes, a_scales, b_codes, b_scales, y, y_dtype, workspace, as_stream(stream));
+  RowsArgs g{};
+  g.x = a_codes;
+  g.xs = static_cast<const uint8_t *>(a_scales);
+  g.w[0] = b_codes;
+  g.s[0] = static_cast<const uint8_t *>(b_scales);
+  g.M = M;
+  g.N = N;
+  g.R = 32 * blocks;
+  g.blocks = blocks;
+  g.w_pitch = 16 * blocks;
+  g.chunks = static_cast<int>(chunks_of(g.R));
+  g.y = y;
+  g.y_dtype = y_dtype;
+  return rows_both(g, as_stream(stream));
 }
 
 size_t caifx_gated_workspace_bytes(int64_t M, int64_t N, int64_t K, int w_kind, int dtype, int backward)
 {
   bool go;
   if (gated_check(M, N, K, w_kind, dtype, go) != CAIFX_OK || !go) return 0;
-  Room room;
-  if (backward) gradient(gated_gradient(M, N, K, w_kind, dtype), room, true, nullptr);
-  else product(gated_product(M, N, K, w_kind, dtype), room, true, nullptr);
-  // (activations at an address that no 16-byte access takes are packed; few rows are all the query leaves out otherwise)
-  if (!backward && room.used == 0) room.take(packed_bytes(M, chunks_of(K), dtype));
-  return room.used;
+  if (backward) return gradient_bytes(gated_gradient(M, N, K, w_kind, dtype));
+  const size_t bytes = product_bytes(gated_product(M, N, K, w_kind, dtype));
+  // few rows are read where they are, but packed first at an address that no 16-byte access takes
+  return bytes > 0 ? bytes : packed_bytes(M, chunks_of(K), dtype);
 }
 
 int caifx_gated_forward(int64_t M, int64_t N, int64_t K, const void *x, const void *w_gate, const void *scales_gate, const void *w_up,
@@ -335,8 +443,7 @@ int caifx_gated_forward(int64_t M, int64_t N, int64_t K, const void *x, const vo
   p.y = hidden;
   p.gate = gate;
   p.up = up;
-  Room room{static_cast<char *>(workspace), 0};
-  return product(p, room, false, as_stream(stream));
+  return product(p, workspace, workspace_bytes, as_stream(stream));
 }
 
 int caifx_gated_backward(int64_t M, int64_t N, int64_t K, const void *grad_hidden, const void *gate, const void *up, const void *w_gate,
@@ -370,8 +477,7 @@ int caifx_gated_backward(int64_t M, int64_t N, int64_t K, const void *grad_hidde
   p.w[1].p = w_up;
   p.w[1].scales = scales_up;
   p.y = dx;
-  Room room{static_cast<char *>(workspace), 0};
-  return gradient(p, room, false, s);
+  return gradient(p, workspace, s);
 }
 
 }  // extern "C"

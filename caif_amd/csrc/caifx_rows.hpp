@@ -7,10 +7,11 @@
 // launch of a usual weight has all of it on its way at once.  The reduction indices inside a chunk are permuted such that a lane's 16
 // bytes of codes are one block of 32 values of one weight row: lane (j, q) of v_mfma_f32_16x16x32 holds block q (then q + 4) of row j,
 // instruction i takes its values 8 i .. 8 i + 7, and the activations follow that order.  The codes become operands by
-// v_cvt_scalef32_pk_{bf16,f16}_fp4 with the block's scale: exact in bf16, in fp16 rounded like any weight that is cast to it.
+// v_cvt_scalef32_pk_{bf16,f16}_fp4 with the block's scale: exact in bf16, in fp16 rounded like any weight that is cast to it.  Where the
+// activations have 4 bits too, the same blocks go into v_mfma_scale_f32_16x16x128_f8f6f4 as they are.
 #pragma once
 
-#include "caifx_internal.hpp"
+#include "caifx_wide.hpp"
 
 namespace caifx {
 
@@ -22,6 +23,7 @@ struct RowsArgs {
   int64_t x_pitch;
   const void *w[2];       // MX codes or dense rows of the compute type
   const uint8_t *s[2];    // MX scales
+  const uint8_t *xs;      // both in 4 bits: scales of x, whose codes are rows of w_pitch bytes
   int64_t M, N, R;        // R: elements of the reduction (direct: a multiple of 8)
   int64_t blocks;         // MX blocks of a weight row
   int64_t w_pitch;        // bytes of a weight row
@@ -32,11 +34,22 @@ struct RowsArgs {
   int y_dtype;
 };
 
-enum { ROWS_MX = 0, ROWS_DENSE = 1 };
+enum { ROWS_MX = 0, ROWS_DENSE = 1, ROWS_BOTH = 2 };      // ROWS_BOTH: weight and activations in microscaled 4 bits
 // first of the eight reduction elements that lane group q holds for instruction u (0 .. 7) of a chunk
 template <int kWeight> __device__ __forceinline__ int rows_element(int u, int q)
 {
   return kWeight == ROWS_MX ? 128 * (u >> 2) + 32 * q + 8 * (u & 3) : 32 * u + 8 * q;
+}
+
+// one block of 32 values of each of 16 rows and 16 columns per lane group, in 4 bits with their scales
+__device__ __forceinline__ floatx4_t mfma_micro(u32x4_t a, u32x4_t b, floatx4_t c, uint32_t sa, uint32_t sb)
+{
+  typedef int eight_t __attribute__((ext_vector_type(8)));
+  const eight_t va = {static_cast<int>(a[0]), static_cast<int>(a[1]), static_cast<int>(a[2]), static_cast<int>(a[3]), 0, 0, 0, 0},
+                vb = {static_cast<int>(b[0]), static_cast<int>(b[1]), static_cast<int>(b[2]), static_cast<int>(b[3]), 0, 0, 0, 0};
+  typedef float four_t __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(floatx4_t, __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, __builtin_bit_cast(four_t, c), 4, 4, 0, static_cast<int>(sa), 0,
+                                                                                       static_cast<int>(sb)));
 }
 
 template <typename CT> struct Mfma16;
@@ -53,19 +66,13 @@ template <> struct Mfma16<f16_t> {
   }
 };
 
-// silu in fp32 from 1 / (1 + exp(-g)) with the exponential of -|g|, whose inverse stays in (0.5, 1]
-__device__ __forceinline__ float gate_act(float g)
-{
-  const float e = expf(-fabsf(g)), high = __builtin_amdgcn_rcpf(1.0f + e);
-  return g * (g < 0.0f ? e * high : high);
-}
-
 // P: pieces of an activation (3: fp32).  NW: weights (2: gate and up; the first half of the NT column tiles is gate's).
 template <typename CT, int P, int kWeight, int NW, int MT, int NT, bool kDirect>
 __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
 {
   constexpr int NC = NT / NW;                // column tiles of one weight
-  constexpr int WV = kWeight == ROWS_MX ? 1 : 4;      // 16-byte pieces of a column tile per half chunk
+  constexpr bool kMicro = kWeight != ROWS_DENSE, kBoth = kWeight == ROWS_BOTH;
+  constexpr int WV = kMicro ? 1 : 4, XV = kBoth ? 1 : 4;      // 16-byte pieces of a column tile and of a row tile per half chunk
   static_assert(NT % NW == 0 && (P == 1 || !kDirect), "");
   __shared__ floatx4_t sums[kRowsWaves / 2][MT * NT][64];
   const int lane = threadIdx.x & 63;
@@ -82,12 +89,18 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
     int64_t n = n0 + (c % NC) * 16 + j;
     n = n < g.N ? n : g.N - 1;
     wp[c] = static_cast<const uint8_t *>(g.w[v]) + n * g.w_pitch;
-    if constexpr (kWeight == ROWS_MX) sp[c] = g.s[v] + n * g.blocks;
+    if constexpr (kMicro) sp[c] = g.s[v] + n * g.blocks;
   }
   const uint8_t *xp[MT];
+  const uint8_t *xsp[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
-    if constexpr (kDirect) {
+    if constexpr (kBoth) {
+      int64_t m = m0 + t * 16 + j;
+      m = m < g.M ? m : g.M - 1;
+      xp[t] = static_cast<const uint8_t *>(g.x) + m * g.w_pitch;
+      xsp[t] = g.xs + m * g.blocks;
+    } else if constexpr (kDirect) {
       int64_t m = m0 + t * 16 + j;
       m = m < g.M ? m : g.M - 1;
       xp[t] = static_cast<const uint8_t *>(g.x) + m * g.x_pitch * 2;
@@ -101,15 +114,16 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
   // half chunk number `at` of this wave: chunk wave + 8 (at / 2), half at & 1
   struct Half {
     u32x4_t w[NT][WV];
-    uint32_t scale[kWeight == ROWS_MX ? NT : 1];
-    u32x4_t x[MT][P][4];
+    uint32_t scale[kMicro ? NT : 1];
+    u32x4_t x[MT][P][XV];
+    uint32_t x_scale[kBoth ? MT : 1];
   };
   const int mine = g.chunks > wave ? 2 * ((g.chunks - 1 - wave) / kRowsWaves + 1) : 0;
   auto load = [&](Half &b, int at) __attribute__((always_inline)) {
     const int use = at < mine ? at : (mine > 0 ? mine - 1 : 0);
     const int chunk = wave + kRowsWaves * (use >> 1), h = use & 1;
     const int64_t c = chunk < g.chunks ? chunk : g.chunks - 1;
-    if constexpr (kWeight == ROWS_MX) {
+    if constexpr (kMicro) {
       const int64_t block = c * 8 + h * 4 + q;
       const bool in = block < g.blocks;
       const int64_t safe = in ? block : g.blocks - 1;
@@ -118,6 +132,14 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
         b.w[t][0] = *reinterpret_cast<const u32x4_t *>(wp[t] + safe * 16);
         b.scale[t] = in ? sp[t][safe] : 0u;
         if (!in) b.w[t][0] = u32x4_t{0, 0, 0, 0};
+      }
+      if constexpr (kBoth) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          b.x[t][0][0] = *reinterpret_cast<const u32x4_t *>(xp[t] + safe * 16);
+          b.x_scale[t] = in ? xsp[t][safe] : 0u;
+        }
+        return;
       }
     } else {
 #pragma unroll
@@ -157,14 +179,20 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
 #pragma unroll
     for (int c = 0; c < NT; ++c)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < XV; ++i) {
+        if constexpr (kBoth) {
+#pragma unroll
+          for (int t = 0; t < MT; ++t) acc[t][c] = mfma_micro(b.x[t][0][0], b.w[c][0], acc[t][c], b.x_scale[t], b.scale[c]);
+          continue;
+        }
         u32x4_t w;
-        if constexpr (kWeight == ROWS_MX) w = mxfp4_eight<CT>(b.w[c][0][i], mxfp4_scale(b.scale[c]));
+        if constexpr (kMicro) w = mxfp4_eight<CT>(b.w[c][0][i], mxfp4_scale(b.scale[c]));
         else w = b.w[c][i];
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
-          for (int p = 0; p < P; ++p) acc[t][c] = Mfma16<CT>::run(b.x[t][p][i], w, acc[t][c]);
+          for (int p = 0; p < P; ++p)
+            if constexpr (!kBoth) acc[t][c] = Mfma16<CT>::run(b.x[t][p][i], w, acc[t][c]);
       }
   };
   Half even, odd;
@@ -239,7 +267,8 @@ int rows_launch(const RowsArgs &g, hipStream_t s)
     const auto forth = [&](const void *p, int64_t bytes) { return p ? const_cast<char *>(static_cast<const char *>(p)) + bytes : nullptr; };
     part.M = g.M - m0;
     part.tiles = g.tiles - static_cast<int>(m0 / 16);
-    part.x = forth(g.x, kDirect ? m0 * g.x_pitch * 2 : m0 / 16 * g.chunks * (P * 8 * 1024));
+    part.x = forth(g.x, kWeight == ROWS_BOTH ? m0 * g.w_pitch : kDirect ? m0 * g.x_pitch * 2 : m0 / 16 * g.chunks * (P * 8 * 1024));
+    part.xs = g.xs ? g.xs + m0 * g.blocks : nullptr;
     part.y = forth(g.y, m0 * g.N * es);
     part.gate = forth(g.gate, m0 * g.N * es);
     part.up = forth(g.up, m0 * g.N * es);
@@ -279,6 +308,7 @@ template <typename CT, int kWeight, int NW> int rows_pick(const RowsArgs &g, int
   return g.M <= 32 ? rows_pick_columns<CT, 1, kWeight, NW, 2, false>(g, s) : rows_pick_columns<CT, 1, kWeight, NW, 4, false>(g, s);
 }
 
+int rows_both(const RowsArgs &g, hipStream_t s);
 int rows_bf16(const RowsArgs &g, int weight, int weights, int pieces, bool direct, hipStream_t s);
 int rows_f16(const RowsArgs &g, int weight, int weights, bool direct, hipStream_t s);
 

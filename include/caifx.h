@@ -209,11 +209,15 @@ CAIFX_API int caifx_qlinear_backward_input_add(int64_t M, int64_t N, int64_t K,
  * with up to 16 rows and the forward with up to 16 rows and K > 4096 run, without it, on kernels that round
  * code * scale to the 16-bit compute type as the reference does, and with it on the few-row kernels that multiply
  * unrounded codes (about 2e-3 of max|out| apart; both within the 1e-2 bound; the few-row input gradient of packed
- * int4 with a 16-bit compute type multiplies the rounded weight either way). */
+ * int4 with a 16-bit compute type multiplies the rounded weight either way).
+ * CAIFX_W_MXFP4: the forward's activations in the kernels' order (some dozens of rows and more, fp32 compute, rows that are no
+ * multiple of 16 bytes), a dense copy of the weight from some hundred rows on, for the input gradient always a transposed one
+ * and the gradients in that order.  With less the forward runs without the dense copy, and otherwise the shape-agnostic kernels. */
 CAIFX_API size_t caifx_qlinear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_dtype, int compute_dtype,
                                      int w_kind, int backward);
 /* The same without the dense copy of large calls: what is left is a few partial tiles, at most 16 MiB for the 16-bit compute
- * types' tiled kernel.  For callers that pay for every allocation (a pool that returns its memory at each synchronisation). */
+ * types' tiled kernel (CAIFX_W_MXFP4: the forward's activations in the kernels' order; 0 for the input gradient).  For callers that
+ * pay for every allocation (a pool that returns its memory at each synchronisation). */
 CAIFX_API size_t caifx_qlinear_partials_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_dtype, int compute_dtype,
                                      int w_kind, int backward);
 
@@ -555,7 +559,8 @@ CAIFX_API int caifx_mxfp4_dequantize(const void *codes, const void *scales, void
 /* y[M,N] = A B^T with both operands in that form, A of M rows and B of N rows of K columns; products and sums are fp32, one rounding
  * to y_dtype.  The codes that fill up a row's last block take part in the sums: they have to be zeros, as caifx_mxfp4_quantize leaves
  * them.  Both codes aligned to 16 bytes.  workspace: caifx_mxfp4_matmul_workspace_bytes (may be 0, CAIFX_ERR_WORKSPACE_TOO_SMALL for
- * less).  CAIFX_ERR_UNSUPPORTED beyond 2^30 rows of either and beyond K = 2^30. */
+ * less).  Bytes above 252, which only a block of NaN has among those that caifx_mxfp4_quantize makes, give values beyond fp32:
+ * infinities or not.  CAIFX_ERR_UNSUPPORTED beyond M = 2^30 and from an N or K of 2^22 on. */
 CAIFX_API int caifx_mxfp4_matmul(int64_t M, int64_t N, int64_t K, const void *a_codes, const void *a_scales, const void *b_codes,
                        const void *b_scales, void *y, int y_dtype, void *workspace, size_t workspace_bytes,
                        caifx_stream_t stream);
@@ -568,7 +573,7 @@ CAIFX_API size_t caifx_mxfp4_matmul_workspace_bytes(int64_t M, int64_t N, int64_
  * w_kind: CAIFX_W_MXFP4, or CAIFX_W_F16 / CAIFX_W_BF16 with dtype the same type (scales NULL then); CAIFX_ERR_UNSUPPORTED for other
  * kinds.  All activations and results are of `dtype`, contiguous, any alignment of it; weights are aligned to 16 bytes.  Results alias
  * no input and no other result.  fp32 uses three bf16 pieces of each activation, which add up to it.  CAIFX_ERR_UNSUPPORTED beyond
- * 2^30 rows and an N or K of 2^26.  workspace: caifx_gated_workspace_bytes, CAIFX_ERR_WORKSPACE_TOO_SMALL for less.
+ * 2^30 rows and from an N or K of 2^22 on.  workspace: caifx_gated_workspace_bytes, CAIFX_ERR_WORKSPACE_TOO_SMALL for less.
  * ------------------------------------------------------------------------- */
 
 /* With g = x w_gate^T and u = x w_up^T in fp32: hidden[M,N] = T(silu(g) * u), gate = T(g), up = T(u).  gate and up are what the
