@@ -581,12 +581,11 @@ double rounds_cost(int64_t tiles, int64_t slots, double full, double base, doubl
   const int64_t rest = tiles % slots;
   return full * static_cast<double>(tiles / slots) + (rest == 0 ? 0.0 : base + per * static_cast<double>(rest));
 }
-double wide_us(const GemmArgs &a, bool backward)
+double wide_us_of(int64_t M, int64_t C, int64_t R)      // the product alone
 {
-  const int64_t C = backward ? a.K : a.N, R = backward ? a.N : a.K;
-  const auto tiles = [&](int64_t bm, int64_t bn) { return (a.M + bm - 1) / bm * ((C + bn - 1) / bn); };
+  const auto tiles = [&](int64_t bm, int64_t bn) { return (M + bm - 1) / bm * ((C + bn - 1) / bn); };
   double step;
-  switch (best_tile(a.M, C, 0)) {
+  switch (best_tile(M, C, 0)) {
     case TILE_256: step = rounds_cost(tiles(256, 256), 256, 1.42, 0.75, 0.0026); break;
     case TILE_128x256: step = rounds_cost(tiles(128, 256), 256, 0.81, 0.25, 0.0022); break;
     default: {
@@ -594,12 +593,16 @@ double wide_us(const GemmArgs &a, bool backward)
       step = t % 512 <= 256 ? rounds_cost(t, 512, 0.82, 0.24, 0.0008) : rounds_cost(t, 512, 0.82, 0.30, 0.0010);
     }
   }
+  return step * static_cast<double>(R / kBK);
+}
+double wide_us(const GemmArgs &a, bool backward)
+{
   // the dense copy, per million weights; of a 16-bit weight beyond 48 million it no longer stays in the memory-side cache
   const double millions = 1e-6 * static_cast<double>(a.N) * static_cast<double>(a.K);
   const double copy = a.w.kind == CAIFX_W_INT8          ? 10.0 + 0.42 * millions
                       : a.w.kind == CAIFX_W_INT4_GROUP ? 10.0 + 0.34 * millions
                                                        : 6.0 + (millions > 48.0 ? 0.78 : 0.40) * millions;
-  return step * static_cast<double>(R / kBK) + copy;
+  return wide_us_of(a.M, backward ? a.K : a.N, backward ? a.N : a.K) + copy;
 }
 // caifx_gemm.hip: 256 x 128 tiles for long reductions with enough of them, else 128 x 128, whose reduction is shared out
 // where at most 128 of them leave compute units idle
@@ -792,6 +795,11 @@ bool wide_takes(int64_t M, int64_t C, int64_t R)
   // (row offsets inside a tile have 32 bits)
   return M > 0 && M <= (int64_t{1} << 30) && C > 0 && C % 8 == 0 && R % kBK == 0 && R >= 2 * kBK && R < (int64_t{1} << 22) &&
          ((M + 127) / 128) * ((C + 63) / 64) <= (int64_t{1} << 30);
+}
+
+double wide_product_us(int64_t M, int64_t C, int64_t R)
+{
+  return wide_us_of(M, C, R);
 }
 
 int wide_product(const WideProduct &p, hipStream_t s)

@@ -230,7 +230,7 @@ __global__ __launch_bounds__(kThreads) void dense_transposed_kernel(Source g, CT
 // Activations in the order in which the row kernels read them: for each tile of 16 rows, chunk of 256 reduction elements and piece, eight
 // kilobytes of which the u-th holds every lane's operand of instruction u.  fp32 in P = 3 pieces: the upper 8 bits of the mantissa, the next
 // 8 and the rest, each cut off and so exact.
-template <typename S, typename CT, int P, int kWeight>
+template <typename S, typename CT, int P>
 __global__ __launch_bounds__(kThreads) void pack_rows_kernel(Source g, unsigned char *__restrict__ out, int chunk0, int chunks)
 {
   const int64_t tile = blockIdx.y + static_cast<int64_t>(blockIdx.z) * gridDim.y;
@@ -240,7 +240,7 @@ __global__ __launch_bounds__(kThreads) void pack_rows_kernel(Source g, unsigned 
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int at = half * kThreads + threadIdx.x, lane = at & 63, u = at >> 6;
-    const int64_t m = tile * 16 + (lane & 15), k = static_cast<int64_t>(c) * kRowsChunk + rows_element<kWeight>(u, lane >> 4);
+    const int64_t m = tile * 16 + (lane & 15), k = static_cast<int64_t>(c) * kRowsChunk + 32 * u + 8 * (lane >> 4);
     if constexpr (P == 1) {
       *reinterpret_cast<u32x4_t *>(to + at * 16) = source8<S, CT>(g, m, k);
     } else {
@@ -327,7 +327,7 @@ int operand_transposed(const void *p, const void *scales, int kind, int64_t rows
   return launch_status();
 }
 
-int operand_rows(const void *p, int kind, int64_t rows, int64_t cols, int to, int weight, void *out, int chunk0, int chunks, hipStream_t s)
+int operand_rows(const void *p, int kind, int64_t rows, int64_t cols, int to, void *out, int chunk0, int chunks, hipStream_t s)
 {
   const Source g = source(p, nullptr, rows, cols);
   const int64_t tiles = (rows + 15) / 16;
@@ -335,17 +335,10 @@ int operand_rows(const void *p, int kind, int64_t rows, int64_t cols, int to, in
   const dim3 grid(static_cast<unsigned>((cols + kRowsChunk - 1) / kRowsChunk), y, static_cast<unsigned>((tiles + y - 1) / y));
   unsigned char *o = static_cast<unsigned char *>(out);
   if (to == CAIFX_F32) {
-    const auto go = [&](auto type_, auto weight_) {
-      hipLaunchKernelGGL((pack_rows_kernel<decltype(type_), bf16_t, 3, decltype(weight_)::value>), grid, dim3(kThreads), 0, s, g, o, chunk0, chunks);
-    };
-    const std::integral_constant<int, ROWS_MX> mx;
-    const std::integral_constant<int, ROWS_DENSE> dense;
-    if (kind == CAIFX_F32) weight == ROWS_MX ? go(float{}, mx) : go(float{}, dense);
-    else weight == ROWS_MX ? go(f16_t{}, mx) : go(f16_t{}, dense);
-  } else if (weight == ROWS_MX) {
-    CAIFX_BY_TARGET(hipLaunchKernelGGL((pack_rows_kernel<S, CT, 1, ROWS_MX>), grid, dim3(kThreads), 0, s, g, o, chunk0, chunks))
+    if (kind == CAIFX_F32) hipLaunchKernelGGL((pack_rows_kernel<float, bf16_t, 3>), grid, dim3(kThreads), 0, s, g, o, chunk0, chunks);
+    else hipLaunchKernelGGL((pack_rows_kernel<f16_t, bf16_t, 3>), grid, dim3(kThreads), 0, s, g, o, chunk0, chunks);
   } else {
-    CAIFX_BY_TARGET(hipLaunchKernelGGL((pack_rows_kernel<S, CT, 1, ROWS_DENSE>), grid, dim3(kThreads), 0, s, g, o, chunk0, chunks))
+    CAIFX_BY_TARGET(hipLaunchKernelGGL((pack_rows_kernel<S, CT, 1>), grid, dim3(kThreads), 0, s, g, o, chunk0, chunks))
   }
   return launch_status();
 }

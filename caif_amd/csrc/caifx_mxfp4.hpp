@@ -17,11 +17,12 @@ int operand_transposed(const void *p, const void *scales, int kind, int64_t rows
                        hipStream_t s);
 // activations for rows_bf16 / rows_f16 with packed operands, `to` CAIFX_F32: three bf16 pieces (kind CAIFX_F32 or CAIFX_F16 then); chunk0: where the
 // source's chunks begin among `chunks`
-int operand_rows(const void *p, int kind, int64_t rows, int64_t cols, int to, int weight, void *out, int chunk0, int chunks, hipStream_t s);
+int operand_rows(const void *p, int kind, int64_t rows, int64_t cols, int to, void *out, int chunk0, int chunks, hipStream_t s);
 
 // y[M, C] = A B^T of two operands in microscaled 4 bits with `blocks` blocks a row, in tiles for the matrix cores.  The workspace is for scales
 // in rows of whole 16 bytes (their addresses are multiples of 16 where none is needed).
 bool mx_gemm_takes(int64_t M, int64_t C, int64_t blocks);
+double mx_gemm_us(int64_t M, int64_t C, int64_t blocks);      // an estimate
 size_t mx_gemm_workspace_bytes(int64_t M, int64_t C, int64_t blocks);
 int mx_gemm(int64_t M, int64_t C, int64_t blocks, const void *a, const void *sa, const void *b, const void *sb, void *d, int d_dtype, void *workspace, hipStream_t s);
 

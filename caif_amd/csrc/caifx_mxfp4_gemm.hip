@@ -336,6 +336,14 @@ bool mx_gemm_takes(int64_t M, int64_t C, int64_t blocks)
   return blocks < (int64_t{1} << 17) && ((M + 127) / 128) * ((C + 127) / 128) <= (int64_t{1} << 30);
 }
 
+double mx_gemm_us(int64_t M, int64_t C, int64_t blocks)
+{
+  const double steps = static_cast<double>((blocks + 7) / 8);
+  const int64_t large = ((M + 255) / 256) * ((C + 255) / 256), small = ((M + 127) / 128) * ((C + 127) / 128);
+  if (large >= 192) return 4.0 + 2.3 * steps * static_cast<double>((large + 255) / 256);
+  return 4.0 + 0.8 * steps * static_cast<double>((small + 511) / 512);
+}
+
 size_t mx_gemm_workspace_bytes(int64_t M, int64_t C, int64_t blocks)
 {
   return blocks % 16 == 0 ? 0 : static_cast<size_t>(M + C) * static_cast<size_t>(padded(blocks));

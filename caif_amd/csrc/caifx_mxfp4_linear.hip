@@ -72,10 +72,27 @@ RowsArgs rows_args(const Product &p)
   return g;
 }
 
-int rows_run(const RowsArgs &g, bool mx, int weights, int compute_dtype, bool direct, hipStream_t s)
+// Runs the row kernels on laid out operands, or adds up what they need of the workspace: the sums of shared reductions.
+int rows_run(RowsArgs g, int kind, int weights, int compute_dtype, bool direct, Room &room, bool only_size, hipStream_t s)
 {
-  const int kind = mx ? ROWS_MX : ROWS_DENSE;
-  return compute_dtype == CAIFX_F16 ? rows_f16(g, kind, weights, direct, s) : rows_bf16(g, kind, weights, pieces_of(compute_dtype), direct, s);
+  const int pieces = pieces_of(compute_dtype);
+  const int tile = rows_tile(g.M, pieces);
+  const double row = kind == ROWS_DENSE ? static_cast<double>(g.w_pitch) : 17.0 * static_cast<double>(g.blocks);
+  const double x = (kind == ROWS_BOTH ? row : 2.0 * pieces * static_cast<double>(g.R)) * (g.M <= 4 && pieces == 1 ? 4 : tile);
+  const RowsPlan plan = rows_plan(g.M, g.N, g.R, weights, tile, row, x);
+  void *partial = plan.splits > 1 ? room.take(static_cast<size_t>(plan.splits) * static_cast<size_t>(g.M) * static_cast<size_t>(g.N) * 4) : nullptr;
+  if (only_size) return CAIFX_OK;
+  g.span = plan.span;
+  g.splits = plan.splits;
+  const RowsArgs asked = g;
+  if (plan.splits > 1) {
+    g.y = partial;
+    g.y_dtype = CAIFX_F32;
+    g.addend = nullptr;
+  }
+  const int st = kind == ROWS_BOTH ? rows_both(g, s) : compute_dtype == CAIFX_F16 ? rows_f16(g, kind, weights, direct, s) : rows_bf16(g, kind, weights, pieces, direct, s);
+  if (st != CAIFX_OK || plan.splits == 1) return st;
+  return splitk_reduce(static_cast<const float *>(partial), plan.splits, g.M * g.N, asked.y, asked.y_dtype, asked.addend, s);
 }
 
 // whether the row kernels can read the activations where they are
@@ -89,8 +106,15 @@ bool aligned16(const void *a, const void *b = nullptr, const void *c = nullptr, 
 // Whether a product with this many rows runs on dense operands (caifx_gemm_wide.hip) instead of the row kernels.
 bool wide_product_pays(const Product &p)
 {
-  if (p.compute_dtype == CAIFX_F32 || !wide_takes(p.M, p.N, up_to(p.R, 64)) || p.N * up_to(p.R, 64) >= (int64_t{1} << 32)) return false;
-  return p.M > (p.w[0].mx ? 256 : 64);
+  const int64_t R = up_to(p.R, 64);
+  if (p.M <= 64 || p.compute_dtype == CAIFX_F32 || !wide_takes(p.M, p.N, R) || p.N * R >= (int64_t{1} << 32)) return false;
+  if (!p.w[0].mx) return true;
+  // The row kernels run at some 640 TFLOP/s from a few hundred rows on; the dense product is twice as fast, behind copies of the weights.
+  // us, rows / dense, bf16: N = 14336, K = 4096, 256 rows 62 / 66, 384 rows 86 / 83; N = 11008 384 rows 72 / 70; N = 4096, K = 14336, 512 rows
+  // 84 / 120; 28672 x 8192, 384 rows 270 / 294, 512 rows 356 / 314.
+  const double weights = p.weights, millions = 1e-6 * weights * static_cast<double>(p.N) * static_cast<double>(R);
+  const double rows = 8.0 + 2.0 * millions * static_cast<double>(p.M) / 640.0;
+  return wide_product_us(p.M, p.weights * p.N, R) + 8.0 * weights + 0.56 * millions < rows;
 }
 
 // The product on dense operands: the weights dequantised into the workspace, activations of another type or length copied.
@@ -152,14 +176,14 @@ int product_rows(const Product &p, Room &room, bool only_size, hipStream_t s)
   if (!direct) {
     void *packed = room.take(packed_bytes(p.M, g.chunks, p.compute_dtype));
     if (!only_size) {
-      const int st = operand_rows(p.x, p.x_dtype, p.M, p.R, p.compute_dtype, p.w[0].mx ? ROWS_MX : ROWS_DENSE, packed, 0, g.chunks, s);
+      const int st = operand_rows(p.x, p.x_dtype, p.M, p.R, p.compute_dtype, packed, 0, g.chunks, s);
       if (st != CAIFX_OK) return st;
     }
     g.x = packed;
   } else {
     g.x = p.x;
   }
-  return only_size ? CAIFX_OK : rows_run(g, p.w[0].mx, p.weights, p.compute_dtype, direct, s);
+  return rows_run(g, p.w[0].mx ? ROWS_MX : ROWS_DENSE, p.weights, p.compute_dtype, direct, room, only_size, s);
 }
 
 // What either way can need.  Results or activations at addresses that the dense product does not take run on the row kernels.
@@ -194,7 +218,11 @@ struct Gradient {
 // Whether a gradient runs on the dense product behind the transposed copies.
 bool wide_gradient_pays(const Gradient &p)
 {
-  return p.compute_dtype != CAIFX_F32 && p.M > 64 && wide_takes(p.M, p.K, up_to(p.N, 64));
+  const int64_t R = up_to(p.N, 64);
+  if (p.compute_dtype == CAIFX_F32 || p.M <= 32 || !wide_takes(p.M, p.K, R)) return false;
+  // (both behind the same copies.  us, rows / dense: 4096 x 14336, 64 rows 76 / 72, 96 rows 99 / 72; 14336 x 4096, 128 rows 93 / 123, 256 rows 123 / 124)
+  const double flops = 2.0 * p.weights * static_cast<double>(p.M) * static_cast<double>(p.N) * static_cast<double>(p.K);
+  return wide_product_us(p.M, p.K, p.weights * R) < 8.0 + flops / 480e6;
 }
 
 int gradient_wide(const Gradient &p, Room &room, bool only_size, hipStream_t s)
@@ -232,10 +260,9 @@ int gradient_rows(const Gradient &p, Room &room, bool only_size, hipStream_t s)
   const int per = static_cast<int>(pitch / kRowsChunk), chunks = per * p.weights;
   void *copy = room.take(static_cast<size_t>(p.K) * static_cast<size_t>(stride) * 2);
   void *packed = room.take(packed_bytes(p.M, chunks, p.compute_dtype));
-  if (only_size) return CAIFX_OK;
-  for (int i = 0; i < p.weights; ++i) {
+  for (int i = 0; i < p.weights && !only_size; ++i) {
     int st = operand_transposed(p.w[i].p, p.w[i].scales, p.w[i].mx ? OPERAND_MX : to, p.N, p.K, to, copy, pitch, stride, i * pitch, s);
-    if (st == CAIFX_OK) st = operand_rows(p.x[i], p.x_dtype, p.M, p.N, p.compute_dtype, ROWS_DENSE, packed, i * per, chunks, s);
+    if (st == CAIFX_OK) st = operand_rows(p.x[i], p.x_dtype, p.M, p.N, p.compute_dtype, packed, i * per, chunks, s);
     if (st != CAIFX_OK) return st;
   }
   RowsArgs g{};
@@ -250,7 +277,7 @@ int gradient_rows(const Gradient &p, Room &room, bool only_size, hipStream_t s)
   g.y = p.y;
   g.addend = p.addend;
   g.y_dtype = p.y_dtype;
-  return rows_run(g, false, 1, p.compute_dtype, false, s);
+  return rows_run(g, ROWS_DENSE, 1, p.compute_dtype, false, room, only_size, s);
 }
 
 size_t gradient_bytes(const Gradient &p)
@@ -331,7 +358,24 @@ namespace {
 
 int64_t blocks_of(int64_t columns) { return (columns + CAIFX_MXFP4_BLOCK - 1) / CAIFX_MXFP4_BLOCK; }
 // whether a product of two operands in 4 bits runs in tiles rather than on the row kernels
-bool tiles_pay(int64_t M, int64_t N, int64_t blocks) { return M > 64 && mx_gemm_takes(M, N, blocks); }
+bool tiles_pay(int64_t M, int64_t N, int64_t blocks)
+{
+  // us, rows / tiles, bf16: N = 14336, K = 4096, 64 rows 16 / 17, 96 rows 25 / 18; N = 4096, K = 14336, 256 rows 37 / 49, 512 rows 66 / 48; N = K =
+  // 4096, 192 rows 13 / 12; 2048 x 1408, 512 rows 7 / 12.
+  return M > 64 && mx_gemm_takes(M, N, blocks) && mx_gemm_us(M, N, blocks) < 4.5 + 64e-9 * static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(blocks) / 0.8;
+}
+
+RowsArgs both_args(int64_t M, int64_t N, int64_t blocks)
+{
+  RowsArgs g{};
+  g.M = M;
+  g.N = N;
+  g.R = 32 * blocks;
+  g.blocks = blocks;
+  g.w_pitch = 16 * blocks;
+  g.chunks = static_cast<int>(chunks_of(g.R));
+  return g;
+}
 
 // what both gated calls check; `go`: there is work
 int gated_check(int64_t M, int64_t N, int64_t K, int w_kind, int dtype, bool &go)
@@ -375,7 +419,10 @@ size_t caifx_mxfp4_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K)
 {
   if (M <= 0 || N <= 0 || K <= 0 || !fits(M, N, K)) return 0;
   const int64_t blocks = blocks_of(K);
-  return tiles_pay(M, N, blocks) ? mx_gemm_workspace_bytes(M, N, blocks) : 0;
+  Room room;
+  rows_run(both_args(M, N, blocks), ROWS_BOTH, 1, CAIFX_BF16, true, room, true, nullptr);
+  const size_t tiles = tiles_pay(M, N, blocks) ? mx_gemm_workspace_bytes(M, N, blocks) : 0;
+  return tiles > room.used ? tiles : room.used;
 }
 
 int caifx_mxfp4_matmul(int64_t M, int64_t N, int64_t K, const void *a_codes, const void *a_scales, const void *b_codes, const void *b_scales, void *y,
@@ -390,22 +437,17 @@ int caifx_mxfp4_matmul(int64_t M, int64_t N, int64_t K, const void *a_codes, con
   if (need > 0 && (!workspace || workspace_bytes < need)) return CAIFX_ERR_WORKSPACE_TOO_SMALL;
   const int64_t blocks = blocks_of(K);
   // (scales at an odd address would need a copy that the query did not count)
-  if (tiles_pay(M, N, blocks) && (need > 0 || (aligned_to(a_scales, 16) && aligned_to(b_scales, 16))))
+  if (tiles_pay(M, N, blocks) && (mx_gemm_workspace_bytes(M, N, blocks) > 0 || (aligned_to(a_scales, 16) && aligned_to(b_scales, 16))))
     return mx_gemm(M, N, blocks, a_codes, a_scales, b_codes, b_scales, y, y_dtype, workspace, as_stream(stream));
-  RowsArgs g{};
+  RowsArgs g = both_args(M, N, blocks);
   g.x = a_codes;
   g.xs = static_cast<const uint8_t *>(a_scales);
   g.w[0] = b_codes;
   g.s[0] = static_cast<const uint8_t *>(b_scales);
-  g.M = M;
-  g.N = N;
-  g.R = 32 * blocks;
-  g.blocks = blocks;
-  g.w_pitch = 16 * blocks;
-  g.chunks = static_cast<int>(chunks_of(g.R));
   g.y = y;
   g.y_dtype = y_dtype;
-  return rows_both(g, as_stream(stream));
+  Room room{static_cast<char *>(workspace), 0};
+  return rows_run(g, ROWS_BOTH, 1, CAIFX_BF16, true, room, false, as_stream(stream));
 }
 
 size_t caifx_gated_workspace_bytes(int64_t M, int64_t N, int64_t K, int w_kind, int dtype, int backward)

@@ -11,8 +11,11 @@ int rows_bf16(const RowsArgs &g, int weight, int weights, int pieces, bool direc
 
 int rows_both(const RowsArgs &g, hipStream_t s)
 {
-  if (g.M <= 16) return rows_pick_columns<bf16_t, 1, ROWS_BOTH, 1, 1, true>(g, s);
-  return g.M <= 32 ? rows_pick_columns<bf16_t, 1, ROWS_BOTH, 1, 2, true>(g, s) : rows_pick_columns<bf16_t, 1, ROWS_BOTH, 1, 4, true>(g, s);
+  switch (rows_tile(g.M, 1)) {
+    case 16: return rows_pick_columns<bf16_t, 1, ROWS_BOTH, 1, 1, 0>(g, s);
+    case 32: return rows_pick_columns<bf16_t, 1, ROWS_BOTH, 1, 2, 0>(g, s);
+    default: return rows_pick_columns<bf16_t, 1, ROWS_BOTH, 1, 4, 0>(g, s);
+  }
 }
 
 }  // namespace caifx

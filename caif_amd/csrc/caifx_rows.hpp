@@ -1,22 +1,69 @@
 // Products with up to some hundred rows of activations and a weight in microscaled 4 bits, or dense in the 16-bit compute type:
 //   y[m, n] = sum_k x[m, k] w[n, k]       and, over two weights (gate and up) at once, hidden = silu(x w0^T) * (x w1^T).
 //
-// Bound by memory with few rows (the weight's bytes), by the L1 from some dozens on.  A workgroup of eight waves owns 16 MT rows and
-// 16 NT weight rows of the result; the waves take the chunks of 256 reduction elements in turn and their sums meet in LDS at the end.
+// Bound by memory with few rows (the weight's bytes), by the L1 from some dozens on: a compute unit has some 100 lines on their way at a
+// time, whatever it asks for, and the activations are read anew for every 16 NT weight rows.  So they are asked for in whole lines, only the
+// rows that there are, and take the operands' order in a wave's own part of LDS (up to 32 rows) or beforehand (see pack_rows_kernel).  A workgroup of eight waves owns 16 MT rows and
+// 16 NT weight rows of the result; the waves take units of 512 reduction elements in turn and their sums meet in LDS at the end.
 // So every wave streams its part of the weight rows straight into matrix-core operands, no wave waits for another in between, and a
-// launch of a usual weight has all of it on its way at once.  The reduction indices inside a chunk are permuted such that a lane's 16
-// bytes of codes are one block of 32 values of one weight row: lane (j, q) of v_mfma_f32_16x16x32 holds block q (then q + 4) of row j,
-// instruction i takes its values 8 i .. 8 i + 7, and the activations follow that order.  The codes become operands by
+// launch of a usual weight has all of it on its way at once.  Lane (j, q) of v_mfma_f32_16x16x32 loads block
+// q of four, 16 bytes, of weight row j, and the four lanes of a row exchange their dwords (two swaps of half waves, two of rows of lanes)
+// so that instruction i takes block i, lane q its values 8 q .. 8 q + 7.  The codes become operands by
 // v_cvt_scalef32_pk_{bf16,f16}_fp4 with the block's scale: exact in bf16, in fp16 rounded like any weight that is cast to it.  Where the
 // activations have 4 bits too, the same blocks go into v_mfma_scale_f32_16x16x128_f8f6f4 as they are.
 #pragma once
 
 #include "caifx_wide.hpp"
 
+#include <type_traits>
+
 namespace caifx {
 
 constexpr int kRowsChunk = 256;              // reduction elements of a chunk: 128 bytes of codes of a weight row
 constexpr int kRowsWaves = 8;
+
+// How a launch is cut up: columns of a workgroup, workgroups that share a reduction.
+struct RowsPlan {
+  int span, splits;
+};
+// Rows of a workgroup's tile.
+inline int rows_tile(int64_t M, int pieces) { return pieces == 3 || M <= 16 ? 16 : M <= 32 ? 32 : 64; }
+// The time of a launch in us, fitted to 60 calls (1 to 64 rows, 1024 x 4096 to 8192 x 28672 and 14336 x 4096): a start, the rounds that a
+// wave's units take, a compute unit's share of the weight at 20.7 KB a us (5.3 TB/s in all) and of the activations, which its caches
+// serve, at 80; a shared reduction costs a second launch and the sums' way there and back.
+inline double rows_us(double rows, double columns, double span, double splits, double units, double weight_row, double x_tile, double result)
+{
+  double rounds = rows * columns * splits / 256;
+  rounds = rounds < 1 ? 1 : rounds;
+  double turns = units / splits / 8;
+  turns = turns < 1 ? 1 : turns;
+  return 2.4 + rounds * (0.55 * turns + span * weight_row / splits / 20700 + x_tile / splits / 80000) + (splits > 1 ? 3.3 + splits * result * 8 / 4.0e6 : 0.0);
+}
+// A compute unit has some 100 lines on their way at a time whatever it asks for, so the launch is as fast as its fullest compute unit: the
+// columns are cut into a multiple of 256 parts, as large as the column tiles allow.  Where that leaves a workgroup few columns, so that
+// the activations are most of what it reads, 2 to 8 workgroups share a reduction of wider parts (N = 4096, K = 14336, 32 rows: 18 us in four,
+// 20 in one; the estimates say where).  x_tile: bytes of the activations that a workgroup reads.
+inline RowsPlan rows_plan(int64_t M, int64_t N, int64_t R, int weights, int tile, double weight_row, double x_tile)
+{
+  const int64_t rows = (M + tile - 1) / tile, most = 64 / weights;
+  const double units = static_cast<double>((R + 511) / 512);
+  RowsPlan best{};
+  double best_us = 0;
+  for (int splits = 1; splits <= 8; splits *= 2) {
+    if (splits > 1 && (weights > 1 || units < 4 * splits || rows * splits > 256)) break;
+    int64_t rounds = (rows * splits + 255) / 256;
+    const auto parts = [&] { return 256 * rounds / (rows * splits); };      // of the columns
+    while ((N + parts() - 1) / parts() > most) ++rounds;
+    const int64_t span = (N + parts() - 1) / parts();
+    const double us = rows_us(static_cast<double>(rows), static_cast<double>((N + span - 1) / span), static_cast<double>(span), splits, units, weight_row, x_tile,
+                              static_cast<double>(M) * static_cast<double>(N));
+    if (splits == 1 || us < best_us) {
+      best = RowsPlan{static_cast<int>(span), splits};
+      best_us = us;
+    }
+  }
+  return best;
+}
 
 struct RowsArgs {
   const void *x;          // direct: [M, x_pitch] of the compute type; packed: see pack_rows_kernel
@@ -24,10 +71,12 @@ struct RowsArgs {
   const void *w[2];       // MX codes or dense rows of the compute type
   const uint8_t *s[2];    // MX scales
   const uint8_t *xs;      // both in 4 bits: scales of x, whose codes are rows of w_pitch bytes
-  int64_t M, N, R;        // R: elements of the reduction (direct: a multiple of 8)
+  int64_t M, N, R;        // R: elements of the reduction, a multiple of 8 for direct activations and dense weights
   int64_t blocks;         // MX blocks of a weight row
   int64_t w_pitch;        // bytes of a weight row
   int chunks, tiles;      // chunks of the reduction, row tiles of 16 in the packed activations
+  int span;               // columns of a workgroup, at most 16 for each of its column tiles
+  int splits;             // workgroups that share a reduction: the z-th writes its sums to y + z M N (fp32)
   void *y;                // [M, N] result, or hidden
   void *gate, *up;        // two weights: kept projections, or null
   const void *addend;     // one weight: y = T(float(T(acc)) + float(addend))
@@ -35,10 +84,16 @@ struct RowsArgs {
 };
 
 enum { ROWS_MX = 0, ROWS_DENSE = 1, ROWS_BOTH = 2 };      // ROWS_BOTH: weight and activations in microscaled 4 bits
-// first of the eight reduction elements that lane group q holds for instruction u (0 .. 7) of a chunk
-template <int kWeight> __device__ __forceinline__ int rows_element(int u, int q)
+
+// dword d of lane group q becomes dword q of lane group d
+__device__ __forceinline__ u32x4_t exchange(u32x4_t v)
 {
-  return kWeight == ROWS_MX ? 128 * (u >> 2) + 32 * q + 8 * (u & 3) : 32 * u + 8 * q;
+  typedef uint32_t two_t __attribute__((ext_vector_type(2)));
+  const two_t a = __builtin_bit_cast(two_t, __builtin_amdgcn_permlane32_swap(v[0], v[2], false, false));
+  const two_t b = __builtin_bit_cast(two_t, __builtin_amdgcn_permlane32_swap(v[1], v[3], false, false));
+  const two_t c = __builtin_bit_cast(two_t, __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false));
+  const two_t d = __builtin_bit_cast(two_t, __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false));
+  return u32x4_t{c[0], c[1], d[0], d[1]};
 }
 
 // one block of 32 values of each of 16 rows and 16 columns per lane group, in 4 bits with their scales
@@ -66,108 +121,169 @@ template <> struct Mfma16<f16_t> {
   }
 };
 
-// P: pieces of an activation (3: fp32).  NW: weights (2: gate and up; the first half of the NT column tiles is gate's).
-template <typename CT, int P, int kWeight, int NW, int MT, int NT, bool kDirect>
+// P: pieces of an activation (3: fp32).  NW: weights (2: gate and up; the first half of the NT column tiles is gate's).  kWhole: rows of
+// whole dwords of scales, at least 16 bytes long: a unit's scales of a weight row are one access (one byte at a time they are more requests
+// than the codes; K = 11008, N = 4096, one row 22.0 us instead of XX).
+// XG: groups of four rows of activations that are read where they are; 0: packed ones.
+template <typename CT, int P, int kWeight, int NW, int MT, int NT, int XG, bool kWhole>
 __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
 {
   constexpr int NC = NT / NW;                // column tiles of one weight
   constexpr bool kMicro = kWeight != ROWS_DENSE, kBoth = kWeight == ROWS_BOTH;
+  constexpr bool kDirect = XG > 0 && !kBoth;
   constexpr int WV = kMicro ? 1 : 4, XV = kBoth ? 1 : 4;      // 16-byte pieces of a column tile and of a row tile per half chunk
-  static_assert(NT % NW == 0 && (P == 1 || !kDirect), "");
-  __shared__ floatx4_t sums[kRowsWaves / 2][MT * NT][64];
+  constexpr int XL = kDirect ? XG : MT * P * XV;              // loads of activations per half chunk
+  // half chunks on their way before the one in hand is used: a second one where a SIMD still holds four waves with it (one row, N = 4096, K =
+  // 14336: 10.2 us instead of 13.3; with 32 registers a half chunk, 16 rows, N = 14336, K = 4096: 11.9 instead of 11.4)
+  constexpr int kRegs = 4 * (NT * WV + XL);
+  constexpr int D = kRegs <= 24 ? 2 : 1;
+  static_assert(NT % NW == 0 && (P == 1 || XG == 0) && (kMicro || !kWhole) && (XG == 0 || XG == 4 * MT || (MT == 1 && XG == 1)), "");
+  // the activations of a half chunk for each wave, [4 XG][16 pieces of 16 bytes]; at the end the waves' sums
+  constexpr int kSums = kRowsWaves / 2 * MT * NT * 1024, kOrder = kDirect ? kRowsWaves * XG * 1024 : 0;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[kSums > kOrder ? kSums : kOrder];
+  auto sums = reinterpret_cast<floatx4_t(*)[MT * NT][64]>(smem);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int j = lane & 15, q = lane >> 4;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (16 * NC), m0 = static_cast<int64_t>(blockIdx.y) * (16 * MT);
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * g.span, m0 = static_cast<int64_t>(blockIdx.y) * (16 * MT);
 
-  // what each lane reads from: rows past the end are the last one again, and are not stored
-  const uint8_t *wp[NT];
-  const uint8_t *sp[NT];
+  // what each lane reads from, as an offset of 32 bits from the first row of the tile (at most 64 rows of 2^24 bytes): rows past the end
+  // are the last one again, and are not stored
+  const uint8_t *w_base[NW], *s_base[NW];
 #pragma unroll
-  for (int c = 0; c < NT; ++c) {
-    const int v = c / NC;
-    int64_t n = n0 + (c % NC) * 16 + j;
-    n = n < g.N ? n : g.N - 1;
-    wp[c] = static_cast<const uint8_t *>(g.w[v]) + n * g.w_pitch;
-    if constexpr (kMicro) sp[c] = g.s[v] + n * g.blocks;
+  for (int v = 0; v < NW; ++v) {
+    w_base[v] = static_cast<const uint8_t *>(g.w[v]) + n0 * g.w_pitch;
+    s_base[v] = kMicro ? g.s[v] + n0 * g.blocks : nullptr;
   }
-  const uint8_t *xp[MT];
-  const uint8_t *xsp[MT];
+  const int columns = g.N - n0 < g.span ? static_cast<int>(g.N - n0) : g.span;
+  uint32_t w_off[NC], s_off[NC];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    if constexpr (kBoth) {
-      int64_t m = m0 + t * 16 + j;
-      m = m < g.M ? m : g.M - 1;
-      xp[t] = static_cast<const uint8_t *>(g.x) + m * g.w_pitch;
-      xsp[t] = g.xs + m * g.blocks;
-    } else if constexpr (kDirect) {
-      int64_t m = m0 + t * 16 + j;
-      m = m < g.M ? m : g.M - 1;
-      xp[t] = static_cast<const uint8_t *>(g.x) + m * g.x_pitch * 2;
-    } else {
-      int64_t tile = (m0 >> 4) + t;
-      tile = tile < g.tiles ? tile : g.tiles - 1;
-      xp[t] = static_cast<const uint8_t *>(g.x) + tile * g.chunks * (P * 8 * 1024) + lane * 16;
+  for (int c = 0; c < NC; ++c) {
+    const int n = c * 16 + j;
+    const uint32_t row = static_cast<uint32_t>(n < columns ? n : columns - 1);
+    w_off[c] = row * static_cast<uint32_t>(g.w_pitch) + q * 16;
+    s_off[c] = row * static_cast<uint32_t>(g.blocks);
+  }
+  const uint8_t *x_base = static_cast<const uint8_t *>(g.x), *xs_base = nullptr;
+  uint32_t x_off[kDirect ? XG : MT], xs_off[kBoth ? MT : 1];
+  if constexpr (kBoth || kDirect) {
+    const int64_t pitch = kBoth ? g.w_pitch : 2 * g.x_pitch;
+    x_base += m0 * pitch;
+    if constexpr (kBoth) xs_base = g.xs + m0 * g.blocks;
+#pragma unroll
+    for (int t = 0; t < (kDirect ? XG : MT); ++t) {
+      // (direct: lane (j, q) reads piece j of the half chunk of row 4 t + q)
+      const int64_t m = m0 + (kDirect ? 4 * t + q : 16 * t + j);
+      const uint32_t row = static_cast<uint32_t>((m < g.M ? m : g.M - 1) - m0);
+      x_off[t] = row * static_cast<uint32_t>(pitch) + (kDirect ? j : q) * 16;
+      if constexpr (kBoth) xs_off[t] = row * static_cast<uint32_t>(g.blocks);
     }
   }
+  // 16 bytes at a base that all lanes share, which the asm keeps in scalar registers: otherwise every load of the loop gets a 64-bit pointer
+  // of its own in vector registers, a hundred of them
+  auto at128 = [](const uint8_t *base, uint32_t off) __attribute__((always_inline)) {
+    uint64_t b = reinterpret_cast<uint64_t>(base);
+    asm("" : "+s"(b), "+v"(off));
+    return *reinterpret_cast<const __attribute__((address_space(1))) u32x4_t *>(b + off);
+  };
 
-  // half chunk number `at` of this wave: chunk wave + 8 (at / 2), half at & 1
+  // A unit is two chunks, four halves of 128 elements; wave w takes units w, w + 8, ..
   struct Half {
     u32x4_t w[NT][WV];
-    uint32_t scale[kMicro ? NT : 1];
-    u32x4_t x[MT][P][XV];
-    uint32_t x_scale[kBoth ? MT : 1];
+    u32x4_t x[XL];
+    uint32_t scale[kMicro && !kWhole ? NT : 1];      // like a dword of Scales; both in 4 bits: the byte of this lane's block
+    uint32_t x_scale[kBoth && !kWhole ? MT : 1];
   };
-  const int mine = g.chunks > wave ? 2 * ((g.chunks - 1 - wave) / kRowsWaves + 1) : 0;
+  struct Scales {
+    u32x4_t w[kWhole ? NT : 1];              // dword h: the scales of half h, a byte for each of its blocks
+    u32x4_t x[kWhole && kBoth ? MT : 1];
+  };
+  const int halves = kMicro ? static_cast<int>((g.blocks + 3) >> 2) : static_cast<int>((g.R + 127) >> 7);
+  const int units = (halves + 3) >> 2;
+  const int z = static_cast<int>(blockIdx.z);
+  const int first = units * z / g.splits + wave, end = units * (z + 1) / g.splits;
+  const int mine = end > first ? (end - 1 - first) / kRowsWaves + 1 : 0;
+  auto load_scales = [&](Scales &to, int unit) __attribute__((always_inline)) {
+    if constexpr (kWhole) {
+      // (a unit that begins less than 16 blocks before the end of a row: the row's last 16, see `behind`)
+      const int64_t at = static_cast<int64_t>(unit) * 16, from = at + 16 <= g.blocks ? at : g.blocks - 16;
+#pragma unroll
+      for (int c = 0; c < NT; ++c) to.w[c] = at128(s_base[c / NC] + from, s_off[c % NC]);
+      if constexpr (kBoth) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) to.x[t] = at128(xs_base + from, xs_off[t]);
+      }
+    }
+  };
+  // half `at` of all; past the end the last one again (it is not used)
   auto load = [&](Half &b, int at) __attribute__((always_inline)) {
-    const int use = at < mine ? at : (mine > 0 ? mine - 1 : 0);
-    const int chunk = wave + kRowsWaves * (use >> 1), h = use & 1;
-    const int64_t c = chunk < g.chunks ? chunk : g.chunks - 1;
+    const int64_t half = at < halves ? at : halves - 1;
     if constexpr (kMicro) {
-      const int64_t block = c * 8 + h * 4 + q;
-      const bool in = block < g.blocks;
-      const int64_t safe = in ? block : g.blocks - 1;
+      // blocks past the end of a row: its last one again, as zeros
+      const int block = static_cast<int>(half) * 4 + q;
+      const bool in = kWhole || block < g.blocks;
+      const uint32_t back = in ? 0u : static_cast<uint32_t>(block - (g.blocks - 1));
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        b.w[t][0] = *reinterpret_cast<const u32x4_t *>(wp[t] + safe * 16);
-        b.scale[t] = in ? sp[t][safe] : 0u;
-        if (!in) b.w[t][0] = u32x4_t{0, 0, 0, 0};
+        b.w[t][0] = at128(w_base[t / NC] + half * 64, w_off[t % NC] - back * 16);
+        if constexpr (!kWhole) {
+          const uint8_t *from = s_base[t / NC] + half * 4;
+          if constexpr (kBoth) {
+            b.scale[t] = in ? from[s_off[t % NC] + q - back] : 0u;
+          } else {
+            // the half's four bytes, those past the end of the row as zeros
+            uint32_t dword = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (half * 4 + i < g.blocks) dword |= static_cast<uint32_t>(from[s_off[t % NC] + i]) << (8 * i);
+            b.scale[t] = dword;
+          }
+          if (!in) b.w[t][0] = u32x4_t{0, 0, 0, 0};
+        }
       }
       if constexpr (kBoth) {
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-          b.x[t][0][0] = *reinterpret_cast<const u32x4_t *>(xp[t] + safe * 16);
-          b.x_scale[t] = in ? xsp[t][safe] : 0u;
+          b.x[t] = at128(x_base + half * 64, x_off[t] - back * 16);
+          if constexpr (!kWhole) b.x_scale[t] = in ? (xs_base + half * 4)[xs_off[t] + q - back] : 0u;
         }
         return;
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int64_t k = c * kRowsChunk + rows_element<kWeight>(4 * h + i, q);
+        // pieces of eight elements past the end of a row: its last one again, as zeros
+        const int k = static_cast<int>(half) * 128 + 32 * i + 8 * q;
         const bool in = k < g.R;
-        const int64_t safe = in ? k : 0;
+        const uint32_t back = in ? 0u : static_cast<uint32_t>(k - (g.R - 8)) * 2;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          b.w[t][i] = *reinterpret_cast<const u32x4_t *>(wp[t] + safe * 2);
+          b.w[t][i] = at128(w_base[t / NC] + half * 256, w_off[t % NC] + 64 * i - back);
           if (!in) b.w[t][i] = u32x4_t{0, 0, 0, 0};
         }
       }
     }
+    if constexpr (kDirect) {
+      const int k = static_cast<int>(half) * 128 + 8 * j;
+      const bool in = kWhole || k < g.R;
+      const uint32_t back = in ? 0u : static_cast<uint32_t>(k - (g.R - 8)) * 2;
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (kDirect) {
-          const int64_t k = c * kRowsChunk + rows_element<kWeight>(4 * h + i, q);
-          const bool in = k < g.R;
-          b.x[t][0][i] = *reinterpret_cast<const u32x4_t *>(xp[t] + (in ? k : 0) * 2);
-          if (!in) b.x[t][0][i] = u32x4_t{0, 0, 0, 0};
-        } else {
-#pragma unroll
-          for (int p = 0; p < P; ++p) b.x[t][p][i] = *reinterpret_cast<const u32x4_t *>(xp[t] + ((c * P + p) * 8 + 4 * h + i) * 1024);
-        }
+      for (int t = 0; t < XG; ++t) {
+        b.x[t] = at128(x_base + half * 256, x_off[t] - back);
+        if (!in) b.x[t] = u32x4_t{0, 0, 0, 0};
       }
+    } else {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        int64_t tile = (m0 >> 4) + t;
+        tile = tile < g.tiles ? tile : g.tiles - 1;
+        const uint8_t *from = x_base + (tile * g.chunks + (half >> 1)) * (P * 8 * 1024);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) b.x[(t * P + p) * 4 + i] = at128(from + (p * 8 + 4 * (half & 1) + i) * 1024, static_cast<uint32_t>(lane) * 16);
+      }
+    }
   };
 
   floatx4_t acc[MT][NT];
@@ -175,37 +291,102 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
   for (int t = 0; t < MT; ++t)
 #pragma unroll
     for (int c = 0; c < NT; ++c) acc[t][c] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  auto compute = [&](const Half &b) __attribute__((always_inline)) {
+  // direct: a wave's rows of a half chunk through its own part of LDS into the operands' order; piece p of row r lies in place p ^ r, so that
+  // the reads of sixteen rows use every bank.  Lanes of rows that were not read hold others': their results are not stored.
+  unsigned char *const order = smem + (kDirect ? wave * (XG * 1024) : 0);
+  auto compute = [&](const Half &b, const Scales &s, int h) __attribute__((always_inline)) {
+    u32x4_t ordered[kDirect ? MT * 4 : 1];
+    if constexpr (kDirect) {
 #pragma unroll
-    for (int c = 0; c < NT; ++c)
+      for (int t = 0; t < XG; ++t) *reinterpret_cast<u32x4_t *>(order + (4 * t + q) * 256 + ((j ^ ((4 * t + q) & 15)) << 4)) = b.x[t];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int i = 0; i < XV; ++i) {
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = XG < 4 ? j & (4 * XG - 1) : 16 * t + j;
+          ordered[t * 4 + i] = *reinterpret_cast<const u32x4_t *>(order + row * 256 + (((4 * i + q) ^ (row & 15)) << 4));
+        }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+      if constexpr (kBoth) {
+        const uint32_t byte = kWhole ? s.w[kWhole ? c : 0][h] >> (8 * q) : b.scale[kWhole ? 0 : c];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          const uint32_t xb = kWhole ? s.x[kWhole ? t : 0][h] >> (8 * q) : b.x_scale[kWhole ? 0 : t];
+          acc[t][c] = mfma_micro(b.x[t], b.w[c][0], acc[t][c], xb, byte);
+        }
+      } else {
+        u32x4_t codes;
+        uint32_t bytes = 0;
+        if constexpr (kMicro) {
+          codes = exchange(b.w[c][0]);
+          bytes = kWhole ? s.w[kWhole ? c : 0][h] : b.scale[kWhole ? 0 : c];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          u32x4_t w;
+          if constexpr (kMicro) w = mxfp4_eight<CT>(codes[i], mxfp4_scale((bytes >> (8 * i)) & 255u));
+          else w = b.w[c][i];
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int p = 0; p < P; ++p) acc[t][c] = Mfma16<CT>::run(kDirect ? ordered[kDirect ? t * 4 + i : 0] : b.x[kDirect ? 0 : (t * P + p) * 4 + i], w, acc[t][c]);
+        }
+      }
+    }
+  };
+  // the halves of unit `unit`; what they leave free is asked for again: the unit's own later halves, then those of unit + 8
+  Half ring[D];
+  Scales scales;
+  auto run = [&](int unit, auto last_, auto part_) __attribute__((always_inline)) {
+    constexpr bool kLast = decltype(last_)::value, kPart = decltype(part_)::value;      // kPart: maybe less than four halves
+    Scales next;
+    if constexpr (!kLast) load_scales(next, unit + kRowsWaves);
+    if constexpr (kWhole && kPart) {
+      // the row's last 16 blocks begin `behind` dwords before this unit's
+      const int behind = 4 * unit + 4 - halves;
+      const auto forth = [&](u32x4_t &v) __attribute__((always_inline)) {
+        v = behind == 1 ? u32x4_t{v[1], v[2], v[3], 0} : behind == 2 ? u32x4_t{v[2], v[3], 0, 0} : u32x4_t{v[3], 0, 0, 0};
+      };
+      if (behind > 0) {
+#pragma unroll
+        for (int c = 0; c < NT; ++c) forth(scales.w[kWhole ? c : 0]);
         if constexpr (kBoth) {
 #pragma unroll
-          for (int t = 0; t < MT; ++t) acc[t][c] = mfma_micro(b.x[t][0][0], b.w[c][0], acc[t][c], b.x_scale[t], b.scale[c]);
-          continue;
+          for (int t = 0; t < MT; ++t) forth(scales.x[kWhole && kBoth ? t : 0]);
         }
-        u32x4_t w;
-        if constexpr (kMicro) w = mxfp4_eight<CT>(b.w[c][0][i], mxfp4_scale(b.scale[c]));
-        else w = b.w[c][i];
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int p = 0; p < P; ++p)
-            if constexpr (!kBoth) acc[t][c] = Mfma16<CT>::run(b.x[t][p][i], w, acc[t][c]);
       }
+    }
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      // (a branch here makes the compiler wait for all that is on its way; without one it asks for more than there are registers for where
+      // the tile is large)
+      if ((D > 1 && !kPart) || 4 * unit + h < halves) compute(ring[h % D], scales, h);
+      __builtin_amdgcn_sched_barrier(0);
+      if (h + D < 4) load(ring[h % D], 4 * unit + h + D);
+      else if constexpr (!kLast) load(ring[h % D], 4 * (unit + kRowsWaves) + h + D - 4);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (!kLast) scales = next;
   };
-  Half even, odd;
-  load(even, 0);
-  for (int at = 0; at < mine; at += 2) {
-    load(odd, at + 1);
-    compute(even);
-    load(even, at + 2);
-    compute(odd);
+  if (mine > 0) {
+    load_scales(scales, first);
+#pragma unroll
+    for (int h = 0; h < D; ++h) load(ring[h], 4 * first + h);
+    int unit = first;
+    for (int t = 1; t < mine; ++t, unit += kRowsWaves) run(unit, std::false_type{}, std::false_type{});
+    if (D == 1 || 4 * unit + 4 > halves) run(unit, std::true_type{}, std::true_type{});
+    else run(unit, std::true_type{}, std::false_type{});
   }
 
   // the eight waves' sums, in a fixed order: wave w + 4's into wave w's, then those four into the result
   constexpr int kHalf = kRowsWaves / 2;
+  if constexpr (kDirect) __syncthreads();      // (their places are others' activations until then)
   if (wave >= kHalf)
 #pragma unroll
     for (int t = 0; t < MT; ++t)
@@ -232,10 +413,10 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
     for (int at = threadIdx.x; at < MT * NC * 256; at += kRowsWaves * 64) {
       const int col = at % (16 * NC), row = at / (16 * NC);
       const int64_t m = m0 + row, n = n0 + col;
-      if (m >= g.M || n >= g.N) continue;
+      if (m >= g.M || col >= columns) continue;
       const int tile = (row >> 4) * NT + (col >> 4);
       const float v = total(tile, row & 15, col & 15);
-      const int64_t to = m * g.N + n;
+      const int64_t to = (z * g.M + m) * g.N + n;
       if constexpr (NW == 2) {
         const float u = total(tile + NC, row & 15, col & 15);
         static_cast<T *>(g.y)[to] = from_f32<T>(gate_act(v) * u);
@@ -255,11 +436,10 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
   else store(float{});
 }
 
-template <typename CT, int P, int kWeight, int NW, int MT, int NT, bool kDirect>
+template <typename CT, int P, int kWeight, int NW, int MT, int NT, int XG>
 int rows_launch(const RowsArgs &g, hipStream_t s)
 {
-  constexpr int NC = NT / NW;
-  const int64_t rows = (g.M + 16 * MT - 1) / (16 * MT), cols = (g.N + 16 * NC - 1) / (16 * NC);
+  const int64_t rows = (g.M + 16 * MT - 1) / (16 * MT), cols = (g.N + g.span - 1) / g.span;
   // a grid's second extent has 65535 blocks: more rows than that go in several launches
   for (int64_t r = 0; r < rows; r += 65535) {
     RowsArgs part = g;
@@ -267,45 +447,46 @@ int rows_launch(const RowsArgs &g, hipStream_t s)
     const auto forth = [&](const void *p, int64_t bytes) { return p ? const_cast<char *>(static_cast<const char *>(p)) + bytes : nullptr; };
     part.M = g.M - m0;
     part.tiles = g.tiles - static_cast<int>(m0 / 16);
-    part.x = forth(g.x, kWeight == ROWS_BOTH ? m0 * g.w_pitch : kDirect ? m0 * g.x_pitch * 2 : m0 / 16 * g.chunks * (P * 8 * 1024));
+    part.x = forth(g.x, kWeight == ROWS_BOTH ? m0 * g.w_pitch : XG > 0 ? m0 * g.x_pitch * 2 : m0 / 16 * g.chunks * (P * 8 * 1024));
     part.xs = g.xs ? g.xs + m0 * g.blocks : nullptr;
     part.y = forth(g.y, m0 * g.N * es);
     part.gate = forth(g.gate, m0 * g.N * es);
     part.up = forth(g.up, m0 * g.N * es);
     part.addend = forth(g.addend, m0 * g.N * es);
-    const dim3 grid(static_cast<unsigned>(cols), static_cast<unsigned>(rows - r < 65535 ? rows - r : 65535));
-    hipLaunchKernelGGL((rows_kernel<CT, P, kWeight, NW, MT, NT, kDirect>), grid, dim3(kRowsWaves * 64), 0, s, part);
+    const dim3 grid(static_cast<unsigned>(cols), static_cast<unsigned>(rows - r < 65535 ? rows - r : 65535), static_cast<unsigned>(g.splits));
+    if constexpr (kWeight != ROWS_DENSE) {
+      const bool whole = g.blocks % 4 == 0 && g.blocks >= 16 && g.R == 32 * g.blocks && aligned_to(g.s[0], 4) && aligned_to(g.s[1], 4) && aligned_to(g.xs, 4);
+      if (whole) hipLaunchKernelGGL((rows_kernel<CT, P, kWeight, NW, MT, NT, XG, true>), grid, dim3(kRowsWaves * 64), 0, s, part);
+      else hipLaunchKernelGGL((rows_kernel<CT, P, kWeight, NW, MT, NT, XG, false>), grid, dim3(kRowsWaves * 64), 0, s, part);
+    } else {
+      hipLaunchKernelGGL((rows_kernel<CT, P, kWeight, NW, MT, NT, XG, false>), grid, dim3(kRowsWaves * 64), 0, s, part);
+    }
   }
   return launch_status();
 }
 
-// Column tiles of a workgroup: as many as leave three quarters of the chip's 256 compute units a workgroup each.
-inline int rows_column_tiles(const RowsArgs &g, int weights, int mt)
-{
-  const int64_t rows = (g.M + 16 * mt - 1) / (16 * mt);
-  for (int nt = 4; nt > weights; nt /= 2)
-    if (rows * ((g.N + 16 * (nt / weights) - 1) / (16 * (nt / weights))) >= 192) return nt;
-  return weights;
-}
-
-template <typename CT, int P, int kWeight, int NW, int MT, bool kDirect>
+template <typename CT, int P, int kWeight, int NW, int MT, int XG>
 int rows_pick_columns(const RowsArgs &g, hipStream_t s)
 {
-  switch (rows_column_tiles(g, NW, MT)) {
-    case 4: return rows_launch<CT, P, kWeight, NW, MT, 4, kDirect>(g, s);
-    case 2: return rows_launch<CT, P, kWeight, NW, MT, 2, kDirect>(g, s);
-    default:
-      if constexpr (NW == 1) return rows_launch<CT, P, kWeight, NW, MT, 1, kDirect>(g, s);
-      else return rows_launch<CT, P, kWeight, NW, MT, 2, kDirect>(g, s);
+  const int tiles = NW * ((g.span + 15) / 16);
+  if (tiles > 2) return rows_launch<CT, P, kWeight, NW, MT, 4, XG>(g, s);
+  if constexpr (NW == 1) {
+    if (tiles == 1) return rows_launch<CT, P, kWeight, NW, MT, 1, XG>(g, s);
   }
+  return rows_launch<CT, P, kWeight, NW, MT, 2, XG>(g, s);
 }
 template <typename CT, int kWeight, int NW> int rows_pick(const RowsArgs &g, int pieces, bool direct, hipStream_t s)
 {
   if constexpr (dtype_code<CT>::value == CAIFX_BF16) {
-    if (pieces == 3) return rows_pick_columns<CT, 3, kWeight, NW, 1, false>(g, s);
+    if (pieces == 3) return rows_pick_columns<CT, 3, kWeight, NW, 1, 0>(g, s);
   }
-  if (direct) return g.M <= 16 ? rows_pick_columns<CT, 1, kWeight, NW, 1, true>(g, s) : rows_pick_columns<CT, 1, kWeight, NW, 2, true>(g, s);
-  return g.M <= 32 ? rows_pick_columns<CT, 1, kWeight, NW, 2, false>(g, s) : rows_pick_columns<CT, 1, kWeight, NW, 4, false>(g, s);
+  switch (rows_tile(g.M, 1)) {
+    case 16:
+      if (!direct) return rows_pick_columns<CT, 1, kWeight, NW, 1, 0>(g, s);
+      return g.M <= 4 ? rows_pick_columns<CT, 1, kWeight, NW, 1, 1>(g, s) : rows_pick_columns<CT, 1, kWeight, NW, 1, 4>(g, s);
+    case 32: return direct ? rows_pick_columns<CT, 1, kWeight, NW, 2, 8>(g, s) : rows_pick_columns<CT, 1, kWeight, NW, 2, 0>(g, s);
+    default: return rows_pick_columns<CT, 1, kWeight, NW, 4, 0>(g, s);
+  }
 }
 
 int rows_both(const RowsArgs &g, hipStream_t s);

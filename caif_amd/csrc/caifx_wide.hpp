@@ -31,5 +31,7 @@ __device__ __forceinline__ float gate_act(float g)
 // whether the kernel takes these sizes; every pointer has to be aligned to 16 bytes
 bool wide_takes(int64_t M, int64_t C, int64_t R);
 int wide_product(const WideProduct &p, hipStream_t s);
+// what a product takes, in us, estimated; gated: C of both weights together, chained: R of both pairs
+double wide_product_us(int64_t M, int64_t C, int64_t R);
 
 }  // namespace caifx
