@@ -209,7 +209,9 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(Wi
       if (t == Q / 2) first();
       const int u = t % (WI * WJ), kk = t / (WI * WJ);
       const int c = u / WI, i = (c & 1) ? WI - 1 - u % WI : u % WI;
-      mfma16<CT>(d[i][c], a[i][kk], b[c][kk]);
+      // (gated: the columns' operand first, so that a lane's four sums are neighbours of a row)
+      if constexpr (kGated) mfma16<CT>(d[i][c], b[c][kk], a[i][kk]);
+      else mfma16<CT>(d[i][c], a[i][kk], b[c][kk]);
       each(t);
       if (t & 1) __builtin_amdgcn_sched_barrier(0);
     }
@@ -340,14 +342,14 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(Wi
 #pragma unroll
       for (int i = 0; i < WI; ++i)
 #pragma unroll
-        for (int c = 0; c < WJ; ++c)
+        for (int c = 0; c < WJ; ++c) {
+          const floatx4_t a = acc[h][0][i][c], u = acc[h][1][i][c];
+          floatx4_t v;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int lrow = h * (BM / 2) + wm * 16 * WI + i * 16 + 4 * kq + r;
-            const float a = acc[h][0][i][c][r], u = acc[h][1][i][c][r];
-            *reinterpret_cast<CT *>(smem + lrow * kPitch + (wn * 16 * WJ + c * 16 + r16) * sizeof(CT)) =
-                from_f32<CT>(what == 0 ? gate_act(a) * u : what == 1 ? a : u);
-          }
+          for (int r = 0; r < 4; ++r) v[r] = what == 0 ? gate_act(a[r]) * u[r] : what == 1 ? a[r] : u[r];
+          *reinterpret_cast<u32x2_t *>(smem + (h * (BM / 2) + wm * 16 * WI + i * 16 + r16) * kPitch + (wn * 16 * WJ + c * 16 + 4 * kq) * sizeof(CT)) =
+              u32x2_t{pack2<CT>(v[0], v[1]), pack2<CT>(v[2], v[3])};
+        }
     __syncthreads();
 #pragma unroll
     for (int b = 0; b < kInstr; ++b) {

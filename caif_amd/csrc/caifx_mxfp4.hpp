@@ -19,8 +19,8 @@ int operand_transposed(const void *p, const void *scales, int kind, int64_t rows
 // source's chunks begin among `chunks`
 int operand_rows(const void *p, int kind, int64_t rows, int64_t cols, int to, void *out, int chunk0, int chunks, hipStream_t s);
 
-// y[M, C] = A B^T of two operands in microscaled 4 bits with `blocks` blocks a row, in tiles for the matrix cores.  The workspace is for scales
-// in rows of whole 16 bytes (their addresses are multiples of 16 where none is needed).
+// y[M, C] = A B^T of two operands in microscaled 4 bits with `blocks` blocks a row, in tiles for the matrix cores.  The workspace is for the
+// scales in another order.
 bool mx_gemm_takes(int64_t M, int64_t C, int64_t blocks);
 double mx_gemm_us(int64_t M, int64_t C, int64_t blocks);      // an estimate
 size_t mx_gemm_workspace_bytes(int64_t M, int64_t C, int64_t blocks);

@@ -3,7 +3,11 @@
 // v_mfma_scale_f32_16x16x128_f8f6f4 takes codes and scales as they are stored: lane (r, q) holds block q of row r, 16 bytes, and the
 // block's byte.  Four times the rate of bf16 from a quarter of the bytes, so the operands' way is the same as in caifx_gemm_wide.hip: a
 // step is 128 bytes of every row (256 values, two instructions deep), tiles of 64 WI x 64 WJ, four waves of a quarter each, half tiles
-// asked for three ahead straight into LDS.  Beside them the scales of two steps, 16 bytes of every row, in a ring of two.
+// asked for three ahead straight into LDS.  Beside them the scales of two steps, 16 bytes of every row, in a ring of two, from a copy that
+// holds the 1 KB of 64 rows together (from the rows themselves each request touches 64 lines, eight times over: 157 us instead of 141 at
+// M = 4096, N = 14336, K = 4096).
+// The columns' operand is the instruction's first one, so that a lane's four sums are neighbours of a row and go to LDS, on their way into
+// whole rows, 8 bytes (fp32: 16) at a time.
 // Blocks past the end of a row count for nothing: both scales are 2^-127 there, and codes have no infinities or NaN.
 #include "caifx_mxfp4.hpp"
 
@@ -17,10 +21,10 @@ constexpr int kBandRows = 1024;            // rows of a band of the tile order
 
 struct MxGemmArgs {
   const uint8_t *a, *b;         // codes [M, pitch], [C, pitch] bytes
-  const uint8_t *sa, *sb;       // scales [M, scale_pitch], [C, scale_pitch], scale_pitch a multiple of 16, zeros behind a row's blocks
+  const uint8_t *sa, *sb;       // scales in the order of order_scales_kernel, `groups` pieces of 16 bytes a row
   void *d;                      // [M, C]
-  int64_t M, C, pitch, scale_pitch;
-  int d_dtype;
+  int64_t M, C, pitch;
+  int groups, d_dtype;
 };
 
 __device__ __forceinline__ void mfma_mx(floatx4_t &acc, const u32x4_t &a, const u32x4_t &b, uint32_t sa, uint32_t sb)
@@ -105,22 +109,18 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void mx_gemm_kernel(MxGe
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(voff), "s"(src) : "memory");
   };
   // the scales of steps 2 group and 2 group + 1: a wave takes 64 rows of either operand (with 128 rows two waves the same ones)
-  const int groups = static_cast<int>(g.scale_pitch >> 4);
-  uint32_t sa_voff, sb_voff;
-  {
-    int64_t m = row0 + (64 * wave) % BM + lane, c = col0 + (64 * wave) % BN + lane;
-    m = m < g.M ? m : g.M - 1;
-    c = c < g.C ? c : g.C - 1;
-    sa_voff = static_cast<uint32_t>((m - row0) * g.scale_pitch);
-    sb_voff = static_cast<uint32_t>((c - col0) * g.scale_pitch);
-  }
-  const uint64_t sa_base = uniform64(reinterpret_cast<uint64_t>(g.sa) + static_cast<uint64_t>(row0 * g.scale_pitch));
-  const uint64_t sb_base = uniform64(reinterpret_cast<uint64_t>(g.sb) + static_cast<uint64_t>(col0 * g.scale_pitch));
+  const int groups = g.groups;
+  const uint32_t s_voff = static_cast<uint32_t>(lane) * 16;
+  const auto scales_of = [&](const uint8_t *scales, int64_t row) __attribute__((always_inline)) {
+    return uniform64(reinterpret_cast<uint64_t>(scales) + static_cast<uint64_t>((row >> 6) * groups) * 1024);
+  };
+  const uint64_t sa_base = scales_of(g.sa, row0 + (64 * wave) % BM < g.M ? row0 + (64 * wave) % BM : row0);      // (past the last row: others' scales)
+  const uint64_t sb_base = scales_of(g.sb, col0 + (64 * wave) % BN < g.C ? col0 + (64 * wave) % BN : col0);
   auto request_scales = [&](int group, int x) __attribute__((always_inline)) {
-    const uint32_t k0 = static_cast<uint32_t>(group < groups ? group : groups - 1) * 16;
+    const uint32_t k0 = static_cast<uint32_t>(group < groups ? group : groups - 1) * 1024;
     const uint64_t src = (x == 0 ? sa_base : sb_base) + k0;
     const uint32_t dst = lds0 + kScales + (group & 1) * kScaleSlot + (x == 0 ? (64 * wave) % BM : BM + (64 * wave) % BN) * 16;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(x == 0 ? sa_voff : sb_voff), "s"(src) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(s_voff), "s"(src) : "memory");
   };
 
   // operand (row tile i of 16 rows, reduction half kk): tiles i and i + 2 lie 32 rows apart, which flips the
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void mx_gemm_kernel(MxGe
       if (t == Q / 2) first();
       const int u = t % (WI * WJ), kk = t / (WI * WJ);
       const int c = u / WI, i = (c & 1) ? WI - 1 - u % WI : u % WI;
-      mfma_mx(d[i][c], a[i][kk].v, b[c][kk].v, a[i][kk].s, b[c][kk].s);
+      mfma_mx(d[i][c], b[c][kk].v, a[i][kk].v, b[c][kk].s, a[i][kk].s);
       each(t);
       if (t & 1) __builtin_amdgcn_sched_barrier(0);
     }
@@ -239,8 +239,8 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void mx_gemm_kernel(MxGe
   // latency), requests past the last step may still be writing LDS, and other waves may still be reading
   asm volatile("s_nop 15\n\ts_nop 15\n\ts_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
-  // store through LDS, whole tile rows at a time (fp32: half of them), row pitch = row + 32 bytes so that the four row groups of a wave's
-  // registers spread over the banks; 16 bytes per lane where the result's rows start at multiples of that, one value otherwise
+  // store through LDS, whole tile rows at a time (fp32: half of them), row pitch = row + 32 bytes so that the rows spread over the banks;
+  // 16 bytes per lane where the result's rows start at multiples of that, one value otherwise
   auto store = [&](auto type_) __attribute__((always_inline)) {
     typedef decltype(type_) T;
     constexpr int kPitch = BN * sizeof(T) + 32;
@@ -261,13 +261,12 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void mx_gemm_kernel(MxGe
 #pragma unroll
           for (int i = 0; i < WI; ++i)
 #pragma unroll
-            for (int c = 0; c < WJ; ++c)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const int lrow = hh * (BM / 2) + wm * 16 * WI + i * 16 + 4 * kq + r;
-                *reinterpret_cast<T *>(smem + lrow * kPitch + (q * (BN / 2) + wn * 16 * WJ + c * 16 + r16) * sizeof(T)) =
-                    from_f32<T>(acc[pass * kPassHalves + hh][q][i][c][r]);
-              }
+            for (int c = 0; c < WJ; ++c) {
+              const floatx4_t v = acc[pass * kPassHalves + hh][q][i][c];
+              unsigned char *to = smem + (hh * (BM / 2) + wm * 16 * WI + i * 16 + r16) * kPitch + (q * (BN / 2) + wn * 16 * WJ + c * 16 + 4 * kq) * sizeof(T);
+              if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2_t *>(to) = u32x2_t{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+              else *reinterpret_cast<floatx4_t *>(to) = v;
+            }
       __syncthreads();
       if (whole) {
 #pragma unroll
@@ -291,17 +290,33 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void mx_gemm_kernel(MxGe
   else store(float{});
 }
 
-// scales [rows, blocks] as rows of `pitch` bytes with zeros behind, four bytes a thread
-__global__ __launch_bounds__(256) void pad_scales_kernel(const uint8_t *__restrict__ scales, uint32_t *__restrict__ out, int64_t rows, int blocks, int pitch)
+// Scales [rows, blocks] of both operands as [rows / 64][groups][64][16]: the 16 bytes of a row that two steps need, 64 rows together, zeros
+// (2^-127) for blocks and rows that there are not.
+__global__ __launch_bounds__(256) void order_scales_kernel(const uint8_t *__restrict__ a, int64_t a_rows, const uint8_t *__restrict__ b, int64_t b_rows,
+                                                           u32x4_t *__restrict__ out, int blocks, int groups)
 {
-  const int words = pitch / 4;
-  for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < rows * words; at += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t row = at / words;
-    const int first = static_cast<int>(at - row * words) * 4;
-    uint32_t v = 0;
+  const int64_t a_pieces = (a_rows + 63) / 64 * groups * 64, pieces = a_pieces + (b_rows + 63) / 64 * groups * 64;
+  const bool dwords = blocks % 4 == 0 && (reinterpret_cast<uintptr_t>(a) & 3) == 0 && (reinterpret_cast<uintptr_t>(b) & 3) == 0;
+  for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < pieces; at += static_cast<int64_t>(gridDim.x) * 256) {
+    const bool second = at >= a_pieces;
+    const int64_t in = second ? at - a_pieces : at, tile = in / (64 * groups);
+    const int within = static_cast<int>(in - tile * 64 * groups), group = within >> 6;
+    const int64_t row = tile * 64 + (within & 63);
+    u32x4_t v = {0, 0, 0, 0};
+    if (row < (second ? b_rows : a_rows)) {
+      const uint8_t *from = (second ? b : a) + row * blocks + group * 16;
+      const int left = blocks - group * 16;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (first + i < blocks) v |= static_cast<uint32_t>(scales[row * blocks + first + i]) << (8 * i);
+      for (int d = 0; d < 4; ++d) {
+        if (dwords) {
+          if (4 * d < left) v[d] = *reinterpret_cast<const uint32_t *>(from + 4 * d);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (4 * d + i < left) v[d] |= static_cast<uint32_t>(from[4 * d + i]) << (8 * i);
+        }
+      }
+    }
     out[at] = v;
   }
 }
@@ -326,7 +341,8 @@ int launch_mx(const MxGemmArgs &g, hipStream_t s)
   return launch_status();
 }
 
-int64_t padded(int64_t blocks) { return (blocks + 15) / 16 * 16; }
+int64_t groups_of(int64_t blocks) { return (blocks + 15) / 16; }
+int64_t scale_bytes(int64_t rows, int64_t blocks) { return (rows + 63) / 64 * groups_of(blocks) * 1024; }
 
 }  // namespace
 
@@ -346,7 +362,7 @@ double mx_gemm_us(int64_t M, int64_t C, int64_t blocks)
 
 size_t mx_gemm_workspace_bytes(int64_t M, int64_t C, int64_t blocks)
 {
-  return blocks % 16 == 0 ? 0 : static_cast<size_t>(M + C) * static_cast<size_t>(padded(blocks));
+  return static_cast<size_t>(scale_bytes(M, blocks) + scale_bytes(C, blocks));
 }
 
 int mx_gemm(int64_t M, int64_t C, int64_t blocks, const void *a, const void *sa, const void *b, const void *sb, void *d, int d_dtype, void *workspace, hipStream_t s)
@@ -354,27 +370,17 @@ int mx_gemm(int64_t M, int64_t C, int64_t blocks, const void *a, const void *sa,
   MxGemmArgs g{};
   g.a = static_cast<const uint8_t *>(a);
   g.b = static_cast<const uint8_t *>(b);
-  g.sa = static_cast<const uint8_t *>(sa);
-  g.sb = static_cast<const uint8_t *>(sb);
   g.d = d;
   g.M = M;
   g.C = C;
   g.pitch = 16 * blocks;
-  g.scale_pitch = padded(blocks);
+  g.groups = static_cast<int>(groups_of(blocks));
   g.d_dtype = d_dtype;
-  if (blocks % 16 != 0 || !aligned_to(sa, 16) || !aligned_to(sb, 16)) {
-    uint8_t *to = static_cast<uint8_t *>(workspace);
-    const auto pad = [&](const uint8_t *from, int64_t rows) {
-      const int64_t words = rows * (g.scale_pitch / 4), grid = (words + 255) / 256;
-      hipLaunchKernelGGL(pad_scales_kernel, dim3(static_cast<unsigned>(grid < (1 << 20) ? grid : (1 << 20))), dim3(256), 0, s, from, reinterpret_cast<uint32_t *>(to),
-                         rows, static_cast<int>(blocks), static_cast<int>(g.scale_pitch));
-      const uint8_t *at = to;
-      to += rows * g.scale_pitch;
-      return at;
-    };
-    g.sa = pad(g.sa, M);
-    g.sb = pad(g.sb, C);
-  }
+  g.sa = static_cast<const uint8_t *>(workspace);
+  g.sb = g.sa + scale_bytes(M, blocks);
+  const int64_t grid = (scale_bytes(M, blocks) + scale_bytes(C, blocks)) / 16 / 256;
+  hipLaunchKernelGGL(order_scales_kernel, dim3(static_cast<unsigned>(grid < 1 ? 1 : grid < (1 << 20) ? grid : (1 << 20))), dim3(256), 0, s, static_cast<const uint8_t *>(sa), M,
+                     static_cast<const uint8_t *>(sb), C, static_cast<u32x4_t *>(workspace), static_cast<int>(blocks), g.groups);
   const bool tail = blocks % 8 != 0;
   // One workgroup of 256 x 256 per compute unit or two of 128 x 128: the large tile reads each operand half as often, and is taken once
   // there are enough of them.

@@ -436,8 +436,7 @@ int caifx_mxfp4_matmul(int64_t M, int64_t N, int64_t K, const void *a_codes, con
   const size_t need = caifx_mxfp4_matmul_workspace_bytes(M, N, K);
   if (need > 0 && (!workspace || workspace_bytes < need)) return CAIFX_ERR_WORKSPACE_TOO_SMALL;
   const int64_t blocks = blocks_of(K);
-  // (scales at an odd address would need a copy that the query did not count)
-  if (tiles_pay(M, N, blocks) && (mx_gemm_workspace_bytes(M, N, blocks) > 0 || (aligned_to(a_scales, 16) && aligned_to(b_scales, 16))))
+  if (tiles_pay(M, N, blocks))
     return mx_gemm(M, N, blocks, a_codes, a_scales, b_codes, b_scales, y, y_dtype, workspace, as_stream(stream));
   RowsArgs g = both_args(M, N, blocks);
   g.x = a_codes;
