@@ -41,9 +41,11 @@ struct WideArgs {
   bool zero_rest;
   unsigned long long *stamps;      // measurement only, see mfma_grouped_tile_stamps
   long long stamps_capacity;
-  // the forms over a pair of weights (WIDE_GATED, WIDE_CHAIN)
-  const void *a2, *b2;
+  // the forms of caifx_wide.hpp
+  const void *b2;
   void *gate, *up;
+  int64_t a_stride, b_stride;
+  int pairs, b_every;
 };
 
 // A result tile has 64 WI rows and 64 WJ columns.  Wave (wm, wn) owns rows h 32 WI + wm 16 WI + [0, 16 WI) and columns
@@ -56,13 +58,13 @@ struct WideArgs {
 // complete in issue order, so the wait for the half tile that is read next is an exact count (a wave issues WI + WJ
 // per half).
 // WIDE_GATED: half g of the columns belongs to the g-th weight, the same BN / 2 columns of each, so that a wave's accumulators of the two
-// halves hold gate and up of the same values and the gating happens where they are.  WIDE_CHAIN: the steps run through the first pair
-// of operands and then through the second.
+// halves hold gate and up of the same values and the gating happens where they are.  WIDE_CHAIN: the steps run through one pair of operands
+// after the other.  WIDE_RAGGED: a result whose rows are no whole, aligned pieces of 16 bytes is stored value by value.
 template <typename CT, int WI, int WJ, bool kGrouped, int kForm = WIDE_PLAIN>
 __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(WideArgs g)
 {
   typedef typename Mfma32<CT>::vec_t vec_t;
-  constexpr bool kGated = kForm == WIDE_GATED, kChain = kForm == WIDE_CHAIN;
+  constexpr bool kGated = (kForm & WIDE_GATED) != 0, kChain = (kForm & WIDE_CHAIN) != 0, kRagged = (kForm & WIDE_RAGGED) != 0;
   constexpr int BM = 64 * WI, BN = 64 * WJ;
   constexpr int BC = kGated ? BN / 2 : BN;      // columns of the result
   constexpr int kASlot = BM / 2 * 128, kBSlot = BN / 2 * 128;      // LDS bytes of half an operand tile
@@ -136,23 +138,35 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(Wi
   }
   const uint64_t a_base = uniform64(reinterpret_cast<uint64_t>(g.a) + static_cast<uint64_t>(row0 * g.R * 2));
   const uint64_t b_base = uniform64(b_ptr + static_cast<uint64_t>(col0 * g.R * 2));
-  const uint64_t b2_base = kForm != WIDE_PLAIN ? uniform64(reinterpret_cast<uint64_t>(g.b2) + static_cast<uint64_t>(col0 * g.R * 2)) : 0;
-  const uint64_t a2_base = kChain ? uniform64(reinterpret_cast<uint64_t>(g.a2) + static_cast<uint64_t>(row0 * g.R * 2)) : 0;
+  const uint64_t b2_base = kGated ? uniform64(reinterpret_cast<uint64_t>(g.b2) + static_cast<uint64_t>(col0 * g.R * 2)) : 0;
   const int part = static_cast<int>(g.R / kBK);
-  const int steps = kChain ? 2 * part : part;
+  const int steps = kChain ? g.pairs * part : part;
   const int last = steps - 1;
+  // chain: where the step that is asked for next has its operands, as offsets from the first pair's
+  int64_t a_at = 0, b_at = 0;
+  int asked = 0, in_part = 0, in_b = 0;
+  auto advance = [&]() __attribute__((always_inline)) {
+    if (asked >= last) return;
+    ++asked;
+    a_at += 128;
+    b_at += 128;
+    if (++in_part == part) {
+      in_part = 0;
+      a_at += g.a_stride - static_cast<int64_t>(part) * 128;
+      b_at -= static_cast<int64_t>(part) * 128;
+      if (++in_b == g.b_every) {
+        in_b = 0;
+        b_at += g.b_stride;
+      }
+    }
+  };
   auto request = [&](int s, int h, int slot, int x) __attribute__((always_inline)) {
     const uint32_t k0 = static_cast<uint32_t>(s < last ? s : last) * 128;          // past the end: the last step again
     const bool is_a = x < WI;
     const int i = is_a ? x : x - WI;
-    uint64_t src;
-    if constexpr (kChain) {
-      // (the second pair begins `part` steps into the sum)
-      const bool second = s >= part;
-      src = (second ? (is_a ? a2_base : b2_base) - static_cast<uint64_t>(part) * 128 : (is_a ? a_base : b_base)) + k0;
-    } else {
-      src = (is_a ? a_base : kGated && h == 1 ? b2_base : b_base) + k0;
-    }
+    uint64_t src = is_a ? a_base : kGated && h == 1 ? b2_base : b_base;
+    if constexpr (kChain) src += static_cast<uint64_t>(is_a ? a_at : b_at);
+    else src += k0;
     const uint32_t dst = lds0 + (is_a ? slot * kASlot : kBBase + slot * kBSlot) + (wave + 4 * i) * 1024;
     const uint32_t voff = is_a ? a_voff[h][is_a ? i : 0] : b_voff[h][is_a ? 0 : i];
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(voff), "s"(src) : "memory");
@@ -188,9 +202,13 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(Wi
         for (int c = 0; c < WJ; ++c) acc[h][q][i][c] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
 #pragma unroll
-  for (int u = 0; u < 4; ++u)
+  for (int u = 0; u < 4; ++u) {
 #pragma unroll
     for (int x = 0; x < kReq; ++x) request(u >> 1, u & 1, u, x);
+    if constexpr (kChain) {
+      if (u & 1) advance();
+    }
+  }
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * kReq) : "memory");
   vec_t a0[WI][2], a1[WI][2], b0[WJ][2], b1[WJ][2];
 #pragma unroll
@@ -244,6 +262,7 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(Wi
     quadrant(acc[1][0], a1, b0, nothing, [&](int t) __attribute__((always_inline)) {
       if (t % WI == WI - 1) b0[(t / WI) % WJ][t / (WI * WJ)] = read_b(S0n, (t / WI) % WJ, t / (WI * WJ));
     });
+    if constexpr (kChain) advance();
   };
   int s = 0;
   for (; s + 2 <= steps; s += 2) {
@@ -255,6 +274,18 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(Wi
   // latency), requests past the last step may still be writing LDS, and other waves may still be reading
   asm volatile("s_nop 15\n\ts_nop 15\n\ts_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
+  // rows [from, from + rows) of the tile, laid out in LDS, one value at a time
+  auto ragged = [&](auto type_, void *to, const void *addend, int from, int rows, int pitch) __attribute__((always_inline)) {
+    typedef decltype(type_) T;
+    for (int at = threadIdx.x; at < rows * BC; at += 256) {
+      const int lrow = at / BC, col = at % BC;
+      const int64_t grow = row0 + from + lrow, gcol = col0 + col;
+      if (grow >= row_end || gcol >= g.C) continue;
+      T v = *reinterpret_cast<const T *>(smem + lrow * pitch + col * sizeof(T));
+      if (addend) v = from_f32<T>(to_f32<T>(v) + to_f32<T>(static_cast<const T *>(addend)[grow * g.C + gcol]));
+      static_cast<T *>(to)[grow * g.C + gcol] = v;
+    }
+  };
   // store through LDS: a pass of whole tile rows (16-bit results: all of them, fp32: one half), row pitch = row + 32
   // bytes so that the four row groups of a wave's registers spread over the banks, then whole rows, 16 bytes per lane.
   // The optional addend is read the same way, a batch of rows ahead (the operand registers are free by now): read row
@@ -287,7 +318,7 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(Wi
 #pragma unroll
     for (int pass = 0; pass < 2 / kPassHalves; ++pass) {
       if (pass > 0) __syncthreads();
-      if constexpr (kAdd) fetch(add[0], pass, 0);
+      if constexpr (kAdd && !kRagged) fetch(add[0], pass, 0);
 #pragma unroll
       for (int hh = 0; hh < kPassHalves; ++hh)
 #pragma unroll
@@ -303,6 +334,10 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(Wi
                     from_f32<T>(acc[pass * kPassHalves + hh][q][i][c][r]);
               }
       __syncthreads();
+      if constexpr (kRagged) {
+        ragged(type_, g.d, kAdd ? g.addend : nullptr, pass * (BM / 2), kRows, kPitch);
+        continue;
+      }
 #pragma unroll
       for (int batch = 0; batch < kInstr / kBatch; ++batch) {
         if constexpr (kAdd) {
@@ -328,45 +363,60 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(Wi
     }
   };
   // gated: the result and, where they are kept, the two projections, one after the other through LDS
-  auto store_gated = [&](auto what_) __attribute__((always_inline)) {
+  auto store_gated = [&](auto type_, auto what_) __attribute__((always_inline)) {
+    typedef decltype(type_) T;
     constexpr int what = decltype(what_)::value;         // 0 hidden, 1 gate, 2 up
-    constexpr int kPitch = BC * sizeof(CT) + 32;
-    constexpr int kLanesPerRow = BC / 8;
+    constexpr int kPitch = BC * sizeof(T) + 32;
+    constexpr int kPer16 = 16 / sizeof(T);
+    constexpr int kLanesPerRow = BC / kPer16;
     constexpr int kRowsPerInstr = 64 / kLanesPerRow;
-    constexpr int kInstr = BM / (4 * kRowsPerInstr);
-    CT *dp = static_cast<CT *>(what == 0 ? g.d : what == 1 ? g.gate : g.up);
+    constexpr int kPassHalves = sizeof(T) == 2 ? 2 : 1;
+    constexpr int kRows = kPassHalves * (BM / 2);
+    T *dp = static_cast<T *>(what == 0 ? g.d : what == 1 ? g.gate : g.up);
     const int chunk = lane % kLanesPerRow;
-    const int64_t gcol = col0 + chunk * 8;
+    const int64_t gcol = col0 + chunk * kPer16;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int pass = 0; pass < 2 / kPassHalves; ++pass) {
+      if (pass > 0 || what > 0) __syncthreads();
 #pragma unroll
-      for (int i = 0; i < WI; ++i)
+      for (int hh = 0; hh < kPassHalves; ++hh)
 #pragma unroll
-        for (int c = 0; c < WJ; ++c) {
-          const floatx4_t a = acc[h][0][i][c], u = acc[h][1][i][c];
-          floatx4_t v;
+        for (int i = 0; i < WI; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = what == 0 ? gate_act(a[r]) * u[r] : what == 1 ? a[r] : u[r];
-          *reinterpret_cast<u32x2_t *>(smem + (h * (BM / 2) + wm * 16 * WI + i * 16 + r16) * kPitch + (wn * 16 * WJ + c * 16 + 4 * kq) * sizeof(CT)) =
-              u32x2_t{pack2<CT>(v[0], v[1]), pack2<CT>(v[2], v[3])};
+          for (int c = 0; c < WJ; ++c) {
+            const floatx4_t a = acc[pass * kPassHalves + hh][0][i][c], u = acc[pass * kPassHalves + hh][1][i][c];
+            floatx4_t v;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = what == 0 ? gate_act(a[r]) * u[r] : what == 1 ? a[r] : u[r];
+            unsigned char *to = smem + (hh * (BM / 2) + wm * 16 * WI + i * 16 + r16) * kPitch + (wn * 16 * WJ + c * 16 + 4 * kq) * sizeof(T);
+            if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2_t *>(to) = u32x2_t{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+            else *reinterpret_cast<floatx4_t *>(to) = v;
+          }
+      __syncthreads();
+      if constexpr (kRagged) {
+        ragged(type_, dp, nullptr, pass * (BM / 2), kRows, kPitch);
+      } else {
+#pragma unroll
+        for (int b = 0; b < kRows / (4 * kRowsPerInstr); ++b) {
+          const int lrow = (b * 4 + wave) * kRowsPerInstr + lane / kLanesPerRow;
+          const int64_t grow = row0 + pass * (BM / 2) + lrow;
+          const u32x4_t v = *reinterpret_cast<const u32x4_t *>(smem + lrow * kPitch + chunk * 16);
+          if (grow < row_end && gcol < g.C) *reinterpret_cast<u32x4_t *>(dp + grow * g.C + gcol) = v;
         }
-    __syncthreads();
-#pragma unroll
-    for (int b = 0; b < kInstr; ++b) {
-      const int lrow = (b * 4 + wave) * kRowsPerInstr + lane / kLanesPerRow;
-      const int64_t grow = row0 + lrow;
-      const u32x4_t v = *reinterpret_cast<const u32x4_t *>(smem + lrow * kPitch + chunk * 16);
-      if (grow < row_end && gcol < g.C) *reinterpret_cast<u32x4_t *>(dp + grow * g.C + gcol) = v;
+      }
     }
   };
   if constexpr (kGated) {
-    store_gated(std::integral_constant<int, 0>{});
-    if (g.gate) {
-      __syncthreads();
-      store_gated(std::integral_constant<int, 1>{});
-      __syncthreads();
-      store_gated(std::integral_constant<int, 2>{});
-    }
+    auto all = [&](auto type_) __attribute__((always_inline)) {
+      store_gated(type_, std::integral_constant<int, 0>{});
+      if (g.gate) {
+        store_gated(type_, std::integral_constant<int, 1>{});
+        store_gated(type_, std::integral_constant<int, 2>{});
+      }
+    };
+    // (fp32 comes as a chain of its bf16 pieces)
+    if constexpr (kChain) all(float{});
+    else all(CT{});
     return;
   }
   auto store_as = [&](auto type_) __attribute__((always_inline)) {
@@ -528,7 +578,7 @@ int launch_dense(const DenseArgs &g, int kind, bool transposed, int experts, hip
 template <typename CT, int WI, int WJ, bool kGrouped, int kForm = WIDE_PLAIN>
 int launch_wide(const WideArgs &g, hipStream_t s)
 {
-  constexpr int BM = 64 * WI, BN = 64 * WJ, BC = kForm == WIDE_GATED ? BN / 2 : BN;
+  constexpr int BM = 64 * WI, BN = 64 * WJ, BC = (kForm & WIDE_GATED) ? BN / 2 : BN;
   constexpr int kRing = (BM + BN) * 256, kStore16 = BM * (BN * 2 + 32), kStore32 = BM / 2 * (BN * 4 + 32);
   constexpr int kStore = kStore16 > kStore32 ? kStore16 : kStore32;
   constexpr int kLds = kRing > kStore ? kRing : kStore;
@@ -647,7 +697,7 @@ template <typename CT, bool kGrouped, int kForm = WIDE_PLAIN>
 int pick_wide(const WideArgs &g, hipStream_t s)
 {
   // (gated: as many tiles as a plain product with both weights' columns has)
-  switch (best_tile(g.M, kForm == WIDE_GATED ? 2 * g.C : g.C, g.num_experts)) {
+  switch (best_tile(g.M, (kForm & WIDE_GATED) ? 2 * g.C : g.C, g.num_experts)) {
     case TILE_256: return launch_wide<CT, 4, 4, kGrouped, kForm>(g, s);
     case TILE_128x256: return launch_wide<CT, 2, 4, kGrouped, kForm>(g, s);
     default: return launch_wide<CT, 2, 2, kGrouped, kForm>(g, s);
@@ -795,7 +845,7 @@ int mfma_wide(const GemmArgs &a, bool backward, hipStream_t s)
 bool wide_takes(int64_t M, int64_t C, int64_t R)
 {
   // (row offsets inside a tile have 32 bits)
-  return M > 0 && M <= (int64_t{1} << 30) && C > 0 && C % 8 == 0 && R % kBK == 0 && R >= 2 * kBK && R < (int64_t{1} << 22) &&
+  return M > 0 && M <= (int64_t{1} << 30) && C > 0 && R % kBK == 0 && R >= 2 * kBK && R < (int64_t{1} << 22) &&
          ((M + 127) / 128) * ((C + 63) / 64) <= (int64_t{1} << 30);
 }
 
@@ -804,11 +854,20 @@ double wide_product_us(int64_t M, int64_t C, int64_t R)
   return wide_us_of(M, C, R);
 }
 
+template <typename CT, int kForm> static int wide_form(const WideArgs &g, int form, hipStream_t s)
+{
+  // (gated fp32, a chain of bf16 pieces, has no fp16 form)
+  if constexpr (dtype_code<CT>::value == CAIFX_BF16 || (kForm & 3) != 3) {
+    if (form == kForm) return pick_wide<CT, false, kForm>(g, s);
+  }
+  if constexpr (kForm > 1) return wide_form<CT, kForm - 1>(g, form, s);
+  else return pick_wide<CT, false>(g, s);
+}
+
 int wide_product(const WideProduct &p, hipStream_t s)
 {
   WideArgs g{};
-  g.a = p.a[0];
-  g.a2 = p.a[1];
+  g.a = p.a;
   g.b = p.b[0];
   g.b2 = p.b[1];
   g.d = p.d;
@@ -818,14 +877,16 @@ int wide_product(const WideProduct &p, hipStream_t s)
   g.M = p.M;
   g.C = p.C;
   g.R = p.R;
+  g.a_stride = p.a_stride;
+  g.b_stride = p.b_stride;
+  g.pairs = p.pairs;
+  g.b_every = p.b_every;
   g.d_dtype = p.d_dtype;
-  const auto go = [&](auto type_) {
-    typedef decltype(type_) CT;
-    if (p.form == WIDE_GATED) return pick_wide<CT, false, WIDE_GATED>(g, s);
-    if (p.form == WIDE_CHAIN) return pick_wide<CT, false, WIDE_CHAIN>(g, s);
-    return pick_wide<CT, false>(g, s);
-  };
-  return p.compute_dtype == CAIFX_BF16 ? go(bf16_t{}) : go(f16_t{});
+  const int64_t whole = p.d_dtype == CAIFX_F32 ? 4 : 8;
+  const bool ragged = p.C % whole != 0 || !aligned_to(p.d, 16) || !aligned_to(p.gate, 16) || !aligned_to(p.up, 16) || !aligned_to(p.addend, 16);
+  const int form = (p.gated ? WIDE_GATED : 0) | (p.pairs > 1 ? WIDE_CHAIN : 0) | (ragged ? WIDE_RAGGED : 0);
+  if (p.compute_dtype == CAIFX_BF16) return wide_form<bf16_t, 7>(g, form, s);
+  return wide_form<f16_t, 7>(g, form, s);
 }
 
 }  // namespace caifx

@@ -144,6 +144,9 @@ struct Source {
   int64_t rows, cols, blocks;
 };
 struct Mx {};                // a source in microscaled 4 bits
+struct Sources {             // one or two of one shape, a launch's last extent
+  Source g[2];
+};
 
 // eight values (n, k .. k + 7) of a source in CT, zeros outside; k is a multiple of 8
 template <typename S, typename CT> __device__ __forceinline__ u32x4_t source8(const Source &g, int64_t n, int64_t k)
@@ -177,11 +180,13 @@ template <typename S, typename CT> __device__ __forceinline__ u32x4_t source8(co
   }
 }
 
-// [rows, cols] as dense rows of CT, `pitch` long with zeros behind the last column, from column `first` of rows `stride` long
+// [rows, cols] as dense rows of CT, `pitch` long with zeros behind the last column; the second source's rows behind the first's
 template <typename S, typename CT>
-__global__ __launch_bounds__(kThreads) void dense_kernel(Source g, CT *__restrict__ out, int64_t pitch, int64_t stride, int64_t first)
+__global__ __launch_bounds__(kThreads) void dense_kernel(Sources two, CT *__restrict__ out, int64_t pitch)
 {
   constexpr int kRounds = 4;
+  const Source g = two.g[blockIdx.z];
+  out += blockIdx.z * g.rows * pitch;
   const int64_t pieces = pitch / kPer;
   for (int64_t n = blockIdx.y; n < g.rows; n += gridDim.y) {
     const int64_t p0 = static_cast<int64_t>(blockIdx.x) * (kThreads * kRounds) + threadIdx.x;
@@ -191,18 +196,20 @@ __global__ __launch_bounds__(kThreads) void dense_kernel(Source g, CT *__restric
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
       const int64_t p = p0 + r * kThreads;
-      if (p < pieces) *reinterpret_cast<u32x4_t *>(out + n * stride + first + p * kPer) = v[r];
+      if (p < pieces) *reinterpret_cast<u32x4_t *>(out + n * pitch + p * kPer) = v[r];
     }
   }
 }
 
-// the same transposed: [cols] rows, each from column `first` of `stride` with the rows' values, zeros up to `pitch` (a multiple of 64).
+// the same transposed: [cols] rows `stride` long with the rows' values, zeros up to a multiple of 64; the second source's `second` values on.
 // A workgroup takes 64 rows x 256 columns: a thread reads eight columns of eight rows and lays them out in LDS as rows of 64 n, which
 // are then written in whole 128-byte lines.  The piece position is rotated by the thread's columns so that the eight lanes of a group
 // use different banks.
 template <typename S, typename CT>
-__global__ __launch_bounds__(kThreads) void dense_transposed_kernel(Source g, CT *__restrict__ out, int64_t stride, int64_t first)
+__global__ __launch_bounds__(kThreads) void dense_transposed_kernel(Sources two, CT *__restrict__ out, int64_t stride, int64_t second)
 {
+  const Source g = two.g[blockIdx.z];
+  out += blockIdx.z * second;
   __shared__ __attribute__((aligned(16))) unsigned char tile[256 * 128];
   const int kl = threadIdx.x & 31, ng = threadIdx.x >> 5;
   const int64_t n0 = static_cast<int64_t>(blockIdx.y) * 64, k0 = static_cast<int64_t>(blockIdx.x) * 256;
@@ -223,46 +230,70 @@ __global__ __launch_bounds__(kThreads) void dense_transposed_kernel(Source g, CT
     const int k = it * 32 + (threadIdx.x >> 3);
     if (k0 + k >= g.cols) continue;
     const u32x4_t v = *reinterpret_cast<const u32x4_t *>(tile + k * 128 + (((piece + (k >> 3)) & 7) << 4));
-    *reinterpret_cast<u32x4_t *>(out + (k0 + k) * stride + first + n0 + 8 * piece) = v;
+    *reinterpret_cast<u32x4_t *>(out + (k0 + k) * stride + n0 + 8 * piece) = v;
+  }
+}
+
+// Eight values (m, k .. k + 7) of activations as three bf16 pieces each, which add up to them: the upper 8 bits of the mantissa, the next 8
+// and the rest, each cut off and so exact.  Zeros outside.
+template <typename S> __device__ __forceinline__ void pieces8(const Source &g, int64_t m, int64_t k, Eight<uint16_t> (&piece)[3])
+{
+  const int64_t left = m < g.rows ? g.cols - k : 0;
+  const Eight<S> e = load8(static_cast<const S *>(g.p) + m * g.cols + k, left > 0 ? (left < kPer ? static_cast<int>(left) : kPer) : 0);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const float value = to_f32<S>(e.v[i]);
+    const uint32_t bits = __builtin_bit_cast(uint32_t, value), high = bits & 0xFFFF0000u;
+    const bool finite = (bits & 0x7F800000u) != 0x7F800000u;
+    const float rest = value - __builtin_bit_cast(float, high);
+    const uint32_t middle = __builtin_bit_cast(uint32_t, rest) & 0xFFFF0000u;
+    const float last = rest - __builtin_bit_cast(float, middle);
+    // a NaN whose upper bits alone would be an infinity stays a NaN
+    const uint32_t nan = !finite && (bits & 0x007FFFFFu) != 0 ? 0x00400000u : 0u;
+    piece[0].v[i] = static_cast<uint16_t>((high | nan) >> 16);
+    piece[1].v[i] = finite ? static_cast<uint16_t>(middle >> 16) : 0;
+    piece[2].v[i] = finite ? static_cast<uint16_t>(__builtin_bit_cast(uint32_t, last) >> 16) : 0;
+  }
+}
+
+// The pieces of fp32 activations as three dense matrices [rows, pitch], one behind the other, zeros behind the last column; the second
+// source's behind the first's.
+template <typename S>
+__global__ __launch_bounds__(kThreads) void pieces_kernel(Sources two, uint16_t *__restrict__ out, int64_t pitch)
+{
+  const Source g = two.g[blockIdx.z];
+  const int64_t piece_size = g.rows * pitch, p = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  out += blockIdx.z * 3 * piece_size;
+  if (p * kPer >= pitch) return;
+  for (int64_t m = blockIdx.y; m < g.rows; m += gridDim.y) {
+    Eight<uint16_t> piece[3];
+    pieces8<S>(g, m, p * kPer, piece);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) *reinterpret_cast<u32x4_t *>(out + i * piece_size + m * pitch + p * kPer) = __builtin_bit_cast(u32x4_t, piece[i]);
   }
 }
 
 // Activations in the order in which the row kernels read them: for each tile of 16 rows, chunk of 256 reduction elements and piece, eight
-// kilobytes of which the u-th holds every lane's operand of instruction u.  fp32 in P = 3 pieces: the upper 8 bits of the mantissa, the next
-// 8 and the rest, each cut off and so exact.
+// kilobytes of which the u-th holds every lane's operand of instruction u.  fp32 in P = 3 pieces.
 template <typename S, typename CT, int P>
-__global__ __launch_bounds__(kThreads) void pack_rows_kernel(Source g, unsigned char *__restrict__ out, int chunk0, int chunks)
+__global__ __launch_bounds__(kThreads) void pack_rows_kernel(Sources two, unsigned char *__restrict__ out, int own, int chunks)
 {
-  const int64_t tile = blockIdx.y + static_cast<int64_t>(blockIdx.z) * gridDim.y;
-  if (tile * 16 >= g.rows) return;
-  const int c = static_cast<int>(blockIdx.x);
-  unsigned char *to = out + (tile * chunks + chunk0 + c) * (P * 8 * 1024);
+  const Source g = two.g[blockIdx.z];
+  const int c = static_cast<int>(blockIdx.x), chunk0 = static_cast<int>(blockIdx.z) * own;
+  for (int64_t tile = blockIdx.y; tile * 16 < g.rows; tile += gridDim.y) {
+    unsigned char *to = out + (tile * chunks + chunk0 + c) * (P * 8 * 1024);
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int at = half * kThreads + threadIdx.x, lane = at & 63, u = at >> 6;
-    const int64_t m = tile * 16 + (lane & 15), k = static_cast<int64_t>(c) * kRowsChunk + 32 * u + 8 * (lane >> 4);
-    if constexpr (P == 1) {
-      *reinterpret_cast<u32x4_t *>(to + at * 16) = source8<S, CT>(g, m, k);
-    } else {
-      const int64_t left = g.cols - k;
-      const Eight<S> e = load8(static_cast<const S *>(g.p) + m * g.cols + k, m < g.rows && left > 0 ? (left < kPer ? static_cast<int>(left) : kPer) : 0);
-      Eight<uint16_t> piece[3];
+    for (int half = 0; half < 2; ++half) {
+      const int at = half * kThreads + threadIdx.x, lane = at & 63, u = at >> 6;
+      const int64_t m = tile * 16 + (lane & 15), k = static_cast<int64_t>(c) * kRowsChunk + 32 * u + 8 * (lane >> 4);
+      if constexpr (P == 1) {
+        *reinterpret_cast<u32x4_t *>(to + at * 16) = source8<S, CT>(g, m, k);
+      } else {
+        Eight<uint16_t> piece[3];
+        pieces8<S>(g, m, k, piece);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const float value = to_f32<S>(e.v[i]);
-        const uint32_t bits = __builtin_bit_cast(uint32_t, value), high = bits & 0xFFFF0000u;
-        const bool finite = (bits & 0x7F800000u) != 0x7F800000u;
-        const float rest = value - __builtin_bit_cast(float, high);
-        const uint32_t middle = __builtin_bit_cast(uint32_t, rest) & 0xFFFF0000u;
-        const float last = rest - __builtin_bit_cast(float, middle);
-        // a NaN whose upper bits alone would be an infinity stays a NaN
-        const uint32_t nan = !finite && (bits & 0x007FFFFFu) != 0 ? 0x00400000u : 0u;
-        piece[0].v[i] = static_cast<uint16_t>((high | nan) >> 16);
-        piece[1].v[i] = finite ? static_cast<uint16_t>(middle >> 16) : 0;
-        piece[2].v[i] = finite ? static_cast<uint16_t>(__builtin_bit_cast(uint32_t, last) >> 16) : 0;
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4_t *>(to + p * 8192 + at * 16) = __builtin_bit_cast(u32x4_t, piece[p]);
       }
-#pragma unroll
-      for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4_t *>(to + p * 8192 + at * 16) = __builtin_bit_cast(u32x4_t, piece[p]);
     }
   }
 }
@@ -290,16 +321,18 @@ __global__ __launch_bounds__(kThreads) void gating_backward_kernel(const T *__re
   }
 }
 
-Source source(const void *p, const void *scales, int64_t rows, int64_t cols)
+Sources sources(const Operand &a)
 {
-  return Source{p, static_cast<const uint8_t *>(scales), rows, cols, (cols + kBlock - 1) / kBlock};
+  const int64_t blocks = (a.cols + kBlock - 1) / kBlock;
+  return Sources{{Source{a.p[0], static_cast<const uint8_t *>(a.scales[0]), a.rows, a.cols, blocks}, Source{a.p[1], static_cast<const uint8_t *>(a.scales[1]), a.rows, a.cols, blocks}}};
 }
+unsigned rows_grid(int64_t rows) { return static_cast<unsigned>(rows < 65535 ? rows : 65535); }
 
 }  // namespace
 
 // one call for the source's and the target's type
 #define CAIFX_BY_SOURCE(...)                                                    \
-  switch (kind) {                                                               \
+  switch (a.kind) {                                                             \
     case OPERAND_MX: { typedef Mx S; __VA_ARGS__; break; }                      \
     case CAIFX_F32: { typedef float S; __VA_ARGS__; break; }                    \
     case CAIFX_F16: { typedef f16_t S; __VA_ARGS__; break; }                    \
@@ -309,36 +342,38 @@ Source source(const void *p, const void *scales, int64_t rows, int64_t cols)
   if (to == CAIFX_BF16) { typedef bf16_t CT; CAIFX_BY_SOURCE(__VA_ARGS__) }     \
   else { typedef f16_t CT; CAIFX_BY_SOURCE(__VA_ARGS__) }
 
-int operand_dense(const void *p, const void *scales, int kind, int64_t rows, int64_t cols, int to, void *out, int64_t pitch, int64_t stride, int64_t first,
-                  hipStream_t s)
+int operand_dense(const Operand &a, int to, void *out, int64_t pitch, hipStream_t s)
 {
-  const Source g = source(p, scales, rows, cols);
-  const dim3 grid(static_cast<unsigned>((pitch / kPer + 1023) / 1024), static_cast<unsigned>(rows < 65535 ? rows : 65535));
-  CAIFX_BY_TARGET(hipLaunchKernelGGL((dense_kernel<S, CT>), grid, dim3(kThreads), 0, s, g, static_cast<CT *>(out), pitch, stride, first))
+  const dim3 grid(static_cast<unsigned>((pitch / kPer + 1023) / 1024), rows_grid(a.rows), static_cast<unsigned>(a.count));
+  CAIFX_BY_TARGET(hipLaunchKernelGGL((dense_kernel<S, CT>), grid, dim3(kThreads), 0, s, sources(a), static_cast<CT *>(out), pitch))
   return launch_status();
 }
 
-int operand_transposed(const void *p, const void *scales, int kind, int64_t rows, int64_t cols, int to, void *out, int64_t pitch, int64_t stride, int64_t first,
-                       hipStream_t s)
+int operand_transposed(const Operand &a, int to, void *out, int64_t pitch, int64_t stride, int64_t second, hipStream_t s)
 {
-  const Source g = source(p, scales, rows, cols);
-  const dim3 grid(static_cast<unsigned>((cols + 255) / 256), static_cast<unsigned>(pitch / 64));
-  CAIFX_BY_TARGET(hipLaunchKernelGGL((dense_transposed_kernel<S, CT>), grid, dim3(kThreads), 0, s, g, static_cast<CT *>(out), stride, first))
+  const dim3 grid(static_cast<unsigned>((a.cols + 255) / 256), static_cast<unsigned>(pitch / 64), static_cast<unsigned>(a.count));
+  CAIFX_BY_TARGET(hipLaunchKernelGGL((dense_transposed_kernel<S, CT>), grid, dim3(kThreads), 0, s, sources(a), static_cast<CT *>(out), stride, second))
   return launch_status();
 }
 
-int operand_rows(const void *p, int kind, int64_t rows, int64_t cols, int to, void *out, int chunk0, int chunks, hipStream_t s)
+int operand_pieces(const Operand &a, void *out, int64_t pitch, hipStream_t s)
 {
-  const Source g = source(p, nullptr, rows, cols);
-  const int64_t tiles = (rows + 15) / 16;
-  const unsigned y = static_cast<unsigned>(tiles < 32768 ? tiles : 32768);
-  const dim3 grid(static_cast<unsigned>((cols + kRowsChunk - 1) / kRowsChunk), y, static_cast<unsigned>((tiles + y - 1) / y));
+  const dim3 grid(static_cast<unsigned>((pitch / kPer + kThreads - 1) / kThreads), rows_grid(a.rows), static_cast<unsigned>(a.count));
+  if (a.kind == CAIFX_F32) hipLaunchKernelGGL((pieces_kernel<float>), grid, dim3(kThreads), 0, s, sources(a), static_cast<uint16_t *>(out), pitch);
+  else hipLaunchKernelGGL((pieces_kernel<f16_t>), grid, dim3(kThreads), 0, s, sources(a), static_cast<uint16_t *>(out), pitch);
+  return launch_status();
+}
+
+int operand_rows(const Operand &a, int to, void *out, int chunks, hipStream_t s)
+{
+  const int own = static_cast<int>((a.cols + kRowsChunk - 1) / kRowsChunk);
+  const dim3 grid(static_cast<unsigned>(own), rows_grid((a.rows + 15) / 16), static_cast<unsigned>(a.count));
   unsigned char *o = static_cast<unsigned char *>(out);
   if (to == CAIFX_F32) {
-    if (kind == CAIFX_F32) hipLaunchKernelGGL((pack_rows_kernel<float, bf16_t, 3>), grid, dim3(kThreads), 0, s, g, o, chunk0, chunks);
-    else hipLaunchKernelGGL((pack_rows_kernel<f16_t, bf16_t, 3>), grid, dim3(kThreads), 0, s, g, o, chunk0, chunks);
+    if (a.kind == CAIFX_F32) hipLaunchKernelGGL((pack_rows_kernel<float, bf16_t, 3>), grid, dim3(kThreads), 0, s, sources(a), o, own, chunks);
+    else hipLaunchKernelGGL((pack_rows_kernel<f16_t, bf16_t, 3>), grid, dim3(kThreads), 0, s, sources(a), o, own, chunks);
   } else {
-    CAIFX_BY_TARGET(hipLaunchKernelGGL((pack_rows_kernel<S, CT, 1>), grid, dim3(kThreads), 0, s, g, o, chunk0, chunks))
+    CAIFX_BY_TARGET(hipLaunchKernelGGL((pack_rows_kernel<S, CT, 1>), grid, dim3(kThreads), 0, s, sources(a), o, own, chunks))
   }
   return launch_status();
 }

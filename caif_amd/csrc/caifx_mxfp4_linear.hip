@@ -79,7 +79,7 @@ int rows_run(RowsArgs g, int kind, int weights, int compute_dtype, bool direct, 
   const int tile = rows_tile(g.M, pieces);
   const double row = kind == ROWS_DENSE ? static_cast<double>(g.w_pitch) : 17.0 * static_cast<double>(g.blocks);
   const double x = (kind == ROWS_BOTH ? row : 2.0 * pieces * static_cast<double>(g.R)) * (g.M <= 4 && pieces == 1 ? 4 : tile);
-  const RowsPlan plan = rows_plan(g.M, g.N, g.R, weights, tile, row, x);
+  const RowsPlan plan = rows_plan(g.M, g.N, g.R, weights, pieces, row, x);
   void *partial = plan.splits > 1 ? room.take(static_cast<size_t>(plan.splits) * static_cast<size_t>(g.M) * static_cast<size_t>(g.N) * 4) : nullptr;
   if (only_size) return CAIFX_OK;
   g.span = plan.span;
@@ -98,46 +98,77 @@ int rows_run(RowsArgs g, int kind, int weights, int compute_dtype, bool direct, 
 // whether the row kernels can read the activations where they are
 bool direct_type(const Product &p) { return p.compute_dtype != CAIFX_F32 && p.x_dtype == p.compute_dtype && p.R % 8 == 0; }
 
-bool aligned16(const void *a, const void *b = nullptr, const void *c = nullptr, const void *d = nullptr)
+// The weights of a product or the activations of a gradient, as a source of operands
+Operand weights_of(const Weight (&w)[2], int count, int64_t rows, int64_t cols, int stored)
 {
-  return aligned_to(a, 16) && aligned_to(b, 16) && aligned_to(c, 16) && aligned_to(d, 16);
+  Operand o{};
+  for (int i = 0; i < count; ++i) {
+    o.p[i] = w[i].p;
+    o.scales[i] = w[i].scales;
+  }
+  o.count = count;
+  o.kind = w[0].mx ? OPERAND_MX : stored;
+  o.rows = rows;
+  o.cols = cols;
+  return o;
+}
+Operand activations_of(const void *x, const void *second, int kind, int64_t rows, int64_t cols)
+{
+  Operand o{};
+  o.p[0] = x;
+  o.p[1] = second;
+  o.count = second ? 2 : 1;
+  o.kind = kind;
+  o.rows = rows;
+  o.cols = cols;
+  return o;
 }
 
 // Whether a product with this many rows runs on dense operands (caifx_gemm_wide.hip) instead of the row kernels.
 bool wide_product_pays(const Product &p)
 {
-  const int64_t R = up_to(p.R, 64);
-  if (p.M <= 64 || p.compute_dtype == CAIFX_F32 || !wide_takes(p.M, p.N, R) || p.N * R >= (int64_t{1} << 32)) return false;
+  const int64_t R = up_to(p.R, 64) < 128 ? 128 : up_to(p.R, 64);
+  const int pieces = pieces_of(p.compute_dtype);
+  if (p.M <= 64 || !wide_takes(p.M, p.N, R) || p.N * R >= (int64_t{1} << 32)) return false;
   if (!p.w[0].mx) return true;
-  // The row kernels run at some 640 TFLOP/s from a few hundred rows on; the dense product is twice as fast, behind copies of the weights.
-  // us, rows / dense, bf16: N = 14336, K = 4096, 256 rows 62 / 66, 384 rows 86 / 83; N = 11008 384 rows 72 / 70; N = 4096, K = 14336, 512 rows
-  // 84 / 120; 28672 x 8192, 384 rows 270 / 294, 512 rows 356 / 314.
+  // The row kernels run at some 640 TFLOP/s from a few hundred rows on, on three pieces at 100; the dense product is twice as fast and more, behind
+  // copies of the weights.  us, rows / dense, bf16: N = 14336, K = 4096, 256 rows 62 / 66, 384 rows 86 / 83; N = 11008 384 rows 72 / 70; N = 4096,
+  // K = 14336, 512 rows 84 / 120; 28672 x 8192, 384 rows 270 / 294, 512 rows 356 / 314.
   const double weights = p.weights, millions = 1e-6 * weights * static_cast<double>(p.N) * static_cast<double>(R);
-  const double rows = 8.0 + 2.0 * millions * static_cast<double>(p.M) / 640.0;
-  return wide_product_us(p.M, p.weights * p.N, R) + 8.0 * weights + 0.56 * millions < rows;
+  const double rows = 8.0 + 2.0 * millions * static_cast<double>(p.M) / (pieces == 3 ? 100.0 : 640.0);
+  return wide_product_us(p.M, p.weights * p.N, pieces * R) + (pieces == 3 ? 12.0 : 8.0) + 0.56 * millions < rows;
 }
 
 // The product on dense operands: the weights dequantised into the workspace, activations of another type or length copied.
 int product_wide(const Product &p, Room &room, bool only_size, hipStream_t s)
 {
-  const int64_t R = up_to(p.R, 64);
-  const int to = p.compute_dtype;
+  const int64_t R = up_to(p.R, 64) < 128 ? 128 : up_to(p.R, 64);
+  const int to = stored_as(p.compute_dtype), pieces = pieces_of(p.compute_dtype);
+  int st = CAIFX_OK;
   WideProduct d{};
-  d.form = p.weights == 2 ? WIDE_GATED : WIDE_PLAIN;
-  for (int i = 0; i < p.weights; ++i) {
-    d.b[i] = p.w[i].p;
-    if (!p.w[i].mx && R == p.R) continue;
-    void *copy = room.take(static_cast<size_t>(p.N) * static_cast<size_t>(R) * 2);
-    d.b[i] = copy;
-    const int st = only_size ? CAIFX_OK : operand_dense(p.w[i].p, p.w[i].scales, p.w[i].mx ? OPERAND_MX : to, p.N, p.R, to, copy, R, R, 0, s);
-    if (st != CAIFX_OK) return st;
+  d.pairs = pieces;
+  d.b_every = pieces;
+  d.gated = p.weights == 2;
+  d.b[0] = p.w[0].p;
+  d.b[1] = p.w[1].p;
+  if (p.w[0].mx || R != p.R) {
+    const size_t one = static_cast<size_t>(p.N) * static_cast<size_t>(R) * 2;
+    char *copy = static_cast<char *>(room.take(p.weights * one));
+    d.b[0] = copy;
+    d.b[1] = copy + (only_size ? 0 : one);
+    if (!only_size) st = operand_dense(weights_of(p.w, p.weights, p.N, p.R, to), to, copy, R, s);
   }
-  d.a[0] = p.x;
-  if (p.x_dtype != to || R != p.R || (!only_size && !aligned_to(p.x, 16))) {
+  d.a = p.x;
+  const Operand x = activations_of(p.x, nullptr, p.x_dtype, p.M, p.R);
+  if (pieces == 3) {
+    d.a_stride = p.M * R * 2;
+    void *copy = room.take(static_cast<size_t>(p.M) * static_cast<size_t>(R) * 6);
+    d.a = copy;
+    if (!only_size && st == CAIFX_OK) st = operand_pieces(x, copy, R, s);
+  } else if (p.x_dtype != to || R != p.R) {
     void *copy = room.take(static_cast<size_t>(p.M) * static_cast<size_t>(R) * 2);
-    d.a[0] = copy;
-    const int st = only_size ? CAIFX_OK : operand_dense(p.x, nullptr, p.x_dtype, p.M, p.R, to, copy, R, R, 0, s);
-    if (st != CAIFX_OK) return st;
+    d.a = copy;
+    if (!only_size && st == CAIFX_OK) st = operand_dense(x, to, copy, R, s);
   }
   d.d = p.y;
   d.gate = p.gate;
@@ -148,35 +179,36 @@ int product_wide(const Product &p, Room &room, bool only_size, hipStream_t s)
   d.R = R;
   d.compute_dtype = to;
   d.d_dtype = p.y_dtype;
-  return only_size ? CAIFX_OK : wide_product(d, s);
+  return only_size || st != CAIFX_OK ? st : wide_product(d, s);
 }
 
 // The product on the row kernels, any sizes and types.
 int product_rows(const Product &p, Room &room, bool only_size, hipStream_t s)
 {
   Product d = p;
+  const int to = stored_as(p.compute_dtype);
+  const int64_t pitch = up_to(p.R, 8);
   // rows of a stored weight start at any multiple of two bytes where R is odd: the row kernels take them from a copy
-  if (!p.w[0].mx && p.R % 8 != 0) {
-    const int64_t pitch = up_to(p.R, 8);
-    for (int i = 0; i < p.weights; ++i) {
-      void *copy = room.take(static_cast<size_t>(p.N) * static_cast<size_t>(pitch) * 2);
-      if (!only_size) {
-        const int st = operand_dense(p.w[i].p, nullptr, stored_as(p.compute_dtype), p.N, p.R, stored_as(p.compute_dtype), copy, pitch, pitch, 0, s);
-        if (st != CAIFX_OK) return st;
-      }
-      d.w[i].p = copy;
+  if (!p.w[0].mx && p.R != pitch) {
+    const size_t one = static_cast<size_t>(p.N) * static_cast<size_t>(pitch) * 2;
+    char *copy = static_cast<char *>(room.take(p.weights * one));
+    d.w[0].p = copy;
+    d.w[1].p = copy + (only_size ? 0 : one);
+    if (!only_size) {
+      const int st = operand_dense(weights_of(p.w, p.weights, p.N, p.R, to), to, copy, pitch, s);
+      if (st != CAIFX_OK) return st;
     }
   }
   RowsArgs g = rows_args(d);
-  if (!p.w[0].mx && p.R % 8 != 0) {
-    g.R = up_to(p.R, 8);
-    g.w_pitch = 2 * g.R;
+  if (!p.w[0].mx && p.R != pitch) {
+    g.R = pitch;
+    g.w_pitch = 2 * pitch;
   }
   const bool direct = p.M <= 32 && direct_type(p) && (only_size || aligned_to(p.x, 16));
   if (!direct) {
     void *packed = room.take(packed_bytes(p.M, g.chunks, p.compute_dtype));
     if (!only_size) {
-      const int st = operand_rows(p.x, p.x_dtype, p.M, p.R, p.compute_dtype, packed, 0, g.chunks, s);
+      const int st = operand_rows(activations_of(p.x, nullptr, p.x_dtype, p.M, p.R), p.compute_dtype, packed, g.chunks, s);
       if (st != CAIFX_OK) return st;
     }
     g.x = packed;
@@ -186,7 +218,7 @@ int product_rows(const Product &p, Room &room, bool only_size, hipStream_t s)
   return rows_run(g, p.w[0].mx ? ROWS_MX : ROWS_DENSE, p.weights, p.compute_dtype, direct, room, only_size, s);
 }
 
-// What either way can need.  Results or activations at addresses that the dense product does not take run on the row kernels.
+// What either way can need.  Activations at addresses that the dense product does not take run on the row kernels.
 size_t product_bytes(const Product &p, bool dense_copy = true)
 {
   Room rows, wide;
@@ -198,8 +230,7 @@ size_t product_bytes(const Product &p, bool dense_copy = true)
 int product(const Product &p, void *workspace, size_t bytes, hipStream_t s)
 {
   Room room{static_cast<char *>(workspace), 0};
-  // (activations at an odd address would need a copy that the query did not count: the row kernels' order has room)
-  if (wide_product_pays(p) && bytes >= product_bytes(p) && aligned16(p.x, p.y, p.addend) && aligned16(p.gate, p.up)) return product_wide(p, room, false, s);
+  if (wide_product_pays(p) && bytes >= product_bytes(p) && aligned_to(p.x, 16)) return product_wide(p, room, false, s);
   return product_rows(p, room, false, s);
 }
 
@@ -218,30 +249,35 @@ struct Gradient {
 // Whether a gradient runs on the dense product behind the transposed copies.
 bool wide_gradient_pays(const Gradient &p)
 {
-  const int64_t R = up_to(p.N, 64);
-  if (p.compute_dtype == CAIFX_F32 || p.M <= 32 || !wide_takes(p.M, p.K, R)) return false;
+  const int64_t R = up_to(p.N, 64) < 128 ? 128 : up_to(p.N, 64);
+  const int pieces = pieces_of(p.compute_dtype);
+  if (p.M <= 32 || !wide_takes(p.M, p.K, R)) return false;
   // (both behind the same copies.  us, rows / dense: 4096 x 14336, 64 rows 76 / 72, 96 rows 99 / 72; 14336 x 4096, 128 rows 93 / 123, 256 rows 123 / 124)
   const double flops = 2.0 * p.weights * static_cast<double>(p.M) * static_cast<double>(p.N) * static_cast<double>(p.K);
-  return wide_product_us(p.M, p.K, p.weights * R) < 8.0 + flops / 480e6;
+  return wide_product_us(p.M, p.K, p.weights * pieces * R) + (pieces == 3 ? 15.0 : 0.0) < 8.0 + flops / (pieces == 3 ? 100e6 : 480e6);
 }
 
 int gradient_wide(const Gradient &p, Room &room, bool only_size, hipStream_t s)
 {
-  const int to = p.compute_dtype;
-  const int64_t R = up_to(p.N, 64);
+  const int to = stored_as(p.compute_dtype), pieces = pieces_of(p.compute_dtype);
+  const int64_t R = up_to(p.N, 64) < 128 ? 128 : up_to(p.N, 64);
+  int st = CAIFX_OK;
   WideProduct d{};
-  d.form = p.weights == 2 ? WIDE_CHAIN : WIDE_PLAIN;
-  for (int i = 0; i < p.weights; ++i) {
-    void *copy = room.take(static_cast<size_t>(p.K) * static_cast<size_t>(R) * 2);
-    d.b[i] = copy;
-    int st = only_size ? CAIFX_OK : operand_transposed(p.w[i].p, p.w[i].scales, p.w[i].mx ? OPERAND_MX : to, p.N, p.K, to, copy, R, R, 0, s);
-    if (st != CAIFX_OK) return st;
-    d.a[i] = p.x[i];
-    if (p.x_dtype == to && R == p.N) continue;
-    void *x = room.take(static_cast<size_t>(p.M) * static_cast<size_t>(R) * 2);
-    d.a[i] = x;
-    st = only_size ? CAIFX_OK : operand_dense(p.x[i], nullptr, p.x_dtype, p.M, p.N, to, x, R, R, 0, s);
-    if (st != CAIFX_OK) return st;
+  d.pairs = p.weights * pieces;
+  d.b_every = pieces;
+  d.b_stride = p.K * R * 2;
+  void *copy = room.take(p.weights * static_cast<size_t>(p.K) * static_cast<size_t>(R) * 2);
+  d.b[0] = copy;
+  if (!only_size) st = operand_transposed(weights_of(p.w, p.weights, p.N, p.K, to), to, copy, R, R, p.K * R, s);
+  const Operand x = activations_of(p.x[0], p.x[1], p.x_dtype, p.M, p.N);
+  d.a = p.x[0];
+  d.a_stride = static_cast<const char *>(p.x[1]) - static_cast<const char *>(p.x[0]);
+  if (pieces == 3 || p.x_dtype != to || R != p.N) {
+    const size_t one = static_cast<size_t>(p.M) * static_cast<size_t>(R) * 2;
+    void *operand = room.take(d.pairs * one);
+    d.a = operand;
+    d.a_stride = static_cast<int64_t>(one);
+    if (!only_size && st == CAIFX_OK) st = pieces == 3 ? operand_pieces(x, operand, R, s) : operand_dense(x, to, operand, R, s);
   }
   d.d = p.y;
   d.addend = p.addend;
@@ -250,19 +286,19 @@ int gradient_wide(const Gradient &p, Room &room, bool only_size, hipStream_t s)
   d.R = R;
   d.compute_dtype = to;
   d.d_dtype = p.y_dtype;
-  return only_size ? CAIFX_OK : wide_product(d, s);
+  return only_size || st != CAIFX_OK ? st : wide_product(d, s);
 }
 
 int gradient_rows(const Gradient &p, Room &room, bool only_size, hipStream_t s)
 {
   const int to = stored_as(p.compute_dtype);
   const int64_t pitch = up_to(p.N, kRowsChunk), stride = pitch * p.weights;       // whole chunks of each weight's rows
-  const int per = static_cast<int>(pitch / kRowsChunk), chunks = per * p.weights;
+  const int chunks = static_cast<int>(stride / kRowsChunk);
   void *copy = room.take(static_cast<size_t>(p.K) * static_cast<size_t>(stride) * 2);
   void *packed = room.take(packed_bytes(p.M, chunks, p.compute_dtype));
-  for (int i = 0; i < p.weights && !only_size; ++i) {
-    int st = operand_transposed(p.w[i].p, p.w[i].scales, p.w[i].mx ? OPERAND_MX : to, p.N, p.K, to, copy, pitch, stride, i * pitch, s);
-    if (st == CAIFX_OK) st = operand_rows(p.x[i], p.x_dtype, p.M, p.N, p.compute_dtype, packed, i * per, chunks, s);
+  if (!only_size) {
+    int st = operand_transposed(weights_of(p.w, p.weights, p.N, p.K, to), to, copy, pitch, stride, pitch, s);
+    if (st == CAIFX_OK) st = operand_rows(activations_of(p.x[0], p.x[1], p.x_dtype, p.M, p.N), p.compute_dtype, packed, chunks, s);
     if (st != CAIFX_OK) return st;
   }
   RowsArgs g{};
@@ -280,9 +316,55 @@ int gradient_rows(const Gradient &p, Room &room, bool only_size, hipStream_t s)
   return rows_run(g, ROWS_DENSE, 1, p.compute_dtype, false, room, only_size, s);
 }
 
+// The gradient from the weights as they are stored.
+DxProduct dx_of(const Gradient &p, bool direct)
+{
+  DxProduct d{};
+  d.M = p.M;
+  d.N = p.N;
+  d.K = p.K;
+  d.count = p.weights;
+  for (int i = 0; i < p.weights; ++i) {
+    d.w[i] = p.w[i].p;
+    d.s[i] = p.w[i].scales;
+    d.x[i] = p.x[i];
+  }
+  d.mx = p.w[0].mx;
+  d.direct = direct;
+  d.compute_dtype = p.compute_dtype;
+  d.y = p.y;
+  d.y_dtype = p.y_dtype;
+  d.addend = p.addend;
+  return d;
+}
+bool dx_pays(const Gradient &p)
+{
+  return dx_takes(dx_of(p, false)) && p.M <= 128;
+}
+int gradient_dx(const Gradient &p, Room &room, bool only_size, hipStream_t s)
+{
+  const bool direct = p.compute_dtype != CAIFX_F32 && p.x_dtype == p.compute_dtype && p.N % 8 == 0 && aligned_to(p.x[0], 16) && aligned_to(p.x[1], 16) && !only_size;
+  DxProduct d = dx_of(p, direct);
+  void *partial = room.take(dx_partial_bytes(d));
+  if (!direct) {
+    // (counted in any case: the query does not know the activations' addresses)
+    const int chunks = p.weights * static_cast<int>(chunks_of(p.N));
+    void *packed = room.take(packed_bytes(p.M, chunks, p.compute_dtype));
+    if (only_size) return CAIFX_OK;
+    const int st = operand_rows(activations_of(p.x[0], p.x[1], p.x_dtype, p.M, p.N), p.compute_dtype, packed, chunks, s);
+    if (st != CAIFX_OK) return st;
+    d.x[0] = packed;
+  }
+  return dx_product(d, partial, s);
+}
+
 size_t gradient_bytes(const Gradient &p)
 {
-  Room rows, wide;
+  Room dx, rows, wide;
+  if (dx_pays(p)) {
+    gradient_dx(p, dx, true, nullptr);
+    return dx.used;
+  }
   gradient_rows(p, rows, true, nullptr);
   if (!wide_gradient_pays(p)) return rows.used;
   gradient_wide(p, wide, true, nullptr);
@@ -291,7 +373,8 @@ size_t gradient_bytes(const Gradient &p)
 int gradient(const Gradient &p, void *workspace, hipStream_t s)
 {
   Room room{static_cast<char *>(workspace), 0};
-  if (wide_gradient_pays(p) && aligned16(p.x[0], p.x[1], p.y, p.addend)) return gradient_wide(p, room, false, s);
+  if (dx_pays(p)) return gradient_dx(p, room, false, s);
+  if (wide_gradient_pays(p) && aligned_to(p.x[0], 16) && aligned_to(p.x[1], 16)) return gradient_wide(p, room, false, s);
   return gradient_rows(p, room, false, s);
 }
 

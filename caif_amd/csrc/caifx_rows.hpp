@@ -27,7 +27,7 @@ struct RowsPlan {
   int span, splits;
 };
 // Rows of a workgroup's tile.
-inline int rows_tile(int64_t M, int pieces) { return pieces == 3 || M <= 16 ? 16 : M <= 32 ? 32 : 64; }
+inline int rows_tile(int64_t M, int pieces) { return M <= 16 ? 16 : M <= 32 || pieces == 3 ? 32 : 64; }
 // The time of a launch in us, fitted to 60 calls (1 to 64 rows, 1024 x 4096 to 8192 x 28672 and 14336 x 4096): a start, the rounds that a
 // wave's units take, a compute unit's share of the weight at 20.7 KB a us (5.3 TB/s in all) and of the activations, which its caches
 // serve, at 80; a shared reduction costs a second launch and the sums' way there and back.
@@ -43,9 +43,10 @@ inline double rows_us(double rows, double columns, double span, double splits, d
 // columns are cut into a multiple of 256 parts, as large as the column tiles allow.  Where that leaves a workgroup few columns, so that
 // the activations are most of what it reads, 2 to 8 workgroups share a reduction of wider parts (N = 4096, K = 14336, 32 rows: 18 us in four,
 // 20 in one; the estimates say where).  x_tile: bytes of the activations that a workgroup reads.
-inline RowsPlan rows_plan(int64_t M, int64_t N, int64_t R, int weights, int tile, double weight_row, double x_tile)
+inline RowsPlan rows_plan(int64_t M, int64_t N, int64_t R, int weights, int pieces, double weight_row, double x_tile)
 {
-  const int64_t rows = (M + tile - 1) / tile, most = 64 / weights;
+  const int tile = rows_tile(M, pieces);
+  const int64_t rows = (M + tile - 1) / tile, most = (pieces == 3 && tile == 32 ? 32 : 64) / weights;      // (three pieces of 32 rows: two column tiles)
   const double units = static_cast<double>((R + 511) / 512);
   RowsPlan best{};
   double best_us = 0;
@@ -122,8 +123,8 @@ template <> struct Mfma16<f16_t> {
 };
 
 // P: pieces of an activation (3: fp32).  NW: weights (2: gate and up; the first half of the NT column tiles is gate's).  kWhole: rows of
-// whole dwords of scales, at least 16 bytes long: a unit's scales of a weight row are one access (one byte at a time they are more requests
-// than the codes; K = 11008, N = 4096, one row 22.0 us instead of XX).
+// at least 16 blocks: a unit's scales of a weight row are one access, at any address (one byte at a time they are more requests than the
+// codes; K = 11008, N = 4096, one row 22.0 us instead of 8.6).
 // XG: groups of four rows of activations that are read where they are; 0: packed ones.
 template <typename CT, int P, int kWeight, int NW, int MT, int NT, int XG, bool kWhole>
 __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
@@ -181,11 +182,14 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
   }
   // 16 bytes at a base that all lanes share, which the asm keeps in scalar registers: otherwise every load of the loop gets a 64-bit pointer
   // of its own in vector registers, a hundred of them
-  auto at128 = [](const uint8_t *base, uint32_t off) __attribute__((always_inline)) {
+  typedef u32x4_t anywhere_t __attribute__((aligned(1)));
+  auto at128 = [](const uint8_t *base, uint32_t off, auto aligned_) __attribute__((always_inline)) {
     uint64_t b = reinterpret_cast<uint64_t>(base);
     asm("" : "+s"(b), "+v"(off));
-    return *reinterpret_cast<const __attribute__((address_space(1))) u32x4_t *>(b + off);
+    if constexpr (decltype(aligned_)::value) return *reinterpret_cast<const __attribute__((address_space(1))) u32x4_t *>(b + off);
+    else return static_cast<u32x4_t>(*reinterpret_cast<const __attribute__((address_space(1))) anywhere_t *>(b + off));
   };
+  const std::true_type aligned{};
 
   // A unit is two chunks, four halves of 128 elements; wave w takes units w, w + 8, ..
   struct Half {
@@ -208,10 +212,10 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
       // (a unit that begins less than 16 blocks before the end of a row: the row's last 16, see `behind`)
       const int64_t at = static_cast<int64_t>(unit) * 16, from = at + 16 <= g.blocks ? at : g.blocks - 16;
 #pragma unroll
-      for (int c = 0; c < NT; ++c) to.w[c] = at128(s_base[c / NC] + from, s_off[c % NC]);
+      for (int c = 0; c < NT; ++c) to.w[c] = at128(s_base[c / NC] + from, s_off[c % NC], std::false_type{});
       if constexpr (kBoth) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t) to.x[t] = at128(xs_base + from, xs_off[t]);
+        for (int t = 0; t < MT; ++t) to.x[t] = at128(xs_base + from, xs_off[t], std::false_type{});
       }
     }
   };
@@ -219,13 +223,13 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
   auto load = [&](Half &b, int at) __attribute__((always_inline)) {
     const int64_t half = at < halves ? at : halves - 1;
     if constexpr (kMicro) {
-      // blocks past the end of a row: its last one again, as zeros
+      // blocks past the end of a row: its last one again, as zeros or (kWhole) under a scale of 2^-127 against activations that are zeros
       const int block = static_cast<int>(half) * 4 + q;
-      const bool in = kWhole || block < g.blocks;
+      const bool in = block < g.blocks;
       const uint32_t back = in ? 0u : static_cast<uint32_t>(block - (g.blocks - 1));
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        b.w[t][0] = at128(w_base[t / NC] + half * 64, w_off[t % NC] - back * 16);
+        b.w[t][0] = at128(w_base[t / NC] + half * 64, w_off[t % NC] - back * 16, aligned);
         if constexpr (!kWhole) {
           const uint8_t *from = s_base[t / NC] + half * 4;
           if constexpr (kBoth) {
@@ -244,7 +248,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
       if constexpr (kBoth) {
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-          b.x[t] = at128(x_base + half * 64, x_off[t] - back * 16);
+          b.x[t] = at128(x_base + half * 64, x_off[t] - back * 16, aligned);
           if constexpr (!kWhole) b.x_scale[t] = in ? (xs_base + half * 4)[xs_off[t] + q - back] : 0u;
         }
         return;
@@ -252,26 +256,18 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        // pieces of eight elements past the end of a row: its last one again, as zeros
+        // pieces of eight elements past the end of a row: its last one again, as zeros once it is used
         const int k = static_cast<int>(half) * 128 + 32 * i + 8 * q;
-        const bool in = k < g.R;
-        const uint32_t back = in ? 0u : static_cast<uint32_t>(k - (g.R - 8)) * 2;
+        const uint32_t back = k < g.R ? 0u : static_cast<uint32_t>(k - (g.R - 8)) * 2;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          b.w[t][i] = at128(w_base[t / NC] + half * 256, w_off[t % NC] + 64 * i - back);
-          if (!in) b.w[t][i] = u32x4_t{0, 0, 0, 0};
-        }
+        for (int t = 0; t < NT; ++t) b.w[t][i] = at128(w_base[t / NC] + half * 256, w_off[t % NC] + 64 * i - back, aligned);
       }
     }
     if constexpr (kDirect) {
       const int k = static_cast<int>(half) * 128 + 8 * j;
-      const bool in = kWhole || k < g.R;
-      const uint32_t back = in ? 0u : static_cast<uint32_t>(k - (g.R - 8)) * 2;
+      const uint32_t back = k < g.R ? 0u : static_cast<uint32_t>(k - (g.R - 8)) * 2;
 #pragma unroll
-      for (int t = 0; t < XG; ++t) {
-        b.x[t] = at128(x_base + half * 256, x_off[t] - back);
-        if (!in) b.x[t] = u32x4_t{0, 0, 0, 0};
-      }
+      for (int t = 0; t < XG; ++t) b.x[t] = at128(x_base + half * 256, x_off[t] - back, aligned);
     } else {
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
@@ -281,7 +277,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
 #pragma unroll
         for (int p = 0; p < P; ++p)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) b.x[(t * P + p) * 4 + i] = at128(from + (p * 8 + 4 * (half & 1) + i) * 1024, static_cast<uint32_t>(lane) * 16);
+          for (int i = 0; i < 4; ++i) b.x[(t * P + p) * 4 + i] = at128(from + (p * 8 + 4 * (half & 1) + i) * 1024, static_cast<uint32_t>(lane) * 16, aligned);
       }
     }
   };
@@ -294,7 +290,21 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
   // direct: a wave's rows of a half chunk through its own part of LDS into the operands' order; piece p of row r lies in place p ^ r, so that
   // the reads of sixteen rows use every bank.  Lanes of rows that were not read hold others': their results are not stored.
   unsigned char *const order = smem + (kDirect ? wave * (XG * 1024) : 0);
-  auto compute = [&](const Half &b, const Scales &s, int h) __attribute__((always_inline)) {
+  // kPart: the half may reach past the end of the rows
+  auto compute = [&](Half &b, const Scales &s, int h, int half, auto part_) __attribute__((always_inline)) {
+    constexpr bool kPart = decltype(part_)::value;
+    if constexpr (kPart && kDirect) {
+      if (half * 128 + 8 * j >= g.R)
+#pragma unroll
+        for (int t = 0; t < XG; ++t) b.x[t] = u32x4_t{0, 0, 0, 0};
+    }
+    if constexpr (kPart && !kMicro) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (half * 128 + 32 * i + 8 * q >= g.R)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) b.w[t][i] = u32x4_t{0, 0, 0, 0};
+    }
     u32x4_t ordered[kDirect ? MT * 4 : 1];
     if constexpr (kDirect) {
 #pragma unroll
@@ -348,10 +358,15 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
     Scales next;
     if constexpr (!kLast) load_scales(next, unit + kRowsWaves);
     if constexpr (kWhole && kPart) {
-      // the row's last 16 blocks begin `behind` dwords before this unit's
-      const int behind = 4 * unit + 4 - halves;
+      // the row's last 16 blocks begin `behind` before this unit's: the dwords move up, then the bytes, zeros behind them
+      const int behind = 16 * unit + 16 - static_cast<int>(g.blocks);
       const auto forth = [&](u32x4_t &v) __attribute__((always_inline)) {
-        v = behind == 1 ? u32x4_t{v[1], v[2], v[3], 0} : behind == 2 ? u32x4_t{v[2], v[3], 0, 0} : u32x4_t{v[3], 0, 0, 0};
+        const int d = behind >> 2;
+        const uint32_t t0 = d == 0 ? v[0] : d == 1 ? v[1] : d == 2 ? v[2] : v[3], t1 = d == 0 ? v[1] : d == 1 ? v[2] : d == 2 ? v[3] : 0u,
+                       t2 = d == 0 ? v[2] : d == 1 ? v[3] : 0u, t3 = d == 0 ? v[3] : 0u;
+        const uint32_t r = static_cast<uint32_t>(behind & 3);
+        v = u32x4_t{__builtin_amdgcn_alignbyte(t1, t0, r), __builtin_amdgcn_alignbyte(t2, t1, r), __builtin_amdgcn_alignbyte(t3, t2, r),
+                    __builtin_amdgcn_alignbyte(0u, t3, r)};
       };
       if (behind > 0) {
 #pragma unroll
@@ -366,7 +381,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
     for (int h = 0; h < 4; ++h) {
       // (a branch here makes the compiler wait for all that is on its way; without one it asks for more than there are registers for where
       // the tile is large)
-      if ((D > 1 && !kPart) || 4 * unit + h < halves) compute(ring[h % D], scales, h);
+      if ((D > 1 && !kPart) || 4 * unit + h < halves) compute(ring[h % D], scales, h, 4 * unit + h, part_);
       __builtin_amdgcn_sched_barrier(0);
       if (h + D < 4) load(ring[h % D], 4 * unit + h + D);
       else if constexpr (!kLast) load(ring[h % D], 4 * (unit + kRowsWaves) + h + D - 4);
@@ -380,7 +395,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
     for (int h = 0; h < D; ++h) load(ring[h], 4 * first + h);
     int unit = first;
     for (int t = 1; t < mine; ++t, unit += kRowsWaves) run(unit, std::false_type{}, std::false_type{});
-    if (D == 1 || 4 * unit + 4 > halves) run(unit, std::true_type{}, std::true_type{});
+    if (D == 1 || 512 * (unit + 1) > g.R) run(unit, std::true_type{}, std::true_type{});
     else run(unit, std::true_type{}, std::false_type{});
   }
 
@@ -455,7 +470,7 @@ int rows_launch(const RowsArgs &g, hipStream_t s)
     part.addend = forth(g.addend, m0 * g.N * es);
     const dim3 grid(static_cast<unsigned>(cols), static_cast<unsigned>(rows - r < 65535 ? rows - r : 65535), static_cast<unsigned>(g.splits));
     if constexpr (kWeight != ROWS_DENSE) {
-      const bool whole = g.blocks % 4 == 0 && g.blocks >= 16 && g.R == 32 * g.blocks && aligned_to(g.s[0], 4) && aligned_to(g.s[1], 4) && aligned_to(g.xs, 4);
+      const bool whole = g.blocks >= 16;
       if (whole) hipLaunchKernelGGL((rows_kernel<CT, P, kWeight, NW, MT, NT, XG, true>), grid, dim3(kRowsWaves * 64), 0, s, part);
       else hipLaunchKernelGGL((rows_kernel<CT, P, kWeight, NW, MT, NT, XG, false>), grid, dim3(kRowsWaves * 64), 0, s, part);
     } else {
@@ -469,7 +484,9 @@ template <typename CT, int P, int kWeight, int NW, int MT, int XG>
 int rows_pick_columns(const RowsArgs &g, hipStream_t s)
 {
   const int tiles = NW * ((g.span + 15) / 16);
-  if (tiles > 2) return rows_launch<CT, P, kWeight, NW, MT, 4, XG>(g, s);
+  if constexpr (P == 1 || MT == 1) {
+    if (tiles > 2) return rows_launch<CT, P, kWeight, NW, MT, 4, XG>(g, s);
+  }
   if constexpr (NW == 1) {
     if (tiles == 1) return rows_launch<CT, P, kWeight, NW, MT, 1, XG>(g, s);
   }
@@ -478,7 +495,7 @@ int rows_pick_columns(const RowsArgs &g, hipStream_t s)
 template <typename CT, int kWeight, int NW> int rows_pick(const RowsArgs &g, int pieces, bool direct, hipStream_t s)
 {
   if constexpr (dtype_code<CT>::value == CAIFX_BF16) {
-    if (pieces == 3) return rows_pick_columns<CT, 3, kWeight, NW, 1, 0>(g, s);
+    if (pieces == 3) return rows_tile(g.M, 3) == 16 ? rows_pick_columns<CT, 3, kWeight, NW, 1, 0>(g, s) : rows_pick_columns<CT, 3, kWeight, NW, 2, 0>(g, s);
   }
   switch (rows_tile(g.M, 1)) {
     case 16:

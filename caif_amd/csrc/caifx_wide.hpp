@@ -5,17 +5,19 @@
 
 namespace caifx {
 
-enum {
-  WIDE_PLAIN = 0,      // d = a[0] b[0]^T
-  WIDE_GATED = 1,      // d = silu(a[0] b[0]^T) * (a[0] b[1]^T), the two products kept in gate and up unless those are null; no addend
-  WIDE_CHAIN = 2       // d = a[0] b[0]^T + a[1] b[1]^T, one sum
-};
+// what the kernel's forms combine
+enum { WIDE_PLAIN = 0, WIDE_GATED = 1, WIDE_CHAIN = 2, WIDE_RAGGED = 4 };
 
 struct WideProduct {
-  int form;
-  const void *a[2];       // [M, R] of the compute type
-  const void *b[2];       // [C, R] of the compute type
-  void *d, *gate, *up;    // [M, C] of d_dtype (gated: the compute type)
+  // d = sum over the pairs i of A_i B_i^T: A_i behind `a` by i a_stride bytes, B_i behind b[0] by (i / b_every) b_stride bytes
+  const void *a;          // [M, R] each, of the compute type
+  const void *b[2];       // [C, R] each
+  int64_t a_stride, b_stride;
+  int pairs, b_every;
+  // gated: d = silu(that) * (the same with b[1]), and the two kept in gate and up unless those are null; no addend.  d is of the compute
+  // type, or with several pairs fp32.
+  bool gated;
+  void *d, *gate, *up;    // [M, C] of d_dtype
   const void *addend;     // d = T(float(T(sum)) + float(addend))
   int64_t M, C, R;
   int compute_dtype, d_dtype;
@@ -28,7 +30,7 @@ __device__ __forceinline__ float gate_act(float g)
   return g * (g < 0.0f ? e * high : high);
 }
 
-// whether the kernel takes these sizes; every pointer has to be aligned to 16 bytes
+// whether the kernel takes these sizes; the operands have to be aligned to 16 bytes
 bool wide_takes(int64_t M, int64_t C, int64_t R);
 int wide_product(const WideProduct &p, hipStream_t s);
 // what a product takes, in us, estimated; gated: C of both weights together, chained: R of both pairs

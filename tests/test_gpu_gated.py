@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 KINDS = [("mx", "bf16"), ("mx", "f16"), ("mx", "f32"), ("same", "bf16"), ("same", "f16")]
 SHAPES = [(1, 1, 1), (1, 700, 256), (2, 33, 70), (8, 64, 512), (16, 100, 136), (17, 257, 320), (32, 96, 1001), (33, 72, 256), (65, 130, 2048), (130, 264, 328),
-          (257, 300, 776), (520, 136, 1000)]
+          (257, 300, 776), (520, 136, 1000), (700, 333, 512), (1100, 640, 257), (3, 48, 544), (12, 40, 1185)]
 
 
 def gen(seed):
@@ -74,6 +74,25 @@ def test_backward(M, N, K, kind, dtype):
     check(dx, want, R.bound(want, p.abs() @ eg.abs() + q.abs() @ eu.abs(), 2 * N, dt, pieces))
     none, ga, gb = T.gated_backward(d.cuda(), a.cuda(), b.cuda(), wg, wu, need_dx=False)
     assert none is None and torch.equal(ga, da) and torch.equal(gb, db)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_infinite_weights_stay_in_their_columns(dtype):
+    """An infinity in a stored weight's last row, and one in its last column, reach only what their products reach."""
+    g = gen(2)
+    dt = DTYPES[dtype]
+    for M, N, K in ((3, 33, 40), (20, 41, 100), (100, 70, 130), (300, 70, 264)):
+        w = (0.05 * torch.randn(N, K, generator=g)).to(dt)
+        w[N - 1, 2], w[4, K - 1] = float("inf"), float("-inf")
+        fw = T.FrozenWeight(w.cuda(), T.W_F16 if dt == torch.float16 else T.W_BF16, None, N, K)
+        d, a, b = (1 + torch.rand(M, N, generator=g).to(dt) for _ in range(3))
+        dx, da, db = T.gated_backward(d.cuda(), a.cuda(), b.cuda(), fw, fw)
+        want = (da.double().cpu() + db.double().cpu()) @ w.double()
+        assert torch.equal(dx.isfinite().cpu(), want.isfinite()) and torch.equal(dx.isnan().cpu(), want.isnan())
+        x = 1 + torch.rand(M, K, generator=g).to(dt)
+        _, gate, up = T.gated_forward(x.cuda(), fw, fw, keep=True)
+        want = x.double() @ w.double().T
+        assert torch.equal(gate.isinf().cpu(), want.isinf()) and torch.equal(up.isnan().cpu(), want.isnan())
 
 
 def test_against_differences():

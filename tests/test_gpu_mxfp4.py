@@ -112,6 +112,40 @@ def test_gradient(M, N, K, dtype):
     assert torch.equal(both, (dx.float() + addend.cuda().float()).to(dx.dtype))
 
 
+@pytest.mark.parametrize("K", [512, 513, 544, 577, 608, 640, 700, 799, 832, 991, 1024, 1056, 4096 + 32, 4096 + 96, 4096 + 256, 4096 + 416, 8192 + 1])
+@pytest.mark.parametrize("M", [1, 9, 20, 50])
+def test_ends_of_rows(M, K):
+    """Rows that end anywhere in the kernels' units of 512 values, and in their blocks."""
+    g = gen(M * K)
+    N = 70
+    w, exact = weight(g, N, K)
+    for dtype in (torch.bfloat16, torch.float32):
+        x = torch.randn(M, K, generator=g).to(dtype)
+        within(T.qlinear_forward(x.cuda(), w, T.CODE_OF[dtype], T.CODE_OF[dtype]), x.double() @ exact.T, x.double().abs() @ exact.abs().T, K, 3)
+    a, sa = R.random_weight(g, M, K)
+    p = R.decode(a, sa, K)
+    within(T.mxfp4_matmul(a.cuda(), sa.cuda(), w.wq, w.scales), p @ exact.T, p.abs() @ exact.abs().T, K)
+
+
+@pytest.mark.parametrize("M,N,K", [(300, 1101, 512), (700, 999, 130), (1100, 640, 1000), (2100, 333, 257), (3000, 1024, 64)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_rows(M, N, K, dtype):
+    """Calls that run on dense operands, some into rows that are no whole pieces of 16 bytes, with an addend."""
+    g = gen(M + N + K)
+    w, exact = weight(g, N, K)
+    dt = DTYPES[dtype]
+    code, pieces = T.CODE_OF[dt], 3 if dtype == "f32" else 1
+    x, dy, add = (torch.randn(M, n, generator=g).to(dt) for n in (K, N, N))
+    y = T.qlinear_forward(x.cuda(), w, code, code)
+    within(y, x.double() @ exact.T, x.double().abs() @ exact.abs().T, K, pieces)
+    assert torch.equal(T.qlinear_forward(x.cuda(), w, code, code, addend=add.cuda()), (y.float() + add.cuda().float()).to(dt))
+    dx = T.qlinear_backward_input(dy.cuda(), w, code, code)
+    within(dx, dy.double() @ exact, dy.double().abs() @ exact.abs(), N, pieces)
+    a = T.mxfp4_quantize(x.cuda())
+    p = R.decode(*R.quantize(x), K)
+    within(T.mxfp4_matmul(*a, w.wq, w.scales, code), p @ exact.T, p.abs() @ exact.abs().T, K)
+
+
 @pytest.mark.parametrize("backward", [False, True])
 @pytest.mark.parametrize("xd,cd,yd", [("f32", "bf16", "f32"), ("f32", "f16", "f16"), ("bf16", "f32", "f32"), ("f16", "bf16", "f32"), ("bf16", "bf16", "f16")])
 @pytest.mark.parametrize("M", [5, 70])
