@@ -395,6 +395,50 @@ int gating_backward(const void *grad, const void *gate, const void *up, void *gr
 
 namespace {
 
+// Sums of a shared reduction.  Few values and many parts: a wave of its own for 64 lanes' values, sixteen parts on their way at once.
+template <typename T, int V> __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ partial, int parts, int64_t n, T *y, const T *addend)
+{
+  constexpr int kTogether = 16;
+  struct alignas(V * sizeof(float)) Sums { float e[V]; };
+  struct alignas(V * sizeof(T)) Values { T e[V]; };
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * V;
+  if (i >= n) return;
+  Sums sum{};
+  for (int from = 0; from < parts; from += kTogether) {
+    Sums part[kTogether];
+#pragma unroll
+    for (int p = 0; p < kTogether; ++p) part[p] = *reinterpret_cast<const Sums *>(partial + (from + p < parts ? from + p : parts - 1) * n + i);
+#pragma unroll
+    for (int p = 0; p < kTogether; ++p)
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (from + p < parts) sum.e[e] = from + p == 0 ? part[p].e[e] : sum.e[e] + part[p].e[e];
+  }
+  Values out;
+  if (addend) {
+    const Values add = *reinterpret_cast<const Values *>(addend + i);
+#pragma unroll
+    for (int e = 0; e < V; ++e) out.e[e] = from_f32<T>(to_f32<T>(from_f32<T>(sum.e[e])) + to_f32<T>(add.e[e]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) out.e[e] = from_f32<T>(sum.e[e]);
+  }
+  *reinterpret_cast<Values *>(y + i) = out;
+}
+
+template <typename T> int join(const float *partial, int parts, int64_t n, void *y_, const void *addend_, hipStream_t s)
+{
+  T *y = static_cast<T *>(y_);
+  const T *addend = static_cast<const T *>(addend_);
+  const bool four = n % 4 == 0 && aligned_to(y, 4 * sizeof(T)) && aligned_to(addend, 4 * sizeof(T));
+  const int64_t lanes = four ? n / 4 : n;
+  const int block = lanes < 65536 ? 64 : 256;
+  const dim3 grid(static_cast<unsigned>((lanes + block - 1) / block));
+  if (four) hipLaunchKernelGGL((join_kernel<T, 4>), grid, dim3(block), 0, s, partial, parts, n, y, addend);
+  else hipLaunchKernelGGL((join_kernel<T, 1>), grid, dim3(block), 0, s, partial, parts, n, y, addend);
+  return launch_status();
+}
+
 // CAIFX_OK and `go` for a launch that has work, its shape and workgroups
 int check(int64_t rows, int64_t cols, int dtype, bool missing, bool misaligned, bool &go, dim3 &grid, Shape &shape)
 {
@@ -413,6 +457,14 @@ int check(int64_t rows, int64_t cols, int dtype, bool missing, bool misaligned, 
 }
 
 }  // namespace
+
+int join_sums(const float *partial, int parts, int64_t n, void *y, int y_dtype, const void *addend, hipStream_t s)
+{
+  if (y_dtype == CAIFX_F32) return join<float>(partial, parts, n, y, addend, s);
+  if (y_dtype == CAIFX_F16) return join<f16_t>(partial, parts, n, y, addend, s);
+  return join<bf16_t>(partial, parts, n, y, addend, s);
+}
+
 }  // namespace caifx
 
 using namespace caifx;

@@ -40,6 +40,7 @@ struct DxProduct {
   const void *addend;
 };
 bool dx_takes(const DxProduct &p);
+double dx_us(const DxProduct &p);      // an estimate
 size_t dx_partial_bytes(const DxProduct &p);
 int dx_product(const DxProduct &p, void *partial, hipStream_t s);
 
@@ -49,6 +50,9 @@ bool mx_gemm_takes(int64_t M, int64_t C, int64_t blocks);
 double mx_gemm_us(int64_t M, int64_t C, int64_t blocks);      // an estimate
 size_t mx_gemm_workspace_bytes(int64_t M, int64_t C, int64_t blocks);
 int mx_gemm(int64_t M, int64_t C, int64_t blocks, const void *a, const void *sa, const void *b, const void *sb, void *d, int d_dtype, void *workspace, hipStream_t s);
+
+// y = the sum of `parts` fp32 arrays of n values in order, and the addend: sums of a shared reduction
+int join_sums(const float *partial, int parts, int64_t n, void *y, int y_dtype, const void *addend, hipStream_t s);
 
 int gating_backward(const void *grad, const void *gate, const void *up, void *grad_gate, void *grad_up, int64_t n, int dtype, hipStream_t s);
 

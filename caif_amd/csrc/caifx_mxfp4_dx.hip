@@ -9,7 +9,7 @@
 // and read again, 4 bytes for half a byte of codes.
 // A workgroup of eight waves owns 256 columns, its waves take steps in turn and meet in LDS; workgroups share a reduction, as many as the
 // chip has room for, and a second launch adds their sums in a fixed order.
-// N = 14336, K = 4096, bf16, 16 rows: XX us, behind a transposed copy 75.
+// N = 14336, K = 4096, bf16, 16 rows: 16 us (the weight's bytes alone 6.3), behind a transposed copy 70; 512 rows 110 us, 546 TFLOP/s, and 126.
 #include "caifx_mxfp4.hpp"
 
 #include <type_traits>
@@ -38,12 +38,12 @@ __global__ __launch_bounds__(kWaves * 64) void dx_kernel(DxArgs g)
 {
   typedef u32x2_t codes_t __attribute__((aligned(8)));
   typedef u32x4_t anywhere_t __attribute__((aligned(2)));
-  __shared__ floatx4_t sums[kWaves / 2][kSets][64];
+  __shared__ floatx4_t sums[kWaves / 2][kSets][65];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int j = lane & 15, q = lane >> 4;
   const int64_t k0 = static_cast<int64_t>(blockIdx.x) * kColumns, m0 = static_cast<int64_t>(blockIdx.y) * (16 * MT);
-  // a lane's first column: past the end of a row the last sixteen columns again (the same sums, stored twice or not at all)
+  // a lane's first column: past the end of a row the last sixteen columns again (stored once)
   const int64_t width = kMx ? 32 * g.blocks : g.K;
   const auto first_column = [&](int lane_j) __attribute__((always_inline)) {
     const int64_t k = k0 + kSets * lane_j;
@@ -161,9 +161,9 @@ __global__ __launch_bounds__(kWaves * 64) void dx_kernel(DxArgs g)
     }
   }
 
-  // the waves' sums, in a fixed order, 16 rows at a time
+  // The waves' sums, in a fixed order, 16 rows at a time.  A thread takes four rows of one column at once: neighbouring threads read sets of
+  // sums 1040 bytes apart, sixteen bytes each, and write neighbouring columns.
   constexpr int kHalf = kWaves / 2;
-  const float *flat = reinterpret_cast<const float *>(sums);
   auto store = [&](auto type_) __attribute__((always_inline)) {
     typedef decltype(type_) T;
 #pragma unroll
@@ -177,18 +177,23 @@ __global__ __launch_bounds__(kWaves * 64) void dx_kernel(DxArgs g)
 #pragma unroll
         for (int c = 0; c < kSets; ++c) sums[wave][c][lane] += acc[t][c];
       __syncthreads();
-      for (int i = threadIdx.x; i < 16 * kColumns; i += kWaves * 64) {
-        const int row = i / kColumns, within = i % kColumns;
-        const int64_t m = m0 + 16 * t + row, k = first_column(within / kSets) + within % kSets;
-        if (m >= g.M || k >= g.K) continue;
-        const int from = ((within % kSets) * 64 + (row >> 2) * 16 + within / kSets) * 4 + (row & 3);
-        float v = flat[from];
 #pragma unroll
-        for (int w = 1; w < kHalf; ++w) v += flat[w * (kSets * 256) + from];
+      for (int i = threadIdx.x; i < 4 * kColumns; i += kWaves * 64) {
+        const int four = i / kColumns, within = i % kColumns;
+        const int64_t m = m0 + 16 * t + 4 * four, k = first_column(within / kSets) + within % kSets;
+        floatx4_t v = sums[0][within % kSets][four * 16 + within / kSets];
+#pragma unroll
+        for (int w = 1; w < kHalf; ++w) v += sums[w][within % kSets][four * 16 + within / kSets];
+        if (k >= g.K || k < k0 + within / kSets * kSets) continue;      // (another lane's, where the end of a row moved this one's)
         const int64_t to = (z * g.M + m) * g.K + k;
-        T r = from_f32<T>(v);
-        if (g.addend) r = from_f32<T>(to_f32<T>(r) + to_f32<T>(static_cast<const T *>(g.addend)[to]));
-        static_cast<T *>(g.y)[to] = r;
+#pragma unroll
+        for (int row = 0; row < 4; ++row) {
+          if (m + row >= g.M) break;
+          const int64_t at_row = to + row * g.K;
+          T r = from_f32<T>(v[row]);
+          if (g.addend) r = from_f32<T>(to_f32<T>(r) + to_f32<T>(static_cast<const T *>(g.addend)[at_row]));
+          static_cast<T *>(g.y)[at_row] = r;
+        }
       }
     }
   };
@@ -199,11 +204,12 @@ __global__ __launch_bounds__(kWaves * 64) void dx_kernel(DxArgs g)
 
 int tile_of(int64_t M) { return M <= 16 ? 16 : 32; }
 
-// Workgroups that share a reduction: two for each compute unit in all, each wave at least one step
+// Workgroups that share a reduction: one for each compute unit in all, as many as the registers hold at once (N = 14336, K = 4096, 32 rows: 128
+// workgroups 32 us, 256 26, 512 41), and each wave at least one step
 int splits_of(const DxProduct &p)
 {
   const int64_t total = p.count * ((p.N + 31) / 32), others = (p.K + kColumns - 1) / kColumns * ((p.M + tile_of(p.M) - 1) / tile_of(p.M));
-  int64_t most = 512 / others;
+  int64_t most = 256 / others;
   const int64_t steps = (total + kWaves - 1) / kWaves;
   most = most < steps ? most : steps;
   return static_cast<int>(most < 1 ? 1 : most);
@@ -238,6 +244,16 @@ bool dx_takes(const DxProduct &p)
   return p.M <= 1024 && (p.mx || p.K >= kSets);
 }
 
+double dx_us(const DxProduct &p)
+{
+  const int splits = splits_of(p), pieces = p.compute_dtype == CAIFX_F32 ? 3 : 1;
+  const int64_t others = (p.K + kColumns - 1) / kColumns * ((p.M + tile_of(p.M) - 1) / tile_of(p.M));
+  const int64_t rounds = (others * splits + 255) / 256, steps = (p.count * ((p.N + 31) / 32) + kWaves * splits - 1) / (kWaves * splits);
+  const double step = (pieces == 3 ? 3.4 : 1.85) * (p.mx ? 1.0 : 1.2);
+  const double join = splits > 1 ? 3.0 + 8e-7 * static_cast<double>(splits) * static_cast<double>(p.M) * static_cast<double>(p.K) : 0.0;
+  return 5.0 + (p.direct && pieces == 1 ? 0.0 : 3.0) + join + step * static_cast<double>(rounds * steps);
+}
+
 size_t dx_partial_bytes(const DxProduct &p)
 {
   const int splits = splits_of(p);
@@ -270,7 +286,7 @@ int dx_product(const DxProduct &p, void *partial, hipStream_t s)
   else if (p.compute_dtype == CAIFX_F16) st = p.mx ? launch<f16_t, 1, true>(g, p.direct, s) : launch<f16_t, 1, false>(g, p.direct, s);
   else st = p.mx ? launch<bf16_t, 1, true>(g, p.direct, s) : launch<bf16_t, 1, false>(g, p.direct, s);
   if (st != CAIFX_OK || g.splits == 1) return st;
-  return splitk_reduce(static_cast<const float *>(partial), g.splits, p.M * p.K, p.y, p.y_dtype, p.addend, s);
+  return join_sums(static_cast<const float *>(partial), g.splits, p.M * p.K, p.y, p.y_dtype, p.addend, s);
 }
 
 }  // namespace caifx

@@ -92,7 +92,7 @@ int rows_run(RowsArgs g, int kind, int weights, int compute_dtype, bool direct, 
   }
   const int st = kind == ROWS_BOTH ? rows_both(g, s) : compute_dtype == CAIFX_F16 ? rows_f16(g, kind, weights, direct, s) : rows_bf16(g, kind, weights, pieces, direct, s);
   if (st != CAIFX_OK || plan.splits == 1) return st;
-  return splitk_reduce(static_cast<const float *>(partial), plan.splits, g.M * g.N, asked.y, asked.y_dtype, asked.addend, s);
+  return join_sums(static_cast<const float *>(partial), plan.splits, g.M * g.N, asked.y, asked.y_dtype, asked.addend, s);
 }
 
 // whether the row kernels can read the activations where they are
@@ -246,6 +246,12 @@ struct Gradient {
   const void *addend;
 };
 
+double gradient_rows_us(const Gradient &p)      // an estimate, behind the copies
+{
+  const double flops = 2.0 * p.weights * static_cast<double>(p.M) * static_cast<double>(p.N) * static_cast<double>(p.K);
+  return 8.0 + flops / (pieces_of(p.compute_dtype) == 3 ? 100e6 : 480e6);
+}
+
 // Whether a gradient runs on the dense product behind the transposed copies.
 bool wide_gradient_pays(const Gradient &p)
 {
@@ -253,8 +259,7 @@ bool wide_gradient_pays(const Gradient &p)
   const int pieces = pieces_of(p.compute_dtype);
   if (p.M <= 32 || !wide_takes(p.M, p.K, R)) return false;
   // (both behind the same copies.  us, rows / dense: 4096 x 14336, 64 rows 76 / 72, 96 rows 99 / 72; 14336 x 4096, 128 rows 93 / 123, 256 rows 123 / 124)
-  const double flops = 2.0 * p.weights * static_cast<double>(p.M) * static_cast<double>(p.N) * static_cast<double>(p.K);
-  return wide_product_us(p.M, p.K, p.weights * pieces * R) + (pieces == 3 ? 15.0 : 0.0) < 8.0 + flops / (pieces == 3 ? 100e6 : 480e6);
+  return wide_product_us(p.M, p.K, p.weights * pieces * R) + (pieces == 3 ? 15.0 : 0.0) < gradient_rows_us(p);
 }
 
 int gradient_wide(const Gradient &p, Room &room, bool only_size, hipStream_t s)
@@ -337,9 +342,18 @@ DxProduct dx_of(const Gradient &p, bool direct)
   d.addend = p.addend;
   return d;
 }
+// The stored weights are turned around for every 32 rows again, the copies once: few rows run on dx, many on the copies.  Estimates in us, of
+// the copies with a dense product or the row kernels, and of dx.  Measured, copies / dx: N = 14336, K = 4096, bf16, 16 rows 70 / 16, 128 rows
+// 92 / 38, 512 rows 126 / 110, 768 rows 131 / 188; N = 4096, K = 14336, 256 rows 74 / 65, 384 rows 92 / 94; N = K = 4096, 512 rows 40 / 35, in fp32
+// 89 / 71, a gated block's gradient 80 / 76, of stored weights 82 / 83; 2048 x 1408, 512 rows 22 / 20.
 bool dx_pays(const Gradient &p)
 {
-  return dx_takes(dx_of(p, false)) && p.M <= 128;
+  if (!dx_takes(dx_of(p, false))) return false;
+  const int64_t R = up_to(p.N, 64) < 128 ? 128 : up_to(p.N, 64);
+  const int pieces = pieces_of(p.compute_dtype);
+  const double values = p.weights * static_cast<double>(p.N) * static_cast<double>(p.K);
+  const double product = wide_gradient_pays(p) ? wide_product_us(p.M, p.K, p.weights * pieces * R) + (pieces == 3 ? 15.0 : 0.0) : gradient_rows_us(p);
+  return dx_us(dx_of(p, p.N % 8 == 0)) < product + 12.0 + values * (p.w[0].mx ? 2.53 : 4.0) / 4.4e6 + (pieces == 3 ? 4.0 : 0.0);
 }
 int gradient_dx(const Gradient &p, Room &room, bool only_size, hipStream_t s)
 {
