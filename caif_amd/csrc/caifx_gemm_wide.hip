@@ -45,7 +45,7 @@ struct WideArgs {
   const void *b2;
   void *gate, *up;
   int64_t a_stride, b_stride;
-  int pairs, b_every;
+  int pairs, b_every, parts;
 };
 
 // A result tile has 64 WI rows and 64 WJ columns.  Wave (wm, wn) owns rows h 32 WI + wm 16 WI + [0, 16 WI) and columns
@@ -59,7 +59,7 @@ struct WideArgs {
 // per half).
 // WIDE_GATED: half g of the columns belongs to the g-th weight, the same BN / 2 columns of each, so that a wave's accumulators of the two
 // halves hold gate and up of the same values and the gating happens where they are.  WIDE_CHAIN: the steps run through one pair of operands
-// after the other.  WIDE_RAGGED: a result whose rows are no whole, aligned pieces of 16 bytes is stored value by value.
+// after the other, and `parts` workgroups may share them, the z-th writing its sums (fp32) z M C values behind the first's.  WIDE_RAGGED: a result whose rows are no whole, aligned pieces of 16 bytes is stored value by value.
 template <typename CT, int WI, int WJ, bool kGrouped, int kForm = WIDE_PLAIN>
 __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(WideArgs g)
 {
@@ -140,11 +140,21 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void wide_gemm_kernel(Wi
   const uint64_t b_base = uniform64(b_ptr + static_cast<uint64_t>(col0 * g.R * 2));
   const uint64_t b2_base = kGated ? uniform64(reinterpret_cast<uint64_t>(g.b2) + static_cast<uint64_t>(col0 * g.R * 2)) : 0;
   const int part = static_cast<int>(g.R / kBK);
-  const int steps = kChain ? g.pairs * part : part;
-  const int last = steps - 1;
+  int steps = part;
   // chain: where the step that is asked for next has its operands, as offsets from the first pair's
   int64_t a_at = 0, b_at = 0;
   int asked = 0, in_part = 0, in_b = 0;
+  if constexpr (kChain) {
+    const int64_t total = static_cast<int64_t>(g.pairs) * part, z = blockIdx.y;
+    const int begin = static_cast<int>(total * z / g.parts), pair = begin / part;
+    steps = static_cast<int>(total * (z + 1) / g.parts) - begin;
+    in_part = begin - pair * part;
+    in_b = pair % g.b_every;
+    a_at = pair * g.a_stride + static_cast<int64_t>(in_part) * 128;
+    b_at = pair / g.b_every * g.b_stride + static_cast<int64_t>(in_part) * 128;
+    if (z > 0) g.d = static_cast<float *>(g.d) + z * g.M * g.C;
+  }
+  const int last = steps - 1;
   auto advance = [&]() __attribute__((always_inline)) {
     if (asked >= last) return;
     ++asked;
@@ -592,7 +602,8 @@ int launch_wide(const WideArgs &g, hipStream_t s)
   }
   // grouped: segment lengths live on the device; an upper bound, every expert can add one partial tile
   const int64_t tiles = ((g.M + BM - 1) / BM + (kGrouped ? g.num_experts : 0)) * ((g.C + BC - 1) / BC);
-  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((tiles + 7) / 8 * 8)), dim3(256), kLds, s, g);
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((tiles + 7) / 8 * 8), (kForm & WIDE_CHAIN) ? static_cast<unsigned>(g.parts) : 1u), dim3(256),
+                     kLds, s, g);
   return launch_status();
 }
 
@@ -609,19 +620,20 @@ int64_t row_tiles_of(int64_t M, int experts, int64_t bm)
   const int64_t t = (M + bm - 1) / bm + experts / 2, least = M < experts ? M : experts;
   return t > least ? t : least;
 }
-double step_cost(int tile, int64_t M, int64_t C, int experts)
+// parts: workgroups that share a tile's steps
+double step_cost(int tile, int64_t M, int64_t C, int experts, int parts)
 {
-  const auto tiles = [&](int64_t bm, int64_t bn) { return row_tiles_of(M, experts, bm) * ((C + bn - 1) / bn); };
+  const auto tiles = [&](int64_t bm, int64_t bn) { return row_tiles_of(M, experts, bm) * ((C + bn - 1) / bn) * parts; };
   if (tile == TILE_256) return 1.39 * static_cast<double>((tiles(256, 256) + 255) / 256);
   if (tile == TILE_128x256) return 0.87 * static_cast<double>((tiles(128, 256) + 255) / 256);
   const int64_t t = tiles(128, 128), rest = t % 512;
   return 0.91 * static_cast<double>(t / 512) + (rest == 0 ? 0.0 : rest <= 256 ? 0.49 : 0.91);
 }
-int best_tile(int64_t M, int64_t C, int experts)
+int best_tile(int64_t M, int64_t C, int experts, int parts = 1)
 {
   int best = TILE_256;
   for (int t = TILE_128x256; t <= TILE_128; ++t)
-    if (step_cost(t, M, C, experts) < step_cost(best, M, C, experts)) best = t;
+    if (step_cost(t, M, C, experts, parts) < step_cost(best, M, C, experts, parts)) best = t;
   return best;
 }
 
@@ -633,11 +645,11 @@ double rounds_cost(int64_t tiles, int64_t slots, double full, double base, doubl
   const int64_t rest = tiles % slots;
   return full * static_cast<double>(tiles / slots) + (rest == 0 ? 0.0 : base + per * static_cast<double>(rest));
 }
-double wide_us_of(int64_t M, int64_t C, int64_t R)      // the product alone
+double wide_us_of(int64_t M, int64_t C, int64_t R, int parts = 1)      // the product alone
 {
-  const auto tiles = [&](int64_t bm, int64_t bn) { return (M + bm - 1) / bm * ((C + bn - 1) / bn); };
+  const auto tiles = [&](int64_t bm, int64_t bn) { return (M + bm - 1) / bm * ((C + bn - 1) / bn) * parts; };
   double step;
-  switch (best_tile(M, C, 0)) {
+  switch (best_tile(M, C, 0, parts)) {
     case TILE_256: step = rounds_cost(tiles(256, 256), 256, 1.42, 0.75, 0.0026); break;
     case TILE_128x256: step = rounds_cost(tiles(128, 256), 256, 0.81, 0.25, 0.0022); break;
     default: {
@@ -645,7 +657,7 @@ double wide_us_of(int64_t M, int64_t C, int64_t R)      // the product alone
       step = t % 512 <= 256 ? rounds_cost(t, 512, 0.82, 0.24, 0.0008) : rounds_cost(t, 512, 0.82, 0.30, 0.0010);
     }
   }
-  return step * static_cast<double>(R / kBK);
+  return step * static_cast<double>((R / kBK + parts - 1) / parts);
 }
 double wide_us(const GemmArgs &a, bool backward)
 {
@@ -697,7 +709,7 @@ template <typename CT, bool kGrouped, int kForm = WIDE_PLAIN>
 int pick_wide(const WideArgs &g, hipStream_t s)
 {
   // (gated: as many tiles as a plain product with both weights' columns has)
-  switch (best_tile(g.M, (kForm & WIDE_GATED) ? 2 * g.C : g.C, g.num_experts)) {
+  switch (best_tile(g.M, (kForm & WIDE_GATED) ? 2 * g.C : g.C, g.num_experts, (kForm & WIDE_CHAIN) ? g.parts : 1)) {
     case TILE_256: return launch_wide<CT, 4, 4, kGrouped, kForm>(g, s);
     case TILE_128x256: return launch_wide<CT, 2, 4, kGrouped, kForm>(g, s);
     default: return launch_wide<CT, 2, 2, kGrouped, kForm>(g, s);
@@ -854,6 +866,19 @@ double wide_product_us(int64_t M, int64_t C, int64_t R)
   return wide_us_of(M, C, R);
 }
 
+// Few tiles and many steps: up to eight workgroups share a tile's steps, each at least eight of them, and a second launch adds their sums.
+// us in one part / in the best, with the copies before it: M = 512, C = 4096, R = 14336 126 / 105, in fp32 (three times the steps) 291 / 200; M = 2048,
+// C = 4096, R = 22016 (a gated block's gradient) 418 / 387; M = 1024, C = R = 4096 48 / 59, not taken.
+WideParts wide_parts(int64_t M, int64_t C, int64_t R)
+{
+  WideParts best{1, wide_us_of(M, C, R)};
+  for (int parts = 2; parts <= 8 && R / kBK >= 8 * parts; ++parts) {
+    const double us = wide_us_of(M, C, R, parts) + 4.0 + 1.4e-6 * parts * static_cast<double>(M) * static_cast<double>(C);
+    if (us < best.us) best = WideParts{parts, us};
+  }
+  return best;
+}
+
 template <typename CT, int kForm> static int wide_form(const WideArgs &g, int form, hipStream_t s)
 {
   // (gated fp32, a chain of bf16 pieces, has no fp16 form)
@@ -881,10 +906,11 @@ int wide_product(const WideProduct &p, hipStream_t s)
   g.b_stride = p.b_stride;
   g.pairs = p.pairs;
   g.b_every = p.b_every;
+  g.parts = p.parts;
   g.d_dtype = p.d_dtype;
   const int64_t whole = p.d_dtype == CAIFX_F32 ? 4 : 8;
   const bool ragged = p.C % whole != 0 || !aligned_to(p.d, 16) || !aligned_to(p.gate, 16) || !aligned_to(p.up, 16) || !aligned_to(p.addend, 16);
-  const int form = (p.gated ? WIDE_GATED : 0) | (p.pairs > 1 ? WIDE_CHAIN : 0) | (ragged ? WIDE_RAGGED : 0);
+  const int form = (p.gated ? WIDE_GATED : 0) | (p.pairs > 1 || p.parts > 1 ? WIDE_CHAIN : 0) | (ragged ? WIDE_RAGGED : 0);
   if (p.compute_dtype == CAIFX_BF16) return wide_form<bf16_t, 7>(g, form, s);
   return wide_form<f16_t, 7>(g, form, s);
 }

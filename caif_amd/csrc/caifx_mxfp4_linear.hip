@@ -95,6 +95,21 @@ int rows_run(RowsArgs g, int kind, int weights, int compute_dtype, bool direct, 
   return join_sums(static_cast<const float *>(partial), plan.splits, g.M * g.N, asked.y, asked.y_dtype, asked.addend, s);
 }
 
+// The dense product, in parts where that is faster, or the size of their sums.
+int wide_run(WideProduct d, Room &room, bool only_size, hipStream_t s)
+{
+  d.parts = d.gated ? 1 : wide_parts(d.M, d.C, d.pairs * d.R).parts;
+  if (d.parts == 1) return only_size ? CAIFX_OK : wide_product(d, s);
+  void *partial = room.take(static_cast<size_t>(d.parts) * static_cast<size_t>(d.M) * static_cast<size_t>(d.C) * 4);
+  if (only_size) return CAIFX_OK;
+  const WideProduct asked = d;
+  d.d = partial;
+  d.d_dtype = CAIFX_F32;
+  d.addend = nullptr;
+  const int st = wide_product(d, s);
+  return st != CAIFX_OK ? st : join_sums(static_cast<const float *>(partial), d.parts, d.M * d.C, asked.d, asked.d_dtype, asked.addend, s);
+}
+
 // whether the row kernels can read the activations where they are
 bool direct_type(const Product &p) { return p.compute_dtype != CAIFX_F32 && p.x_dtype == p.compute_dtype && p.R % 8 == 0; }
 
@@ -131,12 +146,15 @@ bool wide_product_pays(const Product &p)
   const int pieces = pieces_of(p.compute_dtype);
   if (p.M <= 64 || !wide_takes(p.M, p.N, R) || p.N * R >= (int64_t{1} << 32)) return false;
   if (!p.w[0].mx) return true;
-  // The row kernels run at some 640 TFLOP/s from a few hundred rows on, on three pieces at 100; the dense product is twice as fast and more, behind
-  // copies of the weights.  us, rows / dense, bf16: N = 14336, K = 4096, 256 rows 62 / 66, 384 rows 86 / 83; N = 11008 384 rows 72 / 70; N = 4096,
-  // K = 14336, 512 rows 84 / 120; 28672 x 8192, 384 rows 270 / 294, 512 rows 356 / 314.
+  // A workgroup of the row kernels takes 64 x 64 results in 4.5 us and 1.3 for every 512 elements of the reduction, 256 of them at a time (few, a
+  // third of that and up), on three pieces they run at 100 TFLOP/s; the dense product is twice as fast and more, behind copies of the weights.
+  // us, rows / dense, bf16: N = 14336, K = 4096, 256 rows 62 / 66, 384 rows 86 / 83; N = 11008 384 rows 72 / 70; N = K = 4096, 256 rows 20 / 41; N =
+  // 4096, K = 14336, 512 rows 84 / 98; 5120 x 794, 512 rows 29 / 23.
   const double weights = p.weights, millions = 1e-6 * weights * static_cast<double>(p.N) * static_cast<double>(R);
-  const double rows = 8.0 + 2.0 * millions * static_cast<double>(p.M) / (pieces == 3 ? 100.0 : 640.0);
-  return wide_product_us(p.M, p.weights * p.N, pieces * R) + (pieces == 3 ? 12.0 : 8.0) + 0.56 * millions < rows;
+  const int64_t groups = (p.M + 63) / 64 * ((p.weights * p.N + 63) / 64);
+  const double rounds = static_cast<double>(groups / 256) + (groups % 256 == 0 ? 0.0 : 0.35 + 0.65 / 256 * static_cast<double>(groups % 256));
+  const double rows = pieces == 3 ? 8.0 + 2.0 * millions * static_cast<double>(p.M) / 100.0 : 5.0 + rounds * (4.5 + 1.3 * static_cast<double>((R + 511) / 512));
+  return (p.weights == 2 ? wide_product_us(p.M, 2 * p.N, pieces * R) : wide_parts(p.M, p.N, pieces * R).us) + (pieces == 3 ? 12.0 : 8.0) + 0.56 * millions < rows;
 }
 
 // The product on dense operands: the weights dequantised into the workspace, activations of another type or length copied.
@@ -179,7 +197,7 @@ int product_wide(const Product &p, Room &room, bool only_size, hipStream_t s)
   d.R = R;
   d.compute_dtype = to;
   d.d_dtype = p.y_dtype;
-  return only_size || st != CAIFX_OK ? st : wide_product(d, s);
+  return st != CAIFX_OK ? st : wide_run(d, room, only_size, s);
 }
 
 // The product on the row kernels, any sizes and types.
@@ -259,7 +277,7 @@ bool wide_gradient_pays(const Gradient &p)
   const int pieces = pieces_of(p.compute_dtype);
   if (p.M <= 32 || !wide_takes(p.M, p.K, R)) return false;
   // (both behind the same copies.  us, rows / dense: 4096 x 14336, 64 rows 76 / 72, 96 rows 99 / 72; 14336 x 4096, 128 rows 93 / 123, 256 rows 123 / 124)
-  return wide_product_us(p.M, p.K, p.weights * pieces * R) + (pieces == 3 ? 15.0 : 0.0) < gradient_rows_us(p);
+  return wide_parts(p.M, p.K, p.weights * pieces * R).us + (pieces == 3 ? 15.0 : 0.0) < gradient_rows_us(p);
 }
 
 int gradient_wide(const Gradient &p, Room &room, bool only_size, hipStream_t s)
@@ -291,7 +309,7 @@ int gradient_wide(const Gradient &p, Room &room, bool only_size, hipStream_t s)
   d.R = R;
   d.compute_dtype = to;
   d.d_dtype = p.y_dtype;
-  return only_size || st != CAIFX_OK ? st : wide_product(d, s);
+  return st != CAIFX_OK ? st : wide_run(d, room, only_size, s);
 }
 
 int gradient_rows(const Gradient &p, Room &room, bool only_size, hipStream_t s)
@@ -352,8 +370,9 @@ bool dx_pays(const Gradient &p)
   const int64_t R = up_to(p.N, 64) < 128 ? 128 : up_to(p.N, 64);
   const int pieces = pieces_of(p.compute_dtype);
   const double values = p.weights * static_cast<double>(p.N) * static_cast<double>(p.K);
-  const double product = wide_gradient_pays(p) ? wide_product_us(p.M, p.K, p.weights * pieces * R) + (pieces == 3 ? 15.0 : 0.0) : gradient_rows_us(p);
-  return dx_us(dx_of(p, p.N % 8 == 0)) < product + 12.0 + values * (p.w[0].mx ? 2.53 : 4.0) / 4.4e6 + (pieces == 3 ? 4.0 : 0.0);
+  const double far = values > 64e6 ? (values - 64e6) * 0.5e-6 : 0.0;      // (copies of more than half of the memory-side cache are read from further away)
+  const double product = wide_gradient_pays(p) ? wide_parts(p.M, p.K, p.weights * pieces * R).us + (pieces == 3 ? 15.0 : 0.0) : gradient_rows_us(p);
+  return dx_us(dx_of(p, p.N % 8 == 0)) < product + 12.0 + values * (p.w[0].mx ? 2.53 : 4.0) / 4.4e6 + far + (pieces == 3 ? 4.0 : 0.0);
 }
 int gradient_dx(const Gradient &p, Room &room, bool only_size, hipStream_t s)
 {

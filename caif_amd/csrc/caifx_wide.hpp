@@ -14,6 +14,7 @@ struct WideProduct {
   const void *b[2];       // [C, R] each
   int64_t a_stride, b_stride;
   int pairs, b_every;
+  int parts;              // workgroups that share a tile's steps; more than one: d holds `parts` fp32 results one behind the other, not gated, no addend
   // gated: d = silu(that) * (the same with b[1]), and the two kept in gate and up unless those are null; no addend.  d is of the compute
   // type, or with several pairs fp32.
   bool gated;
@@ -35,5 +36,11 @@ bool wide_takes(int64_t M, int64_t C, int64_t R);
 int wide_product(const WideProduct &p, hipStream_t s);
 // what a product takes, in us, estimated; gated: C of both weights together, chained: R of both pairs
 double wide_product_us(int64_t M, int64_t C, int64_t R);
+// into how many parts a product that is not gated is best cut, and what it takes with their joining, in us, estimated
+struct WideParts {
+  int parts;
+  double us;
+};
+WideParts wide_parts(int64_t M, int64_t C, int64_t R);
 
 }  // namespace caifx
