@@ -25,6 +25,8 @@ struct MxGemmArgs {
   void *d;                      // [M, C]
   int64_t M, C, pitch;
   int groups, d_dtype;
+  int parts;                    // workgroups that share a tile's steps: the z-th writes its sums to d + z M C (fp32)
+  int halved;                   // tiles at the end of each XCD's list that two workgroups of half the rows take
 };
 
 __device__ __forceinline__ void mfma_mx(floatx4_t &acc, const u32x4_t &a, const u32x4_t &b, uint32_t sa, uint32_t sb)
@@ -37,47 +39,38 @@ __device__ __forceinline__ void mfma_mx(floatx4_t &acc, const u32x4_t &a, const 
 // and half 0 in the middle of the next step's (0,0): there the waves meet, and behind the barrier the freed slot is requested for step
 // s + 2.  Requests complete in issue order, so each wait is an exact count: WI + WJ requests of a wave per half, and two more, the
 // scales of steps s + 2 and s + 3, with half 0 where s + 2 is even.
-template <int WI, int WJ, bool kTail>
-__global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void mx_gemm_kernel(MxGemmArgs g)
+template <int WI, int WJ, bool kTail> __device__ __forceinline__ void mx_tile(MxGemmArgs &g, unsigned char *smem, int64_t row0, int64_t col0)
 {
   constexpr int BM = 64 * WI, BN = 64 * WJ;
   constexpr int kASlot = BM / 2 * 128, kBSlot = BN / 2 * 128;      // LDS bytes of half an operand tile
   constexpr int kBBase = 4 * kASlot;
   constexpr int kScales = kBBase + 4 * kBSlot;                     // scales: [slot][BM + BN rows][16 bytes]
   constexpr int kScaleSlot = (BM + BN) * 16;
-  constexpr int kBand = kBandRows / BM;
   constexpr int kReq = WI + WJ;            // requests of a wave per half step
   constexpr int kMore = 2;                 // requests of a wave for the scales of two steps
   constexpr int Q = 2 * WI * WJ;           // products per quadrant
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1;
   const int r16 = lane & 15, kq = lane >> 4;
 
-  // XCD x (workgroup id mod 8) walks the x-th contiguous eighth of a list that runs through bands of 1024 rows column by column
-  const int64_t col_tiles = (g.C + BN - 1) / BN, row_tiles = (g.M + BM - 1) / BM;
-  const int64_t per_xcd = gridDim.x >> 3;
-  const int64_t pos = static_cast<int64_t>(blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-  if (pos >= row_tiles * col_tiles) return;
-  const int64_t band = pos / (kBand * col_tiles);
-  const int64_t within = pos - band * kBand * col_tiles;
-  const int64_t left = row_tiles - band * kBand;
-  const int64_t band_rows = left < kBand ? left : kBand;
-  const int64_t col0 = (within / band_rows) * BN, row0 = (band * kBand + within % band_rows) * BM;
-
-  const int steps = static_cast<int>((g.pitch + 127) / 128), last = steps - 1;
+  // this workgroup's steps, from an even one on (two share their scales)
+  const int total = static_cast<int>((g.pitch + 127) / 128), z = static_cast<int>(blockIdx.y);
+  const int begin = static_cast<int>(static_cast<int64_t>(total) * z / g.parts) & ~1;
+  const int steps = (z + 1 == g.parts ? total : static_cast<int>(static_cast<int64_t>(total) * (z + 1) / g.parts) & ~1) - begin, last = steps - 1;
+  const bool ends = z + 1 == g.parts;      // it has the rows' last step
+  if (z > 0) g.d = static_cast<float *>(g.d) + z * g.M * g.C;
   // request i of a wave for half h of an operand: 8 rows x 128 bytes; LDS position p of row r holds 16-byte chunk p ^ (r ^ r >> 3) & 7 of
   // the row (operand reads without bank conflicts).  Rows past the end are the last one again and never stored; of a row's last step
   // chunks past its end are its last one again (their scales are 2^-127).
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem));
   uint32_t a_voff[2][WI], b_voff[2][WJ], past[2];
-  const int in_last = static_cast<int>((g.pitch - static_cast<int64_t>(last) * 128) >> 4);      // chunks of the last step
+  const int in_last = static_cast<int>((g.pitch - static_cast<int64_t>(total - 1) * 128) >> 4);      // chunks of the last step
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int lrow = 8 * (wave + 4 * i) + (lane >> 3);
     const int chunk = (lane & 7) ^ ((lrow ^ (lrow >> 3)) & 7);
-    past[i] = chunk >= in_last ? static_cast<uint32_t>(chunk - in_last + 1) * 16 : 0;
+    past[i] = ends && chunk >= in_last ? static_cast<uint32_t>(chunk - in_last + 1) * 16 : 0;
   }
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -96,8 +89,8 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void mx_gemm_kernel(MxGe
       b_voff[h][i] = static_cast<uint32_t>((c - col0) * g.pitch + (((lane & 7) ^ ((lrow ^ (lrow >> 3)) & 7)) << 4));
     }
   }
-  const uint64_t a_base = uniform64(reinterpret_cast<uint64_t>(g.a) + static_cast<uint64_t>(row0 * g.pitch));
-  const uint64_t b_base = uniform64(reinterpret_cast<uint64_t>(g.b) + static_cast<uint64_t>(col0 * g.pitch));
+  const uint64_t a_base = uniform64(reinterpret_cast<uint64_t>(g.a) + static_cast<uint64_t>(row0 * g.pitch + begin * 128));
+  const uint64_t b_base = uniform64(reinterpret_cast<uint64_t>(g.b) + static_cast<uint64_t>(col0 * g.pitch + begin * 128));
   auto request = [&](int s, int h, int slot, int x) __attribute__((always_inline)) {
     const uint32_t k0 = static_cast<uint32_t>(s < last ? s : last) * 128;          // past the end: the last step again
     const bool is_a = x < WI;
@@ -109,7 +102,7 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void mx_gemm_kernel(MxGe
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(voff), "s"(src) : "memory");
   };
   // the scales of steps 2 group and 2 group + 1: a wave takes 64 rows of either operand (with 128 rows two waves the same ones)
-  const int groups = g.groups;
+  const int groups = g.groups, group0 = begin >> 1;
   const uint32_t s_voff = static_cast<uint32_t>(lane) * 16;
   const auto scales_of = [&](const uint8_t *scales, int64_t row) __attribute__((always_inline)) {
     return uniform64(reinterpret_cast<uint64_t>(scales) + static_cast<uint64_t>((row >> 6) * groups) * 1024);
@@ -117,7 +110,7 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void mx_gemm_kernel(MxGe
   const uint64_t sa_base = scales_of(g.sa, row0 + (64 * wave) % BM < g.M ? row0 + (64 * wave) % BM : row0);      // (past the last row: others' scales)
   const uint64_t sb_base = scales_of(g.sb, col0 + (64 * wave) % BN < g.C ? col0 + (64 * wave) % BN : col0);
   auto request_scales = [&](int group, int x) __attribute__((always_inline)) {
-    const uint32_t k0 = static_cast<uint32_t>(group < groups ? group : groups - 1) * 1024;
+    const uint32_t k0 = static_cast<uint32_t>(group0 + group < groups ? group0 + group : groups - 1) * 1024;
     const uint64_t src = (x == 0 ? sa_base : sb_base) + k0;
     const uint32_t dst = lds0 + kScales + (group & 1) * kScaleSlot + (x == 0 ? (64 * wave) % BM : BM + (64 * wave) % BN) * 16;
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(s_voff), "s"(src) : "memory");
@@ -290,6 +283,33 @@ __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void mx_gemm_kernel(MxGe
   else store(float{});
 }
 
+// XCD x (workgroup id mod 8) walks the x-th contiguous eighth of a list that runs through bands of 1024 rows column by column.  A last round
+// that fills less than half of the compute units is run as twice as many tiles of half the rows.
+template <int WI, int WJ, bool kTail, bool kHalves> __global__ __launch_bounds__(256, WI + WJ <= 4 ? 2 : 1) void mx_gemm_kernel(MxGemmArgs g)
+{
+  constexpr int BM = 64 * WI, BN = 64 * WJ, kBand = kBandRows / BM;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int64_t col_tiles = (g.C + BN - 1) / BN, row_tiles = (g.M + BM - 1) / BM;
+  const int64_t per_xcd = (row_tiles * col_tiles + 7) >> 3, whole = per_xcd - g.halved;
+  int64_t at = blockIdx.x >> 3;
+  const bool half = kHalves && at >= whole, lower = half && ((at - whole) & 1);
+  if (half) at = whole + ((at - whole) >> 1);
+  const int64_t pos = static_cast<int64_t>(blockIdx.x & 7) * per_xcd + at;
+  if (pos >= row_tiles * col_tiles) return;
+  const int64_t band = pos / (kBand * col_tiles);
+  const int64_t within = pos - band * kBand * col_tiles;
+  const int64_t left = row_tiles - band * kBand;
+  const int64_t band_rows = left < kBand ? left : kBand;
+  const int64_t col0 = (within / band_rows) * BN, row0 = (band * kBand + within % band_rows) * BM + (lower ? BM / 2 : 0);
+  if constexpr (kHalves) {
+    if (half) {
+      if (row0 < g.M) mx_tile<WI / 2, WJ, kTail>(g, smem, row0, col0);
+      return;
+    }
+  }
+  mx_tile<WI, WJ, kTail>(g, smem, row0, col0);
+}
+
 // Scales [rows, blocks] of both operands as [rows / 64][groups][64][16]: the 16 bytes of a row that two steps need, 64 rows together, zeros
 // (2^-127) for blocks and rows that there are not.
 __global__ __launch_bounds__(256) void order_scales_kernel(const uint8_t *__restrict__ a, int64_t a_rows, const uint8_t *__restrict__ b, int64_t b_rows,
@@ -321,14 +341,14 @@ __global__ __launch_bounds__(256) void order_scales_kernel(const uint8_t *__rest
   }
 }
 
-template <int WI, int WJ, bool kTail>
+template <int WI, int WJ, bool kTail, bool kHalves = false>
 int launch_mx(const MxGemmArgs &g, hipStream_t s)
 {
   constexpr int BM = 64 * WI, BN = 64 * WJ;
   constexpr int kRing = (BM + BN) * 256 + 2 * (BM + BN) * 16, kStore16 = BM * (BN * 2 + 32), kStore32 = BM / 2 * (BN * 4 + 32);
   constexpr int kStore = kStore16 > kStore32 ? kStore16 : kStore32;
   constexpr int kLds = kRing > kStore ? kRing : kStore;
-  auto kern = mx_gemm_kernel<WI, WJ, kTail>;
+  auto kern = mx_gemm_kernel<WI, WJ, kTail, kHalves>;
   static std::atomic<bool> raised{false};
   if (!raised.load(std::memory_order_relaxed)) {
     // the attribute is per kernel and sticky; two threads racing here both set it, which is harmless
@@ -337,7 +357,7 @@ int launch_mx(const MxGemmArgs &g, hipStream_t s)
     raised.store(true, std::memory_order_relaxed);
   }
   const int64_t tiles = ((g.M + BM - 1) / BM) * ((g.C + BN - 1) / BN);
-  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((tiles + 7) / 8 * 8)), dim3(256), kLds, s, g);
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(((tiles + 7) / 8 + g.halved) * 8), static_cast<unsigned>(g.parts)), dim3(256), kLds, s, g);
   return launch_status();
 }
 
@@ -352,41 +372,77 @@ bool mx_gemm_takes(int64_t M, int64_t C, int64_t blocks)
   return blocks < (int64_t{1} << 17) && ((M + 127) / 128) * ((C + 127) / 128) <= (int64_t{1} << 30);
 }
 
-double mx_gemm_us(int64_t M, int64_t C, int64_t blocks)
+namespace {
+
+// One workgroup of 256 x 256 per compute unit or two of 128 x 128: the large tile reads each operand half as often.  Few tiles and many steps: up
+// to eight workgroups share a tile's steps, and a second launch adds their sums.  Measured with the scales' order, us, small / large / large with
+// the last round halved: M = 4096, N = 14336, K = 4096 178 / 157 / 147; M = 1536 72 / 74 / 66; M = 512, N = K = 4096 17 / 34 / 23; small in one / four
+// parts: M = 256, N = 4096, K = 14336 42 / 26, N = 14336, K = 4096 20 / 44.
+struct MxPlan {
+  bool large;
+  int halved, parts;
+  double us;
+};
+MxPlan mx_plan(int64_t M, int64_t C, int64_t blocks)
 {
-  const double steps = static_cast<double>((blocks + 7) / 8);
   const int64_t large = ((M + 255) / 256) * ((C + 255) / 256), small = ((M + 127) / 128) * ((C + 127) / 128);
-  if (large >= 192) return 4.0 + 2.3 * steps * static_cast<double>((large + 255) / 256);
-  return 4.0 + 0.8 * steps * static_cast<double>((small + 511) / 512);
+  const int64_t steps = (blocks + 7) / 8;
+  MxPlan best{};
+  // us of a step: full rounds, and a last one that costs less the fewer tiles it has
+  const auto rounds = [](int64_t tiles, int64_t slots, double full, double base, double per) {
+    const int64_t rest = tiles % slots;
+    return full * static_cast<double>(tiles / slots) + (rest == 0 ? 0.0 : base + per * static_cast<double>(rest));
+  };
+  const auto consider = [&](bool is_large, int halved, int parts, double step) {
+    const double us = 9.0 + step * static_cast<double>((steps + parts - 1) / parts) + (parts > 1 ? 4.0 + 1.4e-6 * parts * static_cast<double>(M) * static_cast<double>(C) : 0.0);
+    if (best.parts == 0 || us < best.us) best = MxPlan{is_large, halved, parts, us};
+  };
+  for (int parts = 1; parts <= 8 && (parts == 1 || steps >= 8 * parts); ++parts) {
+    const int64_t t = small * parts;
+    consider(false, 0, parts, t % 512 <= 256 ? rounds(t, 512, 1.35, 0.58, 0.0004) : rounds(t, 512, 1.35, 0.65, 0.0012));
+    consider(true, 0, parts, rounds(large * parts, 256, 2.2, 1.3, 0.003));
+  }
+  const int64_t rest = (large + 7) / 8 % 32;
+  if (rest > 0 && rest <= 16) consider(true, static_cast<int>(rest), 1, rounds((large + 7) / 8 * 8, 256, 2.2, 0.9, 0.0025));
+  return best;
 }
+
+}  // namespace
+
+double mx_gemm_us(int64_t M, int64_t C, int64_t blocks) { return mx_plan(M, C, blocks).us; }
 
 size_t mx_gemm_workspace_bytes(int64_t M, int64_t C, int64_t blocks)
 {
-  return static_cast<size_t>(scale_bytes(M, blocks) + scale_bytes(C, blocks));
+  const MxPlan p = mx_plan(M, C, blocks);
+  return static_cast<size_t>(scale_bytes(M, blocks) + scale_bytes(C, blocks)) + (p.parts > 1 ? static_cast<size_t>(p.parts) * static_cast<size_t>(M) * static_cast<size_t>(C) * 4 : 0);
 }
 
 int mx_gemm(int64_t M, int64_t C, int64_t blocks, const void *a, const void *sa, const void *b, const void *sb, void *d, int d_dtype, void *workspace, hipStream_t s)
 {
+  const MxPlan p = mx_plan(M, C, blocks);
   MxGemmArgs g{};
   g.a = static_cast<const uint8_t *>(a);
   g.b = static_cast<const uint8_t *>(b);
-  g.d = d;
   g.M = M;
   g.C = C;
   g.pitch = 16 * blocks;
   g.groups = static_cast<int>(groups_of(blocks));
-  g.d_dtype = d_dtype;
+  g.parts = p.parts;
+  g.halved = p.halved;
   g.sa = static_cast<const uint8_t *>(workspace);
   g.sb = g.sa + scale_bytes(M, blocks);
+  void *partial = static_cast<char *>(workspace) + scale_bytes(M, blocks) + scale_bytes(C, blocks);
+  g.d = p.parts > 1 ? partial : d;
+  g.d_dtype = p.parts > 1 ? static_cast<int>(CAIFX_F32) : d_dtype;
   const int64_t grid = (scale_bytes(M, blocks) + scale_bytes(C, blocks)) / 16 / 256;
   hipLaunchKernelGGL(order_scales_kernel, dim3(static_cast<unsigned>(grid < 1 ? 1 : grid < (1 << 20) ? grid : (1 << 20))), dim3(256), 0, s, static_cast<const uint8_t *>(sa), M,
                      static_cast<const uint8_t *>(sb), C, static_cast<u32x4_t *>(workspace), static_cast<int>(blocks), g.groups);
   const bool tail = blocks % 8 != 0;
-  // One workgroup of 256 x 256 per compute unit or two of 128 x 128: the large tile reads each operand half as often, and is taken once
-  // there are enough of them.
-  const bool large = ((M + 255) / 256) * ((C + 255) / 256) >= 192;
-  if (large) return tail ? launch_mx<4, 4, true>(g, s) : launch_mx<4, 4, false>(g, s);
-  return tail ? launch_mx<2, 2, true>(g, s) : launch_mx<2, 2, false>(g, s);
+  int st;
+  if (p.halved) st = tail ? launch_mx<4, 4, true, true>(g, s) : launch_mx<4, 4, false, true>(g, s);
+  else if (p.large) st = tail ? launch_mx<4, 4, true>(g, s) : launch_mx<4, 4, false>(g, s);
+  else st = tail ? launch_mx<2, 2, true>(g, s) : launch_mx<2, 2, false>(g, s);
+  return st != CAIFX_OK || p.parts == 1 ? st : join_sums(static_cast<const float *>(partial), p.parts, M * C, d, d_dtype, nullptr, s);
 }
 
 }  // namespace caifx

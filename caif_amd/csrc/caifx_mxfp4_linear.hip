@@ -476,9 +476,12 @@ int64_t blocks_of(int64_t columns) { return (columns + CAIFX_MXFP4_BLOCK - 1) / 
 // whether a product of two operands in 4 bits runs in tiles rather than on the row kernels
 bool tiles_pay(int64_t M, int64_t N, int64_t blocks)
 {
-  // us, rows / tiles, bf16: N = 14336, K = 4096, 64 rows 16 / 17, 96 rows 25 / 18; N = 4096, K = 14336, 256 rows 37 / 49, 512 rows 66 / 48; N = K =
-  // 4096, 192 rows 13 / 12; 2048 x 1408, 512 rows 7 / 12.
-  return M > 64 && mx_gemm_takes(M, N, blocks) && mx_gemm_us(M, N, blocks) < 4.5 + 64e-9 * static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(blocks) / 0.8;
+  // A workgroup of the row kernels takes 64 x 64 results in 2.2 us and 1.1 for every 512 elements of the reduction, 256 of them at a time.  us, rows /
+  // tiles, bf16: N = 14336, K = 4096, 96 rows 25 / 20; N = 4096, K = 14336, 96 rows 26 / 23, 256 rows 37 / 27; N = K = 4096, 256 rows 14 / 16, 512 rows
+  // 26 / 17; 2048 x 1408, 512 rows 7 / 11.
+  const int64_t groups = (M + 63) / 64 * ((N + 63) / 64);
+  const double rounds = static_cast<double>(groups / 256) + (groups % 256 == 0 ? 0.0 : 0.35 + 0.65 / 256 * static_cast<double>(groups % 256));
+  return M > 64 && mx_gemm_takes(M, N, blocks) && mx_gemm_us(M, N, blocks) < 3.5 + rounds * (2.2 + 1.1 * static_cast<double>((blocks + 15) / 16));
 }
 
 RowsArgs both_args(int64_t M, int64_t N, int64_t blocks)
