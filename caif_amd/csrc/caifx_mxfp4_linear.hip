@@ -222,7 +222,8 @@ int product_rows(const Product &p, Room &room, bool only_size, hipStream_t s)
     g.R = pitch;
     g.w_pitch = 2 * pitch;
   }
-  const bool direct = p.M <= 32 && direct_type(p) && (only_size || aligned_to(p.x, 16));
+  // (a query has no address, and one that calls for a workspace in any case has room for rows at any)
+  const bool direct = p.M <= 32 && direct_type(p) && aligned_to(p.x, 16);
   if (!direct) {
     void *packed = room.take(packed_bytes(p.M, g.chunks, p.compute_dtype));
     if (!only_size) {
@@ -233,7 +234,9 @@ int product_rows(const Product &p, Room &room, bool only_size, hipStream_t s)
   } else {
     g.x = p.x;
   }
-  return rows_run(g, p.w[0].mx ? ROWS_MX : ROWS_DENSE, p.weights, p.compute_dtype, direct, room, only_size, s);
+  const int st = rows_run(g, p.w[0].mx ? ROWS_MX : ROWS_DENSE, p.weights, p.compute_dtype, direct, room, only_size, s);
+  if (only_size && direct && !p.x && room.used > 0) room.take(packed_bytes(p.M, g.chunks, p.compute_dtype));
+  return st;
 }
 
 // What either way can need.  Activations at addresses that the dense product does not take run on the row kernels.
@@ -460,8 +463,7 @@ int mxfp4_linear(const GemmArgs &a, bool backward, hipStream_t s)
 {
   if (!fits(a.M, a.N, a.K)) return CAIFX_ERR_UNSUPPORTED;
   const size_t need = mxfp4_workspace_bytes(a, backward, backward);
-  const bool misaligned = !backward && need == 0 && !aligned_to(a.x, 16);      // (packed then, into room that the query did not count)
-  if (misaligned || (need > 0 && (!a.workspace || a.workspace_bytes < need || !aligned_to(a.workspace, 16)))) return CAIFX_ERR_UNSUPPORTED;
+  if (need > 0 && (!a.workspace || a.workspace_bytes < need || !aligned_to(a.workspace, 16))) return CAIFX_ERR_UNSUPPORTED;
   if (backward) return gradient(gradient_of(a), a.workspace, s);
   return product(product_of(a), a.workspace, a.workspace && aligned_to(a.workspace, 16) ? a.workspace_bytes : 0, s);
 }

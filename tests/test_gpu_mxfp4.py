@@ -336,3 +336,30 @@ def test_static_form():
         assert L.caifx_qlinear_forward_static(M, N, K, x.data_ptr(), T.BF16, T.BF16, w.wq.data_ptr(), T.W_MXFP4, w.scales.data_ptr(), 1, 32, y.data_ptr(), T.F32, s) == 0
         want = T.qlinear_forward(x, w, T.BF16, workspace=torch.empty(need, dtype=torch.uint8, device="cuda"))
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(3, 48, 512), (20, 512, 16384), (32, 1024, 8192), (100, 264, 8192), (300, 512, 2048)])
+def test_activations_at_any_address(M, N, K, dtype, backward):
+    """Activations that no 16-byte access takes, in the workspace of the query: nothing behind it is written."""
+    g = gen(60)
+    L = capi.lib()
+    s = torch.cuda.current_stream().cuda_stream
+    w, exact = weight(g, N, K)
+    t = DTYPES[dtype]
+    c = T.CODE_OF[t]
+    length, C = (N, K) if backward else (K, N)
+    x = torch.randn(M, length, generator=g).to(t).cuda()
+    apart = torch.empty(M * length + 1, dtype=t, device="cuda")
+    apart[1:] = x.view(-1)
+    need = L.caifx_qlinear_workspace_bytes(M, N, K, c, c, T.W_MXFP4, int(backward))
+    fn = L.caifx_qlinear_backward_input if backward else L.caifx_qlinear_forward
+    m = exact if backward else exact.T
+    want, size = x.double().cpu() @ m, x.double().cpu().abs() @ m.abs()
+    for a in (x, apart[1:]):
+        ws = torch.full((need + (1 << 20),), 201, dtype=torch.uint8, device="cuda")
+        y = torch.empty(M, C, dtype=t, device="cuda")
+        assert fn(M, N, K, a.data_ptr(), c, c, w.wq.data_ptr(), T.W_MXFP4, w.scales.data_ptr(), 1, 32, y.data_ptr(), c, ws.data_ptr(), need, s) == 0
+        assert bool((ws[need:] == 201).all())
+        within(y, want, size, length, 3 if dtype == "f32" else 1)
