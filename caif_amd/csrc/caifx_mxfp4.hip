@@ -234,25 +234,17 @@ __global__ __launch_bounds__(kThreads) void dense_transposed_kernel(Sources two,
   }
 }
 
-// Eight values (m, k .. k + 7) of activations as three bf16 pieces each, which add up to them: the upper 8 bits of the mantissa, the next 8
-// and the rest, each cut off and so exact.  Zeros outside.
+// Eight values (m, k .. k + 7) of activations as three bf16 pieces each.  Zeros outside.
 template <typename S> __device__ __forceinline__ void pieces8(const Source &g, int64_t m, int64_t k, Eight<uint16_t> (&piece)[3])
 {
   const int64_t left = m < g.rows ? g.cols - k : 0;
   const Eight<S> e = load8(static_cast<const S *>(g.p) + m * g.cols + k, left > 0 ? (left < kPer ? static_cast<int>(left) : kPer) : 0);
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const float value = to_f32<S>(e.v[i]);
-    const uint32_t bits = __builtin_bit_cast(uint32_t, value), high = bits & 0xFFFF0000u;
-    const bool finite = (bits & 0x7F800000u) != 0x7F800000u;
-    const float rest = value - __builtin_bit_cast(float, high);
-    const uint32_t middle = __builtin_bit_cast(uint32_t, rest) & 0xFFFF0000u;
-    const float last = rest - __builtin_bit_cast(float, middle);
-    // a NaN whose upper bits alone would be an infinity stays a NaN
-    const uint32_t nan = !finite && (bits & 0x007FFFFFu) != 0 ? 0x00400000u : 0u;
-    piece[0].v[i] = static_cast<uint16_t>((high | nan) >> 16);
-    piece[1].v[i] = finite ? static_cast<uint16_t>(middle >> 16) : 0;
-    piece[2].v[i] = finite ? static_cast<uint16_t>(__builtin_bit_cast(uint32_t, last) >> 16) : 0;
+    uint32_t bits[3];
+    pieces_of_f32(to_f32<S>(e.v[i]), bits);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) piece[p].v[i] = static_cast<uint16_t>(bits[p] >> 16);
   }
 }
 

@@ -78,7 +78,7 @@ int rows_run(RowsArgs g, int kind, int weights, int compute_dtype, bool direct, 
   const int pieces = pieces_of(compute_dtype);
   const int tile = rows_tile(g.M, pieces);
   const double row = kind == ROWS_DENSE ? static_cast<double>(g.w_pitch) : 17.0 * static_cast<double>(g.blocks);
-  const double x = (kind == ROWS_BOTH ? row : 2.0 * pieces * static_cast<double>(g.R)) * (g.M <= 4 && pieces == 1 ? 4 : tile);
+  const double x = (kind == ROWS_BOTH ? row : (direct ? 2.0 + (pieces > 1 ? 2.0 : 0.0) : 2.0 * pieces) * static_cast<double>(g.R)) * (g.M <= 4 && (direct || pieces == 1) ? 4 : tile);
   const RowsPlan plan = rows_plan(g.M, g.N, g.R, weights, pieces, row, x);
   void *partial = plan.splits > 1 ? room.take(static_cast<size_t>(plan.splits) * static_cast<size_t>(g.M) * static_cast<size_t>(g.N) * 4) : nullptr;
   if (only_size) return CAIFX_OK;
@@ -110,8 +110,9 @@ int wide_run(WideProduct d, Room &room, bool only_size, hipStream_t s)
   return st != CAIFX_OK ? st : join_sums(static_cast<const float *>(partial), d.parts, d.M * d.C, asked.d, asked.d_dtype, asked.addend, s);
 }
 
-// whether the row kernels can read the activations where they are
-bool direct_type(const Product &p) { return p.compute_dtype != CAIFX_F32 && p.x_dtype == p.compute_dtype && p.R % 8 == 0; }
+// Whether the row kernels read the activations where they are.  fp32 ones are taken apart by every workgroup then, which pays for the launch that
+// packs them for one group of four rows (us, N = K = 4096, direct / packed: 4 rows 6.8 / 10.8, 8 rows 11.9 / 10.9).
+bool direct_rows(const Product &p) { return p.M <= (p.compute_dtype == CAIFX_F32 ? 4 : 32) && p.x_dtype == p.compute_dtype && p.R % 8 == 0 && aligned_to(p.x, 16); }
 
 // The weights of a product or the activations of a gradient, as a source of operands
 Operand weights_of(const Weight (&w)[2], int count, int64_t rows, int64_t cols, int stored)
@@ -147,13 +148,13 @@ bool wide_product_pays(const Product &p)
   if (p.M <= 64 || !wide_takes(p.M, p.N, R) || p.N * R >= (int64_t{1} << 32)) return false;
   if (!p.w[0].mx) return true;
   // A workgroup of the row kernels takes 64 x 64 results in 4.5 us and 1.3 for every 512 elements of the reduction, 256 of them at a time (few, a
-  // third of that and up), on three pieces they run at 100 TFLOP/s; the dense product is twice as fast and more, behind copies of the weights.
+  // third of that and up), on three pieces 32 x 32 in 2.2 and 1.3; the dense product is twice as fast and more, behind copies of the weights.
   // us, rows / dense, bf16: N = 14336, K = 4096, 256 rows 62 / 66, 384 rows 86 / 83; N = 11008 384 rows 72 / 70; N = K = 4096, 256 rows 20 / 41; N =
   // 4096, K = 14336, 512 rows 84 / 98; 5120 x 794, 512 rows 29 / 23.
   const double weights = p.weights, millions = 1e-6 * weights * static_cast<double>(p.N) * static_cast<double>(R);
-  const int64_t groups = (p.M + 63) / 64 * ((p.weights * p.N + 63) / 64);
+  const int64_t tile = pieces == 3 ? 32 : 64, groups = (p.M + tile - 1) / tile * ((p.weights * p.N + tile - 1) / tile);
   const double rounds = static_cast<double>(groups / 256) + (groups % 256 == 0 ? 0.0 : 0.35 + 0.65 / 256 * static_cast<double>(groups % 256));
-  const double rows = pieces == 3 ? 8.0 + 2.0 * millions * static_cast<double>(p.M) / 100.0 : 5.0 + rounds * (4.5 + 1.3 * static_cast<double>((R + 511) / 512));
+  const double rows = 5.0 + rounds * ((pieces == 3 ? 2.2 : 4.5) + 1.3 * static_cast<double>((R + 511) / 512));
   return (p.weights == 2 ? wide_product_us(p.M, 2 * p.N, pieces * R) : wide_parts(p.M, p.N, pieces * R).us) + (pieces == 3 ? 12.0 : 8.0) + 0.56 * millions < rows;
 }
 
@@ -223,7 +224,7 @@ int product_rows(const Product &p, Room &room, bool only_size, hipStream_t s)
     g.w_pitch = 2 * pitch;
   }
   // (a query has no address, and one that calls for a workspace in any case has room for rows at any)
-  const bool direct = p.M <= 32 && direct_type(p) && aligned_to(p.x, 16);
+  const bool direct = direct_rows(p);
   if (!direct) {
     void *packed = room.take(packed_bytes(p.M, g.chunks, p.compute_dtype));
     if (!only_size) {

@@ -67,7 +67,7 @@ inline RowsPlan rows_plan(int64_t M, int64_t N, int64_t R, int weights, int piec
 }
 
 struct RowsArgs {
-  const void *x;          // direct: [M, x_pitch] of the compute type; packed: see pack_rows_kernel
+  const void *x;          // direct: [M, x_pitch] of the compute type, or fp32 for three pieces; packed: see pack_rows_kernel
   int64_t x_pitch;
   const void *w[2];       // MX codes or dense rows of the compute type
   const uint8_t *s[2];    // MX scales
@@ -122,10 +122,26 @@ template <> struct Mfma16<f16_t> {
   }
 };
 
+// A number as three of eight bits of its mantissa each, cut off and so exact, which add up to it; a bf16 in the upper half of every dword.
+__device__ __forceinline__ void pieces_of_f32(float value, uint32_t (&piece)[3])
+{
+  const uint32_t bits = __builtin_bit_cast(uint32_t, value), high = bits & 0xFFFF0000u;
+  const bool finite = (bits & 0x7F800000u) != 0x7F800000u;
+  const float rest = value - __builtin_bit_cast(float, high);
+  const uint32_t middle = __builtin_bit_cast(uint32_t, rest) & 0xFFFF0000u;
+  const float last = rest - __builtin_bit_cast(float, middle);
+  // a NaN whose upper bits alone would be an infinity stays a NaN
+  const uint32_t nan = !finite && (bits & 0x007FFFFFu) != 0 ? 0x00400000u : 0u;
+  piece[0] = high | nan;
+  piece[1] = finite ? middle : 0u;
+  piece[2] = finite ? __builtin_bit_cast(uint32_t, last) : 0u;
+}
+
 // P: pieces of an activation (3: fp32).  NW: weights (2: gate and up; the first half of the NT column tiles is gate's).  kWhole: rows of
 // at least 16 blocks: a unit's scales of a weight row are one access, at any address (one byte at a time they are more requests than the
 // codes; K = 11008, N = 4096, one row 22.0 us instead of 8.6).
-// XG: groups of four rows of activations that are read where they are; 0: packed ones.
+// XG: groups of four rows of activations that are read where they are, fp32 ones (up to four) taken
+// apart on their way through LDS; 0: packed ones.
 template <typename CT, int P, int kWeight, int NW, int MT, int NT, int XG, bool kWhole>
 __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
 {
@@ -133,14 +149,15 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
   constexpr bool kMicro = kWeight != ROWS_DENSE, kBoth = kWeight == ROWS_BOTH;
   constexpr bool kDirect = XG > 0 && !kBoth;
   constexpr int WV = kMicro ? 1 : 4, XV = kBoth ? 1 : 4;      // 16-byte pieces of a column tile and of a row tile per half chunk
-  constexpr int XL = kDirect ? XG : MT * P * XV;              // loads of activations per half chunk
+  constexpr int XW = P == 3 ? 2 : 1;                          // direct: loads of eight elements
+  constexpr int XL = kDirect ? XG * XW : MT * P * XV;         // loads of activations per half chunk
   // half chunks on their way before the one in hand is used: a second one where a SIMD still holds four waves with it (one row, N = 4096, K =
   // 14336: 10.2 us instead of 13.3; with 32 registers a half chunk, 16 rows, N = 14336, K = 4096: 11.9 instead of 11.4)
   constexpr int kRegs = 4 * (NT * WV + XL);
   constexpr int D = kRegs <= 24 ? 2 : 1;
-  static_assert(NT % NW == 0 && (P == 1 || XG == 0) && (kMicro || !kWhole) && (XG == 0 || XG == 4 * MT || (MT == 1 && XG == 1)), "");
-  // the activations of a half chunk for each wave, [4 XG][16 pieces of 16 bytes]; at the end the waves' sums
-  constexpr int kSums = kRowsWaves / 2 * MT * NT * 1024, kOrder = kDirect ? kRowsWaves * XG * 1024 : 0;
+  static_assert(NT % NW == 0 && (P == 1 || XG <= 1) && (kMicro || !kWhole) && (XG == 0 || XG == 4 * MT || (MT == 1 && XG == 1)), "");
+  // the activations of a half chunk for each wave, [P][4 XG][16 pieces of 16 bytes]; at the end the waves' sums
+  constexpr int kSums = kRowsWaves / 2 * MT * NT * 1024, kOrder = kDirect ? kRowsWaves * P * XG * 1024 : 0;
   __shared__ __attribute__((aligned(16))) unsigned char smem[kSums > kOrder ? kSums : kOrder];
   auto sums = reinterpret_cast<floatx4_t(*)[MT * NT][64]>(smem);
   const int lane = threadIdx.x & 63;
@@ -168,7 +185,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
   const uint8_t *x_base = static_cast<const uint8_t *>(g.x), *xs_base = nullptr;
   uint32_t x_off[kDirect ? XG : MT], xs_off[kBoth ? MT : 1];
   if constexpr (kBoth || kDirect) {
-    const int64_t pitch = kBoth ? g.w_pitch : 2 * g.x_pitch;
+    const int64_t pitch = kBoth ? g.w_pitch : 2 * XW * g.x_pitch;
     x_base += m0 * pitch;
     if constexpr (kBoth) xs_base = g.xs + m0 * g.blocks;
 #pragma unroll
@@ -176,7 +193,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
       // (direct: lane (j, q) reads piece j of the half chunk of row 4 t + q)
       const int64_t m = m0 + (kDirect ? 4 * t + q : 16 * t + j);
       const uint32_t row = static_cast<uint32_t>((m < g.M ? m : g.M - 1) - m0);
-      x_off[t] = row * static_cast<uint32_t>(pitch) + (kDirect ? j : q) * 16;
+      x_off[t] = row * static_cast<uint32_t>(pitch) + (kDirect ? j * XW : q) * 16;
       if constexpr (kBoth) xs_off[t] = row * static_cast<uint32_t>(g.blocks);
     }
   }
@@ -265,9 +282,11 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
     }
     if constexpr (kDirect) {
       const int k = static_cast<int>(half) * 128 + 8 * j;
-      const uint32_t back = k < g.R ? 0u : static_cast<uint32_t>(k - (g.R - 8)) * 2;
+      const uint32_t back = k < g.R ? 0u : static_cast<uint32_t>(k - (g.R - 8)) * (2 * XW);
 #pragma unroll
-      for (int t = 0; t < XG; ++t) b.x[t] = at128(x_base + half * 256, x_off[t] - back, aligned);
+      for (int t = 0; t < XG; ++t)
+#pragma unroll
+        for (int i = 0; i < XW; ++i) b.x[t * XW + i] = at128(x_base + half * (256 * XW), x_off[t] - back + 16 * i, aligned);
     } else {
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
@@ -289,14 +308,14 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
     for (int c = 0; c < NT; ++c) acc[t][c] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
   // direct: a wave's rows of a half chunk through its own part of LDS into the operands' order; piece p of row r lies in place p ^ r, so that
   // the reads of sixteen rows use every bank.  Lanes of rows that were not read hold others': their results are not stored.
-  unsigned char *const order = smem + (kDirect ? wave * (XG * 1024) : 0);
+  unsigned char *const order = smem + (kDirect ? wave * (P * XG * 1024) : 0);
   // kPart: the half may reach past the end of the rows
   auto compute = [&](Half &b, const Scales &s, int h, int half, auto part_) __attribute__((always_inline)) {
     constexpr bool kPart = decltype(part_)::value;
     if constexpr (kPart && kDirect) {
       if (half * 128 + 8 * j >= g.R)
 #pragma unroll
-        for (int t = 0; t < XG; ++t) b.x[t] = u32x4_t{0, 0, 0, 0};
+        for (int t = 0; t < XL; ++t) b.x[t] = u32x4_t{0, 0, 0, 0};
     }
     if constexpr (kPart && !kMicro) {
 #pragma unroll
@@ -305,10 +324,28 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
 #pragma unroll
           for (int t = 0; t < NT; ++t) b.w[t][i] = u32x4_t{0, 0, 0, 0};
     }
-    u32x4_t ordered[kDirect ? MT * 4 : 1];
+    u32x4_t ordered[kDirect ? MT * P * 4 : 1];
     if constexpr (kDirect) {
 #pragma unroll
-      for (int t = 0; t < XG; ++t) *reinterpret_cast<u32x4_t *>(order + (4 * t + q) * 256 + ((j ^ ((4 * t + q) & 15)) << 4)) = b.x[t];
+      for (int t = 0; t < XG; ++t) {
+        unsigned char *to = order + (4 * t + q) * 256 + ((j ^ ((4 * t + q) & 15)) << 4);
+        if constexpr (P == 1) {
+          *reinterpret_cast<u32x4_t *>(to) = b.x[t];
+        } else {
+          u32x4_t v[3];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const floatx4_t four = __builtin_bit_cast(floatx4_t, b.x[t * XW + (i >> 1)]);
+            uint32_t even[3], odd[3];
+            pieces_of_f32(four[2 * (i & 1)], even);
+            pieces_of_f32(four[2 * (i & 1) + 1], odd);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) v[p][i] = __builtin_amdgcn_perm(odd[p], even[p], 0x07060302u);
+          }
+#pragma unroll
+          for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4_t *>(to + p * (XG * 1024)) = v[p];
+        }
+      }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -316,7 +353,9 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int row = XG < 4 ? j & (4 * XG - 1) : 16 * t + j;
-          ordered[t * 4 + i] = *reinterpret_cast<const u32x4_t *>(order + row * 256 + (((4 * i + q) ^ (row & 15)) << 4));
+#pragma unroll
+          for (int p = 0; p < P; ++p)
+            ordered[(t * P + p) * 4 + i] = *reinterpret_cast<const u32x4_t *>(order + p * (XG * 1024) + row * 256 + (((4 * i + q) ^ (row & 15)) << 4));
         }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
@@ -345,7 +384,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
 #pragma unroll
           for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int p = 0; p < P; ++p) acc[t][c] = Mfma16<CT>::run(kDirect ? ordered[kDirect ? t * 4 + i : 0] : b.x[kDirect ? 0 : (t * P + p) * 4 + i], w, acc[t][c]);
+            for (int p = 0; p < P; ++p) acc[t][c] = Mfma16<CT>::run(kDirect ? ordered[kDirect ? (t * P + p) * 4 + i : 0] : b.x[kDirect ? 0 : (t * P + p) * 4 + i], w, acc[t][c]);
         }
       }
     }
@@ -462,7 +501,7 @@ int rows_launch(const RowsArgs &g, hipStream_t s)
     const auto forth = [&](const void *p, int64_t bytes) { return p ? const_cast<char *>(static_cast<const char *>(p)) + bytes : nullptr; };
     part.M = g.M - m0;
     part.tiles = g.tiles - static_cast<int>(m0 / 16);
-    part.x = forth(g.x, kWeight == ROWS_BOTH ? m0 * g.w_pitch : XG > 0 ? m0 * g.x_pitch * 2 : m0 / 16 * g.chunks * (P * 8 * 1024));
+    part.x = forth(g.x, kWeight == ROWS_BOTH ? m0 * g.w_pitch : XG > 0 ? m0 * g.x_pitch * (P == 3 ? 4 : 2) : m0 / 16 * g.chunks * (P * 8 * 1024));
     part.xs = g.xs ? g.xs + m0 * g.blocks : nullptr;
     part.y = forth(g.y, m0 * g.N * es);
     part.gate = forth(g.gate, m0 * g.N * es);
@@ -492,16 +531,27 @@ int rows_pick_columns(const RowsArgs &g, hipStream_t s)
   }
   return rows_launch<CT, P, kWeight, NW, MT, 2, XG>(g, s);
 }
+// XG for activations that are read where they are, unless no call does so: a dense copy of one weight is a gradient's, with packed activations
+template <typename CT, int P, int kWeight, int NW, int MT, int XG> int rows_pick_direct(const RowsArgs &g, bool direct, hipStream_t s)
+{
+  if constexpr (kWeight == ROWS_MX || NW == 2) {
+    if (direct) return rows_pick_columns<CT, P, kWeight, NW, MT, XG>(g, s);
+  }
+  return rows_pick_columns<CT, P, kWeight, NW, MT, 0>(g, s);
+}
 template <typename CT, int kWeight, int NW> int rows_pick(const RowsArgs &g, int pieces, bool direct, hipStream_t s)
 {
-  if constexpr (dtype_code<CT>::value == CAIFX_BF16) {
-    if (pieces == 3) return rows_tile(g.M, 3) == 16 ? rows_pick_columns<CT, 3, kWeight, NW, 1, 0>(g, s) : rows_pick_columns<CT, 3, kWeight, NW, 2, 0>(g, s);
+  const bool four = direct && g.M <= 4;
+  // (two stored weights are of the 16-bit compute type)
+  if constexpr (dtype_code<CT>::value == CAIFX_BF16 && (kWeight == ROWS_MX || NW == 1)) {
+    if (pieces == 3) {
+      if (rows_tile(g.M, 3) == 32) return rows_pick_columns<CT, 3, kWeight, NW, 2, 0>(g, s);
+      return rows_pick_direct<CT, 3, kWeight, NW, 1, 1>(g, direct, s);
+    }
   }
   switch (rows_tile(g.M, 1)) {
-    case 16:
-      if (!direct) return rows_pick_columns<CT, 1, kWeight, NW, 1, 0>(g, s);
-      return g.M <= 4 ? rows_pick_columns<CT, 1, kWeight, NW, 1, 1>(g, s) : rows_pick_columns<CT, 1, kWeight, NW, 1, 4>(g, s);
-    case 32: return direct ? rows_pick_columns<CT, 1, kWeight, NW, 2, 8>(g, s) : rows_pick_columns<CT, 1, kWeight, NW, 2, 0>(g, s);
+    case 16: return four ? rows_pick_direct<CT, 1, kWeight, NW, 1, 1>(g, direct, s) : rows_pick_direct<CT, 1, kWeight, NW, 1, 4>(g, direct, s);
+    case 32: return rows_pick_direct<CT, 1, kWeight, NW, 2, 8>(g, direct, s);
     default: return rows_pick_columns<CT, 1, kWeight, NW, 4, 0>(g, s);
   }
 }
