@@ -108,14 +108,12 @@ __global__ __launch_bounds__(kWaves * 64) void dx_kernel(DxArgs g)
 #pragma unroll
     for (int c = 0; c < kSets; ++c) acc[t][c] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
   auto compute = [&](Step &b, int step) __attribute__((always_inline)) {
-    if constexpr (!kMx) {
-      // (an infinity of the last row against those zeros would be a NaN)
-      const int n = (step >= g.steps ? step - g.steps : step) * 32;
-      if (n + 32 > g.N) {
+    // (an infinity of the last row against those zeros would be a NaN)
+    const int n = (step >= g.steps ? step - g.steps : step) * 32;
+    if (n + 32 > g.N) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (n + 8 * q + i >= g.N) b.w[i][0] = b.w[i][kMx ? 0 : 1] = u32x4_t{0, 0, 0, 0};
-      }
+      for (int i = 0; i < 8; ++i)
+        if (n + 8 * q + i >= g.N) b.w[i][0] = b.w[i][kMx ? 0 : 1] = u32x4_t{0, 0, 0, 0};
     }
     // eight columns at a time
 #pragma unroll

@@ -363,3 +363,23 @@ def test_activations_at_any_address(M, N, K, dtype, backward):
         assert fn(M, N, K, a.data_ptr(), c, c, w.wq.data_ptr(), T.W_MXFP4, w.scales.data_ptr(), 1, 32, y.data_ptr(), c, ws.data_ptr(), need, s) == 0
         assert bool((ws[need:] == 201).all())
         within(y, want, size, length, 3 if dtype == "f32" else 1)
+
+
+@pytest.mark.parametrize("N", [1, 33, 60])
+@pytest.mark.parametrize("M", [3, 40, 600])
+def test_gradient_of_weights_beyond_fp16(M, N):
+    """A last row beyond fp16 is infinite in that compute type; what is read in place of the rows behind it counts for nothing."""
+    g = gen(70 + N)
+    K = 100
+    codes, s = R.random_weight(g, N, K)
+    s[N - 1, 1] = 127 + 20
+    exact = R.decode(codes, s, K)
+    w = T.FrozenWeight(codes.cuda(), T.W_MXFP4, s.cuda(), N, K, 1, 32)
+    x = torch.randn(M, N, generator=g).half()
+    y = T.qlinear_backward_input(x.cuda(), w, T.F16, T.F32).cpu()
+    used = exact.half().double()
+    want = x.double() @ used
+    assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.isinf(), want.isinf()) and bool((y[want.isinf()] == want[want.isinf()]).all())
+    ok = want.isfinite().all(dim=0)
+    assert bool((~ok).any())
+    within(y[:, ok].contiguous(), want[:, ok], x.double().abs() @ used[:, ok].abs(), N)
