@@ -206,31 +206,34 @@ __global__ __launch_bounds__(kThreads) void dense_kernel(Sources two, CT *__rest
 // are then written in whole 128-byte lines.  The piece position is rotated by the thread's columns so that the eight lanes of a group
 // use different banks.
 template <typename S, typename CT>
-__global__ __launch_bounds__(kThreads) void dense_transposed_kernel(Sources two, CT *__restrict__ out, int64_t stride, int64_t second)
+__global__ __launch_bounds__(kThreads) void dense_transposed_kernel(Sources two, CT *__restrict__ out, int64_t pitch, int64_t stride, int64_t second)
 {
   const Source g = two.g[blockIdx.z];
   out += blockIdx.z * second;
   __shared__ __attribute__((aligned(16))) unsigned char tile[256 * 128];
   const int kl = threadIdx.x & 31, ng = threadIdx.x >> 5;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.y) * 64, k0 = static_cast<int64_t>(blockIdx.x) * 256;
-  Eight<uint16_t> e[8];
+  const int64_t k0 = static_cast<int64_t>(blockIdx.x) * 256;
+  for (int64_t n0 = static_cast<int64_t>(blockIdx.y) * 64; n0 < pitch; n0 += static_cast<int64_t>(gridDim.y) * 64) {
+    Eight<uint16_t> e[8];
 #pragma unroll
-  for (int r = 0; r < 8; ++r) e[r] = __builtin_bit_cast(Eight<uint16_t>, source8<S, CT>(g, n0 + 8 * ng + r, k0 + 8 * kl));
+    for (int r = 0; r < 8; ++r) e[r] = __builtin_bit_cast(Eight<uint16_t>, source8<S, CT>(g, n0 + 8 * ng + r, k0 + 8 * kl));
+    if (n0 >= static_cast<int64_t>(gridDim.y) * 64) __syncthreads();      // (the tile before this one has been read)
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    Eight<uint16_t> t;
+    for (int c = 0; c < 8; ++c) {
+      Eight<uint16_t> t;
 #pragma unroll
-    for (int r = 0; r < 8; ++r) t.v[r] = e[r].v[c];
-    *reinterpret_cast<u32x4_t *>(tile + (8 * kl + c) * 128 + (((ng + kl) & 7) << 4)) = __builtin_bit_cast(u32x4_t, t);
-  }
-  __syncthreads();
-  const int piece = threadIdx.x & 7;
+      for (int r = 0; r < 8; ++r) t.v[r] = e[r].v[c];
+      *reinterpret_cast<u32x4_t *>(tile + (8 * kl + c) * 128 + (((ng + kl) & 7) << 4)) = __builtin_bit_cast(u32x4_t, t);
+    }
+    __syncthreads();
+    const int piece = threadIdx.x & 7;
 #pragma unroll
-  for (int it = 0; it < 8; ++it) {
-    const int k = it * 32 + (threadIdx.x >> 3);
-    if (k0 + k >= g.cols) continue;
-    const u32x4_t v = *reinterpret_cast<const u32x4_t *>(tile + k * 128 + (((piece + (k >> 3)) & 7) << 4));
-    *reinterpret_cast<u32x4_t *>(out + (k0 + k) * stride + n0 + 8 * piece) = v;
+    for (int it = 0; it < 8; ++it) {
+      const int k = it * 32 + (threadIdx.x >> 3);
+      if (k0 + k >= g.cols) continue;
+      const u32x4_t v = *reinterpret_cast<const u32x4_t *>(tile + k * 128 + (((piece + (k >> 3)) & 7) << 4));
+      *reinterpret_cast<u32x4_t *>(out + (k0 + k) * stride + n0 + 8 * piece) = v;
+    }
   }
 }
 
@@ -343,8 +346,8 @@ int operand_dense(const Operand &a, int to, void *out, int64_t pitch, hipStream_
 
 int operand_transposed(const Operand &a, int to, void *out, int64_t pitch, int64_t stride, int64_t second, hipStream_t s)
 {
-  const dim3 grid(static_cast<unsigned>((a.cols + 255) / 256), static_cast<unsigned>(pitch / 64), static_cast<unsigned>(a.count));
-  CAIFX_BY_TARGET(hipLaunchKernelGGL((dense_transposed_kernel<S, CT>), grid, dim3(kThreads), 0, s, sources(a), static_cast<CT *>(out), stride, second))
+  const dim3 grid(static_cast<unsigned>((a.cols + 255) / 256), rows_grid(pitch / 64), static_cast<unsigned>(a.count));
+  CAIFX_BY_TARGET(hipLaunchKernelGGL((dense_transposed_kernel<S, CT>), grid, dim3(kThreads), 0, s, sources(a), static_cast<CT *>(out), pitch, stride, second))
   return launch_status();
 }
 
