@@ -52,10 +52,9 @@ inline RowsPlan rows_plan(int64_t M, int64_t N, int64_t R, int weights, int piec
   double best_us = 0;
   for (int splits = 1; splits <= 8; splits *= 2) {
     if (splits > 1 && (weights > 1 || units < 4 * splits || rows * splits > 256)) break;
-    int64_t rounds = (rows * splits + 255) / 256;
-    const auto parts = [&] { return 256 * rounds / (rows * splits); };      // of the columns
-    while ((N + parts() - 1) / parts() > most) ++rounds;
-    const int64_t span = (N + parts() - 1) / parts();
+    // rounds of workgroups, as few as leave the columns in parts of at most `most`
+    const int64_t least = (N + most - 1) / most, rounds = (least * rows * splits + 255) / 256;
+    const int64_t parts = 256 * rounds / (rows * splits), span = (N + parts - 1) / parts;
     const double us = rows_us(static_cast<double>(rows), static_cast<double>((N + span - 1) / span), static_cast<double>(span), splits, units, weight_row, x_tile,
                               static_cast<double>(M) * static_cast<double>(N));
     if (splits == 1 || us < best_us) {
