@@ -274,21 +274,18 @@ template <typename S, typename CT, int P>
 __global__ __launch_bounds__(kThreads) void pack_rows_kernel(Sources two, unsigned char *__restrict__ out, int own, int chunks)
 {
   const Source g = two.g[blockIdx.z];
-  const int c = static_cast<int>(blockIdx.x), chunk0 = static_cast<int>(blockIdx.z) * own;
+  const int c = static_cast<int>(blockIdx.x >> 1), chunk0 = static_cast<int>(blockIdx.z) * own;
   for (int64_t tile = blockIdx.y; tile * 16 < g.rows; tile += gridDim.y) {
     unsigned char *to = out + (tile * chunks + chunk0 + c) * (P * 8 * 1024);
+    const int at = static_cast<int>(blockIdx.x & 1) * kThreads + threadIdx.x, lane = at & 63, u = at >> 6;
+    const int64_t m = tile * 16 + (lane & 15), k = static_cast<int64_t>(c) * kRowsChunk + 32 * u + 8 * (lane >> 4);
+    if constexpr (P == 1) {
+      *reinterpret_cast<u32x4_t *>(to + at * 16) = source8<S, CT>(g, m, k);
+    } else {
+      Eight<uint16_t> piece[3];
+      pieces8<S>(g, m, k, piece);
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int at = half * kThreads + threadIdx.x, lane = at & 63, u = at >> 6;
-      const int64_t m = tile * 16 + (lane & 15), k = static_cast<int64_t>(c) * kRowsChunk + 32 * u + 8 * (lane >> 4);
-      if constexpr (P == 1) {
-        *reinterpret_cast<u32x4_t *>(to + at * 16) = source8<S, CT>(g, m, k);
-      } else {
-        Eight<uint16_t> piece[3];
-        pieces8<S>(g, m, k, piece);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4_t *>(to + p * 8192 + at * 16) = __builtin_bit_cast(u32x4_t, piece[p]);
-      }
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4_t *>(to + p * 8192 + at * 16) = __builtin_bit_cast(u32x4_t, piece[p]);
     }
   }
 }
@@ -362,7 +359,7 @@ int operand_pieces(const Operand &a, void *out, int64_t pitch, hipStream_t s)
 int operand_rows(const Operand &a, int to, void *out, int chunks, hipStream_t s)
 {
   const int own = static_cast<int>((a.cols + kRowsChunk - 1) / kRowsChunk);
-  const dim3 grid(static_cast<unsigned>(own), rows_grid((a.rows + 15) / 16), static_cast<unsigned>(a.count));
+  const dim3 grid(static_cast<unsigned>(2 * own), rows_grid((a.rows + 15) / 16), static_cast<unsigned>(a.count));
   unsigned char *o = static_cast<unsigned char *>(out);
   if (to == CAIFX_F32) {
     if (a.kind == CAIFX_F32) hipLaunchKernelGGL((pack_rows_kernel<float, bf16_t, 3>), grid, dim3(kThreads), 0, s, sources(a), o, own, chunks);
