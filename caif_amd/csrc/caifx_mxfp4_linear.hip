@@ -504,7 +504,7 @@ int gated_check(int64_t M, int64_t N, int64_t K, int w_kind, int dtype, bool &go
 {
   go = false;
   if (M < 0 || N <= 0 || K <= 0 || !valid_dtype(dtype)) return CAIFX_ERR_INVALID_ARGUMENT;
-  if (w_kind < CAIFX_W_INT8 || w_kind > CAIFX_W_MXFP4) return CAIFX_ERR_INVALID_ARGUMENT;
+  if (w_kind < CAIFX_W_INT8 || (w_kind > CAIFX_W_BF16 && w_kind != CAIFX_W_MXFP4)) return CAIFX_ERR_INVALID_ARGUMENT;
   const bool stored = (w_kind == CAIFX_W_F16 && dtype == CAIFX_F16) || (w_kind == CAIFX_W_BF16 && dtype == CAIFX_BF16);
   if ((w_kind != CAIFX_W_MXFP4 && !stored) || !fits(M, N, K)) return CAIFX_ERR_UNSUPPORTED;
   go = M > 0;

@@ -86,7 +86,7 @@ def test_gated_backward():
 
 @pytest.mark.parametrize("kind,dtype,status", [
     (T.W_INT8, T.BF16, UNSUPPORTED), (T.W_INT4_GROUP, T.F16, UNSUPPORTED), (T.W_F32, T.F32, UNSUPPORTED), (T.W_F16, T.BF16, UNSUPPORTED),
-    (T.W_BF16, T.F16, UNSUPPORTED), (T.W_BF16, T.F32, UNSUPPORTED), (6, T.BF16, INVALID), (-1, T.BF16, INVALID)])
+    (T.W_BF16, T.F16, UNSUPPORTED), (T.W_BF16, T.F32, UNSUPPORTED), (5, T.BF16, INVALID), (7, T.BF16, INVALID), (-1, T.BF16, INVALID)])
 def test_gated_kinds(kind, dtype, status):
     assert forward(kind=kind, dtype=dtype) == status and backward(kind=kind, dtype=dtype) == status
     assert capi.lib().caifx_gated_workspace_bytes(4, 8, 70, kind, dtype, 0) == 0
