@@ -16,17 +16,22 @@ constexpr int kBlock = CAIFX_MXFP4_BLOCK;
 constexpr int kPer = 8;                               // values of a lane
 constexpr int kLanes = kBlock / kPer;                 // lanes of a block
 constexpr int kThreads = 256;
-constexpr int kTurns = 4;                             // blocks of a lane, all asked for before the first is used
-constexpr int kUnits = kTurns * kThreads / kLanes;    // blocks of a workgroup
+constexpr int kUnits = kThreads / kLanes;             // blocks of a workgroup
 
 template <typename T> struct Eight { T v[kPer]; };
+// the same as whole 16-byte accesses at any address (as eight values the compiler may pull one out of them, two accesses then)
+template <typename T> struct Pieces {
+  typedef uint32_t piece_t __attribute__((ext_vector_type(4), aligned(2), may_alias));
+  piece_t p[sizeof(Eight<T>) / 16];
+};
 
 // eight values from p, `have` of them in the row (zeros for the others); any alignment of T
 template <typename T> __device__ __forceinline__ Eight<T> load8(const T *p, int have)
 {
   Eight<T> e;
   if (have >= kPer) {
-    __builtin_memcpy(&e, p, sizeof e);
+    const Pieces<T> pieces = *reinterpret_cast<const Pieces<T> *>(p);
+    __builtin_memcpy(&e, &pieces, sizeof e);
   } else {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) e.v[i] = i < have ? p[i] : T(0);
@@ -36,7 +41,9 @@ template <typename T> __device__ __forceinline__ Eight<T> load8(const T *p, int 
 template <typename T> __device__ __forceinline__ void store8(T *p, const Eight<T> &e, int have)
 {
   if (have >= kPer) {
-    __builtin_memcpy(p, &e, sizeof e);
+    Pieces<T> pieces;
+    __builtin_memcpy(&pieces, &e, sizeof e);
+    *reinterpret_cast<Pieces<T> *>(p) = pieces;
   } else {
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
@@ -54,9 +61,9 @@ struct Place {
   uint32_t unit;                                      // flat index of its block
   int have;                                           // values inside the row, 0 past the last block
 };
-template <bool kWhole> __device__ __forceinline__ Place place(const Shape &s, int turn)
+template <bool kWhole> __device__ __forceinline__ Place place(const Shape &s)
 {
-  const uint32_t unit = (blockIdx.x * kTurns + turn) * (kThreads / kLanes) + threadIdx.x / kLanes, in = (threadIdx.x % kLanes) * kPer;
+  const uint32_t unit = blockIdx.x * kUnits + threadIdx.x / kLanes, in = (threadIdx.x % kLanes) * kPer;
   if constexpr (kWhole) {
     return {static_cast<int64_t>(unit) * kBlock + in, unit, unit < s.units ? kPer : 0};
   } else {
@@ -67,42 +74,36 @@ template <bool kWhole> __device__ __forceinline__ Place place(const Shape &s, in
   }
 }
 
+// (One block for four lanes: four of them, asked for together, are slower at every size, bf16, 28672 x 8192 115 us instead of 105, 512 x 4096 3.9
+// instead of 3.1.)
 template <typename T, bool kWhole>
 __global__ __launch_bounds__(kThreads) void quantize_kernel(const T *__restrict__ x, uint32_t *__restrict__ codes, uint8_t *__restrict__ scales, Shape s)
 {
-  Place p[kTurns];
-  Eight<T> v[kTurns];
+  const Place p = place<kWhole>(s);
+  const Eight<T> v = load8(x + p.at, p.have);
+  float f[kPer];
+  uint32_t top = 0;
 #pragma unroll
-  for (int k = 0; k < kTurns; ++k) {
-    p[k] = place<kWhole>(s, k);
-    v[k] = load8(x + p[k].at, p[k].have);
+  for (int i = 0; i < kPer; ++i) {
+    f[i] = to_f32<T>(v.v[i]);
+    const uint32_t b = __builtin_bit_cast(uint32_t, f[i]) & 0x7FFFFFFFu;      // magnitudes in the order of their bits
+    top = top > b ? top : b;
   }
-#pragma unroll
-  for (int k = 0; k < kTurns; ++k) {
-    float f[kPer];
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      f[i] = to_f32<T>(v[k].v[i]);
-      const uint32_t b = __builtin_bit_cast(uint32_t, f[i]) & 0x7FFFFFFFu;      // magnitudes in the order of their bits
-      top = top > b ? top : b;
-    }
-    auto with = [&](uint32_t w) { top = top > w ? top : w; };
-    with(__builtin_amdgcn_mov_dpp(top, 0xB1, 0xF, 0xF, true));            // lanes 1 0 3 2
-    with(__builtin_amdgcn_mov_dpp(top, 0x4E, 0xF, 0xF, true));            // lanes 2 3 0 1
-    const uint32_t exponent = top >> 23;
-    const bool finite = exponent < 255;
-    const uint32_t byte = finite ? (exponent > 2 ? exponent - 2 : 0) : 255;
-    const float scale = mxfp4_scale(byte);
-    uint32_t c = 0;
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[0], f[1], scale, 0);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[2], f[3], scale, 1);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[4], f[5], scale, 2);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[6], f[7], scale, 3);
-    if (p[k].unit < s.units) {
-      codes[static_cast<int64_t>(p[k].unit) * kLanes + threadIdx.x % kLanes] = finite ? c : 0u;
-      if (threadIdx.x % kLanes == 0) scales[p[k].unit] = static_cast<uint8_t>(byte);
-    }
+  auto with = [&](uint32_t w) { top = top > w ? top : w; };
+  with(__builtin_amdgcn_mov_dpp(top, 0xB1, 0xF, 0xF, true));            // lanes 1 0 3 2
+  with(__builtin_amdgcn_mov_dpp(top, 0x4E, 0xF, 0xF, true));            // lanes 2 3 0 1
+  const uint32_t exponent = top >> 23;
+  const bool finite = exponent < 255;
+  const uint32_t byte = finite ? (exponent > 2 ? exponent - 2 : 0) : 255;
+  const float scale = mxfp4_scale(byte);
+  uint32_t c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[0], f[1], scale, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[2], f[3], scale, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[4], f[5], scale, 2);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[6], f[7], scale, 3);
+  if (p.unit < s.units) {
+    codes[static_cast<int64_t>(p.unit) * kLanes + threadIdx.x % kLanes] = finite ? c : 0u;
+    if (threadIdx.x % kLanes == 0) scales[p.unit] = static_cast<uint8_t>(byte);
   }
 }
 
@@ -125,16 +126,10 @@ template <typename T> __device__ __forceinline__ Eight<T> values8(uint32_t codes
 template <typename T, bool kWhole>
 __global__ __launch_bounds__(kThreads) void dequantize_kernel(const uint32_t *__restrict__ codes, const uint8_t *__restrict__ scales, T *__restrict__ out, Shape s)
 {
-  Place p[kTurns];
-  uint32_t c[kTurns], byte[kTurns];
-#pragma unroll
-  for (int k = 0; k < kTurns; ++k) {
-    p[k] = place<kWhole>(s, k);
-    c[k] = p[k].have > 0 ? codes[static_cast<int64_t>(p[k].unit) * kLanes + threadIdx.x % kLanes] : 0u;
-    byte[k] = p[k].have > 0 ? scales[p[k].unit] : 0u;
-  }
-#pragma unroll
-  for (int k = 0; k < kTurns; ++k) store8(out + p[k].at, values8<T>(c[k], mxfp4_scale(byte[k])), p[k].have);
+  const Place p = place<kWhole>(s);
+  const uint32_t unit = p.unit < s.units ? p.unit : s.units - 1;      // (nothing of it is stored)
+  const uint32_t c = codes[static_cast<int64_t>(unit) * kLanes + threadIdx.x % kLanes], byte = scales[unit];
+  store8(out + p.at, values8<T>(c, mxfp4_scale(byte)), p.have);
 }
 
 // ------------------------------------------------------------------ operands laid out for the products
@@ -184,21 +179,11 @@ template <typename S, typename CT> __device__ __forceinline__ u32x4_t source8(co
 template <typename S, typename CT>
 __global__ __launch_bounds__(kThreads) void dense_kernel(Sources two, CT *__restrict__ out, int64_t pitch)
 {
-  constexpr int kRounds = 4;
   const Source g = two.g[blockIdx.z];
   out += blockIdx.z * g.rows * pitch;
-  const int64_t pieces = pitch / kPer;
-  for (int64_t n = blockIdx.y; n < g.rows; n += gridDim.y) {
-    const int64_t p0 = static_cast<int64_t>(blockIdx.x) * (kThreads * kRounds) + threadIdx.x;
-    u32x4_t v[kRounds];
-#pragma unroll
-    for (int r = 0; r < kRounds; ++r) v[r] = source8<S, CT>(g, n, (p0 + r * kThreads) * kPer);
-#pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      const int64_t p = p0 + r * kThreads;
-      if (p < pieces) *reinterpret_cast<u32x4_t *>(out + n * pitch + p * kPer) = v[r];
-    }
-  }
+  const int64_t p = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (p * kPer >= pitch) return;
+  for (int64_t n = blockIdx.y; n < g.rows; n += gridDim.y) *reinterpret_cast<u32x4_t *>(out + n * pitch + p * kPer) = source8<S, CT>(g, n, p * kPer);
 }
 
 // the same transposed: [cols] rows `stride` long with the rows' values, zeros up to a multiple of 64; the second source's `second` values on.
@@ -206,34 +191,31 @@ __global__ __launch_bounds__(kThreads) void dense_kernel(Sources two, CT *__rest
 // are then written in whole 128-byte lines.  The piece position is rotated by the thread's columns so that the eight lanes of a group
 // use different banks.
 template <typename S, typename CT>
-__global__ __launch_bounds__(kThreads) void dense_transposed_kernel(Sources two, CT *__restrict__ out, int64_t pitch, int64_t stride, int64_t second)
+__global__ __launch_bounds__(kThreads) void dense_transposed_kernel(Sources two, CT *__restrict__ out, int64_t stride, int64_t second)
 {
   const Source g = two.g[blockIdx.z];
   out += blockIdx.z * second;
   __shared__ __attribute__((aligned(16))) unsigned char tile[256 * 128];
   const int kl = threadIdx.x & 31, ng = threadIdx.x >> 5;
-  const int64_t k0 = static_cast<int64_t>(blockIdx.x) * 256;
-  for (int64_t n0 = static_cast<int64_t>(blockIdx.y) * 64; n0 < pitch; n0 += static_cast<int64_t>(gridDim.y) * 64) {
-    Eight<uint16_t> e[8];
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 64, k0 = static_cast<int64_t>(blockIdx.y) * 256;
+  Eight<uint16_t> e[8];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) e[r] = __builtin_bit_cast(Eight<uint16_t>, source8<S, CT>(g, n0 + 8 * ng + r, k0 + 8 * kl));
-    if (n0 >= static_cast<int64_t>(gridDim.y) * 64) __syncthreads();      // (the tile before this one has been read)
+  for (int r = 0; r < 8; ++r) e[r] = __builtin_bit_cast(Eight<uint16_t>, source8<S, CT>(g, n0 + 8 * ng + r, k0 + 8 * kl));
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      Eight<uint16_t> t;
+  for (int c = 0; c < 8; ++c) {
+    Eight<uint16_t> t;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) t.v[r] = e[r].v[c];
-      *reinterpret_cast<u32x4_t *>(tile + (8 * kl + c) * 128 + (((ng + kl) & 7) << 4)) = __builtin_bit_cast(u32x4_t, t);
-    }
-    __syncthreads();
-    const int piece = threadIdx.x & 7;
+    for (int r = 0; r < 8; ++r) t.v[r] = e[r].v[c];
+    *reinterpret_cast<u32x4_t *>(tile + (8 * kl + c) * 128 + (((ng + kl) & 7) << 4)) = __builtin_bit_cast(u32x4_t, t);
+  }
+  __syncthreads();
+  const int piece = threadIdx.x & 7;
 #pragma unroll
-    for (int it = 0; it < 8; ++it) {
-      const int k = it * 32 + (threadIdx.x >> 3);
-      if (k0 + k >= g.cols) continue;
-      const u32x4_t v = *reinterpret_cast<const u32x4_t *>(tile + k * 128 + (((piece + (k >> 3)) & 7) << 4));
-      *reinterpret_cast<u32x4_t *>(out + (k0 + k) * stride + n0 + 8 * piece) = v;
-    }
+  for (int it = 0; it < 8; ++it) {
+    const int k = it * 32 + (threadIdx.x >> 3);
+    if (k0 + k >= g.cols) continue;
+    const u32x4_t v = *reinterpret_cast<const u32x4_t *>(tile + k * 128 + (((piece + (k >> 3)) & 7) << 4));
+    *reinterpret_cast<u32x4_t *>(out + (k0 + k) * stride + n0 + 8 * piece) = v;
   }
 }
 
@@ -336,15 +318,15 @@ unsigned rows_grid(int64_t rows) { return static_cast<unsigned>(rows < 65535 ? r
 
 int operand_dense(const Operand &a, int to, void *out, int64_t pitch, hipStream_t s)
 {
-  const dim3 grid(static_cast<unsigned>((pitch / kPer + 1023) / 1024), rows_grid(a.rows), static_cast<unsigned>(a.count));
+  const dim3 grid(static_cast<unsigned>((pitch / kPer + kThreads - 1) / kThreads), rows_grid(a.rows), static_cast<unsigned>(a.count));
   CAIFX_BY_TARGET(hipLaunchKernelGGL((dense_kernel<S, CT>), grid, dim3(kThreads), 0, s, sources(a), static_cast<CT *>(out), pitch))
   return launch_status();
 }
 
 int operand_transposed(const Operand &a, int to, void *out, int64_t pitch, int64_t stride, int64_t second, hipStream_t s)
 {
-  const dim3 grid(static_cast<unsigned>((a.cols + 255) / 256), rows_grid(pitch / 64), static_cast<unsigned>(a.count));
-  CAIFX_BY_TARGET(hipLaunchKernelGGL((dense_transposed_kernel<S, CT>), grid, dim3(kThreads), 0, s, sources(a), static_cast<CT *>(out), pitch, stride, second))
+  const dim3 grid(static_cast<unsigned>(pitch / 64), static_cast<unsigned>((a.cols + 255) / 256), static_cast<unsigned>(a.count));
+  CAIFX_BY_TARGET(hipLaunchKernelGGL((dense_transposed_kernel<S, CT>), grid, dim3(kThreads), 0, s, sources(a), static_cast<CT *>(out), stride, second))
   return launch_status();
 }
 
