@@ -143,11 +143,12 @@ struct Sources {             // one or two of one shape, a launch's last extent
   Source g[2];
 };
 
-// eight values (n, k .. k + 7) of a source in CT, zeros outside; k is a multiple of 8
-template <typename S, typename CT> __device__ __forceinline__ u32x4_t source8(const Source &g, int64_t n, int64_t k)
+// eight values (n, k .. k + 7) of a source in CT, zeros outside; k is a multiple of 8.  kInside: all eight are inside, nothing is tested (behind
+// a test the compiler waits for one access before it asks for the next).
+template <typename S, typename CT, bool kInside = false> __device__ __forceinline__ u32x4_t source8(const Source &g, int64_t n, int64_t k)
 {
-  if (n >= g.rows || k >= g.cols) return u32x4_t{0, 0, 0, 0};
-  const int64_t left = g.cols - k;
+  if (!kInside && (n >= g.rows || k >= g.cols)) return u32x4_t{0, 0, 0, 0};
+  const int64_t left = kInside ? kPer : g.cols - k;
   if constexpr (sizeof(S) == 1) {
     const int64_t block = n * g.blocks + (k >> 5);
     uint32_t c = *reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(g.p) + block * 16 + ((k & 31) >> 1));
@@ -199,8 +200,13 @@ __global__ __launch_bounds__(kThreads) void dense_transposed_kernel(Sources two,
   const int kl = threadIdx.x & 31, ng = threadIdx.x >> 5;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 64, k0 = static_cast<int64_t>(blockIdx.y) * 256;
   Eight<uint16_t> e[8];
+  if (n0 + 64 <= g.rows && k0 + 256 <= g.cols) {
 #pragma unroll
-  for (int r = 0; r < 8; ++r) e[r] = __builtin_bit_cast(Eight<uint16_t>, source8<S, CT>(g, n0 + 8 * ng + r, k0 + 8 * kl));
+    for (int r = 0; r < 8; ++r) e[r] = __builtin_bit_cast(Eight<uint16_t>, source8<S, CT, true>(g, n0 + 8 * ng + r, k0 + 8 * kl));
+  } else {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) e[r] = __builtin_bit_cast(Eight<uint16_t>, source8<S, CT>(g, n0 + 8 * ng + r, k0 + 8 * kl));
+  }
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
     Eight<uint16_t> t;
