@@ -9,7 +9,7 @@
 // and read again, 4 bytes for half a byte of codes.
 // A workgroup of eight waves owns 256 columns, its waves take steps in turn and meet in LDS; workgroups share a reduction, as many as the
 // chip has room for, and a second launch adds their sums in a fixed order.
-// N = 14336, K = 4096, bf16, 16 rows: 16 us (the weight's bytes alone 6.3), behind a transposed copy 70; 512 rows 110 us, 546 TFLOP/s, and 126.
+// N = 14336, K = 4096, bf16, 16 rows: 16 us (the weight's bytes alone 6.3), behind a transposed copy 57; 256 rows 66 us, 456 TFLOP/s, and 79.
 #include "caifx_mxfp4.hpp"
 
 #include <type_traits>

@@ -268,26 +268,14 @@ struct Gradient {
   const void *addend;
 };
 
-double gradient_rows_us(const Gradient &p)      // an estimate, behind the copies
-{
-  const double flops = 2.0 * p.weights * static_cast<double>(p.M) * static_cast<double>(p.N) * static_cast<double>(p.K);
-  return 8.0 + flops / (pieces_of(p.compute_dtype) == 3 ? 100e6 : 480e6);
-}
-
-// Whether a gradient runs on the dense product behind the transposed copies.
-bool wide_gradient_pays(const Gradient &p)
-{
-  const int64_t R = up_to(p.N, 64) < 128 ? 128 : up_to(p.N, 64);
-  const int pieces = pieces_of(p.compute_dtype);
-  if (p.M <= 32 || !wide_takes(p.M, p.K, R)) return false;
-  // (both behind the same copies.  us, rows / dense: 4096 x 14336, 64 rows 76 / 72, 96 rows 99 / 72; 14336 x 4096, 128 rows 93 / 123, 256 rows 123 / 124)
-  return wide_parts(p.M, p.K, p.weights * pieces * R).us + (pieces == 3 ? 15.0 : 0.0) < gradient_rows_us(p);
-}
+int64_t reduction_of(const Gradient &p) { return up_to(p.N, 64) < 128 ? 128 : up_to(p.N, 64); }
+// Whether a gradient can run on the dense product behind the transposed copies.
+bool wide_gradient_takes(const Gradient &p) { return p.M > 32 && wide_takes(p.M, p.K, reduction_of(p)); }
 
 int gradient_wide(const Gradient &p, Room &room, bool only_size, hipStream_t s)
 {
   const int to = stored_as(p.compute_dtype), pieces = pieces_of(p.compute_dtype);
-  const int64_t R = up_to(p.N, 64) < 128 ? 128 : up_to(p.N, 64);
+  const int64_t R = reduction_of(p);
   int st = CAIFX_OK;
   WideProduct d{};
   d.pairs = p.weights * pieces;
@@ -316,6 +304,7 @@ int gradient_wide(const Gradient &p, Room &room, bool only_size, hipStream_t s)
   return st != CAIFX_OK ? st : wide_run(d, room, only_size, s);
 }
 
+// The row kernels on the transposed copies: what neither of the others takes, activations at addresses that the dense product does not.
 int gradient_rows(const Gradient &p, Room &room, bool only_size, hipStream_t s)
 {
   const int to = stored_as(p.compute_dtype);
@@ -364,19 +353,19 @@ DxProduct dx_of(const Gradient &p, bool direct)
   d.addend = p.addend;
   return d;
 }
-// The stored weights are turned around for every 32 rows again, the copies once: few rows run on dx, many on the copies.  Estimates in us, of
-// the copies with a dense product or the row kernels, and of dx.  Measured, copies / dx: N = 14336, K = 4096, bf16, 16 rows 70 / 16, 128 rows
-// 92 / 38, 512 rows 126 / 110, 768 rows 131 / 188; N = 4096, K = 14336, 256 rows 74 / 65, 384 rows 92 / 94; N = K = 4096, 512 rows 40 / 35, in fp32
-// 89 / 71, a gated block's gradient 80 / 76, of stored weights 82 / 83; 2048 x 1408, 512 rows 22 / 20.
+// The stored weights are turned around for every 32 rows again, the copies once: few rows run on dx, many on the copies.  Estimates in us of
+// both.  Measured, copies / dx: N = 14336, K = 4096, bf16, 16 rows 57 / 16, 128 rows
+// 61 / 39, 256 rows 79 / 66, 512 rows 96 / 116; N = 4096, K = 14336, 256 rows 66 / 73; N = K = 4096, 512 rows 38 / 36, in fp32 76 / 65, a gated block's
+// gradient 69 / 78; 2048 x 1408, 512 rows 21 / 19.
 bool dx_pays(const Gradient &p)
 {
   if (!dx_takes(dx_of(p, false))) return false;
-  const int64_t R = up_to(p.N, 64) < 128 ? 128 : up_to(p.N, 64);
+  if (!wide_gradient_takes(p)) return true;
   const int pieces = pieces_of(p.compute_dtype);
   const double values = p.weights * static_cast<double>(p.N) * static_cast<double>(p.K);
   const double far = values > 64e6 ? (values - 64e6) * 0.5e-6 : 0.0;      // (copies of more than half of the memory-side cache are read from further away)
-  const double product = wide_gradient_pays(p) ? wide_parts(p.M, p.K, p.weights * pieces * R).us + (pieces == 3 ? 15.0 : 0.0) : gradient_rows_us(p);
-  return dx_us(dx_of(p, p.N % 8 == 0)) < product + 12.0 + values * (p.w[0].mx ? 2.53 : 4.0) / 4.4e6 + far + (pieces == 3 ? 4.0 : 0.0);
+  const double copies = 4.0 + values * (p.w[0].mx ? 2.53 : 4.0) / 4.4e6 + far + (pieces == 3 ? 19.0 : 0.0);
+  return dx_us(dx_of(p, p.N % 8 == 0)) < copies + wide_parts(p.M, p.K, p.weights * pieces * reduction_of(p)).us;
 }
 int gradient_dx(const Gradient &p, Room &room, bool only_size, hipStream_t s)
 {
@@ -403,7 +392,7 @@ size_t gradient_bytes(const Gradient &p)
     return dx.used;
   }
   gradient_rows(p, rows, true, nullptr);
-  if (!wide_gradient_pays(p)) return rows.used;
+  if (!wide_gradient_takes(p)) return rows.used;
   gradient_wide(p, wide, true, nullptr);
   return rows.used > wide.used ? rows.used : wide.used;
 }
@@ -411,7 +400,7 @@ int gradient(const Gradient &p, void *workspace, hipStream_t s)
 {
   Room room{static_cast<char *>(workspace), 0};
   if (dx_pays(p)) return gradient_dx(p, room, false, s);
-  if (wide_gradient_pays(p) && aligned_to(p.x[0], 16) && aligned_to(p.x[1], 16)) return gradient_wide(p, room, false, s);
+  if (wide_gradient_takes(p) && aligned_to(p.x[0], 16) && aligned_to(p.x[1], 16)) return gradient_wide(p, room, false, s);
   return gradient_rows(p, room, false, s);
 }
 
