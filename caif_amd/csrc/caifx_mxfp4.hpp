@@ -32,7 +32,7 @@ struct DxProduct {
   int count;
   const void *w[2], *s[2];
   bool mx;
-  const void *x[2];          // direct: [M, N] of the compute type, N a multiple of 8, aligned to 16 bytes; otherwise x[0] packed by operand_rows
+  const void *x[2];          // direct: [M, N] of the compute type (fp32 too), N a multiple of 8, aligned to 16 bytes; otherwise x[0] packed by operand_rows
   bool direct;
   int compute_dtype;         // CAIFX_F32: three bf16 pieces (mx only)
   void *y;
@@ -40,6 +40,7 @@ struct DxProduct {
   const void *addend;
 };
 bool dx_takes(const DxProduct &p);
+bool dx_reads(const DxProduct &p);      // whether activations that can be direct should be
 double dx_us(const DxProduct &p);      // an estimate
 size_t dx_partial_bytes(const DxProduct &p);
 int dx_product(const DxProduct &p, void *partial, hipStream_t s);

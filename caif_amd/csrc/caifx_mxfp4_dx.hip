@@ -23,7 +23,7 @@ constexpr int kWaves = 8;
 
 struct DxArgs {
   const uint8_t *w[2], *s[2];       // one or two weights of N rows, `pitch` bytes long
-  const uint8_t *x[2];              // direct: [M, N] of the compute type; packed: x[0], see pack_rows_kernel, the second's chunks behind the first's
+  const uint8_t *x[2];              // direct: [M, N] of the compute type (P = 3: fp32); packed: x[0], see pack_rows_kernel, the second's chunks behind the first's
   int64_t M, N, K, blocks, pitch;
   int count, steps;                 // weights; steps of 32 rows of one weight
   int chunks, tiles;                // packed: chunks in all, row tiles of 16
@@ -51,10 +51,11 @@ __global__ __launch_bounds__(kWaves * 64) void dx_kernel(DxArgs g)
   };
   const int64_t column = first_column(j);
 
+  constexpr int XW = kDirect && P == 3 ? 2 : P;      // loads of eight activations: direct fp32 ones are taken apart once they are used
   struct Step {
     u32x4_t w[8][kMx ? 1 : 2];        // (codes: half of it)
     uint32_t scale[8];
-    u32x4_t x[MT][P];
+    u32x4_t x[MT][XW];
   };
   auto load = [&](Step &b, int step) __attribute__((always_inline)) {
     const int second = step >= g.steps ? 1 : 0, at = step - second * g.steps;
@@ -85,8 +86,12 @@ __global__ __launch_bounds__(kWaves * 64) void dx_kernel(DxArgs g)
       for (int t = 0; t < MT; ++t) {
         int64_t m = m0 + 16 * t + j;
         m = m < g.M ? m : g.M - 1;
-        b.x[t][0] = *reinterpret_cast<const u32x4_t *>(x + (m * g.N + (in ? n : 0)) * 2);
-        if (!in) b.x[t][0] = u32x4_t{0, 0, 0, 0};
+        const uint8_t *from = x + (m * g.N + (in ? n : 0)) * (2 * XW);
+#pragma unroll
+        for (int i = 0; i < XW; ++i) {
+          b.x[t][i] = *reinterpret_cast<const u32x4_t *>(from + 16 * i);
+          if (!in) b.x[t][i] = u32x4_t{0, 0, 0, 0};
+        }
       }
     } else {
       // steps of a weight fill whole chunks of eight in the packed order
@@ -115,6 +120,24 @@ __global__ __launch_bounds__(kWaves * 64) void dx_kernel(DxArgs g)
       for (int i = 0; i < 8; ++i)
         if (n + 8 * q + i >= g.N) b.w[i][0] = b.w[i][kMx ? 0 : 1] = u32x4_t{0, 0, 0, 0};
     }
+    u32x4_t x[MT][P];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      if constexpr (kDirect && P == 3) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const floatx4_t four = __builtin_bit_cast(floatx4_t, b.x[t][i >> 1]);
+          uint32_t even[3], odd[3];
+          pieces_of_f32(four[2 * (i & 1)], even);
+          pieces_of_f32(four[2 * (i & 1) + 1], odd);
+#pragma unroll
+          for (int p = 0; p < 3; ++p) x[t][p][i] = __builtin_amdgcn_perm(odd[p], even[p], 0x07060302u);
+        }
+      } else {
+#pragma unroll
+        for (int p = 0; p < P; ++p) x[t][p] = b.x[t][p];
+      }
+    }
     // eight columns at a time
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -132,7 +155,7 @@ __global__ __launch_bounds__(kWaves * 64) void dx_kernel(DxArgs g)
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
-          for (int p = 0; p < P; ++p) acc[t][half * 8 + c] = Mfma16<CT>::run(b.x[t][p], w, acc[t][half * 8 + c]);
+          for (int p = 0; p < P; ++p) acc[t][half * 8 + c] = Mfma16<CT>::run(x[t][p], w, acc[t][half * 8 + c]);
       }
     }
   };
@@ -222,12 +245,10 @@ template <typename CT, int P, bool kMx> int launch(const DxArgs &g, bool direct,
   };
   const std::integral_constant<int, 1> one;
   const std::integral_constant<int, 2> two;
-  if constexpr (P == 1) {
-    if (direct) {
-      if (tile == 16) go(one, std::true_type{});
-      else go(two, std::true_type{});
-      return launch_status();
-    }
+  if (direct) {
+    if (tile == 16) go(one, std::true_type{});
+    else go(two, std::true_type{});
+    return launch_status();
   }
   if (tile == 16) go(one, std::false_type{});
   else go(two, std::false_type{});
@@ -242,14 +263,27 @@ bool dx_takes(const DxProduct &p)
   return p.M <= 1024 && (p.mx || p.K >= kSets);
 }
 
+// steps that a wave of the last workgroup has taken
+static int64_t turns_of(const DxProduct &p)
+{
+  const int splits = splits_of(p);
+  const int64_t others = (p.K + kColumns - 1) / kColumns * ((p.M + tile_of(p.M) - 1) / tile_of(p.M));
+  return (others * splits + 255) / 256 * ((p.count * ((p.N + 31) / 32) + kWaves * splits - 1) / (kWaves * splits));
+}
+
+bool dx_reads(const DxProduct &p)
+{
+  // fp32, us, packed / direct: one step N = 2048, K = 1403, 64 rows 17.2 / 14.7, three 333 rows 24.3 / 22.2, four N = K = 4096, 128 rows 26.6 / 26.6, seven
+  // N = 14336, K = 4096, 64 rows 37.2 / 38.7; 16 rows 21.1 / 18.2
+  return p.compute_dtype != CAIFX_F32 || p.M <= 16 || turns_of(p) <= 4;
+}
+
 double dx_us(const DxProduct &p)
 {
-  const int splits = splits_of(p), pieces = p.compute_dtype == CAIFX_F32 ? 3 : 1;
-  const int64_t others = (p.K + kColumns - 1) / kColumns * ((p.M + tile_of(p.M) - 1) / tile_of(p.M));
-  const int64_t rounds = (others * splits + 255) / 256, steps = (p.count * ((p.N + 31) / 32) + kWaves * splits - 1) / (kWaves * splits);
-  const double step = (pieces == 3 ? 3.4 : 1.85) * (p.mx ? 1.0 : 1.2);
+  const int splits = splits_of(p);
+  const double step = (p.compute_dtype == CAIFX_F32 ? 3.4 : 1.85) * (p.mx ? 1.0 : 1.2);
   const double join = splits > 1 ? 3.0 + 8e-7 * static_cast<double>(splits) * static_cast<double>(p.M) * static_cast<double>(p.K) : 0.0;
-  return 5.0 + (p.direct && pieces == 1 ? 0.0 : 3.0) + join + step * static_cast<double>(rounds * steps);
+  return 5.0 + (p.direct ? 0.0 : 3.0) + join + step * static_cast<double>(turns_of(p));
 }
 
 size_t dx_partial_bytes(const DxProduct &p)
@@ -280,7 +314,7 @@ int dx_product(const DxProduct &p, void *partial, hipStream_t s)
   g.y_dtype = g.splits > 1 ? static_cast<int>(CAIFX_F32) : p.y_dtype;
   g.addend = g.splits > 1 ? nullptr : p.addend;
   int st;
-  if (p.compute_dtype == CAIFX_F32) st = launch<bf16_t, 3, true>(g, false, s);
+  if (p.compute_dtype == CAIFX_F32) st = launch<bf16_t, 3, true>(g, p.direct, s);
   else if (p.compute_dtype == CAIFX_F16) st = p.mx ? launch<f16_t, 1, true>(g, p.direct, s) : launch<f16_t, 1, false>(g, p.direct, s);
   else st = p.mx ? launch<bf16_t, 1, true>(g, p.direct, s) : launch<bf16_t, 1, false>(g, p.direct, s);
   if (st != CAIFX_OK || g.splits == 1) return st;

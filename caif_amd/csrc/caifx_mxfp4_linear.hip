@@ -249,11 +249,17 @@ size_t product_bytes(const Product &p, bool dense_copy = true)
   product_wide(p, wide, true, nullptr);
   return rows.used > wide.used ? rows.used : wide.used;
 }
+// One way of a product, in room that is checked first to hold what it takes at these addresses
+template <typename P> int run_in(int (*way)(const P &, Room &, bool, hipStream_t), const P &p, void *workspace, size_t bytes, hipStream_t s)
+{
+  Room need, room{static_cast<char *>(workspace), 0};
+  way(p, need, true, nullptr);
+  return need.used > bytes ? static_cast<int>(CAIFX_ERR_WORKSPACE_TOO_SMALL) : way(p, room, false, s);
+}
 int product(const Product &p, void *workspace, size_t bytes, hipStream_t s)
 {
-  Room room{static_cast<char *>(workspace), 0};
-  if (wide_product_pays(p) && bytes >= product_bytes(p) && aligned_to(p.x, 16)) return product_wide(p, room, false, s);
-  return product_rows(p, room, false, s);
+  const bool wide = wide_product_pays(p) && bytes >= product_bytes(p) && aligned_to(p.x, 16);
+  return run_in(wide ? product_wide : product_rows, p, workspace, bytes, s);
 }
 
 // y[M,K] = sum over the weights of x[i][M,N] w[i][N,K], as one reduction over their rows
@@ -333,7 +339,7 @@ int gradient_rows(const Gradient &p, Room &room, bool only_size, hipStream_t s)
 }
 
 // The gradient from the weights as they are stored.
-DxProduct dx_of(const Gradient &p, bool direct)
+DxProduct dx_of(const Gradient &p, bool aligned)
 {
   DxProduct d{};
   d.M = p.M;
@@ -346,33 +352,35 @@ DxProduct dx_of(const Gradient &p, bool direct)
     d.x[i] = p.x[i];
   }
   d.mx = p.w[0].mx;
-  d.direct = direct;
   d.compute_dtype = p.compute_dtype;
   d.y = p.y;
   d.y_dtype = p.y_dtype;
   d.addend = p.addend;
+  d.direct = p.x_dtype == p.compute_dtype && p.N % 8 == 0 && aligned && dx_reads(d);
   return d;
 }
+
 // The stored weights are turned around for every 32 rows again, the copies once: few rows run on dx, many on the copies.  Estimates in us of
-// both.  Measured, copies / dx: N = 14336, K = 4096, bf16, 16 rows 57 / 16, 128 rows
-// 61 / 39, 256 rows 79 / 66, 512 rows 96 / 116; N = 4096, K = 14336, 256 rows 66 / 73; N = K = 4096, 512 rows 38 / 36, in fp32 76 / 65, a gated block's
+// both.  Measured, copies / dx: N = 14336, K = 4096, bf16, 16 rows 57 / 16, 128 rows 61 / 39, 256 rows 79 / 66, 512 rows 96 / 116; N = 4096, K = 14336, 256 rows 66 / 73; N = K = 4096, 512 rows 38 / 36, in fp32 76 / 65, a gated block's
 // gradient 69 / 78; 2048 x 1408, 512 rows 21 / 19.
 bool dx_pays(const Gradient &p)
 {
-  if (!dx_takes(dx_of(p, false))) return false;
+  // (chosen by sizes and types alone, as a query has no more: the other way may need another amount of room)
+  const DxProduct d = dx_of(p, true);
+  if (!dx_takes(d)) return false;
   if (!wide_gradient_takes(p)) return true;
   const int pieces = pieces_of(p.compute_dtype);
   const double values = p.weights * static_cast<double>(p.N) * static_cast<double>(p.K);
   const double far = values > 64e6 ? (values - 64e6) * 0.5e-6 : 0.0;      // (copies of more than half of the memory-side cache are read from further away)
   const double copies = 4.0 + values * (p.w[0].mx ? 2.53 : 4.0) / 4.4e6 + far + (pieces == 3 ? 19.0 : 0.0);
-  return dx_us(dx_of(p, p.N % 8 == 0)) < copies + wide_parts(p.M, p.K, p.weights * pieces * reduction_of(p)).us;
+  return dx_us(d) < copies + wide_parts(p.M, p.K, p.weights * pieces * reduction_of(p)).us;
 }
+
 int gradient_dx(const Gradient &p, Room &room, bool only_size, hipStream_t s)
 {
-  const bool direct = p.compute_dtype != CAIFX_F32 && p.x_dtype == p.compute_dtype && p.N % 8 == 0 && aligned_to(p.x[0], 16) && aligned_to(p.x[1], 16) && !only_size;
-  DxProduct d = dx_of(p, direct);
+  DxProduct d = dx_of(p, aligned_to(p.x[0], 16) && aligned_to(p.x[1], 16));
   void *partial = room.take(dx_partial_bytes(d));
-  if (!direct) {
+  if (only_size || !d.direct) {
     // (counted in any case: the query does not know the activations' addresses)
     const int chunks = p.weights * static_cast<int>(chunks_of(p.N));
     void *packed = room.take(packed_bytes(p.M, chunks, p.compute_dtype));
@@ -396,12 +404,10 @@ size_t gradient_bytes(const Gradient &p)
   gradient_wide(p, wide, true, nullptr);
   return rows.used > wide.used ? rows.used : wide.used;
 }
-int gradient(const Gradient &p, void *workspace, hipStream_t s)
+int gradient(const Gradient &p, void *workspace, size_t bytes, hipStream_t s)
 {
-  Room room{static_cast<char *>(workspace), 0};
-  if (dx_pays(p)) return gradient_dx(p, room, false, s);
-  if (wide_gradient_takes(p) && aligned_to(p.x[0], 16) && aligned_to(p.x[1], 16)) return gradient_wide(p, room, false, s);
-  return gradient_rows(p, room, false, s);
+  const bool wide = wide_gradient_takes(p) && aligned_to(p.x[0], 16) && aligned_to(p.x[1], 16);
+  return run_in(dx_pays(p) ? gradient_dx : wide ? gradient_wide : gradient_rows, p, workspace, bytes, s);
 }
 
 Product product_of(const GemmArgs &a)
@@ -454,7 +460,7 @@ int mxfp4_linear(const GemmArgs &a, bool backward, hipStream_t s)
   if (!fits(a.M, a.N, a.K)) return CAIFX_ERR_UNSUPPORTED;
   const size_t need = mxfp4_workspace_bytes(a, backward, backward);
   if (need > 0 && (!a.workspace || a.workspace_bytes < need || !aligned_to(a.workspace, 16))) return CAIFX_ERR_UNSUPPORTED;
-  if (backward) return gradient(gradient_of(a), a.workspace, s);
+  if (backward) return gradient(gradient_of(a), a.workspace, a.workspace_bytes, s);
   return product(product_of(a), a.workspace, a.workspace && aligned_to(a.workspace, 16) ? a.workspace_bytes : 0, s);
 }
 
@@ -629,7 +635,7 @@ int caifx_gated_backward(int64_t M, int64_t N, int64_t K, const void *grad_hidde
   p.w[1].p = w_up;
   p.w[1].scales = scales_up;
   p.y = dx;
-  return gradient(p, workspace, s);
+  return gradient(p, workspace, workspace_bytes, s);
 }
 
 }  // extern "C"
