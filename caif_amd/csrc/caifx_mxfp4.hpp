@@ -32,7 +32,7 @@ struct DxProduct {
   int count;
   const void *w[2], *s[2];
   bool mx;
-  const void *x[2];          // direct: [M, N] of the compute type (fp32 too), N a multiple of 8, aligned to 16 bytes; otherwise x[0] packed by operand_rows
+  const void *x[2];          // direct: [M, N] of the compute type (fp32 too), N at least 8, at any address; otherwise x[0] packed by operand_rows
   bool direct;
   int compute_dtype;         // CAIFX_F32: three bf16 pieces (mx only)
   void *y;

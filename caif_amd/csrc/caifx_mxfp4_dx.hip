@@ -80,18 +80,15 @@ __global__ __launch_bounds__(kWaves * 64) void dx_kernel(DxArgs g)
       }
     }
     if constexpr (kDirect) {
-      const int64_t n = static_cast<int64_t>(at) * 32 + 8 * q;
-      const bool in = n < g.N;
+      // (eight elements that end past the row, or begin there: its last eight)
+      const int64_t n = static_cast<int64_t>(at) * 32 + 8 * q, from_n = n + 8 <= g.N ? n : g.N - 8;
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
         int64_t m = m0 + 16 * t + j;
         m = m < g.M ? m : g.M - 1;
-        const uint8_t *from = x + (m * g.N + (in ? n : 0)) * (2 * XW);
+        const uint8_t *from = x + (m * g.N + from_n) * (2 * XW);
 #pragma unroll
-        for (int i = 0; i < XW; ++i) {
-          b.x[t][i] = *reinterpret_cast<const u32x4_t *>(from + 16 * i);
-          if (!in) b.x[t][i] = u32x4_t{0, 0, 0, 0};
-        }
+        for (int i = 0; i < XW; ++i) b.x[t][i] = *reinterpret_cast<const anywhere_t *>(from + 16 * i);
       }
     } else {
       // steps of a weight fill whole chunks of eight in the packed order
@@ -119,6 +116,12 @@ __global__ __launch_bounds__(kWaves * 64) void dx_kernel(DxArgs g)
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (n + 8 * q + i >= g.N) b.w[i][0] = b.w[i][kMx ? 0 : 1] = u32x4_t{0, 0, 0, 0};
+      if constexpr (kDirect) {
+        const int past = n + 8 * q + 8 - static_cast<int>(g.N);
+        if (past > 0)
+#pragma unroll
+          for (int t = 0; t < MT; ++t) drop_first<XW>(b.x[t], past);
+      }
     }
     u32x4_t x[MT][P];
 #pragma unroll

@@ -112,7 +112,7 @@ int wide_run(WideProduct d, Room &room, bool only_size, hipStream_t s)
 
 // Whether the row kernels read the activations where they are.  fp32 ones are taken apart by every workgroup then, which pays for the launch that
 // packs them for one group of four rows (us, N = K = 4096, direct / packed: 4 rows 6.8 / 10.8, 8 rows 11.9 / 10.9).
-bool direct_rows(const Product &p) { return p.M <= (p.compute_dtype == CAIFX_F32 ? 4 : 32) && p.x_dtype == p.compute_dtype && p.R % 8 == 0 && aligned_to(p.x, 16); }
+bool direct_rows(const Product &p) { return p.M <= (p.compute_dtype == CAIFX_F32 ? 4 : 32) && p.x_dtype == p.compute_dtype && p.R >= 8; }
 
 // The weights of a product or the activations of a gradient, as a source of operands
 Operand weights_of(const Weight (&w)[2], int count, int64_t rows, int64_t cols, int stored)
@@ -223,7 +223,6 @@ int product_rows(const Product &p, Room &room, bool only_size, hipStream_t s)
     g.R = pitch;
     g.w_pitch = 2 * pitch;
   }
-  // (a query has no address, and one that calls for a workspace in any case has room for rows at any)
   const bool direct = direct_rows(p);
   if (!direct) {
     void *packed = room.take(packed_bytes(p.M, g.chunks, p.compute_dtype));
@@ -235,9 +234,7 @@ int product_rows(const Product &p, Room &room, bool only_size, hipStream_t s)
   } else {
     g.x = p.x;
   }
-  const int st = rows_run(g, p.w[0].mx ? ROWS_MX : ROWS_DENSE, p.weights, p.compute_dtype, direct, room, only_size, s);
-  if (only_size && direct && !p.x && room.used > 0) room.take(packed_bytes(p.M, g.chunks, p.compute_dtype));
-  return st;
+  return rows_run(g, p.w[0].mx ? ROWS_MX : ROWS_DENSE, p.weights, p.compute_dtype, direct, room, only_size, s);
 }
 
 // What either way can need.  Activations at addresses that the dense product does not take run on the row kernels.
@@ -339,7 +336,7 @@ int gradient_rows(const Gradient &p, Room &room, bool only_size, hipStream_t s)
 }
 
 // The gradient from the weights as they are stored.
-DxProduct dx_of(const Gradient &p, bool aligned)
+DxProduct dx_of(const Gradient &p)
 {
   DxProduct d{};
   d.M = p.M;
@@ -356,7 +353,7 @@ DxProduct dx_of(const Gradient &p, bool aligned)
   d.y = p.y;
   d.y_dtype = p.y_dtype;
   d.addend = p.addend;
-  d.direct = p.x_dtype == p.compute_dtype && p.N % 8 == 0 && aligned && dx_reads(d);
+  d.direct = p.x_dtype == p.compute_dtype && p.N >= 8 && dx_reads(d);
   return d;
 }
 
@@ -365,8 +362,7 @@ DxProduct dx_of(const Gradient &p, bool aligned)
 // gradient 69 / 78; 2048 x 1408, 512 rows 21 / 19.
 bool dx_pays(const Gradient &p)
 {
-  // (chosen by sizes and types alone, as a query has no more: the other way may need another amount of room)
-  const DxProduct d = dx_of(p, true);
+  const DxProduct d = dx_of(p);
   if (!dx_takes(d)) return false;
   if (!wide_gradient_takes(p)) return true;
   const int pieces = pieces_of(p.compute_dtype);
@@ -378,10 +374,9 @@ bool dx_pays(const Gradient &p)
 
 int gradient_dx(const Gradient &p, Room &room, bool only_size, hipStream_t s)
 {
-  DxProduct d = dx_of(p, aligned_to(p.x[0], 16) && aligned_to(p.x[1], 16));
+  DxProduct d = dx_of(p);
   void *partial = room.take(dx_partial_bytes(d));
-  if (only_size || !d.direct) {
-    // (counted in any case: the query does not know the activations' addresses)
+  if (!d.direct) {
     const int chunks = p.weights * static_cast<int>(chunks_of(p.N));
     void *packed = room.take(packed_bytes(p.M, chunks, p.compute_dtype));
     if (only_size) return CAIFX_OK;
@@ -389,7 +384,7 @@ int gradient_dx(const Gradient &p, Room &room, bool only_size, hipStream_t s)
     if (st != CAIFX_OK) return st;
     d.x[0] = packed;
   }
-  return dx_product(d, partial, s);
+  return only_size ? CAIFX_OK : dx_product(d, partial, s);
 }
 
 size_t gradient_bytes(const Gradient &p)
@@ -571,9 +566,7 @@ size_t caifx_gated_workspace_bytes(int64_t M, int64_t N, int64_t K, int w_kind, 
   bool go;
   if (gated_check(M, N, K, w_kind, dtype, go) != CAIFX_OK || !go) return 0;
   if (backward) return gradient_bytes(gated_gradient(M, N, K, w_kind, dtype));
-  const size_t bytes = product_bytes(gated_product(M, N, K, w_kind, dtype));
-  // few rows are read where they are, but packed first at an address that no 16-byte access takes
-  return bytes > 0 ? bytes : packed_bytes(M, chunks_of(K), dtype);
+  return product_bytes(gated_product(M, N, K, w_kind, dtype));
 }
 
 int caifx_gated_forward(int64_t M, int64_t N, int64_t K, const void *x, const void *w_gate, const void *scales_gate, const void *w_up,

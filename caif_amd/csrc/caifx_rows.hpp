@@ -66,12 +66,12 @@ inline RowsPlan rows_plan(int64_t M, int64_t N, int64_t R, int weights, int piec
 }
 
 struct RowsArgs {
-  const void *x;          // direct: [M, x_pitch] of the compute type, or fp32 for three pieces; packed: see pack_rows_kernel
+  const void *x;          // direct: [M, x_pitch] of the compute type, or fp32 for three pieces, x_pitch at least 8, at any address; packed: see pack_rows_kernel
   int64_t x_pitch;
   const void *w[2];       // MX codes or dense rows of the compute type
   const uint8_t *s[2];    // MX scales
   const uint8_t *xs;      // both in 4 bits: scales of x, whose codes are rows of w_pitch bytes
-  int64_t M, N, R;        // R: elements of the reduction, a multiple of 8 for direct activations and dense weights
+  int64_t M, N, R;        // R: elements of the reduction, a multiple of 8 for dense weights
   int64_t blocks;         // MX blocks of a weight row
   int64_t w_pitch;        // bytes of a weight row
   int chunks, tiles;      // chunks of the reduction, row tiles of 16 in the packed activations
@@ -136,12 +136,35 @@ __device__ __forceinline__ void pieces_of_f32(float value, uint32_t (&piece)[3])
   piece[2] = finite ? __builtin_bit_cast(uint32_t, last) : 0u;
 }
 
+// Eight elements of two bytes (XW = 1) or four, read `gone` elements early: those move out in front, zeros follow behind.
+template <int XW> __device__ __forceinline__ void drop_first(u32x4_t (&v)[XW], int gone)
+{
+  uint32_t a[4 * XW];
+#pragma unroll
+  for (int i = 0; i < 4 * XW; ++i) a[i] = v[i >> 2][i & 3];
+  const auto move = [&](int dwords, bool now) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4 * XW; ++i) a[i] = !now ? a[i] : i + dwords < 4 * XW ? a[i + dwords < 4 * XW ? i + dwords : 0] : 0u;
+  };
+  if constexpr (XW == 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = (gone & 1) ? __builtin_amdgcn_alignbyte(i < 3 ? a[i < 3 ? i + 1 : 0] : 0u, a[i], 2u) : a[i];
+  } else {
+    move(1, gone & 1);
+  }
+  move(XW, gone & 2);
+  move(2 * XW, gone & 4);
+#pragma unroll
+  for (int i = 0; i < 4 * XW; ++i) v[i >> 2][i & 3] = gone >= 8 ? 0u : a[i];
+}
+
 // P: pieces of an activation (3: fp32).  NW: weights (2: gate and up; the first half of the NT column tiles is gate's).  kWhole: rows of
 // at least 16 blocks: a unit's scales of a weight row are one access, at any address (one byte at a time they are more requests than the
 // codes; K = 11008, N = 4096, one row 22.0 us instead of 8.6).
 // XG: groups of four rows of activations that are read where they are, fp32 ones (up to four) taken
-// apart on their way through LDS; 0: packed ones.
-template <typename CT, int P, int kWeight, int NW, int MT, int NT, int XG, bool kWhole>
+// apart on their way through LDS; 0: packed ones.  kOdd: direct rows that do not end with eight elements (one kernel for both takes 8.4 us
+// instead of 8.0 for one row, N = 14336, K = 4096; packed first, K = 4095 takes 3 us more).
+template <typename CT, int P, int kWeight, int NW, int MT, int NT, int XG, bool kWhole, bool kOdd>
 __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
 {
   constexpr int NC = NT / NW;                // column tiles of one weight
@@ -149,12 +172,13 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
   constexpr bool kDirect = XG > 0 && !kBoth;
   constexpr int WV = kMicro ? 1 : 4, XV = kBoth ? 1 : 4;      // 16-byte pieces of a column tile and of a row tile per half chunk
   constexpr int XW = P == 3 ? 2 : 1;                          // direct: loads of eight elements
+  constexpr uint32_t kRoom = kOdd ? 32 : 0;
   constexpr int XL = kDirect ? XG * XW : MT * P * XV;         // loads of activations per half chunk
   // half chunks on their way before the one in hand is used: a second one where a SIMD still holds four waves with it (one row, N = 4096, K =
   // 14336: 10.2 us instead of 13.3; with 32 registers a half chunk, 16 rows, N = 14336, K = 4096: 11.9 instead of 11.4)
   constexpr int kRegs = 4 * (NT * WV + XL);
   constexpr int D = kRegs <= 24 ? 2 : 1;
-  static_assert(NT % NW == 0 && (P == 1 || XG <= 1) && (kMicro || !kWhole) && (XG == 0 || XG == 4 * MT || (MT == 1 && XG == 1)), "");
+  static_assert(NT % NW == 0 && (P == 1 || XG <= 1) && (kMicro || !kWhole) && (XG == 0 || XG == 4 * MT || (MT == 1 && XG == 1)) && (kDirect || !kOdd), "");
   // the activations of a half chunk for each wave, [P][4 XG][16 pieces of 16 bytes]; at the end the waves' sums
   constexpr int kSums = kRowsWaves / 2 * MT * NT * 1024, kOrder = kDirect ? kRowsWaves * P * XG * 1024 : 0;
   __shared__ __attribute__((aligned(16))) unsigned char smem[kSums > kOrder ? kSums : kOrder];
@@ -192,7 +216,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
       // (direct: lane (j, q) reads piece j of the half chunk of row 4 t + q)
       const int64_t m = m0 + (kDirect ? 4 * t + q : 16 * t + j);
       const uint32_t row = static_cast<uint32_t>((m < g.M ? m : g.M - 1) - m0);
-      x_off[t] = row * static_cast<uint32_t>(pitch) + (kDirect ? j * XW : q) * 16;
+      x_off[t] = row * static_cast<uint32_t>(pitch) + (kDirect ? j * XW : q) * 16 + kRoom;
       if constexpr (kBoth) xs_off[t] = row * static_cast<uint32_t>(g.blocks);
     }
   }
@@ -218,6 +242,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
     u32x4_t w[kWhole ? NT : 1];              // dword h: the scales of half h, a byte for each of its blocks
     u32x4_t x[kWhole && kBoth ? MT : 1];
   };
+  const int length = static_cast<int>(kOdd ? g.x_pitch : g.R);      // (dense rows are filled up to a multiple of eight)
   const int halves = kMicro ? static_cast<int>((g.blocks + 3) >> 2) : static_cast<int>((g.R + 127) >> 7);
   const int units = (halves + 3) >> 2;
   const int z = static_cast<int>(blockIdx.z);
@@ -280,12 +305,16 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
       }
     }
     if constexpr (kDirect) {
+      // Eight elements that begin past the row, or (kOdd) end there: its last eight.  Those can begin up to 28 bytes before the half chunk, which
+      // the offset, without a sign, makes room for.
       const int k = static_cast<int>(half) * 128 + 8 * j;
-      const uint32_t back = k < g.R ? 0u : static_cast<uint32_t>(k - (g.R - 8)) * (2 * XW);
+      uint32_t back;
+      if constexpr (kOdd) back = k + 8 > length ? static_cast<uint32_t>(k + 8 - length) * (2 * XW) : 0u;
+      else back = k < g.R ? 0u : static_cast<uint32_t>(k - (g.R - 8)) * (2 * XW);
 #pragma unroll
       for (int t = 0; t < XG; ++t)
 #pragma unroll
-        for (int i = 0; i < XW; ++i) b.x[t * XW + i] = at128(x_base + half * (256 * XW), x_off[t] - back + 16 * i, aligned);
+        for (int i = 0; i < XW; ++i) b.x[t * XW + i] = at128(x_base + half * (256 * XW) - kRoom, x_off[t] - back + 16 * i, std::false_type{});
     } else {
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
@@ -312,9 +341,23 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
   auto compute = [&](Half &b, const Scales &s, int h, int half, auto part_) __attribute__((always_inline)) {
     constexpr bool kPart = decltype(part_)::value;
     if constexpr (kPart && kDirect) {
-      if (half * 128 + 8 * j >= g.R)
+      if constexpr (kOdd) {
+        const int past = half * 128 + 8 * j + 8 - length;
+        if (past > 0)
 #pragma unroll
-        for (int t = 0; t < XL; ++t) b.x[t] = u32x4_t{0, 0, 0, 0};
+          for (int t = 0; t < XG; ++t) {
+            u32x4_t eight[XW];
+#pragma unroll
+            for (int i = 0; i < XW; ++i) eight[i] = b.x[t * XW + i];
+            drop_first<XW>(eight, past);
+#pragma unroll
+            for (int i = 0; i < XW; ++i) b.x[t * XW + i] = eight[i];
+          }
+      } else {
+        if (half * 128 + 8 * j >= g.R)
+#pragma unroll
+          for (int t = 0; t < XL; ++t) b.x[t] = u32x4_t{0, 0, 0, 0};
+      }
     }
     if constexpr (kPart && !kMicro) {
 #pragma unroll
@@ -433,7 +476,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
     for (int h = 0; h < D; ++h) load(ring[h], 4 * first + h);
     int unit = first;
     for (int t = 1; t < mine; ++t, unit += kRowsWaves) run(unit, std::false_type{}, std::false_type{});
-    if (D == 1 || 512 * (unit + 1) > g.R) run(unit, std::true_type{}, std::true_type{});
+    if (D == 1 || 512 * (unit + 1) > (kOdd ? g.x_pitch : g.R)) run(unit, std::true_type{}, std::true_type{});
     else run(unit, std::true_type{}, std::false_type{});
   }
 
@@ -507,12 +550,20 @@ int rows_launch(const RowsArgs &g, hipStream_t s)
     part.up = forth(g.up, m0 * g.N * es);
     part.addend = forth(g.addend, m0 * g.N * es);
     const dim3 grid(static_cast<unsigned>(cols), static_cast<unsigned>(rows - r < 65535 ? rows - r : 65535), static_cast<unsigned>(g.splits));
+    const auto go = [&](auto whole_, auto odd_) {
+      hipLaunchKernelGGL((rows_kernel<CT, P, kWeight, NW, MT, NT, XG, decltype(whole_)::value, decltype(odd_)::value>), grid, dim3(kRowsWaves * 64), 0, s, part);
+    };
+    const auto pick_odd = [&](auto whole_) {
+      if constexpr (XG > 0 && kWeight != ROWS_BOTH) {
+        if (g.x_pitch % 8 != 0) return go(whole_, std::true_type{});
+      }
+      go(whole_, std::false_type{});
+    };
     if constexpr (kWeight != ROWS_DENSE) {
-      const bool whole = g.blocks >= 16;
-      if (whole) hipLaunchKernelGGL((rows_kernel<CT, P, kWeight, NW, MT, NT, XG, true>), grid, dim3(kRowsWaves * 64), 0, s, part);
-      else hipLaunchKernelGGL((rows_kernel<CT, P, kWeight, NW, MT, NT, XG, false>), grid, dim3(kRowsWaves * 64), 0, s, part);
+      if (g.blocks >= 16) pick_odd(std::true_type{});
+      else pick_odd(std::false_type{});
     } else {
-      hipLaunchKernelGGL((rows_kernel<CT, P, kWeight, NW, MT, NT, XG, false>), grid, dim3(kRowsWaves * 64), 0, s, part);
+      pick_odd(std::false_type{});
     }
   }
   return launch_status();

@@ -210,10 +210,10 @@ CAIFX_API int caifx_qlinear_backward_input_add(int64_t M, int64_t N, int64_t K,
  * code * scale to the 16-bit compute type as the reference does, and with it on the few-row kernels that multiply
  * unrounded codes (about 2e-3 of max|out| apart; both within the 1e-2 bound; the few-row input gradient of packed
  * int4 with a 16-bit compute type multiplies the rounded weight either way).
- * CAIFX_W_MXFP4: activations or gradients in the kernels' order (more than 32 rows, fp32 compute, rows that are no multiple of 16
- * bytes), the sums of workgroups that share a reduction, and from some hundred rows on dense copies of the weight (transposed for
+ * CAIFX_W_MXFP4: activations in the kernels' order (more than 32 rows, in fp32 more than 4, those of another type or below eight
+ * columns), the sums of workgroups that share a reduction, and from some hundred rows on dense copies of the weight (transposed for
  * the input gradient) and of operands of another type.  With less the forward runs without the dense copies, and otherwise the
- * shape-agnostic kernels, which also take few rows at an address that no 16-byte access does where the query says 0. */
+ * shape-agnostic kernels. */
 CAIFX_API size_t caifx_qlinear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_dtype, int compute_dtype,
                                      int w_kind, int backward);
 /* The same without the dense copy of large calls: what is left is a few partial tiles, at most 16 MiB for the 16-bit compute

@@ -72,16 +72,16 @@ def test_gated_forward():
     assert all(forward(**{k: AT + 1}) == MISALIGNED for k in ("x", "hidden", "gate", "up"))
     assert forward(wg=AT + 8) == MISALIGNED and forward(wu=AT + 2) == MISALIGNED and forward(x=AT + 2, dtype=T.F32) == MISALIGNED
     assert forward(hidden=AT) == INVALID and forward(gate=ELSE) == INVALID and forward(up=ELSE + 4096) == INVALID
-    need = capi.lib().caifx_gated_workspace_bytes(4, 8, 70, T.W_MXFP4, T.BF16, 0)
-    assert need > 0 and forward(ws=None, bytes=need) == SMALL and forward(bytes=need - 1) == SMALL
+    need = capi.lib().caifx_gated_workspace_bytes(40, 8, 70, T.W_MXFP4, T.BF16, 0)
+    assert need > 0 and forward(M=40, ws=None, bytes=need) == SMALL and forward(M=40, bytes=need - 1) == SMALL
 
 
 def test_gated_backward():
     assert all(backward(**{k: None}) == INVALID for k in ("d", "gate", "up", "wg", "wu", "sg", "su", "gg", "gu"))
     assert all(backward(**{k: AT + 1}) == MISALIGNED for k in ("d", "gate", "up", "gg", "gu", "dx"))
     assert backward(wg=AT + 8) == MISALIGNED and backward(gg=AT) == INVALID and backward(gu=ELSE) == INVALID and backward(dx=ELSE) == INVALID
-    need = capi.lib().caifx_gated_workspace_bytes(4, 8, 70, T.W_MXFP4, T.BF16, 1)
-    assert need > 0 and backward(ws=None, bytes=need) == SMALL and backward(bytes=need - 1) == SMALL
+    need = capi.lib().caifx_gated_workspace_bytes(4, 300, 70, T.W_MXFP4, T.BF16, 1)
+    assert need > 0 and backward(N=300, ws=None, bytes=need) == SMALL and backward(N=300, bytes=need - 1) == SMALL
 
 
 @pytest.mark.parametrize("kind,dtype,status", [
