@@ -383,3 +383,31 @@ def test_gradient_of_weights_beyond_fp16(M, N):
     ok = want.isfinite().all(dim=0)
     assert bool((~ok).any())
     within(y[:, ok].contiguous(), want[:, ok], x.double().abs() @ used[:, ok].abs(), N)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M", [1, 4, 5, 30])
+@pytest.mark.parametrize("length", [1, 7, 8, 9, 15, 31, 129, 130, 135, 257, 511, 513, 1027])
+def test_rows_of_any_length(length, M, dtype):
+    """Rows of activations are read eight elements at a time, also where they end in between: what lies beside them counts for nothing."""
+    g = gen(90 + length)
+    t = DTYPES[dtype]
+    c = T.CODE_OF[t]
+    other = 40
+    x = torch.randn(M, length, generator=g).to(t)
+    beside = torch.full((M * length + 40,), float("nan"), dtype=t, device="cuda")
+    beside[9:9 + M * length] = x.view(-1).cuda()
+    x, used = x.double(), beside[9:9 + M * length].view(M, length)
+    for backward in (False, True):
+        w, exact = weight(g, *((length, other) if backward else (other, length)))
+        m = exact if backward else exact.T
+        y = (T.qlinear_backward_input if backward else T.qlinear_forward)(used, w, c, c)
+        within(y, x @ m, x.abs() @ m.abs(), length, 3 if dtype == "f32" else 1)
+    if dtype == "f32":
+        return
+    # the gated block over two stored weights: rows of either length are copied where eight elements do not fill them
+    kind = T.W_F16 if dtype == "f16" else T.W_BF16
+    a, b = (torch.randn(other, length, generator=g).to(t) for _ in range(2))
+    _, gate, up = T.gated_forward(used, *(T.FrozenWeight(v.cuda(), kind, None, other, length) for v in (a, b)), keep=True)
+    for got, v in ((gate, a.double()), (up, b.double())):
+        within(got, x @ v.T, x.abs() @ v.abs().T, length)
