@@ -411,3 +411,36 @@ def test_rows_of_any_length(length, M, dtype):
     _, gate, up = T.gated_forward(used, *(T.FrozenWeight(v.cuda(), kind, None, other, length) for v in (a, b)), keep=True)
     for got, v in ((gate, a.double()), (up, b.double())):
         within(got, x @ v.T, x.abs() @ v.abs().T, length)
+
+
+# ------------------------------------------------------------------ steps of a tile shared by workgroups, a last round of half tiles
+def on_device(codes, scales, cols):
+    """fp64 on the device, where the large products of the tests below are fast enough"""
+    return R.decode(codes.cuda(), scales.cuda(), cols)
+
+
+@pytest.mark.parametrize("yd", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(256, 512, 8192), (200, 300, 8100), (130, 1000, 4128), (1500, 11000, 96), (1530, 10999, 257)])
+def test_matmul_tiles(M, N, K, yd):
+    g = gen(M + N + K)
+    a, sa = R.random_weight(g, M, K)
+    b, sb = R.random_weight(g, N, K, low=110, high=130)
+    y = T.mxfp4_matmul(a.cuda(), sa.cuda(), b.cuda(), sb.cuda(), T.CODE_OF[DTYPES[yd]])
+    p, q = on_device(a, sa, K), on_device(b, sb, K)
+    within(y, (p @ q.T).cpu(), (p.abs() @ q.abs().T).cpu(), K)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(1100, 4096, 264), (1030, 2000, 70), (1025, 4100, 131)])
+def test_gradient_in_parts(M, N, K, dtype):
+    g = gen(M + N + K)
+    codes, s = R.random_weight(g, N, K)
+    w, exact = T.FrozenWeight(codes.cuda(), T.W_MXFP4, s.cuda(), N, K, 1, 32), on_device(codes, s, K)
+    dt = DTYPES[dtype]
+    code = T.CODE_OF[dt]
+    dy = torch.randn(M, N, generator=g).to(dt).cuda()
+    dx = T.qlinear_backward_input(dy, w, code, code)
+    within(dx, (dy.double() @ exact).cpu(), (dy.double().abs() @ exact.abs()).cpu(), N, 3 if dtype == "f32" else 1)
+    add = torch.randn(M, K, generator=g).to(dt).cuda()
+    assert torch.equal(T.qlinear_backward_input(dy, w, code, code, addend=add), (dx.float() + add.float()).to(dt))
+    assert torch.equal(T.qlinear_backward_input(dy, w, code, code), dx)
