@@ -8,6 +8,8 @@
 // M = 4096, N = 14336, K = 4096).
 // The columns' operand is the instruction's first one, so that a lane's four sums are neighbours of a row and go to LDS, on their way into
 // whole rows, 8 bytes (fp32: 16) at a time.
+// M = 4096, N = 14336, K = 4096: 137 us, 3.5 PFLOP/s.  A step takes 1.59 us where the matrix pipes alone take 1.32, and a tile 9 us more for its first
+// requests and its results, which all compute units write at once.
 // Blocks past the end of a row count for nothing: both scales are 2^-127 there, and codes have no infinities or NaN.
 #include "caifx_mxfp4.hpp"
 
