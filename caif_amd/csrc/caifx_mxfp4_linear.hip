@@ -110,9 +110,16 @@ int wide_run(WideProduct d, Room &room, bool only_size, hipStream_t s)
   return st != CAIFX_OK ? st : join_sums(static_cast<const float *>(partial), d.parts, d.M * d.C, asked.d, asked.d_dtype, asked.addend, s);
 }
 
-// Whether the row kernels read the activations where they are.  fp32 ones are taken apart by every workgroup then, which pays for the launch that
-// packs them for one group of four rows (us, N = K = 4096, direct / packed: 4 rows 6.8 / 10.8, 8 rows 11.9 / 10.9).
-bool direct_rows(const Product &p) { return p.M <= (p.compute_dtype == CAIFX_F32 ? 4 : 32) && p.x_dtype == p.compute_dtype && p.R >= 8; }
+// Whether the row kernels read the activations where they are, each workgroup its rows, which pays for the launch that packs them while all
+// workgroups run at once.  us, packed / direct, bf16: 64 rows, N = 14336, K = 4096 22.1 / 20.7; N = 4096, K = 14336 25.7 / 22.6; 2048 x 1408 8.0 / 7.6;
+// 256 rows, N = K = 4096 19.9 / 16.3; two rounds, 96 rows, N = 11008, K = 2048 21.6 / 23.4.  fp32 ones are taken apart by every workgroup: for one
+// group of four rows (N = K = 4096, 4 rows 10.8 / 6.8, 8 rows 10.9 / 11.9).
+bool direct_rows(const Product &p)
+{
+  if (p.x_dtype != p.compute_dtype || p.R < 8) return false;
+  if (p.compute_dtype == CAIFX_F32) return p.M <= 4;
+  return p.M <= 32 || (p.M + 63) / 64 * ((p.weights * p.N + 63) / 64) <= 256;
+}
 
 // The weights of a product or the activations of a gradient, as a source of operands
 Operand weights_of(const Weight (&w)[2], int count, int64_t rows, int64_t cols, int stored)

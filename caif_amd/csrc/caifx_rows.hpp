@@ -3,7 +3,7 @@
 //
 // Bound by memory with few rows (the weight's bytes), by the L1 from some dozens on: a compute unit has some 100 lines on their way at a
 // time, whatever it asks for, and the activations are read anew for every 16 NT weight rows.  So they are asked for in whole lines, only the
-// rows that there are, and take the operands' order in a wave's own part of LDS (up to 32 rows) or beforehand (see pack_rows_kernel).
+// rows that there are, and take the operands' order in a wave's own part of LDS or, in larger calls, beforehand (see pack_rows_kernel).
 // Measured, bf16: one row, N = 14336, K = 4096 8.0 us (3.9 TB/s); 24 rows in fp16, N = 4096, K = 14336 13.9; eight rows of a gated block over two
 // 14336 x 4096 weights 15.2 (4.1 TB/s).
 // A workgroup of eight waves owns 16 MT rows and 16 NT weight rows of the result; the waves take units of 512 reduction elements in turn and their sums meet in LDS at the end.
@@ -604,7 +604,7 @@ template <typename CT, int kWeight, int NW> int rows_pick(const RowsArgs &g, int
   switch (rows_tile(g.M, 1)) {
     case 16: return four ? rows_pick_direct<CT, 1, kWeight, NW, 1, 1>(g, direct, s) : rows_pick_direct<CT, 1, kWeight, NW, 1, 4>(g, direct, s);
     case 32: return rows_pick_direct<CT, 1, kWeight, NW, 2, 8>(g, direct, s);
-    default: return rows_pick_columns<CT, 1, kWeight, NW, 4, 0>(g, s);
+    default: return rows_pick_direct<CT, 1, kWeight, NW, 4, 16>(g, direct, s);
   }
 }
 

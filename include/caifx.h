@@ -210,7 +210,7 @@ CAIFX_API int caifx_qlinear_backward_input_add(int64_t M, int64_t N, int64_t K,
  * code * scale to the 16-bit compute type as the reference does, and with it on the few-row kernels that multiply
  * unrounded codes (about 2e-3 of max|out| apart; both within the 1e-2 bound; the few-row input gradient of packed
  * int4 with a 16-bit compute type multiplies the rounded weight either way).
- * CAIFX_W_MXFP4: activations in the kernels' order (more than 32 rows, in fp32 more than 4, those of another type or below eight
+ * CAIFX_W_MXFP4: activations in the kernels' order (from some dozens of rows on, in fp32 from five, those of another type or below eight
  * columns), the sums of workgroups that share a reduction, and from some hundred rows on dense copies of the weight (transposed for
  * the input gradient) and of operands of another type.  With less the forward runs without the dense copies, and otherwise the
  * shape-agnostic kernels. */

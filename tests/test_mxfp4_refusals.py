@@ -72,8 +72,8 @@ def test_gated_forward():
     assert all(forward(**{k: AT + 1}) == MISALIGNED for k in ("x", "hidden", "gate", "up"))
     assert forward(wg=AT + 8) == MISALIGNED and forward(wu=AT + 2) == MISALIGNED and forward(x=AT + 2, dtype=T.F32) == MISALIGNED
     assert forward(hidden=AT) == INVALID and forward(gate=ELSE) == INVALID and forward(up=ELSE + 4096) == INVALID
-    need = capi.lib().caifx_gated_workspace_bytes(40, 8, 70, T.W_MXFP4, T.BF16, 0)
-    assert need > 0 and forward(M=40, ws=None, bytes=need) == SMALL and forward(M=40, bytes=need - 1) == SMALL
+    need = capi.lib().caifx_gated_workspace_bytes(40, 8, 70, T.W_MXFP4, T.F32, 0)
+    assert need > 0 and forward(M=40, dtype=T.F32, ws=None, bytes=need) == SMALL and forward(M=40, dtype=T.F32, bytes=need - 1) == SMALL
 
 
 def test_gated_backward():
