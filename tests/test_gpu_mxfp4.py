@@ -444,3 +444,40 @@ def test_gradient_in_parts(M, N, K, dtype):
     add = torch.randn(M, K, generator=g).to(dt).cuda()
     assert torch.equal(T.qlinear_backward_input(dy, w, code, code, addend=add), (dx.float() + add.float()).to(dt))
     assert torch.equal(T.qlinear_backward_input(dy, w, code, code), dx)
+
+
+def test_calls_on_two_streams():
+    """Calls that run at the same time, over the same weight, on two streams keep their results; so do two graphs replayed in turn."""
+    g = gen(120)
+    N, K = 1030, 520
+    w, _ = weight(g, N, K)
+    cases = [(M, dt) for M in (1, 30, 200, 1100) for dt in (torch.bfloat16, torch.float32)]
+    x = [torch.randn(M, K, generator=g).to(dt).cuda() for M, dt in cases]
+    d = [torch.randn(M, N, generator=g).to(dt).cuda() for M, dt in cases]
+    a = T.mxfp4_quantize(x[6])
+
+    def step(i):
+        c = T.CODE_OF[x[i].dtype]
+        return T.qlinear_forward(x[i], w, c, c), T.qlinear_backward_input(d[i], w, c, c), T.gated_forward(x[i], w, w), T.mxfp4_matmul(*a, w.wq, w.scales)
+    want = [step(i) for i in range(len(cases))]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(3):
+        for i in range(len(cases)):
+            with torch.cuda.stream(streams[i % 2]):
+                got.append((i, step(i)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for i, results in got for p, q in zip(results, want[i]))
+    graphs = []
+    for i in (2, 5, 6):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, i, step(i)))
+    for _ in range(3):
+        for graph, i, results in graphs:
+            for r in results:
+                r.zero_()
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for _, i, results in graphs for p, q in zip(results, want[i]))
