@@ -164,8 +164,8 @@ template <int XW> __device__ __forceinline__ void drop_first(u32x4_t (&v)[XW], i
 // at least 16 blocks: a unit's scales of a weight row are one access, at any address (one byte at a time they are more requests than the
 // codes; K = 11008, N = 4096, one row 22.0 us instead of 8.6).
 // XG: groups of four rows of activations that are read where they are, fp32 ones (up to four) taken
-// apart on their way through LDS; 0: packed ones.  kOdd: direct rows that do not end with eight elements (one kernel for both takes 8.4 us
-// instead of 8.0 for one row, N = 14336, K = 4096; packed first, K = 4095 takes 3 us more).
+// apart on their way through LDS; 0: packed ones.  kOdd: direct rows that do not end with eight elements, in 4 bits those that do not end with a
+// block (one kernel for both takes 9.7 us instead of 9.2 for one row, N = 14336, K = 4096, weights in turn; packed first, K = 4095 takes 3 us more).
 template <typename CT, int P, int kWeight, int NW, int MT, int NT, int XG, bool kWhole, bool kOdd>
 __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
 {
@@ -359,6 +359,19 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
         if (half * 128 + 8 * j >= g.R)
 #pragma unroll
           for (int t = 0; t < XL; ++t) b.x[t] = u32x4_t{0, 0, 0, 0};
+      }
+    }
+    if constexpr (kPart && kMicro && !kBoth && (kOdd || XG == 0)) {
+      // codes behind the last column, whose values may be beyond the compute type: an infinity against the activations' zeros would be a NaN
+      const int left = static_cast<int>(g.R) - 32 * (4 * half + q);
+      if ((g.R & 31) != 0 && left < 32) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const int in = left - 8 * d;
+          const uint32_t mask = in >= 8 ? ~0u : in > 0 ? (1u << (4 * in)) - 1u : 0u;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) b.w[t][0][d] &= mask;
+        }
       }
     }
     if constexpr (kPart && !kMicro) {
@@ -557,7 +570,7 @@ int rows_launch(const RowsArgs &g, hipStream_t s)
     };
     const auto pick_odd = [&](auto whole_) {
       if constexpr (XG > 0 && kWeight != ROWS_BOTH) {
-        if (g.x_pitch % 8 != 0) return go(whole_, std::true_type{});
+        if (g.x_pitch % (kWeight == ROWS_MX ? CAIFX_MXFP4_BLOCK : 8) != 0) return go(whole_, std::true_type{});
       }
       go(whole_, std::false_type{});
     };

@@ -71,8 +71,9 @@ enum caifx_dtype { CAIFX_F32 = 0, CAIFX_F16 = 1, CAIFX_BF16 = 2 };
  *                      are ignored.  These cells run on the fp32 matrix-core kernel (operands rounded to a
  *                      16-bit compute type first, fp32 products and sums), not on the fast paths of the quantised kinds.
  *  CAIFX_W_MXFP4:      microscaled 4-bit floating point, codes and scales as caifx_mxfp4_quantize lays them out for N rows of K
- *                      columns (codes aligned to 16 bytes; scale_period and group_size are ignored).  Taken by the plain calls,
- *                      with an addend too; the grouped ones return CAIFX_ERR_UNSUPPORTED.  (5 is no kind.) */
+ *                      columns (codes aligned to 16 bytes; scale_period and group_size are ignored).  Codes that fill up a row's
+ *                      last block count for nothing, whatever they are.  Taken by the plain calls, with an addend too; the grouped
+ *                      ones return CAIFX_ERR_UNSUPPORTED.  (5 is no kind.) */
 enum caifx_weight_kind { CAIFX_W_INT8 = 0, CAIFX_W_INT4_GROUP = 1, CAIFX_W_F32 = 2, CAIFX_W_F16 = 3, CAIFX_W_BF16 = 4, CAIFX_W_MXFP4 = 6 };
 
 CAIFX_API const char *caifx_status_string(int status);
