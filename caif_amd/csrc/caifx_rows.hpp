@@ -164,8 +164,9 @@ template <int XW> __device__ __forceinline__ void drop_first(u32x4_t (&v)[XW], i
 // at least 16 blocks: a unit's scales of a weight row are one access, at any address (one byte at a time they are more requests than the
 // codes; K = 11008, N = 4096, one row 22.0 us instead of 8.6).
 // XG: groups of four rows of activations that are read where they are, fp32 ones (up to four) taken
-// apart on their way through LDS; 0: packed ones.  kOdd: direct rows that do not end with eight elements, in 4 bits those that do not end with a
-// block (one kernel for both takes 9.7 us instead of 9.2 for one row, N = 14336, K = 4096, weights in turn; packed first, K = 4095 takes 3 us more).
+// apart on their way through LDS; 0: packed ones.  kOdd: direct rows that do not end with eight elements, and rows in 4 bits that do not end with
+// a block (one kernel for both takes 9.7 us instead of 9.2 for one row, N = 14336, K = 4096, weights in turn, and 75 instead of 71 for 300 packed
+// ones; packed first, K = 4095 takes 3 us more).
 template <typename CT, int P, int kWeight, int NW, int MT, int NT, int XG, bool kWhole, bool kOdd>
 __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
 {
@@ -180,7 +181,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
   // 14336: 10.2 us instead of 13.3; with 32 registers a half chunk, 16 rows, N = 14336, K = 4096: 11.9 instead of 11.4)
   constexpr int kRegs = 4 * (NT * WV + XL);
   constexpr int D = kRegs <= 24 ? 2 : 1;
-  static_assert(NT % NW == 0 && (P == 1 || XG <= 1) && (kMicro || !kWhole) && (XG == 0 || XG == 4 * MT || (MT == 1 && XG == 1)) && (kDirect || !kOdd), "");
+  static_assert(NT % NW == 0 && (P == 1 || XG <= 1) && (kMicro || !kWhole) && (XG == 0 || XG == 4 * MT || (MT == 1 && XG == 1)) && (kDirect || kWeight == ROWS_MX || !kOdd), "");
   // the activations of a half chunk for each wave, [P][4 XG][16 pieces of 16 bytes]; at the end the waves' sums
   constexpr int kSums = kRowsWaves / 2 * MT * NT * 1024, kOrder = kDirect ? kRowsWaves * P * XG * 1024 : 0;
   __shared__ __attribute__((aligned(16))) unsigned char smem[kSums > kOrder ? kSums : kOrder];
@@ -361,7 +362,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void rows_kernel(RowsArgs g)
           for (int t = 0; t < XL; ++t) b.x[t] = u32x4_t{0, 0, 0, 0};
       }
     }
-    if constexpr (kPart && kMicro && !kBoth && (kOdd || XG == 0)) {
+    if constexpr (kPart && kMicro && kOdd) {
       // codes behind the last column, whose values may be beyond the compute type: an infinity against the activations' zeros would be a NaN
       const int left = static_cast<int>(g.R) - 32 * (4 * half + q);
       if ((g.R & 31) != 0 && left < 32) {
@@ -569,7 +570,7 @@ int rows_launch(const RowsArgs &g, hipStream_t s)
       hipLaunchKernelGGL((rows_kernel<CT, P, kWeight, NW, MT, NT, XG, decltype(whole_)::value, decltype(odd_)::value>), grid, dim3(kRowsWaves * 64), 0, s, part);
     };
     const auto pick_odd = [&](auto whole_) {
-      if constexpr (XG > 0 && kWeight != ROWS_BOTH) {
+      if constexpr (kWeight == ROWS_MX || (XG > 0 && kWeight != ROWS_BOTH)) {
         if (g.x_pitch % (kWeight == ROWS_MX ? CAIFX_MXFP4_BLOCK : 8) != 0) return go(whole_, std::true_type{});
       }
       go(whole_, std::false_type{});
