@@ -165,7 +165,15 @@ bool wide_product_pays(const Product &p)
   return (p.weights == 2 ? wide_product_us(p.M, 2 * p.N, pieces * R) : wide_parts(p.M, p.N, pieces * R).us) + (pieces == 3 ? 12.0 : 8.0) + 0.56 * millions < rows;
 }
 
-// The product on dense operands: the weights dequantised into the workspace, activations of another type or length copied.
+// Whether the dense product reads activations from a copy: of another type or length, or that no 16-byte access takes where they are.  us, 4096 rows, N =
+// 11008, K = 4096, bf16, in place / copied / on the row kernels, which take any address: forward 302 / 300 / 596, gradient 263 / 297 / 953; 300 rows, N = 14336,
+// K = 4096, gradient 72 / 78 / 138.  A size query, which has no address, counts the copy.
+bool copied(int pieces, int x_dtype, int to, int64_t length, int64_t R, const void *x, const void *second)
+{
+  return pieces == 3 || x_dtype != to || length != R || !x || !aligned_to(x, 16) || !aligned_to(second, 16);
+}
+
+// The product on dense operands: the weights dequantised into the workspace, activations copied where they have to be.
 int product_wide(const Product &p, Room &room, bool only_size, hipStream_t s)
 {
   const int64_t R = up_to(p.R, 64) < 128 ? 128 : up_to(p.R, 64);
@@ -191,7 +199,7 @@ int product_wide(const Product &p, Room &room, bool only_size, hipStream_t s)
     void *copy = room.take(static_cast<size_t>(p.M) * static_cast<size_t>(R) * 6);
     d.a = copy;
     if (!only_size && st == CAIFX_OK) st = operand_pieces(x, copy, R, s);
-  } else if (p.x_dtype != to || R != p.R) {
+  } else if (copied(pieces, p.x_dtype, to, p.R, R, p.x, nullptr)) {
     void *copy = room.take(static_cast<size_t>(p.M) * static_cast<size_t>(R) * 2);
     d.a = copy;
     if (!only_size && st == CAIFX_OK) st = operand_dense(x, to, copy, R, s);
@@ -244,25 +252,27 @@ int product_rows(const Product &p, Room &room, bool only_size, hipStream_t s)
   return rows_run(g, p.w[0].mx ? ROWS_MX : ROWS_DENSE, p.weights, p.compute_dtype, direct, room, only_size, s);
 }
 
-// What either way can need.  Activations at addresses that the dense product does not take run on the row kernels.
-size_t product_bytes(const Product &p, bool dense_copy = true)
+// What one way of a product takes of the workspace
+template <typename P> size_t room_of(int (*way)(const P &, Room &, bool, hipStream_t), const P &p)
 {
-  Room rows, wide;
-  product_rows(p, rows, true, nullptr);
-  if (!dense_copy || !wide_product_pays(p)) return rows.used;
-  product_wide(p, wide, true, nullptr);
-  return rows.used > wide.used ? rows.used : wide.used;
+  Room need;
+  way(p, need, true, nullptr);
+  return need.used;
 }
 // One way of a product, in room that is checked first to hold what it takes at these addresses
 template <typename P> int run_in(int (*way)(const P &, Room &, bool, hipStream_t), const P &p, void *workspace, size_t bytes, hipStream_t s)
 {
-  Room need, room{static_cast<char *>(workspace), 0};
-  way(p, need, true, nullptr);
-  return need.used > bytes ? static_cast<int>(CAIFX_ERR_WORKSPACE_TOO_SMALL) : way(p, room, false, s);
+  Room room{static_cast<char *>(workspace), 0};
+  return room_of(way, p) > bytes ? static_cast<int>(CAIFX_ERR_WORKSPACE_TOO_SMALL) : way(p, room, false, s);
+}
+
+size_t product_bytes(const Product &p, bool dense_copy = true)
+{
+  return room_of(dense_copy && wide_product_pays(p) ? product_wide : product_rows, p);
 }
 int product(const Product &p, void *workspace, size_t bytes, hipStream_t s)
 {
-  const bool wide = wide_product_pays(p) && bytes >= product_bytes(p) && aligned_to(p.x, 16);
+  const bool wide = wide_product_pays(p) && bytes >= room_of(product_wide, p);
   return run_in(wide ? product_wide : product_rows, p, workspace, bytes, s);
 }
 
@@ -297,7 +307,7 @@ int gradient_wide(const Gradient &p, Room &room, bool only_size, hipStream_t s)
   const Operand x = activations_of(p.x[0], p.x[1], p.x_dtype, p.M, p.N);
   d.a = p.x[0];
   d.a_stride = static_cast<const char *>(p.x[1]) - static_cast<const char *>(p.x[0]);
-  if (pieces == 3 || p.x_dtype != to || R != p.N) {
+  if (copied(pieces, p.x_dtype, to, p.N, R, p.x[0], p.x[1])) {
     const size_t one = static_cast<size_t>(p.M) * static_cast<size_t>(R) * 2;
     void *operand = room.take(d.pairs * one);
     d.a = operand;
@@ -314,7 +324,7 @@ int gradient_wide(const Gradient &p, Room &room, bool only_size, hipStream_t s)
   return st != CAIFX_OK ? st : wide_run(d, room, only_size, s);
 }
 
-// The row kernels on the transposed copies: what neither of the others takes, activations at addresses that the dense product does not.
+// The row kernels on the transposed copies: what neither of the others takes, weights of nearly 2^22 rows and stored ones of less than 16 columns.
 int gradient_rows(const Gradient &p, Room &room, bool only_size, hipStream_t s)
 {
   const int to = stored_as(p.compute_dtype);
@@ -394,23 +404,12 @@ int gradient_dx(const Gradient &p, Room &room, bool only_size, hipStream_t s)
   return only_size ? CAIFX_OK : dx_product(d, partial, s);
 }
 
-size_t gradient_bytes(const Gradient &p)
+int (*gradient_way(const Gradient &p))(const Gradient &, Room &, bool, hipStream_t)
 {
-  Room dx, rows, wide;
-  if (dx_pays(p)) {
-    gradient_dx(p, dx, true, nullptr);
-    return dx.used;
-  }
-  gradient_rows(p, rows, true, nullptr);
-  if (!wide_gradient_takes(p)) return rows.used;
-  gradient_wide(p, wide, true, nullptr);
-  return rows.used > wide.used ? rows.used : wide.used;
+  return dx_pays(p) ? gradient_dx : wide_gradient_takes(p) ? gradient_wide : gradient_rows;
 }
-int gradient(const Gradient &p, void *workspace, size_t bytes, hipStream_t s)
-{
-  const bool wide = wide_gradient_takes(p) && aligned_to(p.x[0], 16) && aligned_to(p.x[1], 16);
-  return run_in(dx_pays(p) ? gradient_dx : wide ? gradient_wide : gradient_rows, p, workspace, bytes, s);
-}
+size_t gradient_bytes(const Gradient &p) { return room_of(gradient_way(p), p); }
+int gradient(const Gradient &p, void *workspace, size_t bytes, hipStream_t s) { return run_in(gradient_way(p), p, workspace, bytes, s); }
 
 Product product_of(const GemmArgs &a)
 {

@@ -213,7 +213,7 @@ CAIFX_API int caifx_qlinear_backward_input_add(int64_t M, int64_t N, int64_t K,
  * int4 with a 16-bit compute type multiplies the rounded weight either way).
  * CAIFX_W_MXFP4: activations in the kernels' order (from some dozens of rows on, in fp32 from five, those of another type or below eight
  * columns), the sums of workgroups that share a reduction, and from some hundred rows on dense copies of the weight (transposed for
- * the input gradient) and of operands of another type.  With less the forward runs without the dense copies, and otherwise the
+ * the input gradient) and of activations of another type or that do not begin at a multiple of 16 bytes.  With less the forward runs without the dense copies, and otherwise the
  * shape-agnostic kernels. */
 CAIFX_API size_t caifx_qlinear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_dtype, int compute_dtype,
                                      int w_kind, int backward);
