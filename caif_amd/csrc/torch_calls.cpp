@@ -167,6 +167,15 @@ at::Tensor bytes_like(const at::Tensor &x, size_t n)
   return at::empty({static_cast<int64_t>(n)}, x.options().dtype(at::kByte));
 }
 
+// the kernels write the caller's workspace by its address: anything but gapless memory of the input's device would be a fault
+void check_workspace(PyObject *given, const at::Tensor &x)
+{
+  if (given == Py_None) return;
+  const at::Tensor &t = tensor(given);
+  if (t.numel() > 0 && (t.device() != x.device() || !t.is_contiguous()))
+    throw Error{PyExc_ValueError, "the workspace must be contiguous and on the input's device"};
+}
+
 // the caller's workspace, or one of the size the library asks for (none for zero bytes)
 struct Workspace {
   at::Tensor held;
@@ -260,6 +269,7 @@ PyObject *qlinear(PyObject *, PyObject *const *a, Py_ssize_t n)
     const int kind = static_cast<int>(int_attr(w, at_.kind));
     const int64_t period = int_attr(w, at_.period);
     const int group = static_cast<int>(int_attr(w, at_.group));
+    check_workspace(a[6], x);
     c10::OptionalDeviceGuard guard;
     if (kind == CAIFX_W_MXFP4) {
       check_mxfp4(w, N, K, x);
@@ -304,6 +314,7 @@ PyObject *grouped(PyObject *, PyObject *const *a, Py_ssize_t n)
     const Py_ssize_t E = PySequence_Size(list.p);
     if (E < 0) throw Error{nullptr, nullptr};
     // sizes and dtypes are checked here, before anything is launched
+    check_workspace(a[7], x);
     if (x.numel() != rows * in) throw Error{PyExc_ValueError, "the input's size is not a multiple of the reduction length"};
     if (offsets.scalar_type() != at::kInt || offsets.numel() != E + 1) throw Error{PyExc_ValueError, "offsets must be int32 [experts + 1]"};
     if (a[6] != Py_None) {
