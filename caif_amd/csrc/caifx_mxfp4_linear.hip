@@ -76,10 +76,7 @@ RowsArgs rows_args(const Product &p)
 int rows_run(RowsArgs g, int kind, int weights, int compute_dtype, bool direct, Room &room, bool only_size, hipStream_t s)
 {
   const int pieces = pieces_of(compute_dtype);
-  const int tile = rows_tile(g.M, pieces);
-  const double row = kind == ROWS_DENSE ? static_cast<double>(g.w_pitch) : 17.0 * static_cast<double>(g.blocks);
-  const double x = (kind == ROWS_BOTH ? row : (direct ? 2.0 + (pieces > 1 ? 2.0 : 0.0) : 2.0 * pieces) * static_cast<double>(g.R)) * (g.M <= 4 && (direct || pieces == 1) ? 4 : tile);
-  const RowsPlan plan = rows_plan(g.M, g.N, g.R, weights, pieces, row, x);
+  const RowsPlan plan = rows_plan_of(kind, weights, pieces, direct, g.M, g.N, g.R, g.blocks, g.w_pitch);
   void *partial = plan.splits > 1 ? room.take(static_cast<size_t>(plan.splits) * static_cast<size_t>(g.M) * static_cast<size_t>(g.N) * 4) : nullptr;
   if (only_size) return CAIFX_OK;
   g.span = plan.span;
@@ -162,7 +159,7 @@ bool wide_product_pays(const Product &p)
   const int64_t tile = pieces == 3 ? 32 : 64, groups = (p.M + tile - 1) / tile * ((p.weights * p.N + tile - 1) / tile);
   const double rounds = static_cast<double>(groups / 256) + (groups % 256 == 0 ? 0.0 : 0.35 + 0.65 / 256 * static_cast<double>(groups % 256));
   const double rows = 5.0 + rounds * ((pieces == 3 ? 2.2 : 4.5) + 1.3 * static_cast<double>((R + 511) / 512));
-  return (p.weights == 2 ? wide_product_us(p.M, 2 * p.N, pieces * R) : wide_parts(p.M, p.N, pieces * R).us) + (pieces == 3 ? 12.0 : 8.0) + 0.56 * millions < rows;
+  return (p.weights == 2 ? wide_us_of(p.M, 2 * p.N, pieces * R) : wide_parts(p.M, p.N, pieces * R).us) + (pieces == 3 ? 12.0 : 8.0) + 0.56 * millions < rows;
 }
 
 // Whether the dense product reads activations from a copy: of another type or length, or that no 16-byte access takes where they are.  us, 4096 rows, N =

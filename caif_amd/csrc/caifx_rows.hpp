@@ -15,6 +15,7 @@
 // activations have 4 bits too, the same blocks go into v_mfma_scale_f32_16x16x128_f8f6f4 as they are.
 #pragma once
 
+#include "caifx_rows_plan.hpp"
 #include "caifx_wide.hpp"
 
 #include <type_traits>
@@ -23,49 +24,6 @@ namespace caifx {
 
 constexpr int kRowsChunk = 256;              // reduction elements of a chunk: 128 bytes of codes of a weight row
 constexpr int kRowsWaves = 8;
-
-// How a launch is cut up: columns of a workgroup, workgroups that share a reduction.
-struct RowsPlan {
-  int span, splits;
-};
-// Rows of a workgroup's tile.
-inline int rows_tile(int64_t M, int pieces) { return M <= 16 ? 16 : M <= 32 || pieces == 3 ? 32 : 64; }
-// The time of a launch in us, fitted to 60 calls (1 to 64 rows, 1024 x 4096 to 8192 x 28672 and 14336 x 4096): a start, the rounds that a
-// wave's units take, a compute unit's share of the weight at 20.7 KB a us (5.3 TB/s in all) and of the activations, which its caches
-// serve, at 80; a shared reduction costs a second launch and the sums' way there and back.
-inline double rows_us(double rows, double columns, double span, double splits, double units, double weight_row, double x_tile, double result)
-{
-  double rounds = rows * columns * splits / 256;
-  rounds = rounds < 1 ? 1 : rounds;
-  double turns = units / splits / 8;
-  turns = turns < 1 ? 1 : turns;
-  return 2.4 + rounds * (0.55 * turns + span * weight_row / splits / 20700 + x_tile / splits / 80000) + (splits > 1 ? 3.3 + splits * result * 8 / 4.0e6 : 0.0);
-}
-// A compute unit has some 100 lines on their way at a time whatever it asks for, so the launch is as fast as its fullest compute unit: the
-// columns are cut into a multiple of 256 parts, as large as the column tiles allow.  Where that leaves a workgroup few columns, so that
-// the activations are most of what it reads, 2 to 8 workgroups share a reduction of wider parts (N = 4096, K = 14336, 32 rows: 18 us in four,
-// 20 in one; the estimates say where).  x_tile: bytes of the activations that a workgroup reads.
-inline RowsPlan rows_plan(int64_t M, int64_t N, int64_t R, int weights, int pieces, double weight_row, double x_tile)
-{
-  const int tile = rows_tile(M, pieces);
-  const int64_t rows = (M + tile - 1) / tile, most = (pieces == 3 && tile == 32 ? 32 : 64) / weights;      // (three pieces of 32 rows: two column tiles)
-  const double units = static_cast<double>((R + 511) / 512);
-  RowsPlan best{};
-  double best_us = 0;
-  for (int splits = 1; splits <= 8; splits *= 2) {
-    if (splits > 1 && (weights > 1 || units < 4 * splits || rows * splits > 256)) break;
-    // rounds of workgroups, as few as leave the columns in parts of at most `most`
-    const int64_t least = (N + most - 1) / most, rounds = (least * rows * splits + 255) / 256;
-    const int64_t parts = 256 * rounds / (rows * splits), span = (N + parts - 1) / parts;
-    const double us = rows_us(static_cast<double>(rows), static_cast<double>((N + span - 1) / span), static_cast<double>(span), splits, units, weight_row, x_tile,
-                              static_cast<double>(M) * static_cast<double>(N));
-    if (splits == 1 || us < best_us) {
-      best = RowsPlan{static_cast<int>(span), splits};
-      best_us = us;
-    }
-  }
-  return best;
-}
 
 struct RowsArgs {
   const void *x;          // direct: [M, x_pitch] of the compute type, or fp32 for three pieces, x_pitch at least 8, at any address; packed: see pack_rows_kernel
@@ -84,8 +42,6 @@ struct RowsArgs {
   const void *addend;     // one weight: y = T(float(T(acc)) + float(addend))
   int y_dtype;
 };
-
-enum { ROWS_MX = 0, ROWS_DENSE = 1, ROWS_BOTH = 2 };      // ROWS_BOTH: weight and activations in microscaled 4 bits
 
 // dword d of lane group q becomes dword q of lane group d
 __device__ __forceinline__ u32x4_t exchange(u32x4_t v)
@@ -588,9 +544,9 @@ int rows_launch(const RowsArgs &g, hipStream_t s)
 template <typename CT, int P, int kWeight, int NW, int MT, int XG>
 int rows_pick_columns(const RowsArgs &g, hipStream_t s)
 {
-  const int tiles = NW * ((g.span + 15) / 16);
+  const int tiles = rows_column_tiles(g.span, NW);
   if constexpr (P == 1 || MT == 1) {
-    if (tiles > 2) return rows_launch<CT, P, kWeight, NW, MT, 4, XG>(g, s);
+    if (tiles == 4) return rows_launch<CT, P, kWeight, NW, MT, 4, XG>(g, s);
   }
   if constexpr (NW == 1) {
     if (tiles == 1) return rows_launch<CT, P, kWeight, NW, MT, 1, XG>(g, s);

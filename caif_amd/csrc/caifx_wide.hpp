@@ -2,6 +2,7 @@
 #pragma once
 
 #include "caifx_internal.hpp"
+#include "caifx_wide_plan.hpp"
 
 namespace caifx {
 
@@ -34,13 +35,5 @@ __device__ __forceinline__ float gate_act(float g)
 // whether the kernel takes these sizes; the operands have to be aligned to 16 bytes
 bool wide_takes(int64_t M, int64_t C, int64_t R);
 int wide_product(const WideProduct &p, hipStream_t s);
-// what a product takes, in us, estimated; gated: C of both weights together, chained: R of both pairs
-double wide_product_us(int64_t M, int64_t C, int64_t R);
-// into how many parts a product that is not gated is best cut, and what it takes with their joining, in us, estimated
-struct WideParts {
-  int parts;
-  double us;
-};
-WideParts wide_parts(int64_t M, int64_t C, int64_t R);
 
 }  // namespace caifx

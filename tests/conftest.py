@@ -53,3 +53,10 @@ def few_plans(tmp_path_factory):
     """How the few-row forward kernel cuts calls (rows, columns, reduction, kind): row tiles, their 16-row blocks, workgroups per reduction
     and the units of each; zeros where another kernel takes the call."""
     return _plans(tmp_path_factory, "few_plan")
+
+
+@pytest.fixture(scope="session")
+def mxfp4_plans(tmp_path_factory):
+    """Which forms products over 4-bit weights and gated blocks run in, see tests/cpp/mxfp4_plan.cpp: (0, rows, columns, reduction, kind, weights,
+    pieces, direct) for the row kernels, (1, rows, columns, reduction, gated) for the dense product."""
+    return _plans(tmp_path_factory, "mxfp4_plan")

@@ -46,9 +46,10 @@ def pieces_of(dtype):
 
 
 # ------------------------------------------------------------------ few rows: the columns of a weight are cut into about 256 parts
-# N = 14336 and 14339 give a workgroup 56 and 57 columns, four column tiles; 6001 two; K = 8200 beside 4096 columns is shared by several workgroups
+# N = 14336 and 14339 give a workgroup 56 and 57 columns, four column tiles; 6001 two; a reduction of 14337 beside 4096 columns is shared by several workgroups
 FEW = [(1, 14336, 1056), (4, 14339, 1403), (3, 14336, 330), (9, 14336, 1403), (16, 14339, 300), (24, 14336, 2048), (24, 14339, 1185), (50, 14336, 1056),
-       (64, 14339, 471), (100, 14336, 776), (2, 6001, 1403), (30, 6001, 520), (1, 4096, 8200), (24, 4096, 8193), (12, 4090, 16384)]
+       (64, 14339, 471), (100, 14336, 776), (2, 6001, 1403), (30, 6001, 520), (1, 4096, 8200), (24, 4096, 14337), (12, 4090, 16384),
+       (50, 4096, 14336)]
 
 
 @pytest.mark.parametrize("M,N,K", FEW)
@@ -130,8 +131,8 @@ def test_gradient(M, N, K, dtype):
 
 
 # ------------------------------------------------------------------ dense products: tiles of every size, several operand pairs, rows of any width
-# tiles of 256 x 256 (1030 x 4100, 2048 x 11008, 2041 x 11001, 1500 x 6000), 128 x 256 (2048 x 11001) and 128 x 128
-DENSE = [(1030, 4100, 1088), (2048, 11008, 520), (2041, 11001, 1003), (330, 4100, 1088), (333, 2003, 1403), (1500, 6000, 1088)]
+# gated: tiles of 256 x 256 (1030 x 4100, 2048 x 11008, 2041 x 11001), 128 x 256 (2048 x 5501) and 128 x 128
+DENSE = [(1030, 4100, 1088), (2048, 11008, 520), (2041, 11001, 1003), (2048, 5501, 600), (330, 4100, 1088), (333, 2003, 1403), (1500, 6000, 1088)]
 
 
 @pytest.mark.parametrize("M,N,K", DENSE)
