@@ -104,9 +104,9 @@ int mfma_f32_forward(const GemmArgs &a, hipStream_t s);
 int mfma_f32_backward(const GemmArgs &a, hipStream_t s);
 size_t mfma_f32_workspace_bytes(const GemmArgs &a, bool backward);
 
-// CAIFX_W_MXFP4, forward and input gradient, with an addend too.  UNSUPPORTED with less workspace than mxfp4_workspace_bytes (the forward
-// runs without its dense copy), for activations that are not aligned to 16 bytes where that is 0, and from 2^22 of N or K on: the
-// shape-agnostic kernels take those.
+// CAIFX_W_MXFP4, forward and input gradient, with an addend too, activations at any address.  UNSUPPORTED with less workspace than
+// mxfp4_workspace_bytes (the forward runs without its dense copy) or one that is not aligned to 16 bytes, and from 2^22 of N or K on:
+// the shape-agnostic kernels take those.
 int mxfp4_linear(const GemmArgs &a, bool backward, hipStream_t s);
 size_t mxfp4_workspace_bytes(const GemmArgs &a, bool backward, bool dense_copy);
 

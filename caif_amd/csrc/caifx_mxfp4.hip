@@ -281,7 +281,10 @@ __global__ __launch_bounds__(kThreads) void pack_rows_kernel(Sources two, unsign
 }
 
 // The gating's backward: grad_up = T(d g s), grad_gate = T(d u s (1 + g (1 - s))), s = 1 / (1 + exp(-g)).  Bound by memory: five tensors
-// (bf16, 2048 x 11008 42 us, 5.3 TB/s).  The results are rounded before the products that they go into, as the caller gets them.
+// (bf16, 2048 x 11008 42 us, 5.3 TB/s).  The results are rounded before the products that they go into: dx is the product of the gradients that
+// the caller gets, as where the projections' gradients are taken one after the other.  In bf16 dx is 2.35e-3 from 64 bits so (2-norm; 2048 rows, N =
+// 11008, K = 4096), 1.66e-3, its own rounding alone, with unrounded factors; those would be two bf16 pieces each, twice the matrix
+// instructions, 245 us more on 360.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void gating_backward_kernel(const T *__restrict__ grad, const T *__restrict__ gate, const T *__restrict__ up,
                                                                    T *__restrict__ grad_gate, T *__restrict__ grad_up, int64_t n)

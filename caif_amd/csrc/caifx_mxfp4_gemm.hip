@@ -8,8 +8,8 @@
 // M = 4096, N = 14336, K = 4096).
 // The columns' operand is the instruction's first one, so that a lane's four sums are neighbours of a row and go to LDS, on their way into
 // whole rows, 8 bytes (fp32: 16) at a time.
-// M = 4096, N = 14336, K = 4096: 137 us, 3.5 PFLOP/s.  A step takes 1.59 us where the matrix pipes alone take 1.32, and a tile 9 us more for its first
-// requests and its results, which all compute units write at once.
+// M = 4096, N = 14336, K = 4096: 137 us, 3.5 PFLOP/s, behind 5.5 for the scales' order.  A step takes 1.59 us where the matrix pipes alone
+// take 1.32, and a tile 9 us more for its first requests and its results, which all compute units write at once.
 // Blocks past the end of a row count for nothing: both scales are 2^-127 there, and codes have no infinities or NaN.
 #include "caifx_mxfp4.hpp"
 
@@ -63,8 +63,9 @@ template <int WI, int WJ, bool kTail> __device__ __forceinline__ void mx_tile(Mx
   const bool ends = z + 1 == g.parts;      // it has the rows' last step
   if (z > 0) g.d = static_cast<float *>(g.d) + z * g.M * g.C;
   // request i of a wave for half h of an operand: 8 rows x 128 bytes; LDS position p of row r holds 16-byte chunk p ^ (r ^ r >> 3) & 7 of
-  // the row (operand reads without bank conflicts).  Rows past the end are the last one again and never stored; of a row's last step
-  // chunks past its end are its last one again (their scales are 2^-127).
+  // the row, so that eight neighbouring lanes' operand reads use eight times four banks (the counters call half of the cycles in which LDS
+  // is busy conflicts all the same, as they do in caifx_gemm_wide.hip, which has no scales).  Rows past the end are the last one again and
+  // never stored; of a row's last step chunks past its end are its last one again (their scales are 2^-127).
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem));
   uint32_t a_voff[2][WI], b_voff[2][WJ], past[2];
   const int in_last = static_cast<int>((g.pitch - static_cast<int64_t>(total - 1) * 128) >> 4);      // chunks of the last step

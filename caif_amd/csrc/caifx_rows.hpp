@@ -4,8 +4,9 @@
 // Bound by memory with few rows (the weight's bytes), by the L1 from some dozens on: a compute unit has some 100 lines on their way at a
 // time, whatever it asks for, and the activations are read anew for every 16 NT weight rows.  So they are asked for in whole lines, only the
 // rows that there are, and take the operands' order in a wave's own part of LDS or, in larger calls, beforehand (see pack_rows_kernel).
-// Measured, bf16: one row, N = 14336, K = 4096 8.0 us (3.9 TB/s); 24 rows in fp16, N = 4096, K = 14336 13.9; eight rows of a gated block over two
-// 14336 x 4096 weights 15.2 (4.1 TB/s).
+// Measured, bf16, weights in turn so that none stays in the caches: one row, N = 14336, K = 4096 10.2 us (3.1 TB/s), 16 rows 11.8, one row of a gated
+// block over two such weights 19.2 (3.3 TB/s).  A weight used again and again, 31 MB that come half from the memory-side cache: one row 8.0; 24 rows in
+// fp16, N = 4096, K = 14336 13.9; eight rows of the gated block 15.2.
 // A workgroup of eight waves owns 16 MT rows and 16 NT weight rows of the result; the waves take units of 512 reduction elements in turn and their sums meet in LDS at the end.
 // So every wave streams its part of the weight rows straight into matrix-core operands, no wave waits for another in between, and a
 // launch of a usual weight has all of it on its way at once.  Lane (j, q) of v_mfma_f32_16x16x32 loads block

@@ -73,9 +73,10 @@ enum caifx_dtype { CAIFX_F32 = 0, CAIFX_F16 = 1, CAIFX_BF16 = 2 };
  *  CAIFX_W_MXFP4:      microscaled 4-bit floating point, codes and scales as caifx_mxfp4_quantize lays them out for N rows of K
  *                      columns (codes aligned to 16 bytes; scale_period and group_size are ignored).  Codes that fill up a row's
  *                      last block count for nothing, whatever they are.  Scale bytes 253 and 254, which quantising never gives,
- *                      take codes of 4 and 6, or from 2 on, beyond fp32: a result with one of them is an infinity, where
- *                      products are fp32 an infinity or a NaN.  fp16 compute rounds weights to fp16, infinities too.  Taken by the plain calls, with an addend too; the grouped
- *                      ones return CAIFX_ERR_UNSUPPORTED.  (5 is no kind.) */
+ *                      take codes of 4 and 6, or from 2 on, beyond fp32: a result with one of them is an infinity, with fp32 as
+ *                      the compute type an infinity or a NaN.  fp16 as the compute type rounds weights to it, beyond it to
+ *                      infinities.  Taken by the plain calls, with an addend too; the grouped ones return
+ *                      CAIFX_ERR_UNSUPPORTED.  (5 is no kind.) */
 enum caifx_weight_kind { CAIFX_W_INT8 = 0, CAIFX_W_INT4_GROUP = 1, CAIFX_W_F32 = 2, CAIFX_W_F16 = 3, CAIFX_W_BF16 = 4, CAIFX_W_MXFP4 = 6 };
 
 CAIFX_API const char *caifx_status_string(int status);
@@ -215,8 +216,8 @@ CAIFX_API int caifx_qlinear_backward_input_add(int64_t M, int64_t N, int64_t K,
  * int4 with a 16-bit compute type multiplies the rounded weight either way).
  * CAIFX_W_MXFP4: activations in the kernels' order (from some dozens of rows on, in fp32 from five, those of another type or below eight
  * columns), the sums of workgroups that share a reduction, and from some hundred rows on dense copies of the weight (transposed for
- * the input gradient) and of activations of another type or that do not begin at a multiple of 16 bytes.  With less the forward runs without the dense copies, and otherwise the
- * shape-agnostic kernels. */
+ * the input gradient) and of activations of another type or that do not begin at a multiple of 16 bytes.  With less the forward runs
+ * without the dense copies, and otherwise the shape-agnostic kernels. */
 CAIFX_API size_t caifx_qlinear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_dtype, int compute_dtype,
                                      int w_kind, int backward);
 /* The same without the dense copy of large calls: what is left is a few partial tiles, at most 16 MiB for the 16-bit compute
@@ -578,7 +579,8 @@ CAIFX_API size_t caifx_mxfp4_matmul_workspace_bytes(int64_t M, int64_t N, int64_
  * kinds.  All activations and results are of `dtype`, contiguous, any alignment of it; weights are aligned to 16 bytes.  Results alias
  * no input and no other result.  fp32 uses three bf16 pieces of each activation, which add up to it (weights beyond fp32: as said at
  * CAIFX_W_MXFP4).  CAIFX_ERR_UNSUPPORTED beyond
- * 2^30 rows and from an N or K of 2^22 on.  workspace: caifx_gated_workspace_bytes, CAIFX_ERR_WORKSPACE_TOO_SMALL for less.
+ * 2^30 rows and from an N or K of 2^22 on.  workspace: caifx_gated_workspace_bytes, CAIFX_ERR_WORKSPACE_TOO_SMALL for less.  Stored
+ * weights with a K that is no multiple of 8 are copied into it by every forward of few rows, both of them (N = 14336, K = 4100: 235 MB).
  * ------------------------------------------------------------------------- */
 
 /* With g = x w_gate^T and u = x w_up^T in fp32: hidden[M,N] = T(silu(g) * u), gate = T(g), up = T(u).  gate and up are what the
@@ -588,7 +590,7 @@ CAIFX_API int caifx_gated_forward(int64_t M, int64_t N, int64_t K, const void *x
                         void *workspace, size_t workspace_bytes, caifx_stream_t stream);
 /* With g, u = gate, up and s = 1 / (1 + exp(-g)):
  *   grad_up = T(grad_hidden * g s),  grad_gate = T(grad_hidden * u * s (1 + g (1 - s))),
- *   dx[M,K] = T(grad_gate w_gate + grad_up w_up), one sum of 2 N products.
+ *   dx[M,K] = T(grad_gate w_gate + grad_up w_up), one sum of 2 N products of the rounded grad_gate and grad_up.
  * dx may be NULL (a first layer): then only the gating's gradients are formed, and the weights and scales may be NULL too. */
 CAIFX_API int caifx_gated_backward(int64_t M, int64_t N, int64_t K, const void *grad_hidden, const void *gate, const void *up,
                          const void *w_gate, const void *scales_gate, const void *w_up, const void *scales_up, int w_kind,
