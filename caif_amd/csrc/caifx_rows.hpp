@@ -81,6 +81,7 @@ template <> struct Mfma16<f16_t> {
 };
 
 // A number as three of eight bits of its mantissa each, cut off and so exact, which add up to it; a bf16 in the upper half of every dword.
+// (bf16 has no numbers below 2^-133: what a number of less than 2^-109 has beneath that is lost.)
 __device__ __forceinline__ void pieces_of_f32(float value, uint32_t (&piece)[3])
 {
   const uint32_t bits = __builtin_bit_cast(uint32_t, value), high = bits & 0xFFFF0000u;

@@ -72,11 +72,12 @@ enum caifx_dtype { CAIFX_F32 = 0, CAIFX_F16 = 1, CAIFX_BF16 = 2 };
  *                      16-bit compute type first, fp32 products and sums), not on the fast paths of the quantised kinds.
  *  CAIFX_W_MXFP4:      microscaled 4-bit floating point, codes and scales as caifx_mxfp4_quantize lays them out for N rows of K
  *                      columns (codes aligned to 16 bytes; scale_period and group_size are ignored).  Codes that fill up a row's
- *                      last block count for nothing, whatever they are.  Scale bytes 253 and 254, which quantising never gives,
- *                      take codes of 4 and 6, or from 2 on, beyond fp32: a result with one of them is an infinity, with fp32 as
- *                      the compute type an infinity or a NaN.  fp16 as the compute type rounds weights to it, beyond it to
- *                      infinities.  Taken by the plain calls, with an addend too; the grouped ones return
- *                      CAIFX_ERR_UNSUPPORTED.  (5 is no kind.) */
+ *                      last block count for nothing, whatever they are.  fp32 as the compute type multiplies three bf16 pieces
+ *                      of each activation, which add up to it but for what it has beneath 2^-133.  Scale bytes 253 and 254,
+ *                      which quantising never gives, take codes of 4 and 6, or from 2 on, beyond fp32: a result with one of
+ *                      them is an infinity, with fp32 as the compute type an infinity or a NaN.  fp16 as the compute type rounds
+ *                      weights to it, beyond it to infinities.  Taken by the plain calls, with an addend too; the grouped ones
+ *                      return CAIFX_ERR_UNSUPPORTED.  (5 is no kind.) */
 enum caifx_weight_kind { CAIFX_W_INT8 = 0, CAIFX_W_INT4_GROUP = 1, CAIFX_W_F32 = 2, CAIFX_W_F16 = 3, CAIFX_W_BF16 = 4, CAIFX_W_MXFP4 = 6 };
 
 CAIFX_API const char *caifx_status_string(int status);
@@ -577,8 +578,7 @@ CAIFX_API size_t caifx_mxfp4_matmul_workspace_bytes(int64_t M, int64_t N, int64_
  * and the backward pass of that part (:266-316).
  * w_kind: CAIFX_W_MXFP4, or CAIFX_W_F16 / CAIFX_W_BF16 with dtype the same type (scales NULL then); CAIFX_ERR_UNSUPPORTED for other
  * kinds.  All activations and results are of `dtype`, contiguous, any alignment of it; weights are aligned to 16 bytes.  Results alias
- * no input and no other result.  fp32 uses three bf16 pieces of each activation, which add up to it (weights beyond fp32: as said at
- * CAIFX_W_MXFP4).  CAIFX_ERR_UNSUPPORTED beyond
+ * no input and no other result.  fp32: as said at CAIFX_W_MXFP4.  CAIFX_ERR_UNSUPPORTED beyond
  * 2^30 rows and from an N or K of 2^22 on.  workspace: caifx_gated_workspace_bytes, CAIFX_ERR_WORKSPACE_TOO_SMALL for less.  Stored
  * weights with a K that is no multiple of 8 are copied into it by every forward of few rows, both of them (N = 14336, K = 4100: 235 MB).
  * ------------------------------------------------------------------------- */
