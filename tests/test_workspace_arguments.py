@@ -27,3 +27,19 @@ def test_host_memory_and_gaps(kind, backward):
                 call(x, w, T.BF16, workspace=workspace)
         with pytest.raises(ValueError, match="workspace"):
             call(x, w, T.BF16, workspace=torch.empty(1 << 16, dtype=torch.uint8, device="cuda:1"))
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_expert_segments(backward):
+    with FakeTensorMode():
+        class Experts:
+            weights = [weight(T.W_INT8), weight(T.W_INT8)]
+            N, K, w_kind, scale_period, group_size = 8, 128, T.W_INT8, 8, 128
+            wq_ptrs = torch.empty(2, dtype=torch.int64, device="cuda")
+            scales_ptrs = torch.empty(2, dtype=torch.int64, device="cuda")
+        x = torch.empty(4, 8 if backward else 128, dtype=torch.bfloat16, device="cuda")
+        offsets = torch.empty(3, dtype=torch.int32, device="cuda")
+        call = T.qlinear_grouped_backward_input if backward else T.qlinear_grouped_forward
+        for workspace in (torch.empty(1 << 16, dtype=torch.uint8), torch.empty(1, dtype=torch.uint8, device="cuda").expand(1 << 16)):
+            with pytest.raises(ValueError, match="workspace"):
+                call(x, offsets, Experts, T.BF16, workspace=workspace)
